@@ -117,6 +117,53 @@ ORL_API int orl_attn_fwd_noalloc(const void* q, const void* k, const void* v, vo
                                  long long nk, int heads, int head_dim, float scale, const int32_t* cu_q_host,
                                  const int32_t* cu_k_host, int n_seg, int* status_host, void* stream);
 
+/* ---------------------------------------------------------------- attention, backward
+ * The gradients the reference gets from FlashAttention's autograd (attention.py:39-53): with S = scale q k^T,
+ * P = exp(S - lse), delta = sum_d dout out - dlse:  dv = P^T dout, dS = P * (dout v^T - delta), dq = scale dS k,
+ * dk = scale dS^T q. Deterministic: no atomics, key rows shared by several segments are summed in a fixed order. */
+
+#define ORL_ATTN_BWD_KV 0 /* the item's rows are key rows, its ranges the query rows that read them */
+#define ORL_ATTN_BWD_Q 1  /* the item's rows are query rows, its ranges the key rows they read */
+
+/* One backward work item: up to 128 rows of one head. */
+typedef struct orl_attn_bwd_work {
+  int32_t row0;     /* first row */
+  int32_t rows;     /* 1..128 */
+  int32_t head;
+  int32_t kind;     /* ORL_ATTN_BWD_KV or ORL_ATTN_BWD_Q */
+  int32_t range0;   /* first of its ranges */
+  int32_t n_ranges; /* 0: the rows' gradients are zero */
+  int32_t n_tiles;  /* 128-row tiles of its ranges */
+  int32_t pad;
+} orl_attn_bwd_work;
+
+/* Work list of a backward call for segments given as in orl_attn_plan_ranges (key ranges may overlap, query ranges
+ * may not) over nq query and nk key rows; rows of no segment get zero gradients. Returns the item count and stores
+ * the number of ranges (pairs first row, rows); if a buffer is NULL or too small returns -(items + 1000). */
+ORL_API int orl_attn_bwd_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start,
+                              const int32_t* k_len, int n_seg, int heads, long long nq, long long nk,
+                              orl_attn_bwd_work* work, int work_capacity, int32_t* ranges, int ranges_capacity,
+                              int* n_ranges);
+
+/* dq [nq, heads, head_dim], dk / dv [nk, heads, head_dim] bf16 from the forward's inputs, out and lse [heads, nq], the
+ * gradient dout of out and, unless NULL, dlse [heads, nq] of lse. work_dev / ranges_dev: the plan in device memory.
+ * stats_dev: scratch of 2 * heads * nq floats, 16-byte aligned. */
+ORL_API int orl_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                         const float* lse, const float* dlse, void* dq, void* dk, void* dv, long long nq, long long nk,
+                         int heads, int head_dim, float scale, const orl_attn_bwd_work* work_dev, int n_items,
+                         const int32_t* ranges_dev, float* stats_dev, int* err_dev, void* stream);
+
+/* As orl_attn_bwd with cu_seqlens in DEVICE memory, planned on the device (see orl_attn_fwd_cu). scratch_dev: at
+ * least orl_attn_bwd_cu_scratch(nq, nk, n_seg, heads) bytes, 16-byte aligned. At most 4096 segments. */
+ORL_API int orl_attn_bwd_cu(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                            const float* lse, const float* dlse, void* dq, void* dk, void* dv, long long nq,
+                            long long nk, int heads, int head_dim, float scale, const int32_t* cu_q_dev,
+                            const int32_t* cu_k_dev, int n_seg, void* scratch_dev, long long scratch_bytes,
+                            float* stats_dev, int* err_dev, void* stream);
+
+/* Bytes of scratch orl_attn_bwd_cu needs. */
+ORL_API long long orl_attn_bwd_cu_scratch(long long nq, long long nk, int n_seg, int heads);
+
 /* One row-range copy of a pack: `nbytes` from base[src_slot] + src_off to base[dst_slot] + dst_off. */
 typedef struct orl_copy_run {
   int32_t src_slot; /* index into src_bases */

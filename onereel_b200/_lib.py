@@ -47,6 +47,8 @@ class Path(ctypes.Structure):
 
 # numpy views of the same layouts (for building tables without Python loops over ctypes objects)
 WORK_DTYPE = np.dtype([(n, np.int32) for n, _ in AttnWork._fields_])
+BWD_WORK_DTYPE = np.dtype([(n, np.int32) for n in ('row0', 'rows', 'head', 'kind', 'range0', 'n_ranges', 'n_tiles',
+                                                    'pad')])
 RUN_DTYPE = np.dtype([('src_slot', np.int32), ('dst_slot', np.int32), ('src_off', np.int64), ('dst_off', np.int64),
                       ('vec0', np.int64)])
 assert WORK_DTYPE.itemsize == ctypes.sizeof(AttnWork) == 32 and RUN_DTYPE.itemsize == ctypes.sizeof(CopyRun) == 32
@@ -66,6 +68,12 @@ SIGNATURES = {
     'orl_attn_fwd_cu_capacity': (c_ll, [c_ll, c_int, c_int]),
     'orl_attn_fwd_noalloc': (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_ll, c_ll, c_int, c_int, c_float, P_I32, P_I32,
                                      c_int, c_vp, c_vp]),
+    'orl_attn_bwd_plan': (c_int, [P_I32, P_I32, P_I32, P_I32, c_int, c_int, c_ll, c_ll, c_vp, c_int, c_vp, c_int,
+                                  ctypes.POINTER(c_int)]),
+    'orl_attn_bwd': (c_int, [c_vp] * 10 + [c_ll, c_ll, c_int, c_int, c_float, c_vp, c_int, c_vp, c_vp, c_vp, c_vp]),
+    'orl_attn_bwd_cu': (c_int, [c_vp] * 10 + [c_ll, c_ll, c_int, c_int, c_float, c_vp, c_vp, c_int, c_vp, c_ll, c_vp,
+                                              c_vp, c_vp]),
+    'orl_attn_bwd_cu_scratch': (c_ll, [c_ll, c_ll, c_int, c_int]),
     'orl_pack_prepare': (c_ll, [c_vp, P_I64, c_int]),
     'orl_pack': (c_int, [c_vp, c_int, c_ll, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp]),
     'orl_peer_barrier': (c_int, [ctypes.POINTER(c_vp), c_int, c_int, c_int, ctypes.c_ulonglong, c_vp, c_vp]),

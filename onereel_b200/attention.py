@@ -6,6 +6,11 @@ selects FlashAttention-2/-3 by BACKEND; here every value runs the sm_100a kernel
 and 'auto' are accepted so existing callers keep working). There is no CPU or library fallback: inputs must be bf16
 CUDA tensors with head_dim 64 or 128.
 
+Gradients: like the reference's FlashAttention calls, `varlen`, `varlen_lse`, `packed`, `packed_lse`,
+`overlapping_ranges` and `dense` are differentiable in q, k and v (also through the log-sum-exp) when autograd is on
+and an input requires a gradient; the backward pass (onereel_b200/csrc/attn_bwd.cu) recomputes the probabilities and is
+deterministic. `attend_grad` is the same computation as a plain call. First derivatives only.
+
 Kernel failures: the kernel never hangs; a bounded wait that gives up sets a per-device error word. `check()`
 synchronises and raises if it is set (tests and benchmarks call it; it costs a device sync).
 """
@@ -15,6 +20,7 @@ from collections import OrderedDict
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
 from onereel_b200.pack import pack_rows
@@ -205,23 +211,30 @@ def _cu_to_ranges(cu_q, cu_k):
 _CU_WORK = {}    # (device, stream) -> work-list scratch of orl_attn_fwd_cu (uint8), grown as needed
 
 
-def _attend_cu(q, k, v, cu_q, cu_k, lse):
-    """cu_seqlens on the device: orl_attn_fwd_cu plans the work list on the GPU, no host synchronisation. The
-    scratch is per (device, stream), so calls on one stream reuse it in order."""
-    _check_inputs(q, k, v)
+def _check_cu(q, cu_q, cu_k):
     for name, c in (('cu_seqlens_q', cu_q), ('cu_seqlens_k', cu_k)):
         if c.dtype != torch.int32 or c.dim() != 1 or c.device != q.device or not c.is_contiguous():
             raise TypeError(f'{name} must be a contiguous int32 tensor on {q.device}')
     if cu_q.numel() != cu_k.numel() or cu_q.numel() < 1:
         raise ValueError('cu_seqlens_q and cu_seqlens_k differ in length')
+
+
+def _attend_cu(q, k, v, cu_q, cu_k, lse, own_scratch=False):
+    """cu_seqlens on the device: orl_attn_fwd_cu plans the work list on the GPU, no host synchronisation. The
+    scratch is per (device, stream), so calls on one stream reuse it in order; own_scratch: scratch of this call alone
+    (safe in captured graphs that replay side by side)."""
+    _check_inputs(q, k, v)
+    _check_cu(q, cu_q, cu_k)
     Nq, H, Dh = q.shape
     dev = q.device
     n_seg = cu_q.numel() - 1
     need = L.check(L.lib().orl_attn_fwd_cu_capacity(Nq, n_seg, H), 'orl_attn_fwd_cu_capacity')
     stream = torch.cuda.current_stream(dev)
     key = (dev.index, stream.cuda_stream)
-    work = _CU_WORK.get(key)
-    if work is None or work.numel() < need * L.WORK_DTYPE.itemsize:
+    work = None if own_scratch else _CU_WORK.get(key)
+    if own_scratch:
+        work = torch.empty(need * L.WORK_DTYPE.itemsize, dtype=torch.uint8, device=dev)
+    elif work is None or work.numel() < need * L.WORK_DTYPE.itemsize:
         work = _CU_WORK[key] = torch.empty(need * L.WORK_DTYPE.itemsize, dtype=torch.uint8, device=dev)
     out = torch.empty_like(q)
     lse_t = torch.empty(H, Nq, dtype=torch.float32, device=dev) if lse else None
@@ -233,20 +246,180 @@ def _attend_cu(q, k, v, cu_q, cu_k, lse):
     return out, lse_t
 
 
+# ------------------------------------------------------------------------------------------------ gradients
+
+_BWD_PLANS: OrderedDict = OrderedDict()
+
+
+def _plan_bwd(q_start, q_len, k_start, k_len, heads: int, nq: int, nk: int, device):
+    """device work list and ranges of the backward pass for segments given as (start, length) rows (cached like
+    `plan`): (items uint8 [32 n], ranges int32 [m, 2], n)"""
+    key = (tuple(q_start), tuple(q_len), tuple(k_start), tuple(k_len), heads, nq, nk, str(device))
+    hit = _BWD_PLANS.get(key)
+    if hit is not None:
+        _BWD_PLANS.move_to_end(key)
+        return hit
+    arrs = [np.ascontiguousarray(x, dtype=np.int32) for x in (q_start, q_len, k_start, k_len)]
+    args = [L.i32p(a) for a in arrs] + [len(arrs[0]), heads, nq, nk]
+    n_ranges = L.c_int(0)
+    n = L.lib().orl_attn_bwd_plan(*args, None, 0, None, 0, n_ranges)
+    if n <= -1000:
+        work = np.zeros(-n - 1000, dtype=L.BWD_WORK_DTYPE)
+        ranges = np.zeros((max(n_ranges.value, 1), 2), dtype=np.int32)
+        n = L.lib().orl_attn_bwd_plan(*args, work.ctypes.data, len(work), ranges.ctypes.data, n_ranges.value, n_ranges)
+    else:
+        work, ranges = np.zeros(1, dtype=L.BWD_WORK_DTYPE), np.zeros((1, 2), dtype=np.int32)
+    L.check(n, 'orl_attn_bwd_plan')
+    res = (torch.from_numpy(work.view(np.uint8)).to(device), torch.from_numpy(ranges).to(device), n)
+    _BWD_PLANS[key] = res
+    if len(_BWD_PLANS) > 512:
+        _BWD_PLANS.popitem(last=False)
+    return res
+
+
+def _grad_buffers(q, k, v, out, lse, dout, dlse):
+    """the checked, contiguous gradient inputs, the gradient tensors and the statistics scratch of a backward call"""
+    Nq, H, Dh = q.shape
+    for name, x, shape, dtype in (('out', out, q.shape, torch.bfloat16), ('dout', dout, q.shape, torch.bfloat16),
+                                  ('lse', lse, (H, Nq), torch.float32), ('dlse', dlse, (H, Nq), torch.float32)):
+        if x is None and name == 'dlse':
+            continue
+        if not (isinstance(x, torch.Tensor) and x.device == q.device and x.dtype == dtype):
+            raise TypeError(f'{name} must be a {dtype} tensor on {q.device}')
+        if tuple(x.shape) != tuple(shape):
+            raise ValueError(f'{name} must have shape {tuple(shape)}, got {tuple(x.shape)}')
+    def c(x):                                    # contiguous and 16-byte aligned (a gradient may be any view)
+        x = x.contiguous()
+        return x if x.data_ptr() % 16 == 0 else x.clone()
+    dlse = None if dlse is None else c(dlse)
+    stats = torch.empty(2 * H * Nq, dtype=torch.float32, device=q.device)
+    return c(out), lse.contiguous(), c(dout), dlse, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), stats
+
+
+def _bwd_pointers(q, k, v, out, lse, dout, dlse, dq, dk, dv):
+    return [x.data_ptr() for x in (q, k, v, out, dout, lse)] + [None if dlse is None else dlse.data_ptr()] + \
+        [x.data_ptr() for x in (dq, dk, dv)]
+
+
+def attend_grad(q, k, v, out, lse, dout, q_start, q_len, k_start, k_len, dlse=None, scale=None):
+    """(dq, dk, dv) of `attend` on the same segments from its out and lse, the gradient dout of out and (optional) dlse
+    of lse. Query ranges must not overlap; key ranges may, and a shared key row's gradient is the sum over its readers.
+    Rows of no segment get zeros."""
+    _check_inputs(q, k, v)
+    Nq, H, Dh = q.shape
+    dev = q.device
+    with torch.cuda.device(dev):
+        out, lse, dout, dlse, dq, dk, dv, stats = _grad_buffers(q, k, v, out, lse, dout, dlse)
+        work, ranges, n = _plan_bwd(q_start, q_len, k_start, k_len, H, Nq, k.shape[0], dev)
+        L.check(L.lib().orl_attn_bwd(*_bwd_pointers(q, k, v, out, lse, dout, dlse, dq, dk, dv), Nq, k.shape[0], H, Dh,
+                                     Dh ** -0.5 if scale is None else float(scale), work.data_ptr(), n,
+                                     ranges.data_ptr(), stats.data_ptr(), _err_word(dev).data_ptr(),
+                                     torch.cuda.current_stream(dev).cuda_stream), 'orl_attn_bwd')
+    return dq, dk, dv
+
+
+def _attend_cu_grad(q, k, v, out, lse, dout, dlse, cu_q, cu_k):
+    """attend_grad for cu_seqlens on the device, planned there (orl_attn_bwd_cu)"""
+    Nq, H, Dh = q.shape
+    Nk, dev, n_seg = k.shape[0], q.device, cu_q.numel() - 1
+    with torch.cuda.device(dev):
+        out, lse, dout, dlse, dq, dk, dv, stats = _grad_buffers(q, k, v, out, lse, dout, dlse)
+        need = L.check(L.lib().orl_attn_bwd_cu_scratch(Nq, Nk, n_seg, H), 'orl_attn_bwd_cu_scratch')
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+        L.check(L.lib().orl_attn_bwd_cu(*_bwd_pointers(q, k, v, out, lse, dout, dlse, dq, dk, dv), Nq, Nk, H, Dh,
+                                        Dh ** -0.5, cu_q.data_ptr(), cu_k.data_ptr(), n_seg, scratch.data_ptr(), need,
+                                        stats.data_ptr(), _err_word(dev).data_ptr(),
+                                        torch.cuda.current_stream(dev).cuda_stream), 'orl_attn_bwd_cu')
+    return dq, dk, dv
+
+
+class _Ranges(torch.autograd.Function):
+    """attend on (start, length) segments, differentiable in q, k, v"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, segments):
+        with torch.cuda.device(q.device):
+            out, lse = attend(q, k, v, *segments, lse=True)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.segments = segments
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dlse):
+        if dout is None and dlse is None:
+            return None, None, None, None
+        q, k, v, out, lse = ctx.saved_tensors
+        dout = torch.zeros_like(out) if dout is None else dout
+        return *attend_grad(q, k, v, out, lse, dout, *ctx.segments, dlse=dlse), None
+
+
+class _Varlen(torch.autograd.Function):
+    """attention on device cu_seqlens, differentiable in q, k, v; neither pass synchronises with the host"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k):
+        with torch.cuda.device(q.device):
+            out, lse = _attend_cu(q, k, v, cu_q, cu_k, lse=True, own_scratch=True)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dlse):
+        if dout is None and dlse is None:
+            return None, None, None, None, None
+        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        dout = torch.zeros_like(out) if dout is None else dout
+        return *_attend_cu_grad(q, k, v, out, lse, dout, dlse, cu_q, cu_k), None, None
+
+
+class _PackRows(torch.autograd.Function):
+    """row tensors packed back to back (pack_rows); every part's gradient is its rows of the packed gradient"""
+
+    @staticmethod
+    def forward(ctx, *parts):
+        ctx.lengths = [p.shape[0] for p in parts]
+        return pack_rows(parts, parts[0].new_empty(sum(ctx.lengths), *parts[0].shape[1:]))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return g.split(ctx.lengths)
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def _attend_ranges(q, k, v, q_start, q_len, k_start, k_len, lse=False):
+    """(out, lse or None) of host-planned segments, differentiable where an input asks for it"""
+    if _wants_grad(q, k, v):
+        _check_inputs(q, k, v)
+        return _Ranges.apply(q, k, v, (q_start, q_len, k_start, k_len))
+    return attend(q, k, v, q_start, q_len, k_start, k_len, lse=True if lse else None)
+
+
 def varlen(q, k, v, cu_q, cu_k, max_q, max_k):
     """attention.py:39-43: packed q [Nq, H, D], k / v [Nk, H, D] -> out [Nq, H, D]. cu_seqlens as device int32
     tensors (as the reference passes them) are planned on the GPU without a host sync; host lists are planned on
     the host."""
     if isinstance(cu_q, torch.Tensor) and cu_q.is_cuda:
+        if _wants_grad(q, k, v):
+            return _Varlen.apply(q, k, v, cu_q, cu_k)[0]
         return _attend_cu(q, k, v, cu_q, cu_k, lse=False)[0]
-    return attend(q, k, v, *_cu_to_ranges(cu_q, cu_k))[0]
+    return _attend_ranges(q, k, v, *_cu_to_ranges(cu_q, cu_k))[0]
 
 
 def varlen_lse(q, k, v, cu_q, cu_k, max_q, max_k):
     """attention.py:46-53: (out [Nq, H, D], lse [H, Nq] fp32, natural log)"""
     if isinstance(cu_q, torch.Tensor) and cu_q.is_cuda:
+        if _wants_grad(q, k, v):
+            return _Varlen.apply(q, k, v, cu_q, cu_k)
         return _attend_cu(q, k, v, cu_q, cu_k, lse=True)
-    return attend(q, k, v, *_cu_to_ranges(cu_q, cu_k), lse=True)
+    return _attend_ranges(q, k, v, *_cu_to_ranges(cu_q, cu_k), lse=True)
 
 
 def _pack_segments(segments):
@@ -254,13 +427,16 @@ def _pack_segments(segments):
     lk = [s[1].shape[0] for s in segments]
     q0 = segments[0][0]
     H, Dh = q0.shape[1:]
-    qp = q0.new_empty(sum(lq), H, Dh)
-    kp = q0.new_empty(sum(lk), H, Dh)
-    vp = q0.new_empty(sum(lk), H, Dh)
     c = lambda x: x if x.is_contiguous() else x.contiguous()
-    pack_rows([c(s[0]) for s in segments], qp)
-    pack_rows([c(s[1]) for s in segments], kp)
-    pack_rows([c(s[2]) for s in segments], vp)
+    if _wants_grad(*(x for s in segments for x in s)):
+        qp, kp, vp = (_PackRows.apply(*(c(s[i]) for s in segments)) for i in range(3))
+    else:
+        qp = q0.new_empty(sum(lq), H, Dh)
+        kp = q0.new_empty(sum(lk), H, Dh)
+        vp = q0.new_empty(sum(lk), H, Dh)
+        pack_rows([c(s[0]) for s in segments], qp)
+        pack_rows([c(s[1]) for s in segments], kp)
+        pack_rows([c(s[2]) for s in segments], vp)
     cq, ck = np.cumsum([0] + lq), np.cumsum([0] + lk)
     return qp, kp, vp, lq, list(cq[:-1]), lk, list(ck[:-1])
 
@@ -268,7 +444,7 @@ def _pack_segments(segments):
 def packed_lse(segments):
     """attention.py:56-62: list of (out, lse [H, n]) per segment, one kernel call"""
     qp, kp, vp, lq, qs, lk, ks = _pack_segments(segments)
-    o, lse = attend(qp, kp, vp, qs, lq, ks, lk, lse=True)
+    o, lse = _attend_ranges(qp, kp, vp, qs, lq, ks, lk, lse=True)
     return list(zip(o.split(lq), lse.split(lq, dim=1)))
 
 
@@ -276,7 +452,7 @@ def packed(segments):
     """attention.py:65-71: segments = list of (q, k, v) -> list of outputs, one gather/pack launch per tensor and one
     attention launch"""
     qp, kp, vp, lq, qs, lk, ks = _pack_segments(segments)
-    return attend(qp, kp, vp, qs, lq, ks, lk)[0].split(lq)
+    return _attend_ranges(qp, kp, vp, qs, lq, ks, lk)[0].split(lq)
 
 
 def overlapping_ranges(q, k, v, q_ranges, k_ranges):
@@ -286,7 +462,7 @@ def overlapping_ranges(q, k, v, q_ranges, k_ranges):
     ql = [b - a for a, b in q_ranges]
     if qs and (qs[0] != 0 or any(qs[i] + ql[i] != qs[i + 1] for i in range(len(qs) - 1)) or qs[-1] + ql[-1] != q.shape[0]):
         raise ValueError('q_ranges must tile q in order')
-    return attend(q, k, v, qs, ql, [a for a, _ in k_ranges], [b - a for a, b in k_ranges])[0]
+    return _attend_ranges(q, k, v, qs, ql, [a for a, _ in k_ranges], [b - a for a, b in k_ranges])[0]
 
 
 def dense(q, k, v):
@@ -294,7 +470,7 @@ def dense(q, k, v):
     B, S, H, Dh = q.shape
     Sk = k.shape[1]
     c = lambda x: x.reshape(B * x.shape[1], H, Dh).contiguous()
-    o = attend(c(q), c(k), c(v), [b * S for b in range(B)], [S] * B, [b * Sk for b in range(B)], [Sk] * B)[0]
+    o = _attend_ranges(c(q), c(k), c(v), [b * S for b in range(B)], [S] * B, [b * Sk for b in range(B)], [Sk] * B)[0]
     return o.view(B, S, H, Dh)
 
 

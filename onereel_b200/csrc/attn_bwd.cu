@@ -1,0 +1,1004 @@
+// Packed variable-length scene attention, backward, bf16 in / fp32 accumulate / bf16 out, for sm_100a.
+//
+// With S = scale q k^T, P = exp(S - lse) (recomputed from the forward's log-sum-exp), o = P v and incoming gradients
+// dO of o and dL of lse:
+//   delta_i = sum_d dO_id o_id - dL_i        dP = dO v^T        dS = P * (dP - delta)
+//   dq = scale dS k        dk = scale dS^T q        dv = P^T dO
+// delta and lse * log2(e) come from a first, memory-bound kernel ([heads, nq] pairs). The main kernel has two kinds of
+// work items, both a block of up to 128 rows of one head that stays resident while tiles of 128 rows stream past it:
+//   kDkv: K / V rows resident, the q / dO rows that read them stream:  S^T = K q^T, dP^T = V dO^T,
+//         dV += P^T dO, dK += dS^T q. Its ranges are every query range that reads the rows, so key ranges that several
+//         segments share are summed in fp32 in a fixed order.
+//   kDq:  q / dO rows resident, their K / V rows stream:               S = q K^T, dP = dO V^T, dQ += dS K.
+// S and dP are computed twice (seven products of the size of S instead of five). In exchange nothing is added across
+// CTAs: no atomics, no fp32 dQ in memory, the same bits on every run.
+//
+// A CTA is the forward's: warp 0 streams tiles by TMA, warp 1 owns TMEM and issues the MMAs, warps 2-3 prepare each
+// tile (row statistics of streamed queries; zeros in the shared-memory rows past a range's end, so that what lies
+// there - other segments, or NaN in rows no segment owns - enters no product), warps 4-11 hold P and dS: a warp owns 16
+// TMEM lanes, a thread two rows and 32 of their 128 columns each. P and dS go back to TMEM as bf16 and are the A
+// operand of the accumulating MMAs.
+// TMEM columns, kDkv: S^T / P^T [0,128), dP^T / dS^T [128,256), dV [256,256+D), dK [256+D,256+2D): while the compute
+// warps work on P the tensor pipe runs dK of the previous tile and dP of this one; while they work on dS, dV and the
+// next S. kDq: S / dS [0,128) and [128,256) by turns, dP [256,384), dQ [384,384+D).
+// Every mbarrier wait is bounded as in the forward: a stuck pipeline sets the error word and winds down.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <mutex>
+#include <new>
+#include <vector>
+
+#include "orl_common.h"
+#include "ptx.cuh"
+#include "tensor_map.cuh"
+
+namespace orl {
+
+using BwdWork = orl_attn_bwd_work;
+static_assert(sizeof(BwdWork) == 32, "backward work item layout");
+constexpr int kDkv = ORL_ATTN_BWD_KV, kDq = ORL_ATTN_BWD_Q;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct BwdCfg {
+  static constexpr int kChunks = D / 64;              // 128-byte swizzle columns per row
+  static constexpr int kTileBytes = 128 * D * 2;      // one 128-row bf16 tile
+  static constexpr int kChunkBytes = 128 * 128;       // one 128-row x 64-column chunk
+  static constexpr int kStages = (D == 128) ? 2 : 4;  // ring depth of streamed tile pairs
+  // resident tiles R0, R1 (K, V or q, dO), streamed tiles T0, T1 (q, dO or K, V)
+  static constexpr int kROff = 0;
+  static constexpr int kTOff = 2 * kTileBytes;
+  static constexpr int kStatOff = kTOff + 2 * kStages * kTileBytes;   // float2 (lse2, delta) of 128 streamed rows
+  static constexpr int kValidOff = kStatOff + kStages * 1024;         // int: rows of the tile inside its range
+  static constexpr int kBarOff = kValidOff + 16 * ((kStages * 4 + 15) / 16);
+  static constexpr int kBarR = 0;                       // resident tiles landed
+  static constexpr int kBarT0 = 1;                      // streamed tiles landed, per stage
+  static constexpr int kBarT1 = kBarT0 + kStages;
+  static constexpr int kBarAux = kBarT1 + kStages;      // statistics and zeroed rows ready, per stage
+  static constexpr int kBarE = kBarAux + kStages;       // stage free
+  static constexpr int kBarS = kBarE + kStages;         // S computed (two buffers in kDq)
+  static constexpr int kBarDp = kBarS + 2;              // dP computed
+  static constexpr int kBarP = kBarDp + 1;              // kDkv: P stored; kDq: dP read
+  static constexpr int kBarDs = kBarP + 1;              // dS stored
+  static constexpr int kBarDone = kBarDs + 1;
+  static constexpr int kBarDrain = kBarDone + 1;
+  static constexpr int kNumBars = kBarDrain + 1;
+  static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
+  static constexpr uint32_t kTmemCols = 512;
+  static constexpr uint32_t kColDv = 256, kColDk = 256 + D;       // kDkv (S at 0, dP at 128)
+  static constexpr uint32_t kColDp = 256, kColDq = 384;           // kDq (S at 0 and 128)
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+constexpr int kBwdThreads = 384;
+constexpr int kAuxThreads = 64;
+// register split as in the forward: 4 x 32 x 120 + 8 x 32 x 192 = 384 x 168
+constexpr int kBwdLaunchRegs = 168, kBwdRegsLow = 120, kBwdRegsHigh = 192;
+static_assert(4 * kBwdRegsLow + 8 * kBwdRegsHigh == 12 * kBwdLaunchRegs, "register split must add up to the launch total");
+
+__device__ __forceinline__ void bwd_drain_wait(uint32_t bar, uint32_t parity, int* err) {
+  const unsigned long long t0 = global_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (global_ns() - t0 > kWaitLimitNs) {
+      atomicOr(err, kErrTimeoutDrain);
+      return;
+    }
+  }
+}
+
+struct BwdShared {
+  uint8_t* smem;         // 1024-aligned tile area
+  uint32_t sbase;        // its shared-window address
+  uint32_t bar0;         // address of barrier 0
+  volatile int* abort_flag;
+  __device__ uint32_t bar(int i) const { return bar0 + 8u * i; }
+};
+
+// the tiles of an item's ranges in order: each range cut into 128-row tiles, the last one of a range shorter
+struct TileWalk {
+  const int2* ranges;
+  int left;              // ranges not yet begun
+  int row, rest;         // next row and rows left in the current range
+  __device__ TileWalk(const int2* r, int n) : ranges(r), left(n), row(0), rest(0) {}
+  // moves to the next tile: its first row, its rows in the return value
+  __device__ int next(int& first) {
+    while (rest <= 0) {
+      if (left == 0) return 0;
+      const int2 r = __ldg(ranges++);
+      --left;
+      row = r.x;
+      rest = r.y;
+    }
+    first = row;
+    const int n = min(128, rest);
+    row += 128;
+    rest -= 128;
+    return n;
+  }
+};
+
+// ---------------------------------------------------------------------------------------------- TMA producer
+template <int D>
+__device__ __forceinline__ void bwd_producer(const BwdShared& sh, const CUtensorMap* r0, const CUtensorMap* r1,
+                                             const CUtensorMap* t0, const CUtensorMap* t1, const BwdWork& wi,
+                                             const int2* ranges, int* err) {
+  using C = BwdCfg<D>;
+  const uint64_t pol_r = policy_evict_first();
+  const uint64_t pol_t = policy_evict_last();
+  const int x0 = wi.head * D;
+  mbar_expect_tx(sh.bar(C::kBarR), 2 * C::kTileBytes);
+  for (int c = 0; c < C::kChunks; ++c) {
+    tma_load_2d(sh.sbase + C::kROff + c * C::kChunkBytes, r0, sh.bar(C::kBarR), x0 + 64 * c, wi.row0, pol_r);
+    tma_load_2d(sh.sbase + C::kROff + C::kTileBytes + c * C::kChunkBytes, r1, sh.bar(C::kBarR), x0 + 64 * c, wi.row0,
+                pol_r);
+  }
+  TileWalk walk(ranges, wi.n_ranges);
+  int issued = 0;
+  for (int j = 0; j < wi.n_tiles; ++j) {
+    const int s = j % C::kStages;
+    int y = 0;
+    walk.next(y);
+    if (j >= C::kStages && !mbar_wait(sh.bar(C::kBarE + s), ((j / C::kStages) - 1) & 1, sh.abort_flag)) {
+      atomicOr(err, kErrTimeoutLoad);
+      break;
+    }
+    const uint32_t a = sh.sbase + C::kTOff + 2 * s * C::kTileBytes;
+    mbar_expect_tx(sh.bar(C::kBarT0 + s), C::kTileBytes);
+    for (int c = 0; c < C::kChunks; ++c)
+      tma_load_2d(a + c * C::kChunkBytes, t0, sh.bar(C::kBarT0 + s), x0 + 64 * c, y, pol_t);
+    mbar_expect_tx(sh.bar(C::kBarT1 + s), C::kTileBytes);
+    for (int c = 0; c < C::kChunks; ++c)
+      tma_load_2d(a + C::kTileBytes + c * C::kChunkBytes, t1, sh.bar(C::kBarT1 + s), x0 + 64 * c, y, pol_t);
+    issued = j + 1;
+  }
+  if (*sh.abort_flag) {
+    // wind down: every copy this thread started must land before the CTA's shared memory is released
+    bwd_drain_wait(sh.bar(C::kBarR), 0, err);
+    for (int j = issued > C::kStages ? issued - C::kStages : 0; j < issued; ++j) {
+      const int s = j % C::kStages;
+      bwd_drain_wait(sh.bar(C::kBarT0 + s), (j / C::kStages) & 1, err);
+      bwd_drain_wait(sh.bar(C::kBarT1 + s), (j / C::kStages) & 1, err);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- tile preparation
+// 64 threads (t = 0..63). Per streamed tile: the number of its rows inside the range; in kDkv the statistics of its
+// query rows (lse2 = +inf past the end, so P = 0 there); zeros over the shared-memory rows past the end. In kDq only
+// T0 (K) needs them: the columns of S and dP past the end are masked, but dS K sums over K's rows.
+template <int D>
+__device__ __forceinline__ void bwd_aux(const BwdShared& sh, const BwdWork& wi, const int2* ranges,
+                                        const float2* __restrict__ stats, long long nq, int t, int* err) {
+  using C = BwdCfg<D>;
+  const bool dkv = wi.kind == kDkv;
+  const float2* st = stats + static_cast<long long>(wi.head) * nq;
+  TileWalk walk(ranges, wi.n_ranges);
+  for (int j = 0; j < wi.n_tiles; ++j) {
+    const int s = j % C::kStages;
+    int row = 0;
+    const int valid = walk.next(row);
+    float2 a = make_float2(INFINITY, 0.f), b = a;
+    if (dkv) {
+      if (t < valid) a = __ldg(st + row + t);
+      if (t + 64 < valid) b = __ldg(st + row + t + 64);
+    }
+    bool ok = true;
+    if (j >= C::kStages) ok = mbar_wait(sh.bar(C::kBarE + s), ((j / C::kStages) - 1) & 1, sh.abort_flag);
+    if (ok && valid < 128) {
+      ok = mbar_wait(sh.bar(C::kBarT0 + s), (j / C::kStages) & 1, sh.abort_flag);
+      if (ok && dkv) ok = mbar_wait(sh.bar(C::kBarT1 + s), (j / C::kStages) & 1, sh.abort_flag);
+    }
+    if (!ok) {
+      if (t == 0) atomicOr(err, kErrTimeoutLoad);
+      return;
+    }
+    if (dkv) {
+      float2* dst = reinterpret_cast<float2*>(sh.smem + C::kStatOff + s * 1024);
+      dst[t] = a;
+      dst[t + 64] = b;
+    }
+    if (t == 0) *reinterpret_cast<int*>(sh.smem + C::kValidOff + 4 * s) = valid;
+    if (valid < 128) {
+      uint8_t* tiles = sh.smem + C::kTOff + 2 * s * C::kTileBytes;
+      const int n_chunks = dkv ? 2 * C::kChunks : C::kChunks;   // T0's chunks, then T1's
+      for (int c = 0; c < n_chunks; ++c)
+        for (int o = valid * 128 + t * 16; o < C::kChunkBytes; o += kAuxThreads * 16)
+          *reinterpret_cast<uint4*>(tiles + c * C::kChunkBytes + o) = make_uint4(0u, 0u, 0u, 0u);
+      fence_async_smem();
+    }
+    mbar_arrive(sh.bar(C::kBarAux + s));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- MMA issuer
+template <int D>
+struct BwdMma {
+  using C = BwdCfg<D>;
+  static constexpr uint32_t kIdescS = idesc_bf16(128, 128, false, false);
+  static constexpr uint32_t kIdescA = idesc_bf16(128, D, false, true);
+  // D[col] = R (resident tile r) * T (streamed tile t of stage s)^T
+  static __device__ __forceinline__ void product(const BwdShared& sh, uint32_t d, int r, int t, int s) {
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint32_t off = (kk >> 2) * C::kChunkBytes + (kk & 3) * 32;
+      const uint64_t a = smem_desc_sw128(sh.sbase + C::kROff + r * C::kTileBytes + off, 16, 1024);
+      const uint64_t b = smem_desc_sw128(sh.sbase + C::kTOff + (2 * s + t) * C::kTileBytes + off, 16, 1024);
+      mma_ss(d, a, b, kIdescS, kk > 0 ? 1u : 0u);
+    }
+  }
+  // D[col] (+)= A (bf16 in TMEM, 128 x 128) * T (streamed tile t of stage s, MN-major)
+  static __device__ __forceinline__ void accumulate(const BwdShared& sh, uint32_t d, uint32_t a, int t, int s,
+                                                    bool acc) {
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      const uint64_t b =
+          smem_desc_sw128(sh.sbase + C::kTOff + (2 * s + t) * C::kTileBytes + kk * 2048, C::kChunkBytes, 1024);
+      mma_ts(d, a + kk * 8, b, kIdescA, (acc || kk > 0) ? 1u : 0u);
+    }
+  }
+};
+
+template <int D>
+__device__ __forceinline__ void bwd_mma(const BwdShared& sh, uint32_t tmem, const BwdWork& wi, int* err) {
+  using C = BwdCfg<D>;
+  using M = BwdMma<D>;
+  const int n = wi.n_tiles;
+  const bool dkv = wi.kind == kDkv;
+  auto wait = [&](int bar, int phase) { return mbar_wait(sh.bar(bar), phase & 1, sh.abort_flag); };
+  // S of tile j: its streamed T0, prepared
+  auto issue_s = [&](int j) {
+    const int s = j % C::kStages, ph = j / C::kStages;
+    if (!wait(C::kBarT0 + s, ph) || !wait(C::kBarAux + s, ph)) return false;
+    const int buf = dkv ? 0 : (j & 1);
+    M::product(sh, tmem + 128 * buf, 0, 0, s);
+    mma_commit(sh.bar(C::kBarS + buf));
+    return true;
+  };
+  bool ok = wait(C::kBarR, 0) && issue_s(0);
+  for (int j = 0; ok && j < n; ++j) {
+    const int s = j % C::kStages, ph = j / C::kStages;
+    ok = wait(C::kBarT1 + s, ph);
+    if (!ok) break;
+    if (dkv) {
+      // dP overwrites dS of tile j - 1, whose dK MMA was issued before
+      M::product(sh, tmem + 128, 1, 1, s);
+      mma_commit(sh.bar(C::kBarDp));
+      ok = wait(C::kBarP, j);
+      if (!ok) break;
+      tc_fence_after();
+      M::accumulate(sh, tmem + C::kColDv, tmem, 1, s, j > 0);
+      if (j + 1 < n) ok = issue_s(j + 1);
+      ok = ok && wait(C::kBarDs, j);
+      if (!ok) break;
+      tc_fence_after();
+      M::accumulate(sh, tmem + C::kColDk, tmem + 128, 0, s, j > 0);
+    } else {
+      ok = j == 0 || wait(C::kBarP, j - 1);          // dP of tile j - 1 read
+      if (!ok) break;
+      tc_fence_after();
+      M::product(sh, tmem + C::kColDp, 1, 1, s);
+      mma_commit(sh.bar(C::kBarDp));
+      if (j + 1 < n) ok = issue_s(j + 1);            // over dS of tile j - 1, whose dQ MMA was issued before
+      ok = ok && wait(C::kBarDs, j);
+      if (!ok) break;
+      tc_fence_after();
+      M::accumulate(sh, tmem + C::kColDq, tmem + 128 * (j & 1), 0, s, j > 0);
+    }
+    mma_commit(sh.bar(C::kBarE + s));
+  }
+  if (ok) {
+    mma_commit(sh.bar(C::kBarDone));
+  } else {
+    atomicOr(err, kErrTimeoutMma);
+    mma_commit(sh.bar(C::kBarDrain));
+    bwd_drain_wait(sh.bar(C::kBarDrain), 0, err);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- P and dS
+// Thread layout of the .16x256b / .16x128b TMEM shapes: warp sw owns lanes 32 (sw % 4) + 16 (sw / 4) + [0, 16); its
+// thread holds the rows lane / 4 and lane / 4 + 8 of that block, register 4r + 2i + e of a 64-column load: row i,
+// column 8r + 2 (lane % 4) + e.
+struct BwdThread {
+  int cq, row;           // lane % 4; tile row of the first of the two rows
+  uint32_t lane_off;     // TMEM lane field
+  __device__ BwdThread(int sw, int lane)
+      : cq(lane & 3),
+        row(32 * (sw & 3) + 16 * (sw >> 2) + (lane >> 2)),
+        lane_off(static_cast<uint32_t>(32 * (sw & 3) + 16 * (sw >> 2)) << 16) {}
+};
+
+// rows of an accumulator scaled to bf16: tile row r of the item -> dst row row0 + r, columns head * D ..
+template <int D>
+__device__ __forceinline__ void bwd_store(uint32_t acc, const BwdThread& th, const BwdWork& wi, float f,
+                                          __nv_bfloat16* __restrict__ dst, int heads) {
+  const bool v0 = th.row < wi.rows, v1 = th.row + 8 < wi.rows;
+  __nv_bfloat16* o0 = dst + (static_cast<long long>(wi.row0) + th.row) * heads * D + wi.head * D + 2 * th.cq;
+  __nv_bfloat16* o1 = o0 + 8ll * heads * D;
+#pragma unroll
+  for (int ch = 0; ch < D / 64; ++ch) {
+    uint32_t o[32];
+    tmem_ld_16x256b_x8(acc + th.lane_off + 64 * ch, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int col = 64 * ch + 8 * r;
+      if (v0)
+        *reinterpret_cast<uint32_t*>(o0 + col) =
+            pack_bf16x2(__uint_as_float(o[4 * r + 0]) * f, __uint_as_float(o[4 * r + 1]) * f);
+      if (v1)
+        *reinterpret_cast<uint32_t*>(o1 + col) =
+            pack_bf16x2(__uint_as_float(o[4 * r + 2]) * f, __uint_as_float(o[4 * r + 3]) * f);
+    }
+  }
+}
+
+// rows no product reaches (keys no query reads, queries without keys): zero gradients
+template <int D>
+__device__ __forceinline__ void bwd_zero(const BwdThread& th, const BwdWork& wi, __nv_bfloat16* __restrict__ dst,
+                                         int heads) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (th.row + 8 * i >= wi.rows) continue;
+    __nv_bfloat16* o = dst + (static_cast<long long>(wi.row0) + th.row + 8 * i) * heads * D + wi.head * D + 2 * th.cq;
+    for (int col = 0; col < D; col += 8) *reinterpret_cast<uint32_t*>(o + col) = 0u;
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tmem, const BwdThread& th,
+                                                const BwdWork& wi, float scale, __nv_bfloat16* __restrict__ dk,
+                                                __nv_bfloat16* __restrict__ dv, int heads, int* err) {
+  using C = BwdCfg<D>;
+  const float scale_log2 = scale * kLog2e;
+  const uint32_t s_addr = tmem + th.lane_off, dp_addr = s_addr + 128;
+  bool ok = true;
+  uint32_t p[64];                               // scores, then P in fp32
+  for (int j = 0; j < wi.n_tiles; ++j) {
+    const int s = j % C::kStages, ph = (j / C::kStages) & 1;
+    ok = mbar_wait(sh.bar(C::kBarAux + s), ph, sh.abort_flag) && mbar_wait(sh.bar(C::kBarS), j & 1, sh.abort_flag);
+    if (!ok) break;
+    tc_fence_after();
+    // (lse2, delta) of columns 8r + 2 cq + {0, 1}: one 16-byte load
+    const float4* st = reinterpret_cast<const float4*>(sh.smem + C::kStatOff + s * 1024) + th.cq;
+    tmem_ld_16x256b_x8(s_addr, p);
+    tmem_ld_16x256b_x8(s_addr + 64, p + 32);
+    tmem_wait_ld();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[16];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float4 c = st[4 * (8 * h + r)];
+        uint32_t* x = p + 4 * (8 * h + r);
+        const float a0 = ex2(fmaf(__uint_as_float(x[0]), scale_log2, -c.x));
+        const float a1 = ex2(fmaf(__uint_as_float(x[1]), scale_log2, -c.z));
+        const float b0 = ex2(fmaf(__uint_as_float(x[2]), scale_log2, -c.x));
+        const float b1 = ex2(fmaf(__uint_as_float(x[3]), scale_log2, -c.z));
+        x[0] = __float_as_uint(a0);
+        x[1] = __float_as_uint(a1);
+        x[2] = __float_as_uint(b0);
+        x[3] = __float_as_uint(b1);
+        w[2 * r] = pack_bf16x2(a0, a1);
+        w[2 * r + 1] = pack_bf16x2(b0, b1);
+      }
+      tmem_st_16x128b_x8(s_addr + 32 * h, w);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(sh.bar(C::kBarP));
+    ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
+    if (!ok) break;
+    tc_fence_after();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t d[32], w[16];
+      tmem_ld_16x256b_x8(dp_addr + 64 * h, d);
+      tmem_wait_ld();
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float4 c = st[4 * (8 * h + r)];
+        const uint32_t* x = p + 4 * (8 * h + r);
+        const float a0 = __uint_as_float(x[0]) * (__uint_as_float(d[4 * r + 0]) - c.y);
+        const float a1 = __uint_as_float(x[1]) * (__uint_as_float(d[4 * r + 1]) - c.w);
+        const float b0 = __uint_as_float(x[2]) * (__uint_as_float(d[4 * r + 2]) - c.y);
+        const float b1 = __uint_as_float(x[3]) * (__uint_as_float(d[4 * r + 3]) - c.w);
+        w[2 * r] = pack_bf16x2(a0, a1);
+        w[2 * r + 1] = pack_bf16x2(b0, b1);
+      }
+      // dS words of half h go over the dP columns [32 h, 32 h + 32), which half 0 has loaded
+      tmem_st_16x128b_x8(dp_addr + 32 * h, w);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(sh.bar(C::kBarDs));
+  }
+  if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
+  if (!ok) {
+    atomicOr(err, kErrTimeoutSoftmax);
+    return;
+  }
+  tc_fence_after();
+  bwd_store<D>(tmem + C::kColDv, th, wi, 1.f, dv, heads);
+  bwd_store<D>(tmem + C::kColDk, th, wi, scale, dk, heads);
+}
+
+template <int D>
+__device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tmem, const BwdThread& th,
+                                               const BwdWork& wi, float scale, const float2* __restrict__ stats,
+                                               long long nq, __nv_bfloat16* __restrict__ dq, int heads, int* err) {
+  using C = BwdCfg<D>;
+  const float scale_log2 = scale * kLog2e;
+  const float2* st = stats + static_cast<long long>(wi.head) * nq + wi.row0 + th.row;
+  const float2 st0 = th.row < wi.rows ? __ldg(st) : make_float2(INFINITY, 0.f);
+  const float2 st1 = th.row + 8 < wi.rows ? __ldg(st + 8) : make_float2(INFINITY, 0.f);
+  const uint32_t dp_addr = tmem + C::kColDp + th.lane_off;
+  bool ok = true;
+  uint32_t p[64];
+  for (int j = 0; j < wi.n_tiles; ++j) {
+    const int s = j % C::kStages, ph = (j / C::kStages) & 1;
+    const uint32_t s_addr = tmem + 128 * (j & 1) + th.lane_off;
+    ok = mbar_wait(sh.bar(C::kBarAux + s), ph, sh.abort_flag) &&
+         mbar_wait(sh.bar(C::kBarS + (j & 1)), (j >> 1) & 1, sh.abort_flag);
+    if (!ok) break;
+    tc_fence_after();
+    const int valid = *reinterpret_cast<const volatile int*>(sh.smem + C::kValidOff + 4 * s);
+    tmem_ld_16x256b_x8(s_addr, p);
+    tmem_ld_16x256b_x8(s_addr + 64, p + 32);
+    tmem_wait_ld();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      uint32_t* x = p + 4 * r;
+      x[0] = __float_as_uint(ex2(fmaf(__uint_as_float(x[0]), scale_log2, -st0.x)));
+      x[1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[1]), scale_log2, -st0.x)));
+      x[2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[2]), scale_log2, -st1.x)));
+      x[3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[3]), scale_log2, -st1.x)));
+    }
+    ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
+    if (!ok) break;
+    tc_fence_after();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t d[32], w[16];
+      tmem_ld_16x256b_x8(dp_addr + 64 * h, d);
+      tmem_wait_ld();
+      if (h == 1) {
+        tc_fence_before();
+        mbar_arrive(sh.bar(C::kBarP));
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const uint32_t* x = p + 4 * (8 * h + r);
+        float a0 = __uint_as_float(x[0]) * (__uint_as_float(d[4 * r + 0]) - st0.y);
+        float a1 = __uint_as_float(x[1]) * (__uint_as_float(d[4 * r + 1]) - st0.y);
+        float b0 = __uint_as_float(x[2]) * (__uint_as_float(d[4 * r + 2]) - st1.y);
+        float b1 = __uint_as_float(x[3]) * (__uint_as_float(d[4 * r + 3]) - st1.y);
+        if (valid < 128) {
+          // keys past the range: whatever their rows held, they add nothing
+          const int col = 64 * h + 8 * r + 2 * th.cq;
+          a0 = col < valid ? a0 : 0.f;
+          b0 = col < valid ? b0 : 0.f;
+          a1 = col + 1 < valid ? a1 : 0.f;
+          b1 = col + 1 < valid ? b1 : 0.f;
+        }
+        w[2 * r] = pack_bf16x2(a0, a1);
+        w[2 * r + 1] = pack_bf16x2(b0, b1);
+      }
+      tmem_st_16x128b_x8(s_addr + 32 * h, w);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(sh.bar(C::kBarDs));
+  }
+  if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
+  if (!ok) {
+    atomicOr(err, kErrTimeoutSoftmax);
+    return;
+  }
+  tc_fence_after();
+  bwd_store<D>(tmem + C::kColDq, th, wi, scale, dq, heads);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                    const BwdWork* __restrict__ work, const int2* __restrict__ ranges,
+                    const float2* __restrict__ stats, __nv_bfloat16* __restrict__ dq, __nv_bfloat16* __restrict__ dk,
+                    __nv_bfloat16* __restrict__ dv, long long nq, int heads, float scale, int* __restrict__ err,
+                    const int* __restrict__ n_items_dev) {
+  using C = BwdCfg<D>;
+  // a grid sized by an upper bound (work list planned on the device): CTAs past the planned count have no item
+  if (n_items_dev != nullptr && static_cast<int>(blockIdx.x) >= __ldg(n_items_dev)) return;
+  extern __shared__ uint8_t smem_raw[];
+  BwdShared sh;
+  sh.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  sh.sbase = smem_u32(sh.smem);
+  sh.bar0 = sh.sbase + C::kBarOff;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sh.smem + C::kBarOff + C::kNumBars * 8);
+  sh.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const BwdWork wi = work[blockIdx.x];
+  const bool dkv = wi.kind == kDkv;
+
+  if (threadIdx.x == 0) {
+    mbar_init(sh.bar(C::kBarR), 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(sh.bar(C::kBarT0 + s), 1);
+      mbar_init(sh.bar(C::kBarT1 + s), 1);
+      mbar_init(sh.bar(C::kBarAux + s), kAuxThreads);
+      mbar_init(sh.bar(C::kBarE + s), 1);
+    }
+    mbar_init(sh.bar(C::kBarS), 1);
+    mbar_init(sh.bar(C::kBarS + 1), 1);
+    mbar_init(sh.bar(C::kBarDp), 1);
+    mbar_init(sh.bar(C::kBarP), 256);
+    mbar_init(sh.bar(C::kBarDs), 256);
+    mbar_init(sh.bar(C::kBarDone), 1);
+    mbar_init(sh.bar(C::kBarDrain), 1);
+    *sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int2* rg = ranges + wi.range0;
+
+  if (warp < 4) {
+    // warpgroup 0 returns registers at one program point (all four warps), then splits into its roles
+    regs_dec<kBwdRegsLow>();
+    if (wi.n_tiles > 0) {
+      if (warp == 0) {
+        if (elect_one()) {
+          if (dkv) bwd_producer<D>(sh, &tm_k, &tm_v, &tm_q, &tm_do, wi, rg, err);
+          else bwd_producer<D>(sh, &tm_q, &tm_do, &tm_k, &tm_v, wi, rg, err);
+        }
+      } else if (warp == 1) {
+        if (elect_one()) bwd_mma<D>(sh, tmem, wi, err);
+      } else {
+        bwd_aux<D>(sh, wi, rg, stats, nq, threadIdx.x - 64, err);
+      }
+    }
+  } else {
+    regs_inc<kBwdRegsHigh>();
+    const BwdThread th(warp - 4, lane);
+    if (wi.n_tiles == 0) {
+      if (dkv) {
+        bwd_zero<D>(th, wi, dk, heads);
+        bwd_zero<D>(th, wi, dv, heads);
+      } else {
+        bwd_zero<D>(th, wi, dq, heads);
+      }
+    } else if (dkv) {
+      bwd_compute_dkv<D>(sh, tmem, th, wi, scale, dk, dv, heads, err);
+    } else {
+      bwd_compute_dq<D>(sh, tmem, th, wi, scale, stats, nq, dq, heads, err);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- row statistics
+// stats[h][row] = (lse * log2 e, sum_d dO o - dL). Memory bound: dO and o are read once, 16 bytes per thread, D / 8
+// lanes per (row, head); a block covers 32 rows x 8 heads and writes its pairs through shared memory, so that the
+// head-major statistics are written in runs of 32 rows.
+template <int D>
+__global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const __nv_bfloat16* __restrict__ out,
+                                                             const __nv_bfloat16* __restrict__ dout,
+                                                             const float* __restrict__ lse,
+                                                             const float* __restrict__ dlse,
+                                                             float2* __restrict__ stats, long long nq, int heads) {
+  constexpr int kLanes = D / 8;                 // lanes per (row, head)
+  constexpr int kPer = 256 / kLanes;            // (row, head) pairs per pass: 8 heads x kPer / 8 rows
+  __shared__ float delta[8][33];
+  const int t = threadIdx.x, g = t / kLanes, l = t % kLanes;
+  const long long row0 = 32ll * blockIdx.x;
+  const int h0 = 8 * blockIdx.y;
+  const int h = h0 + g % 8;
+#pragma unroll
+  for (int i = 0; i < 32 / (kPer / 8); ++i) {
+    const int r = i * (kPer / 8) + g / 8;
+    const long long row = row0 + r;
+    float sum = 0.f;
+    if (row < nq && h < heads) {
+      const long long at = (row * heads + h) * D + 8 * l;
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(out + at));
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(dout + at));
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]));
+        const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[e]));
+        sum += u.x * v.x + u.y * v.y;
+      }
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (l == 0) delta[g % 8][r] = sum;
+  }
+  __syncthreads();
+  const int hh = h0 + (t >> 5);
+  const long long row = row0 + (t & 31);
+  if (hh < heads && row < nq) {
+    const long long at = static_cast<long long>(hh) * nq + row;
+    float d = delta[t >> 5][t & 31];
+    if (dlse != nullptr) d -= dlse[at];
+    stats[at] = make_float2(lse[at] * kLog2e, d);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+
+template <int D>
+static int launch_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                           const float* lse, const float* dlse, void* dq, void* dk, void* dv, long long nq,
+                           long long nk, int heads, float scale, const BwdWork* work, int n_items, const int2* ranges,
+                           float2* stats, int* err, cudaStream_t stream, const int* n_items_dev) {
+  using C = BwdCfg<D>;
+  // an empty side has no tiles to load: its maps only need a valid address
+  if (nk == 0) k = v = q;
+  if (nq == 0) q = dout = k;
+  const long long rq = nq > 0 ? nq : nk, rk = nk > 0 ? nk : nq;
+  CUtensorMap mq, mk, mv, mdo;
+  const long long w = static_cast<long long>(heads) * D;
+  int rc;
+  if ((rc = make_rows_map(&mq, q, rq, w, w, 128)) != ORL_OK) return rc;
+  if ((rc = make_rows_map(&mdo, dout, rq, w, w, 128)) != ORL_OK) return rc;
+  if ((rc = make_rows_map(&mk, k, rk, w, w, 128)) != ORL_OK) return rc;
+  if ((rc = make_rows_map(&mv, v, rk, w, w, 128)) != ORL_OK) return rc;
+  static std::mutex mu;
+  static bool attr_set[kMaxDevices] = {};
+  static int launch_regs = 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return ORL_ERR_LAUNCH;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!attr_set[dev]) {
+      if (cudaFuncSetAttribute(attn_bwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) !=
+          cudaSuccess)
+        return ORL_ERR_LAUNCH;
+      cudaFuncAttributes fa{};
+      if (cudaFuncGetAttributes(&fa, attn_bwd_kernel<D>) != cudaSuccess) return ORL_ERR_LAUNCH;
+      launch_regs = fa.numRegs;
+      attr_set[dev] = true;
+    }
+  }
+  // as in the forward: a build with another register count could leave the split's increase waiting, so it never runs
+  if (launch_regs != kBwdLaunchRegs) return ORL_ERR_UNSUPPORTED;
+  if (nq > 0) {
+    const dim3 grid(static_cast<unsigned>((nq + 31) / 32), static_cast<unsigned>((heads + 7) / 8));
+    attn_bwd_stats_kernel<D><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(out),
+                                                       static_cast<const __nv_bfloat16*>(dout), lse, dlse, stats, nq,
+                                                       heads);
+    if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
+  }
+  attn_bwd_kernel<D><<<n_items, kBwdThreads, C::kSmemBytes, stream>>>(
+      mq, mk, mv, mdo, work, ranges, stats, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
+      static_cast<__nv_bfloat16*>(dv), nq, heads, scale, err, n_items_dev);
+  return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
+}
+
+static bool bwd_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+static int check_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+                     void* dq, void* dk, void* dv, long long nq, long long nk, int heads, int head_dim, float scale,
+                     const void* stats, const int* err) {
+  if (nq < 0 || nk < 0 || nq > 0x7fffffffLL || nk > 0x7fffffffLL || heads <= 0 || !(scale > 0.f) || err == nullptr)
+    return ORL_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128) return ORL_ERR_UNSUPPORTED;
+  if (static_cast<long long>(heads) * head_dim > 0x7fffffffLL) return ORL_ERR_ARG;
+  if (nq > 0 && (q == nullptr || out == nullptr || dout == nullptr || lse == nullptr || dq == nullptr ||
+                 stats == nullptr))
+    return ORL_ERR_ARG;
+  if (nk > 0 && (k == nullptr || v == nullptr || dk == nullptr || dv == nullptr)) return ORL_ERR_ARG;
+  for (const void* p : {q, k, v, out, dout, static_cast<const void*>(dq), static_cast<const void*>(dk),
+                        static_cast<const void*>(dv), stats})
+    if (!bwd_aligned(p)) return ORL_ERR_ALIGN;
+  return ORL_OK;
+}
+
+// Work list of the backward, on the host. Key rows are cut at every start and end of a segment's keys: inside one of
+// the resulting intervals all rows are read by the same segments.
+struct BwdPlan {
+  std::vector<BwdWork> items;
+  std::vector<int2> ranges;
+};
+
+static int plan_bwd(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start, const int32_t* k_len,
+                    int n_seg, int heads, long long nq, long long nk, BwdPlan& plan) {
+  struct Block {
+    int row0, rows, kind, range0, n_ranges, n_tiles;
+  };
+  std::vector<Block> blocks;
+  std::vector<int> by_q;                                  // segments with query rows, by first row
+  for (int i = 0; i < n_seg; ++i) {
+    if (q_len[i] < 0 || k_len[i] < 0 || q_start[i] < 0 || k_start[i] < 0) return ORL_ERR_ARG;
+    if (static_cast<long long>(q_start[i]) + q_len[i] > nq || static_cast<long long>(k_start[i]) + k_len[i] > nk)
+      return ORL_ERR_ARG;
+    if (q_len[i] > 0) by_q.push_back(i);
+  }
+  auto cut = [&](long long lo, long long hi, int kind, int range0, int n_ranges, int n_tiles) {
+    for (long long r = lo; r < hi; r += 128)
+      blocks.push_back({static_cast<int>(r), static_cast<int>(std::min<long long>(128, hi - r)), kind, range0, n_ranges,
+                        n_tiles});
+  };
+  // queries: one range of keys per segment; rows of no segment get zeros
+  std::sort(by_q.begin(), by_q.end(), [&](int a, int b) { return q_start[a] < q_start[b]; });
+  long long at = 0;
+  for (int i : by_q) {
+    if (q_start[i] < at) return ORL_ERR_ARG;              // two segments share a query row
+    cut(at, q_start[i], kDq, 0, 0, 0);
+    plan.ranges.push_back({k_start[i], k_len[i]});
+    cut(q_start[i], static_cast<long long>(q_start[i]) + q_len[i], kDq, static_cast<int>(plan.ranges.size()) - 1, 1,
+        (k_len[i] + 127) / 128);
+    at = static_cast<long long>(q_start[i]) + q_len[i];
+  }
+  cut(at, nq, kDq, 0, 0, 0);
+  // keys: the elementary intervals, each with the query ranges of the segments that cover it (in segment order)
+  std::vector<long long> cuts = {0, nk};
+  for (int i = 0; i < n_seg; ++i)
+    if (q_len[i] > 0 && k_len[i] > 0) {
+      cuts.push_back(k_start[i]);
+      cuts.push_back(static_cast<long long>(k_start[i]) + k_len[i]);
+    }
+  std::sort(cuts.begin(), cuts.end());
+  cuts.erase(std::unique(cuts.begin(), cuts.end()), cuts.end());
+  for (size_t c = 0; c + 1 < cuts.size(); ++c) {
+    const int range0 = static_cast<int>(plan.ranges.size());
+    int n = 0;
+    long long tiles = 0;
+    for (int i = 0; i < n_seg; ++i)
+      if (q_len[i] > 0 && k_len[i] > 0 && k_start[i] <= cuts[c] &&
+          static_cast<long long>(k_start[i]) + k_len[i] >= cuts[c + 1]) {
+        plan.ranges.push_back({q_start[i], q_len[i]});
+        tiles += (q_len[i] + 127) / 128;
+        ++n;
+      }
+    if (tiles > 0x7fffffffLL || plan.ranges.size() > 0x7ffffff0u) return ORL_ERR_CAPACITY;
+    cut(cuts[c], cuts[c + 1], kDkv, range0, n, static_cast<int>(tiles));
+  }
+  // longest first; a dkv tile has four products and a dq tile three. Blocks of one head and segment stay adjacent.
+  auto cost = [](const Block& b) { return static_cast<long long>(b.n_tiles) * (b.kind == kDkv ? 4 : 3); };
+  std::vector<int> order(blocks.size());
+  for (size_t i = 0; i < order.size(); ++i) order[i] = static_cast<int>(i);
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return cost(blocks[a]) > cost(blocks[b]); });
+  if (static_cast<long long>(blocks.size()) * heads > 0x3fffffffLL) return ORL_ERR_CAPACITY;
+  plan.items.reserve(blocks.size() * heads);
+  for (size_t lo = 0; lo < order.size();) {
+    // blocks of the same kind and ranges: head by head, so that concurrent CTAs share the streamed tiles in L2
+    size_t hi = lo + 1;
+    auto same = [&](const Block& a, const Block& b) {
+      return a.kind == b.kind && a.range0 == b.range0 && a.n_ranges == b.n_ranges;
+    };
+    while (hi < order.size() && same(blocks[order[lo]], blocks[order[hi]])) ++hi;
+    for (int h = 0; h < heads; ++h)
+      for (size_t x = lo; x < hi; ++x) {
+        const Block& b = blocks[order[x]];
+        plan.items.push_back({b.row0, b.rows, h, b.kind, b.range0, b.n_ranges, b.n_tiles, 0});
+      }
+    lo = hi;
+  }
+  return ORL_OK;
+}
+
+}  // namespace orl
+
+using namespace orl;
+
+extern "C" int orl_attn_bwd_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start,
+                                 const int32_t* k_len, int n_seg, int heads, long long nq, long long nk,
+                                 orl_attn_bwd_work* work, int work_capacity, int32_t* ranges, int ranges_capacity,
+                                 int* n_ranges) {
+  if (n_seg < 0 || heads <= 0 || nq < 0 || nk < 0 || nq > 0x7fffffffLL || nk > 0x7fffffffLL || n_ranges == nullptr)
+    return ORL_ERR_ARG;
+  if (n_seg > 0 && (q_start == nullptr || q_len == nullptr || k_start == nullptr || k_len == nullptr))
+    return ORL_ERR_ARG;
+  try {
+    BwdPlan plan;
+    const int rc = plan_bwd(q_start, q_len, k_start, k_len, n_seg, heads, nq, nk, plan);
+    if (rc != ORL_OK) return rc;
+    const int n = static_cast<int>(plan.items.size());
+    *n_ranges = static_cast<int>(plan.ranges.size());
+    if (n == 0) return 0;
+    if (work == nullptr || work_capacity < n || (ranges == nullptr && *n_ranges > 0) || ranges_capacity < *n_ranges)
+      return -n - 1000;                                   // caller sizes the buffers
+    std::copy(plan.items.begin(), plan.items.end(), work);
+    for (int i = 0; i < *n_ranges; ++i) {
+      ranges[2 * i] = plan.ranges[i].x;
+      ranges[2 * i + 1] = plan.ranges[i].y;
+    }
+    return n;
+  } catch (const std::bad_alloc&) {
+    return ORL_ERR_CAPACITY;
+  }
+}
+
+extern "C" int orl_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                            const float* lse, const float* dlse, void* dq, void* dk, void* dv, long long nq,
+                            long long nk, int heads, int head_dim, float scale, const orl_attn_bwd_work* work_dev,
+                            int n_items, const int32_t* ranges_dev, float* stats_dev, int* err_dev,
+                            void* stream_ptr) {
+  const int rc = check_bwd(q, k, v, out, dout, lse, dq, dk, dv, nq, nk, heads, head_dim, scale, stats_dev, err_dev);
+  if (rc != ORL_OK) return rc;
+  if (n_items < 0 || (n_items > 0 && work_dev == nullptr)) return ORL_ERR_ARG;
+  if (n_items == 0) return ORL_OK;
+  auto launch = head_dim == 64 ? launch_attn_bwd<64> : launch_attn_bwd<128>;
+  return launch(q, k, v, out, dout, lse, dlse, dq, dk, dv, nq, nk, heads, scale, work_dev, n_items,
+                reinterpret_cast<const int2*>(ranges_dev), reinterpret_cast<float2*>(stats_dev), err_dev,
+                static_cast<cudaStream_t>(stream_ptr), nullptr);
+}
+
+// ------------------------------------------------------------------------------------------------ device plan
+// orl_attn_bwd_cu: cu_seqlens on the device, the work list planned there (one block). Keys of different segments do
+// not overlap, so a segment's key rows have one query range and its query rows one key range: ranges[i] = segment
+// i's query range, ranges[n_seg + i] its key range. Rows before the first and after the last segment get zeros.
+// Scratch: a 32-byte header (slot 0: item count), the items, then the ranges.
+namespace orl {
+
+constexpr int kBwdPlanMaxSeg = 4096;
+
+__global__ void __launch_bounds__(1024)
+    attn_bwd_plan_kernel(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, int n_seg, int heads,
+                         long long nq, long long nk, BwdWork* __restrict__ work, int2* __restrict__ ranges,
+                         long long capacity, int* __restrict__ err) {
+  // groups: n_seg dkv, n_seg dq, then the rows outside the segments (dkv before / after, dq before / after)
+  extern __shared__ int plan_smem[];
+  const int n_grp = 2 * n_seg + 4;
+  int* s_row = plan_smem;                   // [n_grp] first row
+  int* s_len = s_row + n_grp;               // [n_grp] rows
+  int* s_tiles = s_len + n_grp;             // [n_grp] streamed tiles
+  int* s_grp = s_tiles + n_grp;             // [n_grp] group at each rank
+  int* s_end = s_grp + n_grp;               // [n_grp] end of each rank's items
+  __shared__ int bad, total, n_ranked;
+  const int t = threadIdx.x;
+  if (t == 0) bad = total = n_ranked = 0;
+  __syncthreads();
+  for (int i = t; i < n_seg; i += blockDim.x) {
+    const long long q0 = cu_q[i], q1 = cu_q[i + 1], k0 = cu_k[i], k1 = cu_k[i + 1];
+    if (q0 < 0 || q1 < q0 || q1 > nq || k0 < 0 || k1 < k0 || k1 > nk) bad = 1;
+    const int lq = static_cast<int>(q1 - q0), lk = static_cast<int>(k1 - k0);
+    s_row[i] = static_cast<int>(k0);
+    s_len[i] = lk;
+    s_tiles[i] = (lq + 127) >> 7;
+    s_row[n_seg + i] = static_cast<int>(q0);
+    s_len[n_seg + i] = lq;
+    s_tiles[n_seg + i] = (lk + 127) >> 7;
+    ranges[i] = make_int2(static_cast<int>(q0), lq);
+    ranges[n_seg + i] = make_int2(static_cast<int>(k0), lk);
+  }
+  if (t < 4) {
+    const int32_t* cu = t < 2 ? cu_k : cu_q;
+    const long long n = t < 2 ? nk : nq;
+    const int first = cu[0], last = cu[n_seg];
+    if (first < 0 || first > n || last < 0 || last > n) bad = 1;
+    const int lo = (t & 1) ? last : 0;
+    s_row[2 * n_seg + t] = lo;
+    s_len[2 * n_seg + t] = (t & 1) ? static_cast<int>(n - lo) : first;
+    s_tiles[2 * n_seg + t] = 0;
+  }
+  __syncthreads();
+  if (bad) {
+    if (t == 0) {
+      work[0].row0 = 0;
+      atomicOr(err, kErrPlan);
+    }
+    return;
+  }
+  auto is_dkv = [&](int g) { return g < n_seg || (g >= 2 * n_seg && g < 2 * n_seg + 2); };
+  auto cost = [&](int g) { return static_cast<long long>(s_tiles[g]) * (is_dkv(g) ? 4 : 3); };
+  auto items = [&](int g) { return heads * ((s_len[g] + 127) >> 7); };
+  for (int g = t; g < n_grp; g += blockDim.x) {
+    if (s_len[g] == 0) continue;
+    const long long cg = cost(g);
+    int rank = 0, before = 0;
+    for (int x = 0; x < n_grp; ++x) {
+      if (s_len[x] == 0) continue;
+      const long long cx = cost(x);
+      if (cx > cg || (cx == cg && x < g)) {
+        ++rank;
+        before += items(x);
+      }
+    }
+    s_grp[rank] = g;
+    s_end[rank] = before + items(g);
+    atomicAdd(&n_ranked, 1);
+    atomicAdd(&total, items(g));
+  }
+  __syncthreads();
+  const int n = total, m = n_ranked;
+  if (static_cast<long long>(n) + 1 > capacity) {
+    if (t == 0) {
+      work[0].row0 = 0;
+      atomicOr(err, kErrPlan);
+    }
+    return;
+  }
+  for (int it = t; it < n; it += blockDim.x) {
+    int lo = 0, hi = m - 1;                 // first rank whose items end after it
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_end[mid] > it) hi = mid; else lo = mid + 1;
+    }
+    const int g = s_grp[lo];
+    const int chunks = (s_len[g] + 127) >> 7;
+    const int r = it - (lo > 0 ? s_end[lo - 1] : 0);
+    const int h = r / chunks, c = r - h * chunks;
+    BwdWork w;
+    w.row0 = s_row[g] + 128 * c;
+    w.rows = min(128, s_len[g] - 128 * c);
+    w.head = h;
+    w.kind = is_dkv(g) ? kDkv : kDq;
+    w.range0 = g < 2 * n_seg ? g : 0;
+    w.n_ranges = s_tiles[g] > 0 ? 1 : 0;
+    w.n_tiles = s_tiles[g];
+    w.pad = 0;
+    work[1 + it] = w;
+  }
+  if (t == 0) work[0].row0 = n;
+}
+
+}  // namespace orl
+
+extern "C" long long orl_attn_bwd_cu_scratch(long long nq, long long nk, int n_seg, int heads) {
+  if (nq < 0 || nk < 0 || n_seg < 0 || heads <= 0) return ORL_ERR_ARG;
+  // every group of rows may end in a short block: n_seg + 2 groups on each side
+  const long long items = heads * ((nq + 127) / 128 + (nk + 127) / 128 + 2ll * (n_seg + 2));
+  return 32 * (1 + items) + 16ll * n_seg;
+}
+
+extern "C" int orl_attn_bwd_cu(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                               const float* lse, const float* dlse, void* dq, void* dk, void* dv, long long nq,
+                               long long nk, int heads, int head_dim, float scale, const int32_t* cu_q_dev,
+                               const int32_t* cu_k_dev, int n_seg, void* scratch_dev, long long scratch_bytes,
+                               float* stats_dev, int* err_dev, void* stream_ptr) {
+  const int rc = check_bwd(q, k, v, out, dout, lse, dq, dk, dv, nq, nk, heads, head_dim, scale, stats_dev, err_dev);
+  if (rc != ORL_OK) return rc;
+  if (n_seg < 0 || cu_q_dev == nullptr || cu_k_dev == nullptr || scratch_dev == nullptr) return ORL_ERR_ARG;
+  if (!bwd_aligned(scratch_dev)) return ORL_ERR_ALIGN;
+  if (n_seg > kBwdPlanMaxSeg) return ORL_ERR_CAPACITY;
+  const long long need = orl_attn_bwd_cu_scratch(nq, nk, n_seg, heads);
+  if (scratch_bytes < need) return ORL_ERR_CAPACITY;
+  const long long items = (need - 32 - 16ll * n_seg) / 32;
+  if (items > 0x3fffffffLL) return ORL_ERR_CAPACITY;
+  if (nq == 0 && nk == 0) return ORL_OK;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  const int smem = 20 * (2 * n_seg + 4);
+  static std::mutex mu;
+  static bool attr_set[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return ORL_ERR_LAUNCH;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!attr_set[dev]) {
+      if (cudaFuncSetAttribute(attn_bwd_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               20 * (2 * kBwdPlanMaxSeg + 4)) != cudaSuccess)
+        return ORL_ERR_LAUNCH;
+      attr_set[dev] = true;
+    }
+  }
+  BwdWork* work = static_cast<BwdWork*>(scratch_dev);
+  int2* ranges = reinterpret_cast<int2*>(work + 1 + items);
+  attn_bwd_plan_kernel<<<1, 1024, smem, stream>>>(cu_q_dev, cu_k_dev, n_seg, heads, nq, nk, work, ranges, 1 + items,
+                                                  err_dev);
+  if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
+  auto launch = head_dim == 64 ? launch_attn_bwd<64> : launch_attn_bwd<128>;
+  return launch(q, k, v, out, dout, lse, dlse, dq, dk, dv, nq, nk, heads, scale, work + 1, static_cast<int>(items),
+                ranges, reinterpret_cast<float2*>(stats_dev), err_dev, stream, reinterpret_cast<const int*>(work));
+}

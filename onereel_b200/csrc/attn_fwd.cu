@@ -28,6 +28,7 @@
 
 #include "orl_common.h"
 #include "ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace orl {
 
@@ -60,7 +61,6 @@ struct AttnCfg {
 };
 
 constexpr int kThreads = 384;
-constexpr int kMaxDevices = 64;
 // register split: the launch has 384 threads x 168 registers; warpgroup 0 (producer, MMA issuer, two idle warps)
 // keeps kRegsLow, the two softmax warpgroups get kRegsHigh (4 x 32 x kRegsLow + 8 x 32 x kRegsHigh = 384 x 168)
 constexpr int kLaunchRegs = 168, kRegsLow = 120, kRegsHigh = 192;
@@ -477,36 +477,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------------------------------------ host side
 
-// cuTensorMapEncodeTiled (driver API, cuda.h), fetched through the runtime so the library needs no -lcuda.
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
 // 2-D bf16 map over rows x (heads * D) with 128-row x 64-column boxes, 128-byte swizzle, zero fill out of bounds.
 static int make_rows_map(CUtensorMap* map, const void* base, long long rows, int row_elems) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return ORL_ERR_DRIVER;
-  cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_elems), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_elems) * 2};
-  cuuint32_t box[2] = {64, 128};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? ORL_OK : ORL_ERR_TENSOR_MAP;
+  return make_rows_map(map, base, rows, row_elems, row_elems, 128);
 }
 
 template <int D>

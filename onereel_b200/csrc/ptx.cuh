@@ -124,6 +124,10 @@ __device__ __forceinline__ void bulk_wait() {
   asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Orders this thread's earlier ordinary shared-memory writes before later accesses of the asynchronous proxy (TMA,
+// tcgen05.mma operand reads) that an mbarrier arrival after it releases.
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // L2 eviction-priority policies for cache_hint operands.
 __device__ __forceinline__ uint64_t policy_evict_last() {
   uint64_t p;
