@@ -209,6 +209,17 @@ ORL_API int orl_qk_norm_rope(const void* x, void* y, const void* weight, const f
                              long long rows, int heads, int head_dim, int per_head, float eps, int sin_shift,
                              long long rope_ld, const int32_t* row_map, void* stream);
 
+/* Gradients of orl_qk_norm_rope (without a row map): dx [rows, heads * head_dim] bf16 and dweight (bf16, the weight's
+ * size) from the gradient dy of y and the forward's x, weight and tables. Deterministic. scratch: device fp32,
+ * orl_qk_norm_rope_bwd_scratch elements. heads * head_dim at most 8192. */
+ORL_API int orl_qk_norm_rope_bwd(const void* x, const void* dy, const void* weight, const float* cos_t,
+                                 const float* sin_t, void* dx, void* dweight, float* scratch, long long rows,
+                                 int heads, int head_dim, int per_head, float eps, int sin_shift, long long rope_ld,
+                                 void* stream);
+
+/* fp32 elements of scratch orl_qk_norm_rope_bwd needs. */
+ORL_API long long orl_qk_norm_rope_bwd_scratch(long long rows, int heads, int head_dim, int per_head);
+
 /* In-place rotary rotation of listed rows (no norm), for moving shared-frame keys of a packed K to their adjacent
  * temporal positions (hunyuan15.py:127-150 `_move_shared`, which applies R(-src) then R(dst) with two
  * apply_rotary_emb calls): x [*, heads * head_dim] bf16; row rows[i] rotated by table row i of cos_t / sin_t

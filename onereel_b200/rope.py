@@ -5,6 +5,7 @@ into a Triton kernel)."""
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
 
@@ -13,7 +14,8 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
                  eps: float, per_head: bool, sin_shift: int, out: torch.Tensor | None = None,
                  row_map: torch.Tensor | None = None) -> torch.Tensor:
     """x [rows, heads * D] (or [1, rows, heads * D]) bf16 -> [rows, heads, D] bf16, normalised and rotated; cos / sin
-    [rows, D] (any float dtype; converted to fp32 contiguous). out / row_map: write row i to out[row_map[i]]."""
+    [rows, D] (any float dtype; converted to fp32 contiguous). out / row_map: write row i to out[row_map[i]].
+    Differentiable in x and weight (first derivatives; the tables get none) unless out or row_map is given."""
     if x.dim() == 3:
         x = x[0]
     if not (x.is_cuda and x.dtype == torch.bfloat16):
@@ -24,6 +26,13 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
     w = weight.to(device=x.device, dtype=torch.bfloat16).contiguous()
     c = cos.to(device=x.device, dtype=torch.float32).reshape(rows, -1).contiguous()
     s = sin.to(device=x.device, dtype=torch.float32).reshape(rows, -1).contiguous()
+    if (out is None and row_map is None and torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)):
+        return _QkNormRope.apply(x, w, c, s, heads, float(eps), int(per_head), int(sin_shift))
+    return _forward(x, w, c, s, heads, eps, per_head, sin_shift, out, row_map)
+
+
+def _forward(x, w, c, s, heads, eps, per_head, sin_shift, out=None, row_map=None):
+    rows, Dh = x.shape[0], x.shape[1] // heads
     if out is None:
         out = torch.empty(rows, heads, Dh, dtype=torch.bfloat16, device=x.device)
     rm = None if row_map is None else row_map.to(device=x.device, dtype=torch.int32).contiguous()
@@ -32,6 +41,46 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
                                      None if rm is None else rm.data_ptr(),
                                      torch.cuda.current_stream(x.device).cuda_stream), 'orl_qk_norm_rope')
     return out
+
+
+class _QkNormRope(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, w, c, s, heads, eps, per_head, sin_shift):
+        ctx.save_for_backward(x, w, c, s)
+        ctx.args = heads, eps, per_head, sin_shift
+        with torch.cuda.device(x.device):
+            return _forward(x, w, c, s, heads, eps, per_head, sin_shift)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, c, s = ctx.saved_tensors
+        dx, dw = qk_norm_rope_grad(x, w, c, s, dy, *ctx.args)
+        return dx, dw, None, None, None, None, None, None
+
+
+def qk_norm_rope_grad(x, weight, cos, sin, dy, heads: int, eps: float, per_head: bool, sin_shift: int):
+    """(dx, dweight) of qk_norm_rope (orl_qk_norm_rope_bwd): x [rows, heads * D] and weight bf16, cos / sin fp32
+    [rows, D], all contiguous as the forward used them; dy [rows, heads, D] bf16"""
+    rows, hidden = x.shape
+    if dy.dtype != torch.bfloat16 or dy.device != x.device:
+        raise TypeError(f'qk_norm_rope: dy must be bf16 on {x.device}')
+    if dy.shape != (rows, heads, hidden // heads):
+        raise ValueError(f'qk_norm_rope: dy must have shape {(rows, heads, hidden // heads)}, got {tuple(dy.shape)}')
+    dy = dy.contiguous()
+    dy = dy if dy.data_ptr() % 16 == 0 else dy.clone()
+    with torch.cuda.device(x.device):
+        n = L.check(L.lib().orl_qk_norm_rope_bwd_scratch(rows, heads, hidden // heads, int(per_head)),
+                    'orl_qk_norm_rope_bwd_scratch')
+        scratch = torch.empty(n, dtype=torch.float32, device=x.device)
+        dx, dw = torch.empty_like(x), torch.empty_like(weight)
+        L.check(L.lib().orl_qk_norm_rope_bwd(x.data_ptr(), dy.data_ptr(), weight.data_ptr(), cos.data_ptr(),
+                                             sin.data_ptr(), dx.data_ptr(), dw.data_ptr(), scratch.data_ptr(), rows,
+                                             heads, hidden // heads, int(per_head), float(eps), int(sin_shift),
+                                             cos.shape[1], torch.cuda.current_stream(x.device).cuda_stream),
+                'orl_qk_norm_rope_bwd')
+    return dx, dw
 
 
 def rotate_rows(x: torch.Tensor, rows: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, sin_shift: int = 0):
