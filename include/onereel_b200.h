@@ -244,6 +244,39 @@ ORL_API int orl_peer_gather(const void* const* src, void* const* dst, int planes
                             long long seg_bytes, long long src_row0, long long src_stride, long long dst_pstride,
                             long long dst_stride, void* stream);
 
+/* ---------------------------------------------------------------- linear layers with their epilogue
+ * The projections and feed-forward layers around the attention, which the reference runs as separate torch ops:
+ * y = residual + gate * act(x w^T + bias), x [m, k] (row stride ldx), w [n, k] (row stride ldw), bias / gate [n],
+ * residual [m, n] (row stride ldr), y [m, n], all bf16, accumulated and finished in fp32. n, k and the row strides are
+ * multiples of 8 elements, pointers 16-byte aligned; bias, gate, residual may be NULL. */
+
+#define ORL_ACT_NONE 0
+#define ORL_ACT_GELU_TANH 1 /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+#define ORL_ACT_SILU 2      /* z / (1 + exp(-z)) */
+
+/* z (optional, [m, n]): receives x w^T + bias, which the backward pass of an activation or a gate needs. err_dev: as
+ * in orl_attn_fwd. */
+ORL_API int orl_linear(const void* x, long long ldx, const void* w, long long ldw, const void* bias, const void* gate,
+                       const void* residual, long long ldr, void* y, void* z, long long m, long long n, long long k,
+                       int act, int* err_dev, void* stream);
+
+/* dz = gate * dy * act'(z) [m, n] (NULL: not written), dbias = column sums of dz, dgate = column sums of dy * act(z)
+ * (bf16 [n], NULL: not computed). dy has row stride lddy; z may be NULL without activation and gate. Deterministic.
+ * scratch: device fp32, orl_linear_dz_scratch elements, needed for dbias or dgate. */
+ORL_API int orl_linear_dz(const void* dy, long long lddy, const void* z, const void* gate, int act, void* dz,
+                          void* dbias, void* dgate, float* scratch, long long m, long long n, void* stream);
+
+/* fp32 elements of scratch orl_linear_dz needs. */
+ORL_API long long orl_linear_dz_scratch(long long m, long long n);
+
+/* dx [m, k] = dz [m, n] w [n, k] */
+ORL_API int orl_linear_dx(const void* dz, long long lddz, const void* w, long long ldw, void* dx, long long m,
+                          long long n, long long k, int* err_dev, void* stream);
+
+/* dw [n, k] = dz [m, n]^T x [m, k] */
+ORL_API int orl_linear_dw(const void* dz, long long lddz, const void* x, long long ldx, void* dw, long long m,
+                          long long n, long long k, int* err_dev, void* stream);
+
 /* ---------------------------------------------------------------- frame memory (src/onereel/frame_memory.py) */
 
 /* Per-frame pooling of one layer's hidden states (frame_memory.py:76-85 `collect`, an index_add_ of the rows into

@@ -1,0 +1,660 @@
+// Linear layers with their epilogue, bf16 in / fp32 accumulate / bf16 out, for sm_100a:
+//   y = residual + gate * act(x w^T + bias)          x [m, k], w [n, k], bias / gate [n], residual / y [m, n]
+// and their gradients:  dz = gate dy act'(z) (z = x w^T + bias, which the forward keeps), dx = dz w, dw = dz^T x,
+// db = sum dz, dgate = sum dy act(z).
+//
+// gemm_kernel computes C = A B^T over operands whose contraction dimension is contiguous (K-major) or not (MN-major:
+// the tcgen05 descriptors read such tiles transposed), so dx and dw need no transposed copies. Persistent and warp
+// specialised: warp 0 streams 64-deep A and B tiles by TMA into a ring, warp 1 issues the MMAs into one of two TMEM
+// accumulators, warps 4-7 drain the other: bias, activation, gate, residual and the bf16 stores run under the next
+// tile's MMAs. kCtas = 2: a cluster of two CTAs owns a 256 x 256 tile (tcgen05 cta_group::2): each holds half of A's
+// rows and half of B's, so an SM reads 64 bytes of shared memory per clock where a 128 x 256 tile of its own would read
+// 96 and fill as much again. Rows and columns past the ends are zeros (TMA fill) and are not stored.
+// Every mbarrier wait is bounded (ptx.cuh).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <mutex>
+
+#include "column_sum.cuh"
+#include "orl_common.h"
+#include "ptx.cuh"
+#include "tensor_map.cuh"
+
+namespace orl {
+
+// ------------------------------------------------------------------------------------------------ activations
+// With t = 1 / (1 + exp(-a)): silu a = z, gelu_tanh a = 2 sqrt(2 / pi) (z + 0.044715 z^3) (tanh(u) = 2 sigmoid(2u) - 1);
+// act = z t in both.
+constexpr float kLog2eF = 1.4426950408889634f;
+constexpr float kGelu = 1.5957691216057308f;          // 2 sqrt(2 / pi)
+constexpr float kGelu3 = 0.044715f;
+
+__device__ __forceinline__ float sigmoid(float a) { return __fdividef(1.0f, 1.0f + ex2(-a * kLog2eF)); }
+
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == ORL_ACT_GELU_TANH) return z * sigmoid(kGelu * (z + kGelu3 * z * z * z));
+  if (act == ORL_ACT_SILU) return z * sigmoid(z);
+  return z;
+}
+
+// act(z) and act'(z)
+__device__ __forceinline__ float2 activate_slope(float z, int act) {
+  if (act == ORL_ACT_NONE) return make_float2(z, 1.0f);
+  const bool gelu = act == ORL_ACT_GELU_TANH;
+  const float t = sigmoid(gelu ? kGelu * (z + kGelu3 * z * z * z) : z);
+  const float da = gelu ? kGelu * (1.0f + 3.0f * kGelu3 * z * z) : 1.0f;
+  const float s = t * (1.0f - t);                     // 0 far out, where z^2 may be infinite
+  return make_float2(z * t, s == 0.0f ? t : t + z * da * s);
+}
+
+__device__ __forceinline__ void unpack8(uint4 r, float (&f)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+
+// what happens to a product on its way out; null pointers: not there
+struct Epilogue {
+  const __nv_bfloat16* bias;
+  const __nv_bfloat16* gate;
+  const __nv_bfloat16* residual;
+  long long ldr;
+  __nv_bfloat16* y;        // [m, n]
+  __nv_bfloat16* z;        // [m, n]: x w^T + bias, kept for the backward pass
+  int act;
+};
+
+// eight columns n0.. of one row: f = products in, y out
+__device__ __forceinline__ void finish8(const Epilogue& ep, long long row, int n0, int n, float (&f)[8]) {
+  const long long at = row * n + n0;
+  float t[8];
+  if (ep.bias != nullptr) {
+    unpack8(__ldg(reinterpret_cast<const uint4*>(ep.bias + n0)), t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] += t[i];
+  }
+  if (ep.z != nullptr) *reinterpret_cast<uint4*>(ep.z + at) = pack8(f);
+  if (ep.act != ORL_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = activate(f[i], ep.act);
+  }
+  if (ep.gate != nullptr) {
+    unpack8(__ldg(reinterpret_cast<const uint4*>(ep.gate + n0)), t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= t[i];
+  }
+  if (ep.residual != nullptr) {
+    unpack8(*reinterpret_cast<const uint4*>(ep.residual + row * ep.ldr + n0), t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] += t[i];
+  }
+  *reinterpret_cast<uint4*>(ep.y + at) = pack8(f);
+}
+
+// ------------------------------------------------------------------------------------------------ matrix product
+
+constexpr int kGemmThreads = 256;
+constexpr int kBk = 64;                                // contraction depth of a stage: one 128-byte swizzle row
+
+template <int kCtas, int BN>
+struct GemmCfg {
+  static constexpr int kTileM = 128 * kCtas;           // rows of C per cluster
+  static constexpr int kBRows = BN / kCtas;            // columns of C whose B each CTA holds
+  static constexpr int kABytes = 128 * kBk * 2;
+  static constexpr int kBBytes = kBRows * kBk * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = (196 * 1024) / kStageBytes;
+  static constexpr int kBarOff = kStages * kStageBytes;
+  static constexpr int kBarFull = 0;
+  static constexpr int kBarEmpty = kStages;
+  static constexpr int kBarAccFull = 2 * kStages;      // + accumulator
+  static constexpr int kBarAccEmpty = kBarAccFull + 2;
+  static constexpr int kBarDrain = kBarAccEmpty + 2;
+  static constexpr int kNumBars = kBarDrain + 1;
+  static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
+  static constexpr uint32_t kTmemCols = 2 * BN;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+  static_assert(kTmemCols == 128 || kTmemCols == 256 || kTmemCols == 512, "TMEM allocation size");
+};
+
+struct GemmShape {
+  int m, n, k;             // C [m, n], contraction k
+  int tiles_m, tiles_n;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// arrive on the barrier at the same shared-memory offset in CTA 0 of the cluster
+__device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, 0;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar)
+      : "memory");
+}
+// 2-D tiled load (no multicast) into this CTA whose bytes complete on the barrier of the pair's CTA 0 (the address
+// with the CTA's bit cleared)
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y,
+                                                 uint64_t cache_hint) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar & 0xFEFFFFFFu), "r"(x), "r"(y), "l"(cache_hint)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrive on the barrier at this offset in both CTAs of the pair once the MMAs issued before have completed
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+struct GemmShared {
+  uint32_t sbase, bar0;
+  volatile int* abort_flag;
+  __device__ uint32_t bar(int i) const { return bar0 + 8u * i; }
+};
+
+// tile -> (tile row, tile column): groups of eight tile rows, columns outermost in a group, so that the tiles in flight
+// share A and B tiles in L2
+__device__ __forceinline__ int2 tile_at(const GemmShape& g, int t) {
+  constexpr int kGroup = 8;
+  const int per = kGroup * g.tiles_n;
+  const int first = (t / per) * kGroup;
+  const int rows = min(kGroup, g.tiles_m - first);
+  const int r = t % per;
+  return make_int2(first + r % rows, r / rows);
+}
+
+template <int kCtas, int BN, bool kAmn, bool kBmn>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                const __grid_constant__ GemmShape g, const __grid_constant__ Epilogue ep, int* __restrict__ err) {
+  using C = GemmCfg<kCtas, BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOff + C::kNumBars * 8);
+  GemmShared sh;
+  sh.sbase = smem_u32(smem);
+  sh.bar0 = sh.sbase + C::kBarOff;
+  sh.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kCtas == 2 ? static_cast<int>(cluster_rank()) : 0;
+  const int cluster = blockIdx.x / kCtas, n_clusters = gridDim.x / kCtas;
+  const int n_tiles = g.tiles_m * g.tiles_n;
+  const int n_k = (g.k + kBk - 1) / kBk;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(sh.bar(C::kBarFull + s), 1);
+      mbar_init(sh.bar(C::kBarEmpty + s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sh.bar(C::kBarAccFull + i), 1);
+      mbar_init(sh.bar(C::kBarAccEmpty + i), 4 * kCtas);
+    }
+    mbar_init(sh.bar(C::kBarDrain), 1);
+    *sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    if (kCtas == 2) {
+      tmem_alloc_pair(smem_u32(tmem_slot), C::kTmemCols);
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (kCtas == 2) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      tma_prefetch_map(&tm_a);
+      tma_prefetch_map(&tm_b);
+      const uint64_t pol = policy_evict_last();
+      auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+        if (kCtas == 2) tma_load_2d_pair(dst, map, bar, x, y, pol);
+        else tma_load_2d(dst, map, bar, x, y, pol);
+      };
+      int it = 0;
+      bool ok = true;
+      for (int t = cluster; ok && t < n_tiles; t += n_clusters) {
+        const int2 at = tile_at(g, t);
+        const int m0 = at.x * C::kTileM + 128 * rank, n0 = at.y * BN + C::kBRows * rank;
+        for (int kb = 0; kb < n_k; ++kb, ++it) {
+          const int s = it % C::kStages;
+          if (it >= C::kStages && !mbar_wait(sh.bar(C::kBarEmpty + s), ((it / C::kStages) - 1) & 1, sh.abort_flag)) {
+            atomicOr(err, kErrTimeoutLoad);
+            ok = false;
+            break;
+          }
+          const uint32_t a = sh.sbase + s * C::kStageBytes, b = a + C::kABytes, bar = sh.bar(C::kBarFull + s);
+          if (rank == 0) mbar_expect_tx(bar, kCtas * C::kStageBytes);
+          const int k0 = kb * kBk;
+          if (kAmn) {
+            for (int c = 0; c < 2; ++c) load(a + c * 8192, &tm_a, bar, m0 + 64 * c, k0);
+          } else {
+            load(a, &tm_a, bar, k0, m0);
+          }
+          if (kBmn) {
+            for (int c = 0; c < C::kBRows / 64; ++c) load(b + c * 8192, &tm_b, bar, n0 + 64 * c, k0);
+          } else {
+            load(b, &tm_b, bar, k0, n0);
+          }
+        }
+      }
+      if (*sh.abort_flag && rank == 0) {
+        // wind down: the copies in flight (both CTAs' complete on CTA 0's barriers) land before shared memory goes
+        for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i) {
+          const unsigned long long t0 = global_ns();
+          while (!mbar_try_wait(sh.bar(C::kBarFull + i % C::kStages), (i / C::kStages) & 1))
+            if (global_ns() - t0 > kWaitLimitNs) {
+              atomicOr(err, kErrTimeoutDrain);
+              break;
+            }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (CTA 0 of a pair)
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t kIdesc = idesc_bf16(C::kTileM, BN, kAmn, kBmn);
+      auto commit = [&](uint32_t bar) {
+        if (kCtas == 2) mma_commit_pair(bar);
+        else mma_commit(bar);
+      };
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int t = cluster; ok && t < n_tiles; t += n_clusters, ++n) {
+        const int buf = n & 1;
+        if (n >= 2) ok = mbar_wait(sh.bar(C::kBarAccEmpty + buf), ((n >> 1) - 1) & 1, sh.abort_flag);
+        tc_fence_after();
+        const uint32_t d = tmem + buf * BN;
+        for (int kb = 0; ok && kb < n_k; ++kb, ++it) {
+          const int s = it % C::kStages;
+          ok = mbar_wait(sh.bar(C::kBarFull + s), (it / C::kStages) & 1, sh.abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a = sh.sbase + s * C::kStageBytes, b = a + C::kABytes;
+#pragma unroll
+          for (int kk = 0; kk < kBk / 16; ++kk) {
+            // K-major: 16 columns on; MN-major: 16 rows of 128 bytes on, 64-column blocks 8 KiB apart
+            const uint64_t da = kAmn ? smem_desc_sw128(a + kk * 2048, 8192, 1024) : smem_desc_sw128(a + kk * 32, 16, 1024);
+            const uint64_t db = kBmn ? smem_desc_sw128(b + kk * 2048, 8192, 1024) : smem_desc_sw128(b + kk * 32, 16, 1024);
+            if (kCtas == 2) mma_ss_pair(d, da, db, kIdesc, (kb | kk) ? 1u : 0u);
+            else mma_ss(d, da, db, kIdesc, (kb | kk) ? 1u : 0u);
+          }
+          commit(sh.bar(C::kBarEmpty + s));
+        }
+        if (ok) commit(sh.bar(C::kBarAccFull + buf));
+      }
+      if (!ok) {
+        atomicOr(err, kErrTimeoutMma);
+        commit(sh.bar(C::kBarDrain));
+        const unsigned long long t0 = global_ns();
+        while (!mbar_try_wait(sh.bar(C::kBarDrain), 0))
+          if (global_ns() - t0 > kWaitLimitNs) {
+            atomicOr(err, kErrTimeoutDrain);
+            break;
+          }
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue: one row per thread
+    int n = 0;
+    for (int t = cluster; t < n_tiles; t += n_clusters, ++n) {
+      const int buf = n & 1;
+      const int2 at = tile_at(g, t);
+      const long long row = static_cast<long long>(at.x) * C::kTileM + 128 * rank + 32 * (warp - 4) + lane;
+      const int n0 = at.y * BN;
+      if (!mbar_wait(sh.bar(C::kBarAccFull + buf), (n >> 1) & 1, sh.abort_flag)) {
+        atomicOr(err, kErrTimeoutSoftmax);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * BN + (static_cast<uint32_t>(32 * (warp - 4)) << 16);
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        if (n0 + c >= g.n) break;
+        uint32_t v[32];
+        tmem_ld32(acc + c, v);
+        tmem_wait_ld();
+        if (row < g.m) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (n0 + c + 8 * i < g.n) {
+              float f[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[8 * i + e]);
+              finish8(ep, row, n0 + c + 8 * i, g.n, f);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (kCtas == 2) mbar_arrive_leader(sh.bar(C::kBarAccEmpty + buf));
+        else mbar_arrive(sh.bar(C::kBarAccEmpty + buf));
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (kCtas == 2) cluster_sync();           // the peer may still arrive on, or read, this CTA's shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    if (kCtas == 2) tmem_dealloc_pair(tmem, C::kTmemCols);
+    else tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// m <= kRowsMax rows: the weight is read once and little else happens, so tensor-core tiles would leave most SMs idle
+// (n / 64 CTAs). One warp per output column pair streams their weight rows with 16-byte loads; x is in shared memory.
+constexpr int kRowsMax = 4;
+constexpr int kRowsWarps = 8;
+
+template <int M>
+__global__ void __launch_bounds__(32 * kRowsWarps) linear_rows_kernel(const __nv_bfloat16* __restrict__ x,
+                                                                      long long ldx,
+                                                                      const __nv_bfloat16* __restrict__ w,
+                                                                      long long ldw, int n, int k, Epilogue ep) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = 8 * (blockIdx.x * kRowsWarps + warp);
+  if (n0 >= n) return;                                  // n is a multiple of 8
+  float acc[M][8];
+#pragma unroll
+  for (int r = 0; r < M; ++r)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[r][c] = 0.f;
+  for (int e = 8 * lane; e < k; e += 256) {
+    uint4 wr[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) wr[c] = __ldcs(reinterpret_cast<const uint4*>(w + (n0 + c) * ldw + e));
+    float xf[M][8];
+#pragma unroll
+    for (int r = 0; r < M; ++r) unpack8(__ldg(reinterpret_cast<const uint4*>(x + r * ldx + e)), xf[r]);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      float wf[8];
+      unpack8(wr[c], wf);
+#pragma unroll
+      for (int r = 0; r < M; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[r][c] = fmaf(xf[r][i], wf[i], acc[r][c]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < M; ++r)
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[r][c] += __shfl_xor_sync(0xffffffffu, acc[r][c], o);
+#pragma unroll
+  for (int r = 0; r < M; ++r)
+    if (lane == r) finish8(ep, r, n0, n, acc[r]);
+}
+
+// ------------------------------------------------------------------------------------------------ dz and column sums
+// dz = gate * dy * act'(z), with the column sums of dz (bias) and of dy * act(z) (gate). Memory bound. A block covers
+// 256 columns (8 per thread, 32 threads across) and a strip of rows (8 at a time); its sums are one partial row.
+constexpr int kDzBlocks = 1184;                          // at most, over rows and columns: 8 per SM
+
+__global__ void __launch_bounds__(256) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, long long lddy,
+                                                        const __nv_bfloat16* __restrict__ z,
+                                                        const __nv_bfloat16* __restrict__ gate, int act, int m, int n,
+                                                        __nv_bfloat16* __restrict__ dz, float* __restrict__ part_b,
+                                                        float* __restrict__ part_g) {
+  __shared__ float red[8][257];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int col = 256 * blockIdx.x + 8 * tx;
+  const bool on = col < n;
+  float sb[8], sg[8], gf[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    sb[i] = sg[i] = 0.f;
+    gf[i] = 1.f;
+  }
+  if (on && gate != nullptr) unpack8(__ldg(reinterpret_cast<const uint4*>(gate + col)), gf);
+  if (on) {
+    for (int r = 8 * blockIdx.y + ty; r < m; r += 8 * gridDim.y) {
+      const long long at = static_cast<long long>(r) * n + col;
+      float d[8], h[8];
+      unpack8(*reinterpret_cast<const uint4*>(dy + r * lddy + col), d);
+      if (z != nullptr) {
+        unpack8(*reinterpret_cast<const uint4*>(z + at), h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 a = activate_slope(h[i], act);
+          sg[i] += d[i] * a.x;
+          d[i] *= gf[i] * a.y;
+        }
+      }
+      if (dz != nullptr) *reinterpret_cast<uint4*>(dz + at) = pack8(d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sb[i] += d[i];
+    }
+  }
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    float* part = which == 0 ? part_b : part_g;
+    if (part == nullptr) continue;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[ty][8 * tx + i] = which == 0 ? sb[i] : sg[i];
+    __syncthreads();
+    const int c = threadIdx.x;
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a += red[i][c];
+    if (256 * blockIdx.x + c < n) part[static_cast<long long>(blockIdx.y) * n + 256 * blockIdx.x + c] = a;
+  }
+}
+
+static int dz_strips(int m, int n) {
+  const int cols = (n + 255) / 256;
+  return std::max(1, std::min((m + 7) / 8, kDzBlocks / cols));
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+
+template <int kCtas, int BN, bool kAmn, bool kBmn>
+static int launch_gemm(const void* a, long long lda, const void* b, long long ldb, GemmShape g, const Epilogue& ep,
+                       int* err, cudaStream_t stream) {
+  using C = GemmCfg<kCtas, BN>;
+  g.tiles_m = (g.m + C::kTileM - 1) / C::kTileM;
+  g.tiles_n = (g.n + BN - 1) / BN;
+  if (static_cast<long long>(g.tiles_m) * g.tiles_n > 0x7fffffffLL) return ORL_ERR_ARG;
+  CUtensorMap ma, mb;
+  int rc;
+  rc = kAmn ? make_rows_map(&ma, a, g.k, g.m, lda, kBk) : make_rows_map(&ma, a, g.m, g.k, lda, 128);
+  if (rc != ORL_OK) return rc;
+  rc = kBmn ? make_rows_map(&mb, b, g.k, g.n, ldb, kBk) : make_rows_map(&mb, b, g.n, g.k, ldb, C::kBRows);
+  if (rc != ORL_OK) return rc;
+  auto kernel = gemm_kernel<kCtas, BN, kAmn, kBmn>;
+  static std::mutex mu;
+  static int clusters[kMaxDevices] = {};                 // clusters resident at once
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return ORL_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCtas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int most;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (clusters[dev] == 0) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) != cudaSuccess)
+        return ORL_ERR_LAUNCH;
+      cfg.gridDim = dim3(kCtas);
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) return ORL_ERR_LAUNCH;
+      clusters[dev] = n;
+    }
+    most = clusters[dev];
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::min(most, g.tiles_m * g.tiles_n)));
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, g, ep, err) == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
+}
+
+// Tile choice: the pair's 256 x 256 tile reads the least shared memory per MMA, but needs enough tiles to occupy the 74
+// pairs; below that, 128 x 64 tiles spread the work (and the streaming of the weight) over more SMs.
+template <bool kAmn, bool kBmn>
+static int gemm(const void* a, long long lda, const void* b, long long ldb, int m, int n, int k, const Epilogue& ep,
+                int* err, cudaStream_t stream) {
+  GemmShape g{m, n, k, 0, 0};
+  const long long big = (static_cast<long long>(m) + 255) / 256 * ((n + 255) / 256);
+  if (big >= 64) return launch_gemm<2, 256, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
+  return launch_gemm<1, 64, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
+}
+
+static bool lin_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+static int check_linear(long long m, long long n, long long k) {
+  if (m < 0 || n <= 0 || k <= 0 || m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return ORL_ERR_ARG;
+  if ((n & 7) || (k & 7)) return ORL_ERR_ALIGN;
+  return ORL_OK;
+}
+
+}  // namespace orl
+
+using namespace orl;
+
+extern "C" int orl_linear(const void* x, long long ldx, const void* w, long long ldw, const void* bias,
+                          const void* gate, const void* residual, long long ldr, void* y, void* z, long long m,
+                          long long n, long long k, int act, int* err_dev, void* stream_ptr) {
+  int rc = check_linear(m, n, k);
+  if (rc != ORL_OK) return rc;
+  if (act < ORL_ACT_NONE || act > ORL_ACT_SILU || w == nullptr || err_dev == nullptr) return ORL_ERR_ARG;
+  if (m > 0 && (x == nullptr || y == nullptr)) return ORL_ERR_ARG;
+  if (ldx < k || ldw < k || (residual != nullptr && ldr < n)) return ORL_ERR_ARG;
+  if ((ldx & 7) || (ldw & 7) || (residual != nullptr && (ldr & 7))) return ORL_ERR_ALIGN;
+  for (const void* p : {x, w, bias, gate, residual, static_cast<const void*>(y), static_cast<const void*>(z)})
+    if (!lin_aligned(p)) return ORL_ERR_ALIGN;
+  if (m == 0) return ORL_OK;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  auto bf = [](const void* p) { return static_cast<const __nv_bfloat16*>(p); };
+  const Epilogue ep{bf(bias), bf(gate), bf(residual), ldr, static_cast<__nv_bfloat16*>(y),
+                    static_cast<__nv_bfloat16*>(z), act};
+  if (m <= kRowsMax) {
+    const unsigned grid = static_cast<unsigned>((n / 8 + kRowsWarps - 1) / kRowsWarps);
+    const int nn = static_cast<int>(n), kk = static_cast<int>(k);
+    switch (m) {
+      case 1: linear_rows_kernel<1><<<grid, 32 * kRowsWarps, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
+      case 2: linear_rows_kernel<2><<<grid, 32 * kRowsWarps, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
+      case 3: linear_rows_kernel<3><<<grid, 32 * kRowsWarps, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
+      default: linear_rows_kernel<4><<<grid, 32 * kRowsWarps, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep);
+    }
+    return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
+  }
+  return gemm<false, false>(x, ldx, w, ldw, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k), ep, err_dev,
+                            stream);
+}
+
+extern "C" long long orl_linear_dz_scratch(long long m, long long n) {
+  if (check_linear(m, n, 8) != ORL_OK) return ORL_ERR_ARG;
+  return 2ll * dz_strips(static_cast<int>(m), static_cast<int>(n)) * n;
+}
+
+extern "C" int orl_linear_dz(const void* dy, long long lddy, const void* z, const void* gate, int act, void* dz,
+                             void* dbias, void* dgate, float* scratch, long long m, long long n, void* stream_ptr) {
+  int rc = check_linear(m, n, 8);
+  if (rc != ORL_OK) return rc;
+  if (act < ORL_ACT_NONE || act > ORL_ACT_SILU || (m > 0 && dy == nullptr) || lddy < n) return ORL_ERR_ARG;
+  if ((act != ORL_ACT_NONE || gate != nullptr || dgate != nullptr) && z == nullptr && m > 0) return ORL_ERR_ARG;
+  if ((dbias != nullptr || dgate != nullptr) && scratch == nullptr) return ORL_ERR_ARG;
+  if (lddy & 7) return ORL_ERR_ALIGN;
+  for (const void* p : {dy, z, gate, static_cast<const void*>(dz)})
+    if (!lin_aligned(p)) return ORL_ERR_ALIGN;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  const int strips = dz_strips(static_cast<int>(m), static_cast<int>(n));
+  float* part_b = dbias != nullptr ? scratch : nullptr;
+  float* part_g = dgate != nullptr ? scratch + static_cast<long long>(strips) * n : nullptr;
+  const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(strips));
+  linear_dz_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(dy), lddy,
+                                             static_cast<const __nv_bfloat16*>(z),
+                                             static_cast<const __nv_bfloat16*>(gate), act, static_cast<int>(m),
+                                             static_cast<int>(n), static_cast<__nv_bfloat16*>(dz), part_b, part_g);
+  if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
+  if (part_b != nullptr && (rc = column_sum(part_b, strips, static_cast<int>(n), n, dbias, stream)) != ORL_OK) return rc;
+  if (part_g != nullptr) return column_sum(part_g, strips, static_cast<int>(n), n, dgate, stream);
+  return ORL_OK;
+}
+
+extern "C" int orl_linear_dx(const void* dz, long long lddz, const void* w, long long ldw, void* dx, long long m,
+                             long long n, long long k, int* err_dev, void* stream_ptr) {
+  const int rc = check_linear(m, n, k);
+  if (rc != ORL_OK) return rc;
+  if (w == nullptr || err_dev == nullptr || lddz < n || ldw < k || (m > 0 && (dz == nullptr || dx == nullptr)))
+    return ORL_ERR_ARG;
+  if ((lddz & 7) || (ldw & 7) || !lin_aligned(dz) || !lin_aligned(w) || !lin_aligned(dx)) return ORL_ERR_ALIGN;
+  if (m == 0) return ORL_OK;
+  const Epilogue ep{nullptr, nullptr, nullptr, 0, static_cast<__nv_bfloat16*>(dx), nullptr, ORL_ACT_NONE};
+  return gemm<false, true>(dz, lddz, w, ldw, static_cast<int>(m), static_cast<int>(k), static_cast<int>(n), ep, err_dev,
+                           static_cast<cudaStream_t>(stream_ptr));
+}
+
+extern "C" int orl_linear_dw(const void* dz, long long lddz, const void* x, long long ldx, void* dw, long long m,
+                             long long n, long long k, int* err_dev, void* stream_ptr) {
+  const int rc = check_linear(m, n, k);
+  if (rc != ORL_OK) return rc;
+  if (dw == nullptr || err_dev == nullptr || lddz < n || ldx < k || (m > 0 && (dz == nullptr || x == nullptr)))
+    return ORL_ERR_ARG;
+  if ((lddz & 7) || (ldx & 7) || !lin_aligned(dz) || !lin_aligned(x) || !lin_aligned(dw)) return ORL_ERR_ALIGN;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (m == 0)
+    return cudaMemsetAsync(dw, 0, 2 * static_cast<size_t>(n) * k, stream) == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
+  const Epilogue ep{nullptr, nullptr, nullptr, 0, static_cast<__nv_bfloat16*>(dw), nullptr, ORL_ACT_NONE};
+  return gemm<true, true>(dz, lddz, x, ldx, static_cast<int>(n), static_cast<int>(k), static_cast<int>(m), ep, err_dev,
+                          stream);
+}

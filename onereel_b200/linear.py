@@ -1,0 +1,145 @@
+"""Linear layers with their epilogue on the B200 matrix kernels (onereel_b200/csrc/linear.cu): the projections and
+feed-forward layers around the scene attention, with bias, activation, gate and residual in the kernel that computes the
+product, and their gradients.
+
+There is no CPU or library fallback: bf16 CUDA tensors, feature sizes that are multiples of 8. A wait of a kernel that
+gave up is reported by onereel_b200.attention.check().
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from onereel_b200 import _lib as L
+from onereel_b200.attention import _err_word
+
+ACTIVATIONS = {None: 0, 'gelu_tanh': 1, 'silu': 2}
+
+
+def _check(name, t, shape, device):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.bfloat16):
+        raise TypeError(f'{name} must be a bf16 CUDA tensor (the B200 path has no fallback), got '
+                        f'{getattr(t, "dtype", type(t))} on {getattr(t, "device", "?")}')
+    if t.device != device:
+        raise ValueError(f'{name} is on {t.device}, x on {device}')
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{name} must have shape {tuple(shape)}, got {tuple(t.shape)}')
+
+
+def _rows(t):
+    """t as the kernels read it: unit column stride, row stride a multiple of 8 and at least the row, 16-byte base (a
+    copy where a view does not have them)"""
+    ok = t.stride(1) == 1 and t.data_ptr() % 16 == 0 and \
+        (t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1]))
+    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(t):
+    t = t.reshape(-1)
+    return t if t.stride(0) == 1 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+           residual: torch.Tensor | None = None, gate: torch.Tensor | None = None) -> torch.Tensor:
+    """residual + gate * activation(x weight^T + bias), accumulated and finished in fp32, rounded once.
+
+    x [..., K], weight [N, K], bias [N], gate of N elements (one factor per output feature, e.g. [1, 1, N]), residual
+    and the result [..., N]; activation None, 'gelu_tanh' or 'silu'; bf16 CUDA tensors, K and N multiples of 8. Views
+    whose rows are strided by multiples of 8 elements are read in place, others are copied. Differentiable in every
+    tensor (first derivatives; deterministic); with an activation or a gate the product is kept for the backward pass."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f'unknown activation {activation!r}: one of {sorted(map(str, ACTIVATIONS))}')
+    _check('x', x, None, getattr(x, 'device', None))
+    dev = x.device
+    _check('weight', weight, None, dev)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f'shape mismatch x {tuple(x.shape)} weight {tuple(weight.shape)}')
+    N, K = weight.shape
+    if N % 8 or K % 8 or N == 0 or K == 0:
+        raise ValueError(f'feature sizes must be positive multiples of 8, got {K} -> {N}')
+    shape = (*x.shape[:-1], N)
+    if bias is not None:
+        _check('bias', bias, (N,), dev)
+    if residual is not None:
+        _check('residual', residual, shape, dev)
+    if gate is not None:
+        _check('gate', gate, None, dev)
+        if gate.numel() != N:
+            raise ValueError(f'gate must have {N} elements, got {tuple(gate.shape)}')
+    args = [x.reshape(-1, K), weight, bias, None if gate is None else gate.reshape(-1),
+            None if residual is None else residual.reshape(-1, N)]
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        y = _Linear.apply(*args, act)
+    else:
+        y = _forward(*args, act, keep=False)[0]
+    return y.view(shape)
+
+
+def _forward(x, w, b, gate, residual, act, keep):
+    """(y, z or None): the kernel call; keep: also store z = x w^T + bias"""
+    M, N, K, dev = x.shape[0], w.shape[0], x.shape[1], x.device
+    with torch.cuda.device(dev):
+        x, w = _rows(x), _rows(w)
+        b, gate = (None if t is None else _vector(t) for t in (b, gate))
+        residual = None if residual is None else _rows(residual)
+        y = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
+        z = torch.empty_like(y) if keep else None
+        L.check(L.lib().orl_linear(x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ptr(b), _ptr(gate), _ptr(residual),
+                                   0 if residual is None else _ld(residual), y.data_ptr(), _ptr(z), M, N, K, act,
+                                   _err_word(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
+                'orl_linear')
+    return y, z
+
+
+class _Linear(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, w, b, gate, residual, act):
+        # z is needed for act' and for the gate's gradient; without them dz is dy itself
+        y, z = _forward(x, w, b, gate, residual, act, keep=act != 0 or gate is not None)
+        ctx.save_for_backward(x, w, gate, z)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, gate, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        (M, K), N, dev = x.shape, w.shape[0], x.device
+        with torch.cuda.device(dev):
+            stream, err = torch.cuda.current_stream(dev).cuda_stream, _err_word(dev).data_ptr()
+            d = _rows(dy)
+            dx = dw = db = dgate = None
+            gv = None if gate is None else _vector(gate)
+            dz = d if z is None else torch.empty(M, N, dtype=torch.bfloat16, device=dev)
+            if need[2]:
+                db = torch.empty(N, dtype=torch.bfloat16, device=dev)
+            if need[3]:
+                dgate = torch.empty(N, dtype=torch.bfloat16, device=dev)
+            if db is not None or dgate is not None or (z is not None and (need[0] or need[1])):
+                scratch = torch.empty(L.check(L.lib().orl_linear_dz_scratch(M, N), 'orl_linear_dz_scratch'),
+                                      dtype=torch.float32, device=dev)
+                L.check(L.lib().orl_linear_dz(d.data_ptr(), _ld(d), _ptr(z), _ptr(gv), ctx.act,
+                                              None if z is None else dz.data_ptr(), _ptr(db), _ptr(dgate),
+                                              scratch.data_ptr(), M, N, stream), 'orl_linear_dz')
+            if need[0]:
+                wr = _rows(w)
+                dx = torch.empty(M, K, dtype=torch.bfloat16, device=dev)
+                L.check(L.lib().orl_linear_dx(dz.data_ptr(), _ld(dz), wr.data_ptr(), _ld(wr), dx.data_ptr(), M, N, K,
+                                              err, stream), 'orl_linear_dx')
+            if need[1]:
+                xr = _rows(x)
+                dw = torch.empty(N, K, dtype=torch.bfloat16, device=dev)
+                L.check(L.lib().orl_linear_dw(dz.data_ptr(), _ld(dz), xr.data_ptr(), _ld(xr), dw.data_ptr(), M, N, K,
+                                              err, stream), 'orl_linear_dw')
+        return dx, dw, db, dgate, dy if need[4] else None, None
