@@ -134,7 +134,7 @@ typedef struct orl_attn_bwd_work {
   int32_t range0;   /* first of its ranges */
   int32_t n_ranges; /* 0: the rows' gradients are zero */
   int32_t n_tiles;  /* 128-row tiles of its ranges */
-  int32_t pad;
+  int32_t whole;    /* 1: its tiles hold all keys of their queries, so delta is summed from them in fp32 */
 } orl_attn_bwd_work;
 
 /* Work list of a backward call for segments given as in orl_attn_plan_ranges (key ranges may overlap, query ranges

@@ -48,7 +48,7 @@ class Path(ctypes.Structure):
 # numpy views of the same layouts (for building tables without Python loops over ctypes objects)
 WORK_DTYPE = np.dtype([(n, np.int32) for n, _ in AttnWork._fields_])
 BWD_WORK_DTYPE = np.dtype([(n, np.int32) for n in ('row0', 'rows', 'head', 'kind', 'range0', 'n_ranges', 'n_tiles',
-                                                    'pad')])
+                                                    'whole')])
 RUN_DTYPE = np.dtype([('src_slot', np.int32), ('dst_slot', np.int32), ('src_off', np.int64), ('dst_off', np.int64),
                       ('vec0', np.int64)])
 assert WORK_DTYPE.itemsize == ctypes.sizeof(AttnWork) == 32 and RUN_DTYPE.itemsize == ctypes.sizeof(CopyRun) == 32

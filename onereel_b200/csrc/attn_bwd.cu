@@ -21,6 +21,12 @@
 // TMEM columns, kDkv: S^T / P^T [0,128), dP^T / dS^T [128,256), dV [256,256+D), dK [256+D,256+2D): while the compute
 // warps work on P the tensor pipe runs dK of the previous tile and dP of this one; while they work on dS, dV and the
 // next S. kDq: S / dS [0,128) and [128,256) by turns, dP [256,384), dQ [384,384+D).
+//
+// delta from the forward's bf16 o carries o's rounding. Over many keys that is lost in the rounding of dS, but over a few
+// keys dS is a small difference of large terms (two keys: dq 0.0040 off in the 2-norm instead of 0.0024; 32 keys and
+// more: the same). Where a tile holds all keys of its queries, delta = sum_j P dP - dL is therefore taken from the
+// tile itself in fp32.
+//
 // Every mbarrier wait is bounded as in the forward: a stuck pipeline sets the error word and winds down.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -54,7 +60,8 @@ struct BwdCfg {
   static constexpr int kTOff = 2 * kTileBytes;
   static constexpr int kStatOff = kTOff + 2 * kStages * kTileBytes;   // float2 (lse2, delta) of 128 streamed rows
   static constexpr int kValidOff = kStatOff + kStages * 1024;         // int: rows of the tile inside its range
-  static constexpr int kBarOff = kValidOff + 16 * ((kStages * 4 + 15) / 16);
+  static constexpr int kRedOff = kValidOff + 16 * ((kStages * 4 + 15) / 16);   // float: column sums per warp
+  static constexpr int kBarOff = kRedOff + 8 * 128 * 4;
   static constexpr int kBarR = 0;                       // resident tiles landed
   static constexpr int kBarT0 = 1;                      // streamed tiles landed, per stage
   static constexpr int kBarT1 = kBarT0 + kStages;
@@ -172,10 +179,18 @@ __device__ __forceinline__ void bwd_producer(const BwdShared& sh, const CUtensor
 // T0 (K) needs them: the columns of S and dP past the end are masked, but dS K sums over K's rows.
 template <int D>
 __device__ __forceinline__ void bwd_aux(const BwdShared& sh, const BwdWork& wi, const int2* ranges,
-                                        const float2* __restrict__ stats, long long nq, int t, int* err) {
+                                        const float2* __restrict__ stats, const float* __restrict__ dlse, long long nq,
+                                        int t, int* err) {
   using C = BwdCfg<D>;
   const bool dkv = wi.kind == kDkv;
   const float2* st = stats + static_cast<long long>(wi.head) * nq;
+  const float* dl = dlse == nullptr ? nullptr : dlse + static_cast<long long>(wi.head) * nq;
+  // (lse2, delta) of a query row; where the tile gives sum_j P dP itself, its other term -dL
+  auto row_stats = [&](long long row) {
+    float2 x = __ldg(st + row);
+    if (wi.whole) x.y = dl == nullptr ? 0.f : -__ldg(dl + row);
+    return x;
+  };
   TileWalk walk(ranges, wi.n_ranges);
   for (int j = 0; j < wi.n_tiles; ++j) {
     const int s = j % C::kStages;
@@ -183,8 +198,8 @@ __device__ __forceinline__ void bwd_aux(const BwdShared& sh, const BwdWork& wi, 
     const int valid = walk.next(row);
     float2 a = make_float2(INFINITY, 0.f), b = a;
     if (dkv) {
-      if (t < valid) a = __ldg(st + row + t);
-      if (t + 64 < valid) b = __ldg(st + row + t + 64);
+      if (t < valid) a = row_stats(row + t);
+      if (t + 64 < valid) b = row_stats(row + t + 64);
     }
     bool ok = true;
     if (j >= C::kStages) ok = mbar_wait(sh.bar(C::kBarE + s), ((j / C::kStages) - 1) & 1, sh.abort_flag);
@@ -349,6 +364,44 @@ __device__ __forceinline__ void bwd_zero(const BwdThread& th, const BwdWork& wi,
   }
 }
 
+// Adds sum_j P dP over the tile's key rows to the delta of each of its query columns (stage s): rows of a thread, lanes
+// of a warp by shuffles, the eight warps through shared memory.
+template <int D>
+__device__ __forceinline__ void bwd_column_delta(const BwdShared& sh, uint32_t dp_addr, const BwdThread& th, int rows,
+                                              const uint32_t (&p)[64], int s) {
+  using C = BwdCfg<D>;
+  const int t = threadIdx.x - 128;                    // 0..255
+  float* red = reinterpret_cast<float*>(sh.smem + C::kRedOff);
+  const float m0 = th.row < rows ? 1.f : 0.f, m1 = th.row + 8 < rows ? 1.f : 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t d[32];
+    tmem_ld_16x256b_x8(dp_addr + 64 * h, d);
+    tmem_wait_ld();
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const uint32_t* x = p + 4 * (8 * h + r);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // rows past the range may hold anything: they are not multiplied in
+        float a = m0 != 0.f ? __uint_as_float(x[e]) * __uint_as_float(d[4 * r + e]) : 0.f;
+        if (m1 != 0.f) a = fmaf(__uint_as_float(x[2 + e]), __uint_as_float(d[4 * r + 2 + e]), a);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if ((t & 31) < 4) red[128 * (t >> 5) + 64 * h + 8 * r + 2 * th.cq + e] = a;
+      }
+    }
+  }
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  if (t < 128) {
+    float a = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) a += red[128 * w + t];
+    reinterpret_cast<float2*>(sh.smem + C::kStatOff + s * 1024)[t].y += a;
+  }
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
 template <int D>
 __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tmem, const BwdThread& th,
                                                 const BwdWork& wi, float scale, __nv_bfloat16* __restrict__ dk,
@@ -394,6 +447,7 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
     ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
     if (!ok) break;
     tc_fence_after();
+    if (wi.whole) bwd_column_delta<D>(sh, dp_addr, th, wi.rows, p, s);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t d[32], w[16];
@@ -430,12 +484,12 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
 template <int D>
 __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tmem, const BwdThread& th,
                                                const BwdWork& wi, float scale, const float2* __restrict__ stats,
-                                               long long nq, __nv_bfloat16* __restrict__ dq, int heads, int* err) {
+                                               const float* __restrict__ dlse, long long nq, __nv_bfloat16* __restrict__ dq, int heads, int* err) {
   using C = BwdCfg<D>;
   const float scale_log2 = scale * kLog2e;
   const float2* st = stats + static_cast<long long>(wi.head) * nq + wi.row0 + th.row;
-  const float2 st0 = th.row < wi.rows ? __ldg(st) : make_float2(INFINITY, 0.f);
-  const float2 st1 = th.row + 8 < wi.rows ? __ldg(st + 8) : make_float2(INFINITY, 0.f);
+  float2 st0 = th.row < wi.rows ? __ldg(st) : make_float2(INFINITY, 0.f);
+  float2 st1 = th.row + 8 < wi.rows ? __ldg(st + 8) : make_float2(INFINITY, 0.f);
   const uint32_t dp_addr = tmem + C::kColDp + th.lane_off;
   bool ok = true;
   uint32_t p[64];
@@ -461,6 +515,32 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
     ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
     if (!ok) break;
     tc_fence_after();
+    if (wi.whole) {
+      // all keys of these queries are here: delta = sum_j P dP - dL, a quad of threads per row
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t d[32];
+        tmem_ld_16x256b_x8(dp_addr + 64 * h, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (64 * h + 8 * r + 2 * th.cq + e < valid) {
+              s0 = fmaf(__uint_as_float(p[4 * (8 * h + r) + e]), __uint_as_float(d[4 * r + e]), s0);
+              s1 = fmaf(__uint_as_float(p[4 * (8 * h + r) + 2 + e]), __uint_as_float(d[4 * r + 2 + e]), s1);
+            }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+        s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+      }
+      const float* dl = dlse == nullptr ? nullptr : dlse + static_cast<long long>(wi.head) * nq + wi.row0 + th.row;
+      st0.y = s0 - (dl != nullptr && th.row < wi.rows ? __ldg(dl) : 0.f);
+      st1.y = s1 - (dl != nullptr && th.row + 8 < wi.rows ? __ldg(dl + 8) : 0.f);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t d[32], w[16];
@@ -508,7 +588,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                     const BwdWork* __restrict__ work, const int2* __restrict__ ranges,
-                    const float2* __restrict__ stats, __nv_bfloat16* __restrict__ dq, __nv_bfloat16* __restrict__ dk,
+                    const float2* __restrict__ stats, const float* __restrict__ dlse, __nv_bfloat16* __restrict__ dq,
+                    __nv_bfloat16* __restrict__ dk,
                     __nv_bfloat16* __restrict__ dv, long long nq, int heads, float scale, int* __restrict__ err,
                     const int* __restrict__ n_items_dev) {
   using C = BwdCfg<D>;
@@ -567,7 +648,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       } else if (warp == 1) {
         if (elect_one()) bwd_mma<D>(sh, tmem, wi, err);
       } else {
-        bwd_aux<D>(sh, wi, rg, stats, nq, threadIdx.x - 64, err);
+        bwd_aux<D>(sh, wi, rg, stats, dlse, nq, threadIdx.x - 64, err);
       }
     }
   } else {
@@ -583,7 +664,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     } else if (dkv) {
       bwd_compute_dkv<D>(sh, tmem, th, wi, scale, dk, dv, heads, err);
     } else {
-      bwd_compute_dq<D>(sh, tmem, th, wi, scale, stats, nq, dq, heads, err);
+      bwd_compute_dq<D>(sh, tmem, th, wi, scale, stats, dlse, nq, dq, heads, err);
     }
   }
 
@@ -690,7 +771,7 @@ static int launch_attn_bwd(const void* q, const void* k, const void* v, const vo
     if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
   }
   attn_bwd_kernel<D><<<n_items, kBwdThreads, C::kSmemBytes, stream>>>(
-      mq, mk, mv, mdo, work, ranges, stats, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
+      mq, mk, mv, mdo, work, ranges, stats, dlse, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
       static_cast<__nv_bfloat16*>(dv), nq, heads, scale, err, n_items_dev);
   return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
 }
@@ -724,7 +805,7 @@ struct BwdPlan {
 static int plan_bwd(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start, const int32_t* k_len,
                     int n_seg, int heads, long long nq, long long nk, BwdPlan& plan) {
   struct Block {
-    int row0, rows, kind, range0, n_ranges, n_tiles;
+    int row0, rows, kind, range0, n_ranges, n_tiles, whole;
   };
   std::vector<Block> blocks;
   std::vector<int> by_q;                                  // segments with query rows, by first row
@@ -734,23 +815,23 @@ static int plan_bwd(const int32_t* q_start, const int32_t* q_len, const int32_t*
       return ORL_ERR_ARG;
     if (q_len[i] > 0) by_q.push_back(i);
   }
-  auto cut = [&](long long lo, long long hi, int kind, int range0, int n_ranges, int n_tiles) {
+  auto cut = [&](long long lo, long long hi, int kind, int range0, int n_ranges, int n_tiles, bool whole) {
     for (long long r = lo; r < hi; r += 128)
       blocks.push_back({static_cast<int>(r), static_cast<int>(std::min<long long>(128, hi - r)), kind, range0, n_ranges,
-                        n_tiles});
+                        n_tiles, whole ? 1 : 0});
   };
   // queries: one range of keys per segment; rows of no segment get zeros
   std::sort(by_q.begin(), by_q.end(), [&](int a, int b) { return q_start[a] < q_start[b]; });
   long long at = 0;
   for (int i : by_q) {
     if (q_start[i] < at) return ORL_ERR_ARG;              // two segments share a query row
-    cut(at, q_start[i], kDq, 0, 0, 0);
+    cut(at, q_start[i], kDq, 0, 0, 0, false);
     plan.ranges.push_back({k_start[i], k_len[i]});
     cut(q_start[i], static_cast<long long>(q_start[i]) + q_len[i], kDq, static_cast<int>(plan.ranges.size()) - 1, 1,
-        (k_len[i] + 127) / 128);
+        (k_len[i] + 127) / 128, k_len[i] > 0 && k_len[i] <= 128);
     at = static_cast<long long>(q_start[i]) + q_len[i];
   }
-  cut(at, nq, kDq, 0, 0, 0);
+  cut(at, nq, kDq, 0, 0, 0, false);
   // keys: the elementary intervals, each with the query ranges of the segments that cover it (in segment order)
   std::vector<long long> cuts = {0, nk};
   for (int i = 0; i < n_seg; ++i)
@@ -764,15 +845,17 @@ static int plan_bwd(const int32_t* q_start, const int32_t* q_len, const int32_t*
     const int range0 = static_cast<int>(plan.ranges.size());
     int n = 0;
     long long tiles = 0;
+    bool whole = cuts[c + 1] - cuts[c] <= 128;            // every reader's keys are exactly this block
     for (int i = 0; i < n_seg; ++i)
       if (q_len[i] > 0 && k_len[i] > 0 && k_start[i] <= cuts[c] &&
           static_cast<long long>(k_start[i]) + k_len[i] >= cuts[c + 1]) {
         plan.ranges.push_back({q_start[i], q_len[i]});
         tiles += (q_len[i] + 127) / 128;
+        whole = whole && k_start[i] == cuts[c] && k_len[i] == cuts[c + 1] - cuts[c];
         ++n;
       }
     if (tiles > 0x7fffffffLL || plan.ranges.size() > 0x7ffffff0u) return ORL_ERR_CAPACITY;
-    cut(cuts[c], cuts[c + 1], kDkv, range0, n, static_cast<int>(tiles));
+    cut(cuts[c], cuts[c + 1], kDkv, range0, n, static_cast<int>(tiles), whole && n > 0);
   }
   // longest first; a dkv tile has four products and a dq tile three. Blocks of one head and segment stay adjacent.
   auto cost = [](const Block& b) { return static_cast<long long>(b.n_tiles) * (b.kind == kDkv ? 4 : 3); };
@@ -791,7 +874,7 @@ static int plan_bwd(const int32_t* q_start, const int32_t* q_len, const int32_t*
     for (int h = 0; h < heads; ++h)
       for (size_t x = lo; x < hi; ++x) {
         const Block& b = blocks[order[x]];
-        plan.items.push_back({b.row0, b.rows, h, b.kind, b.range0, b.n_ranges, b.n_tiles, 0});
+        plan.items.push_back({b.row0, b.rows, h, b.kind, b.range0, b.n_ranges, b.n_tiles, b.whole});
       }
     lo = hi;
   }
@@ -948,7 +1031,9 @@ __global__ void __launch_bounds__(1024)
     w.range0 = g < 2 * n_seg ? g : 0;
     w.n_ranges = s_tiles[g] > 0 ? 1 : 0;
     w.n_tiles = s_tiles[g];
-    w.pad = 0;
+    // the segment's keys fit one tile (a dkv block is then the whole segment)
+    const int keys = g < 2 * n_seg ? s_len[g % n_seg] : 0;
+    w.whole = w.n_tiles > 0 && keys > 0 && keys <= 128 ? 1 : 0;
     work[1 + it] = w;
   }
   if (t == 0) work[0].row0 = n;

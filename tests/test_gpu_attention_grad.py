@@ -260,3 +260,22 @@ def test_refusals():
     with pytest.raises(L.OrlError):
         A.check()
     A.check()
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('lk', [2, 3, 7, 31, 128, 129])
+def test_few_keys_keep_their_precision(lk, D):
+    """with few keys dS is a small difference of large terms: the gradients stay within the two roundings that remain
+    (dS or P, and the result), whatever the rounding of out. A rounding's relative error in the 2-norm is
+    u sqrt(E[1 / m^2] / 3) = 0.425 u for a significand m spread evenly in its logarithm; a quarter more for the data."""
+    from onereel_b200 import attention as A
+    H, lq = 3, [300, 40]
+    q, k, v, dout, dlse = inputs(sum(lq), 2 * lk, H, D, seed=lk)
+    segs = (starts(lq), lq, [0, lk], [lk, lk])
+    out, lse = A.attend(q, k, v, *segs, lse=True)
+    got = A.attend_grad(q, k, v, out, lse, dout, *segs, dlse=dlse)
+    want = attention_grads(q, k, v, dout, *segs, dlse=dlse)
+    tol = 1.25 * 2 ** 0.5 * 0.425 * 2.0 ** -8
+    for t, n in zip(got, ('dq', 'dk', 'dv')):
+        rel = ((t.double() - want[n][0]).norm() / want[n][0].norm()).item()
+        assert rel < tol, (n, rel)
