@@ -18,9 +18,12 @@
 // there - other segments, or NaN in rows no segment owns - enters no product), warps 4-11 hold P and dS: a warp owns 16
 // TMEM lanes, a thread two rows and 32 of their 128 columns each. P and dS go back to TMEM as bf16 and are the A
 // operand of the accumulating MMAs.
-// TMEM columns, kDkv: S^T / P^T [0,128), dP^T / dS^T [128,256), dV [256,256+D), dK [256+D,256+2D): while the compute
-// warps work on P the tensor pipe runs dK of the previous tile and dP of this one; while they work on dS, dV and the
-// next S. kDq: S / dS [0,128) and [128,256) by turns, dP [256,384), dQ [384,384+D).
+// TMEM columns, kDkv: S^T / P^T [0,128), dP^T / dS^T [128,256), dV [256,256+D), dK [256+D,256+2D) - all 512 at D = 128.
+// While the compute warps work on P(j) the tensor pipe runs dK(j-1) and dP(j); while they work on dS(j), dV(j) and
+// S(j+1). P is handed over in two halves, so dV begins under the second half's exponentials.
+// kDq: S [0,128), dP / dS [128,256) and [256,384) by turns, dQ [384,384+D). One step of the compute warps takes dS(j) from
+// dP(j) and the P(j) in their registers, and P(j+1) from S(j+1): the exponentials (MUFU) of one tile run beside the
+// arithmetic of the other, and S(j+2), dP(j+1) and dQ(j-1) are computed under them.
 //
 // delta from the forward's bf16 o carries o's rounding. Over many keys that is lost in the rounding of dS, but over a few
 // keys dS is a small difference of large terms (two keys: dq 0.0040 off in the 2-norm instead of 0.0024; 32 keys and
@@ -36,6 +39,7 @@
 #include <cstdint>
 #include <mutex>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "orl_common.h"
@@ -54,32 +58,46 @@ struct BwdCfg {
   static constexpr int kChunks = D / 64;              // 128-byte swizzle columns per row
   static constexpr int kTileBytes = 128 * D * 2;      // one 128-row bf16 tile
   static constexpr int kChunkBytes = 128 * 128;       // one 128-row x 64-column chunk
-  static constexpr int kStages = (D == 128) ? 2 : 4;  // ring depth of streamed tile pairs
-  // resident tiles R0, R1 (K, V or q, dO), streamed tiles T0, T1 (q, dO or K, V)
+  // Resident tiles R0, R1 (K, V or q, dO); rings of streamed tiles T0 (q or K) and T1 (dO or V). kDq has S of tile
+  // j + 2 issued before dQ of tile j, so K needs three stages; at D = 128 that is all the shared memory there is.
+  __host__ __device__ static constexpr int stages0(bool dkv) { return D == 64 ? 4 : dkv ? 2 : 3; }
+  static constexpr int kStages1 = D == 64 ? 4 : 2;
+  static constexpr int kMaxStages = 4;
   static constexpr int kROff = 0;
-  static constexpr int kTOff = 2 * kTileBytes;
-  static constexpr int kStatOff = kTOff + 2 * kStages * kTileBytes;   // float2 (lse2, delta) of 128 streamed rows
-  static constexpr int kValidOff = kStatOff + kStages * 1024;         // int: rows of the tile inside its range
-  static constexpr int kRedOff = kValidOff + 16 * ((kStages * 4 + 15) / 16);   // float: column sums per warp
-  static constexpr int kBarOff = kRedOff + 8 * 128 * 4;
+  static constexpr int kT1Off = 2 * kTileBytes;
+  static constexpr int kT0Off = kT1Off + kStages1 * kTileBytes;
+  // kDkv: (lse2, delta) of the 128 streamed rows per stage, and column sums per warp (both after its last T0 stage)
+  static constexpr int kStatBytes = 2 * 4 * 36 * 4;   // lse2, delta: four groups of 32 columns, padded (see stat_at)
+  static constexpr int kStatOff = kT0Off + stages0(true) * kTileBytes;
+  static constexpr int kRedOff = kStatOff + kMaxStages * kStatBytes;
+  static constexpr int kDkvEnd = kRedOff + 8 * 128 * 4;
+  static constexpr int kDqEnd = kT0Off + stages0(false) * kTileBytes;
+  static constexpr int kValidOff = kDkvEnd > kDqEnd ? kDkvEnd : kDqEnd;   // int per stage: rows inside the range
+  static constexpr int kBarOff = kValidOff + 16;
   static constexpr int kBarR = 0;                       // resident tiles landed
   static constexpr int kBarT0 = 1;                      // streamed tiles landed, per stage
-  static constexpr int kBarT1 = kBarT0 + kStages;
-  static constexpr int kBarAux = kBarT1 + kStages;      // statistics and zeroed rows ready, per stage
-  static constexpr int kBarE = kBarAux + kStages;       // stage free
-  static constexpr int kBarS = kBarE + kStages;         // S computed (two buffers in kDq)
-  static constexpr int kBarDp = kBarS + 2;              // dP computed
-  static constexpr int kBarP = kBarDp + 1;              // kDkv: P stored; kDq: dP read
-  static constexpr int kBarDs = kBarP + 1;              // dS stored
-  static constexpr int kBarDone = kBarDs + 1;
+  static constexpr int kBarT1 = kBarT0 + kMaxStages;
+  static constexpr int kBarAux = kBarT1 + kMaxStages;   // statistics and zeroed rows ready, per T0 stage
+  static constexpr int kBarE0 = kBarAux + kMaxStages;   // stage free
+  static constexpr int kBarE1 = kBarE0 + kMaxStages;
+  static constexpr int kBarS = kBarE1 + kMaxStages;     // S computed
+  static constexpr int kBarDp = kBarS + 1;              // dP computed (kDq: two buffers)
+  static constexpr int kBarP = kBarDp + 2;              // kDkv: half of P stored (two); kDq: S read
+  // dS stored. kDq: two by turns, since dS(j + 1) may be complete before the issuing thread has seen dS(j)
+  static constexpr int kBarDs = kBarP + 2;
+  static constexpr int kBarDone = kBarDs + 2;
   static constexpr int kBarDrain = kBarDone + 1;
   static constexpr int kNumBars = kBarDrain + 1;
   static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColDv = 256, kColDk = 256 + D;       // kDkv (S at 0, dP at 128)
-  static constexpr uint32_t kColDp = 256, kColDq = 384;           // kDq (S at 0 and 128)
+  static constexpr uint32_t kColDp = 128, kColDq = 384;           // kDq (S at 0; dP at 128 and 256)
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
+
+// Where the statistic of streamed row c lies: a thread of the compute warps needs columns 8r + 2 cq + {0, 1}, here 32
+// consecutive floats of group cq (eight 16-byte loads); groups 36 floats apart fall into different banks.
+__device__ __forceinline__ int stat_at(int c) { return 36 * ((c >> 1) & 3) + 2 * (c >> 3) + (c & 1); }
 
 constexpr int kBwdThreads = 384;
 constexpr int kAuxThreads = 64;
@@ -143,33 +161,37 @@ __device__ __forceinline__ void bwd_producer(const BwdShared& sh, const CUtensor
     tma_load_2d(sh.sbase + C::kROff + C::kTileBytes + c * C::kChunkBytes, r1, sh.bar(C::kBarR), x0 + 64 * c, wi.row0,
                 pol_r);
   }
+  const int n0 = C::stages0(wi.kind == kDkv);
+  auto stream = [&](int j, int y, int stages, int off, int bar_full, int bar_empty, const CUtensorMap* map) {
+    const int s = j % stages;
+    if (j >= stages && !mbar_wait(sh.bar(bar_empty + s), ((j / stages) - 1) & 1, sh.abort_flag)) return false;
+    mbar_expect_tx(sh.bar(bar_full + s), C::kTileBytes);
+    for (int c = 0; c < C::kChunks; ++c)
+      tma_load_2d(sh.sbase + off + s * C::kTileBytes + c * C::kChunkBytes, map, sh.bar(bar_full + s), x0 + 64 * c, y,
+                  pol_t);
+    return true;
+  };
   TileWalk walk(ranges, wi.n_ranges);
-  int issued = 0;
+  int issued0 = 0, issued1 = 0;
   for (int j = 0; j < wi.n_tiles; ++j) {
-    const int s = j % C::kStages;
     int y = 0;
     walk.next(y);
-    if (j >= C::kStages && !mbar_wait(sh.bar(C::kBarE + s), ((j / C::kStages) - 1) & 1, sh.abort_flag)) {
+    bool ok = stream(j, y, n0, C::kT0Off, C::kBarT0, C::kBarE0, t0);
+    if (ok) issued0 = j + 1;
+    ok = ok && stream(j, y, C::kStages1, C::kT1Off, C::kBarT1, C::kBarE1, t1);
+    if (!ok) {
       atomicOr(err, kErrTimeoutLoad);
       break;
     }
-    const uint32_t a = sh.sbase + C::kTOff + 2 * s * C::kTileBytes;
-    mbar_expect_tx(sh.bar(C::kBarT0 + s), C::kTileBytes);
-    for (int c = 0; c < C::kChunks; ++c)
-      tma_load_2d(a + c * C::kChunkBytes, t0, sh.bar(C::kBarT0 + s), x0 + 64 * c, y, pol_t);
-    mbar_expect_tx(sh.bar(C::kBarT1 + s), C::kTileBytes);
-    for (int c = 0; c < C::kChunks; ++c)
-      tma_load_2d(a + C::kTileBytes + c * C::kChunkBytes, t1, sh.bar(C::kBarT1 + s), x0 + 64 * c, y, pol_t);
-    issued = j + 1;
+    issued1 = j + 1;
   }
   if (*sh.abort_flag) {
     // wind down: every copy this thread started must land before the CTA's shared memory is released
     bwd_drain_wait(sh.bar(C::kBarR), 0, err);
-    for (int j = issued > C::kStages ? issued - C::kStages : 0; j < issued; ++j) {
-      const int s = j % C::kStages;
-      bwd_drain_wait(sh.bar(C::kBarT0 + s), (j / C::kStages) & 1, err);
-      bwd_drain_wait(sh.bar(C::kBarT1 + s), (j / C::kStages) & 1, err);
-    }
+    for (int j = issued0 > n0 ? issued0 - n0 : 0; j < issued0; ++j)
+      bwd_drain_wait(sh.bar(C::kBarT0 + j % n0), (j / n0) & 1, err);
+    for (int j = issued1 > C::kStages1 ? issued1 - C::kStages1 : 0; j < issued1; ++j)
+      bwd_drain_wait(sh.bar(C::kBarT1 + j % C::kStages1), (j / C::kStages1) & 1, err);
   }
 }
 
@@ -191,9 +213,10 @@ __device__ __forceinline__ void bwd_aux(const BwdShared& sh, const BwdWork& wi, 
     if (wi.whole) x.y = dl == nullptr ? 0.f : -__ldg(dl + row);
     return x;
   };
+  const int n0 = C::stages0(dkv);
   TileWalk walk(ranges, wi.n_ranges);
   for (int j = 0; j < wi.n_tiles; ++j) {
-    const int s = j % C::kStages;
+    const int s = j % n0, s1 = j % C::kStages1;
     int row = 0;
     const int valid = walk.next(row);
     float2 a = make_float2(INFINITY, 0.f), b = a;
@@ -202,27 +225,30 @@ __device__ __forceinline__ void bwd_aux(const BwdShared& sh, const BwdWork& wi, 
       if (t + 64 < valid) b = row_stats(row + t + 64);
     }
     bool ok = true;
-    if (j >= C::kStages) ok = mbar_wait(sh.bar(C::kBarE + s), ((j / C::kStages) - 1) & 1, sh.abort_flag);
+    if (j >= n0) ok = mbar_wait(sh.bar(C::kBarE0 + s), ((j / n0) - 1) & 1, sh.abort_flag);
     if (ok && valid < 128) {
-      ok = mbar_wait(sh.bar(C::kBarT0 + s), (j / C::kStages) & 1, sh.abort_flag);
-      if (ok && dkv) ok = mbar_wait(sh.bar(C::kBarT1 + s), (j / C::kStages) & 1, sh.abort_flag);
+      ok = mbar_wait(sh.bar(C::kBarT0 + s), (j / n0) & 1, sh.abort_flag);
+      if (ok && dkv) ok = mbar_wait(sh.bar(C::kBarT1 + s1), (j / C::kStages1) & 1, sh.abort_flag);
     }
     if (!ok) {
       if (t == 0) atomicOr(err, kErrTimeoutLoad);
       return;
     }
     if (dkv) {
-      float2* dst = reinterpret_cast<float2*>(sh.smem + C::kStatOff + s * 1024);
-      dst[t] = a;
-      dst[t + 64] = b;
+      float* dst = reinterpret_cast<float*>(sh.smem + C::kStatOff + s * C::kStatBytes);
+      dst[stat_at(t)] = a.x;
+      dst[stat_at(t + 64)] = b.x;
+      dst[144 + stat_at(t)] = a.y;
+      dst[144 + stat_at(t + 64)] = b.y;
     }
     if (t == 0) *reinterpret_cast<int*>(sh.smem + C::kValidOff + 4 * s) = valid;
     if (valid < 128) {
-      uint8_t* tiles = sh.smem + C::kTOff + 2 * s * C::kTileBytes;
-      const int n_chunks = dkv ? 2 * C::kChunks : C::kChunks;   // T0's chunks, then T1's
-      for (int c = 0; c < n_chunks; ++c)
+      for (int c = 0; c < (dkv ? 2 : 1) * C::kChunks; ++c) {    // T0's chunks, then T1's
+        uint8_t* chunk = sh.smem + (c < C::kChunks ? C::kT0Off + s * C::kTileBytes + c * C::kChunkBytes
+                                                   : C::kT1Off + s1 * C::kTileBytes + (c - C::kChunks) * C::kChunkBytes);
         for (int o = valid * 128 + t * 16; o < C::kChunkBytes; o += kAuxThreads * 16)
-          *reinterpret_cast<uint4*>(tiles + c * C::kChunkBytes + o) = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(chunk + o) = make_uint4(0u, 0u, 0u, 0u);
+      }
       fence_async_smem();
     }
     mbar_arrive(sh.bar(C::kBarAux + s));
@@ -235,25 +261,24 @@ struct BwdMma {
   using C = BwdCfg<D>;
   static constexpr uint32_t kIdescS = idesc_bf16(128, 128, false, false);
   static constexpr uint32_t kIdescA = idesc_bf16(128, D, false, true);
-  // D[col] = R (resident tile r) * T (streamed tile t of stage s)^T
-  static __device__ __forceinline__ void product(const BwdShared& sh, uint32_t d, int r, int t, int s) {
+  // Descriptors are built once per tile and stepped by a constant: building one per MMA costs the issuing thread more
+  // (67 clocks measured per MMA) than the MMA takes (64 clocks at N = 128), stepping them 20.
+  static __device__ __forceinline__ uint64_t k_major(uint32_t tile) { return smem_desc_sw128(tile, 16, 1024); }
+  static __device__ __forceinline__ uint64_t mn_major(uint32_t tile) { return smem_desc_sw128(tile, C::kChunkBytes, 1024); }
+  // D[col] = R (resident tile, K-major descriptor) * T (streamed tile, K-major)^T
+  static __device__ __forceinline__ void product(uint32_t d, uint64_t r, uint64_t t) {
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
-      const uint32_t off = (kk >> 2) * C::kChunkBytes + (kk & 3) * 32;
-      const uint64_t a = smem_desc_sw128(sh.sbase + C::kROff + r * C::kTileBytes + off, 16, 1024);
-      const uint64_t b = smem_desc_sw128(sh.sbase + C::kTOff + (2 * s + t) * C::kTileBytes + off, 16, 1024);
-      mma_ss(d, a, b, kIdescS, kk > 0 ? 1u : 0u);
+      const uint64_t off = ((kk >> 2) * C::kChunkBytes + (kk & 3) * 32) >> 4;
+      mma_ss(d, r + off, t + off, kIdescS, kk > 0 ? 1u : 0u);
     }
   }
-  // D[col] (+)= A (bf16 in TMEM, 128 x 128) * T (streamed tile t of stage s, MN-major)
-  static __device__ __forceinline__ void accumulate(const BwdShared& sh, uint32_t d, uint32_t a, int t, int s,
-                                                    bool acc) {
+  // D[col] (+)= A (bf16 in TMEM, 128 x 128) * T (streamed tile, MN-major), A's columns [16 kLo, 16 kHi)
+  template <int kLo, int kHi>
+  static __device__ __forceinline__ void accumulate(uint32_t d, uint32_t a, uint64_t t, bool acc) {
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      const uint64_t b =
-          smem_desc_sw128(sh.sbase + C::kTOff + (2 * s + t) * C::kTileBytes + kk * 2048, C::kChunkBytes, 1024);
-      mma_ts(d, a + kk * 8, b, kIdescA, (acc || kk > 0) ? 1u : 0u);
-    }
+    for (int kk = kLo; kk < kHi; ++kk)
+      mma_ts(d, a + kk * 8, t + ((kk * 2048) >> 4), kIdescA, (acc || kk > 0) ? 1u : 0u);
   }
 };
 
@@ -263,47 +288,72 @@ __device__ __forceinline__ void bwd_mma(const BwdShared& sh, uint32_t tmem, cons
   using M = BwdMma<D>;
   const int n = wi.n_tiles;
   const bool dkv = wi.kind == kDkv;
+  const int n0 = C::stages0(dkv);
+  const uint64_t r0 = M::k_major(sh.sbase + C::kROff), r1 = M::k_major(sh.sbase + C::kROff + C::kTileBytes);
   auto wait = [&](int bar, int phase) { return mbar_wait(sh.bar(bar), phase & 1, sh.abort_flag); };
-  // S of tile j: its streamed T0, prepared
-  auto issue_s = [&](int j) {
-    const int s = j % C::kStages, ph = j / C::kStages;
-    if (!wait(C::kBarT0 + s, ph) || !wait(C::kBarAux + s, ph)) return false;
-    const int buf = dkv ? 0 : (j & 1);
-    M::product(sh, tmem + 128 * buf, 0, 0, s);
-    mma_commit(sh.bar(C::kBarS + buf));
-    return true;
+  auto tile0 = [&](int j) { return sh.sbase + C::kT0Off + (j % n0) * C::kTileBytes; };
+  auto tile1 = [&](int j) { return sh.sbase + C::kT1Off + (j % C::kStages1) * C::kTileBytes; };
+  // The tiles a product needs are waited for well before its operand from the compute warps is: a wait costs about 90
+  // clocks even when the tile is there, and behind P or dS it would be on the critical path.
+  auto ready0 = [&](int j) {                           // T0 of tile j, prepared
+    const int s = j % n0, ph = j / n0;
+    return wait(C::kBarT0 + s, ph) && wait(C::kBarAux + s, ph);
   };
-  bool ok = wait(C::kBarR, 0) && issue_s(0);
-  for (int j = 0; ok && j < n; ++j) {
-    const int s = j % C::kStages, ph = j / C::kStages;
-    ok = wait(C::kBarT1 + s, ph);
-    if (!ok) break;
-    if (dkv) {
+  auto ready1 = [&](int j) { return wait(C::kBarT1 + j % C::kStages1, j / C::kStages1); };
+  auto issue_s = [&](int j) {
+    M::product(tmem, r0, M::k_major(tile0(j)));
+    mma_commit(sh.bar(C::kBarS));
+  };
+  bool ok = wait(C::kBarR, 0) && ready0(0) && ready1(0);
+  if (ok) issue_s(0);
+  if (dkv) {
+    for (int j = 0; ok && j < n; ++j) {
       // dP overwrites dS of tile j - 1, whose dK MMA was issued before
-      M::product(sh, tmem + 128, 1, 1, s);
+      M::product(tmem + 128, r1, M::k_major(tile1(j)));
       mma_commit(sh.bar(C::kBarDp));
       ok = wait(C::kBarP, j);
       if (!ok) break;
       tc_fence_after();
-      M::accumulate(sh, tmem + C::kColDv, tmem, 1, s, j > 0);
-      if (j + 1 < n) ok = issue_s(j + 1);
+      M::template accumulate<0, 4>(tmem + C::kColDv, tmem, M::mn_major(tile1(j)), j > 0);
+      if (j + 1 < n) ok = ready0(j + 1);
+      ok = ok && wait(C::kBarP + 1, j);
+      if (!ok) break;
+      tc_fence_after();
+      M::template accumulate<4, 8>(tmem + C::kColDv, tmem, M::mn_major(tile1(j)), true);
+      if (j + 1 < n) issue_s(j + 1);                   // over P of this tile, whose dV MMA was issued before
+      mma_commit(sh.bar(C::kBarE1 + j % C::kStages1));
+      if (j + 1 < n) ok = ready1(j + 1);
       ok = ok && wait(C::kBarDs, j);
       if (!ok) break;
       tc_fence_after();
-      M::accumulate(sh, tmem + C::kColDk, tmem + 128, 0, s, j > 0);
-    } else {
-      ok = j == 0 || wait(C::kBarP, j - 1);          // dP of tile j - 1 read
-      if (!ok) break;
-      tc_fence_after();
-      M::product(sh, tmem + C::kColDp, 1, 1, s);
-      mma_commit(sh.bar(C::kBarDp));
-      if (j + 1 < n) ok = issue_s(j + 1);            // over dS of tile j - 1, whose dQ MMA was issued before
-      ok = ok && wait(C::kBarDs, j);
-      if (!ok) break;
-      tc_fence_after();
-      M::accumulate(sh, tmem + C::kColDq, tmem + 128 * (j & 1), 0, s, j > 0);
+      M::template accumulate<0, 8>(tmem + C::kColDk, tmem + 128, M::mn_major(tile0(j)), j > 0);
+      mma_commit(sh.bar(C::kBarE0 + j % n0));
     }
-    mma_commit(sh.bar(C::kBarE + s));
+  } else {
+    // dP of tile j into its buffer, over dS of tile j - 2, whose dQ MMA was issued before
+    auto issue_dp = [&](int j) {
+      M::product(tmem + C::kColDp + 128 * (j & 1), r1, M::k_major(tile1(j)));
+      mma_commit(sh.bar(C::kBarDp + (j & 1)));
+      mma_commit(sh.bar(C::kBarE1 + j % C::kStages1));
+    };
+    if (ok) issue_dp(0);
+    if (ok && n > 1) ok = ready0(1) && wait(C::kBarP, 0) && ready1(1);          // S of tile 0 read
+    if (ok && n > 1) issue_s(1);
+    for (int j = 0; ok && j < n; ++j) {
+      if (j + 1 < n) issue_dp(j + 1);
+      if (j + 2 < n) {
+        ok = ready0(j + 2) && wait(C::kBarP, j + 1);
+        if (!ok) break;
+        tc_fence_after();
+        issue_s(j + 2);
+        ok = ready1(j + 2);
+      }
+      ok = ok && wait(C::kBarDs + (j & 1), j >> 1);
+      if (!ok) break;
+      tc_fence_after();
+      M::template accumulate<0, 8>(tmem + C::kColDq, tmem + C::kColDp + 128 * (j & 1), M::mn_major(tile0(j)), j > 0);
+      mma_commit(sh.bar(C::kBarE0 + j % n0));
+    }
   }
   if (ok) {
     mma_commit(sh.bar(C::kBarDone));
@@ -397,7 +447,7 @@ __device__ __forceinline__ void bwd_column_delta(const BwdShared& sh, uint32_t d
     float a = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) a += red[128 * w + t];
-    reinterpret_cast<float2*>(sh.smem + C::kStatOff + s * 1024)[t].y += a;
+    reinterpret_cast<float*>(sh.smem + C::kStatOff + s * C::kStatBytes)[144 + stat_at(t)] += a;
   }
   asm volatile("bar.sync 1, 256;" ::: "memory");
 }
@@ -409,15 +459,21 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
   using C = BwdCfg<D>;
   const float scale_log2 = scale * kLog2e;
   const uint32_t s_addr = tmem + th.lane_off, dp_addr = s_addr + 128;
+  constexpr int n0 = C::stages0(true);
   bool ok = true;
   uint32_t p[64];                               // scores, then P in fp32
   for (int j = 0; j < wi.n_tiles; ++j) {
-    const int s = j % C::kStages, ph = (j / C::kStages) & 1;
-    ok = mbar_wait(sh.bar(C::kBarAux + s), ph, sh.abort_flag) && mbar_wait(sh.bar(C::kBarS), j & 1, sh.abort_flag);
+    const int s = j % n0;
+    ok = mbar_wait(sh.bar(C::kBarAux + s), (j / n0) & 1, sh.abort_flag);
+    if (!ok) break;
+    // statistics of columns 8r + 2 cq + {0, 1}, two r per load, read before the wait for S (dP)
+    const float4* st = reinterpret_cast<const float4*>(sh.smem + C::kStatOff + s * C::kStatBytes) + 9 * th.cq;
+    float4 c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = st[i];
+    ok = mbar_wait(sh.bar(C::kBarS), j & 1, sh.abort_flag);
     if (!ok) break;
     tc_fence_after();
-    // (lse2, delta) of columns 8r + 2 cq + {0, 1}: one 16-byte load
-    const float4* st = reinterpret_cast<const float4*>(sh.smem + C::kStatOff + s * 1024) + th.cq;
     tmem_ld_16x256b_x8(s_addr, p);
     tmem_ld_16x256b_x8(s_addr + 64, p + 32);
     tmem_wait_ld();
@@ -426,12 +482,13 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
       uint32_t w[16];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        const float4 c = st[4 * (8 * h + r)];
+        const float4 c4 = c[4 * h + (r >> 1)];
+        const float l0 = (r & 1) ? c4.z : c4.x, l1 = (r & 1) ? c4.w : c4.y;
         uint32_t* x = p + 4 * (8 * h + r);
-        const float a0 = ex2(fmaf(__uint_as_float(x[0]), scale_log2, -c.x));
-        const float a1 = ex2(fmaf(__uint_as_float(x[1]), scale_log2, -c.z));
-        const float b0 = ex2(fmaf(__uint_as_float(x[2]), scale_log2, -c.x));
-        const float b1 = ex2(fmaf(__uint_as_float(x[3]), scale_log2, -c.z));
+        const float a0 = ex2(fmaf(__uint_as_float(x[0]), scale_log2, -l0));
+        const float a1 = ex2(fmaf(__uint_as_float(x[1]), scale_log2, -l1));
+        const float b0 = ex2(fmaf(__uint_as_float(x[2]), scale_log2, -l0));
+        const float b1 = ex2(fmaf(__uint_as_float(x[3]), scale_log2, -l1));
         x[0] = __float_as_uint(a0);
         x[1] = __float_as_uint(a1);
         x[2] = __float_as_uint(b0);
@@ -440,14 +497,16 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
         w[2 * r + 1] = pack_bf16x2(b0, b1);
       }
       tmem_st_16x128b_x8(s_addr + 32 * h, w);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(sh.bar(C::kBarP + h));
     }
-    tmem_wait_st();
-    tc_fence_before();
-    mbar_arrive(sh.bar(C::kBarP));
     ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
     if (!ok) break;
     tc_fence_after();
     if (wi.whole) bwd_column_delta<D>(sh, dp_addr, th, wi.rows, p, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = st[36 + i];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t d[32], w[16];
@@ -455,12 +514,13 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
       tmem_wait_ld();
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        const float4 c = st[4 * (8 * h + r)];
+        const float4 c4 = c[4 * h + (r >> 1)];
+        const float l0 = (r & 1) ? c4.z : c4.x, l1 = (r & 1) ? c4.w : c4.y;
         const uint32_t* x = p + 4 * (8 * h + r);
-        const float a0 = __uint_as_float(x[0]) * (__uint_as_float(d[4 * r + 0]) - c.y);
-        const float a1 = __uint_as_float(x[1]) * (__uint_as_float(d[4 * r + 1]) - c.w);
-        const float b0 = __uint_as_float(x[2]) * (__uint_as_float(d[4 * r + 2]) - c.y);
-        const float b1 = __uint_as_float(x[3]) * (__uint_as_float(d[4 * r + 3]) - c.w);
+        const float a0 = __uint_as_float(x[0]) * (__uint_as_float(d[4 * r + 0]) - l0);
+        const float a1 = __uint_as_float(x[1]) * (__uint_as_float(d[4 * r + 1]) - l1);
+        const float b0 = __uint_as_float(x[2]) * (__uint_as_float(d[4 * r + 2]) - l0);
+        const float b1 = __uint_as_float(x[3]) * (__uint_as_float(d[4 * r + 3]) - l1);
         w[2 * r] = pack_bf16x2(a0, a1);
         w[2 * r + 1] = pack_bf16x2(b0, b1);
       }
@@ -490,46 +550,108 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
   const float2* st = stats + static_cast<long long>(wi.head) * nq + wi.row0 + th.row;
   float2 st0 = th.row < wi.rows ? __ldg(st) : make_float2(INFINITY, 0.f);
   float2 st1 = th.row + 8 < wi.rows ? __ldg(st + 8) : make_float2(INFINITY, 0.f);
-  const uint32_t dp_addr = tmem + C::kColDp + th.lane_off;
-  bool ok = true;
-  uint32_t p[64];
-  for (int j = 0; j < wi.n_tiles; ++j) {
-    const int s = j % C::kStages, ph = (j / C::kStages) & 1;
-    const uint32_t s_addr = tmem + 128 * (j & 1) + th.lane_off;
-    ok = mbar_wait(sh.bar(C::kBarAux + s), ph, sh.abort_flag) &&
-         mbar_wait(sh.bar(C::kBarS + (j & 1)), (j >> 1) & 1, sh.abort_flag);
-    if (!ok) break;
+  const uint32_t s_addr = tmem + th.lane_off;
+  constexpr int n0 = C::stages0(false);
+  uint32_t p[64];                               // P of the current tile, fp32
+  auto prob = [&](const uint32_t* x, uint32_t* y) {
+    y[0] = __float_as_uint(ex2(fmaf(__uint_as_float(x[0]), scale_log2, -st0.x)));
+    y[1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[1]), scale_log2, -st0.x)));
+    y[2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[2]), scale_log2, -st1.x)));
+    y[3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[3]), scale_log2, -st1.x)));
+  };
+  auto valid_of = [&](int j) { return *reinterpret_cast<const volatile int*>(sh.smem + C::kValidOff + 4 * (j % n0)); };
+  auto wait_s = [&](int j) {
+    return mbar_wait(sh.bar(C::kBarAux + j % n0), (j / n0) & 1, sh.abort_flag) &&
+           mbar_wait(sh.bar(C::kBarS), j & 1, sh.abort_flag);
+  };
+  // dS of tile j over its dP, 32 keys at a time (the next 32 keys' loads in flight); kNext: P of tile j + 1 from its S
+  // in the same sweep; kMask: a tile whose last keys are past the range, which add nothing whatever their rows held
+  auto step = [&](int j, int valid, auto next, auto mask) {
+    constexpr bool kNext = decltype(next)::value, kMask = decltype(mask)::value;
+    const uint32_t dp_addr = tmem + C::kColDp + 128 * (j & 1) + th.lane_off;
+    uint32_t d[2][16], s[64];
+    if (kNext) {
+      tmem_ld_16x256b_x8(s_addr, s);
+      tmem_ld_16x256b_x8(s_addr + 64, s + 32);
+    }
+    tmem_ld_16x256b_x4(dp_addr, d[0]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = i & 1;
+      tmem_wait_ld();
+      if (i == 0 && kNext) {
+        tc_fence_before();
+        mbar_arrive(sh.bar(C::kBarP));          // S of tile j + 1 is in registers
+      }
+      if (i < 3) tmem_ld_16x256b_x4(dp_addr + 32 * (i + 1), d[b ^ 1]);
+      uint32_t w[8];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        uint32_t* x = p + 16 * i + 4 * r;
+        const uint32_t* g = d[b] + 4 * r;
+        float a0 = __uint_as_float(x[0]) * (__uint_as_float(g[0]) - st0.y);
+        float a1 = __uint_as_float(x[1]) * (__uint_as_float(g[1]) - st0.y);
+        float b0 = __uint_as_float(x[2]) * (__uint_as_float(g[2]) - st1.y);
+        float b1 = __uint_as_float(x[3]) * (__uint_as_float(g[3]) - st1.y);
+        if (kMask) {
+          const int col = 32 * i + 8 * r + 2 * th.cq;
+          a0 = col < valid ? a0 : 0.f;
+          b0 = col < valid ? b0 : 0.f;
+          a1 = col + 1 < valid ? a1 : 0.f;
+          b1 = col + 1 < valid ? b1 : 0.f;
+        }
+        w[2 * r] = pack_bf16x2(a0, a1);
+        w[2 * r + 1] = pack_bf16x2(b0, b1);
+        if (kNext) prob(s + 16 * i + 4 * r, x);
+      }
+      // words [16 i, 16 i + 16) lie over dP columns that are in registers already
+      tmem_st_16x128b_x4(dp_addr + 16 * i, w);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(sh.bar(C::kBarDs + (j & 1)));
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  bool ok = wait_s(0);
+  int valid = 0;
+  if (ok) {
     tc_fence_after();
-    const int valid = *reinterpret_cast<const volatile int*>(sh.smem + C::kValidOff + 4 * s);
+    valid = valid_of(0);
     tmem_ld_16x256b_x8(s_addr, p);
     tmem_ld_16x256b_x8(s_addr + 64, p + 32);
     tmem_wait_ld();
+    tc_fence_before();
+    mbar_arrive(sh.bar(C::kBarP));
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      uint32_t* x = p + 4 * r;
-      x[0] = __float_as_uint(ex2(fmaf(__uint_as_float(x[0]), scale_log2, -st0.x)));
-      x[1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[1]), scale_log2, -st0.x)));
-      x[2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[2]), scale_log2, -st1.x)));
-      x[3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[3]), scale_log2, -st1.x)));
+    for (int r = 0; r < 16; ++r) prob(p + 4 * r, p + 4 * r);
+  }
+  for (int j = 0; ok && j < wi.n_tiles; ++j) {
+    const bool next = j + 1 < wi.n_tiles;
+    const int now = valid;
+    if (next) {
+      ok = wait_s(j + 1);
+      if (!ok) break;
+      valid = valid_of(j + 1);
     }
-    ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
+    ok = mbar_wait(sh.bar(C::kBarDp + (j & 1)), (j >> 1) & 1, sh.abort_flag);
     if (!ok) break;
     tc_fence_after();
     if (wi.whole) {
       // all keys of these queries are here: delta = sum_j P dP - dL, a quad of threads per row
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t d[32];
-        tmem_ld_16x256b_x8(dp_addr + 64 * h, d);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t d[16];
+        tmem_ld_16x256b_x4(tmem + C::kColDp + th.lane_off + 32 * i, d);
         tmem_wait_ld();
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (64 * h + 8 * r + 2 * th.cq + e < valid) {
-              s0 = fmaf(__uint_as_float(p[4 * (8 * h + r) + e]), __uint_as_float(d[4 * r + e]), s0);
-              s1 = fmaf(__uint_as_float(p[4 * (8 * h + r) + 2 + e]), __uint_as_float(d[4 * r + 2 + e]), s1);
+            if (32 * i + 8 * r + 2 * th.cq + e < now) {
+              s0 = fmaf(__uint_as_float(p[16 * i + 4 * r + e]), __uint_as_float(d[4 * r + e]), s0);
+              s1 = fmaf(__uint_as_float(p[16 * i + 4 * r + 2 + e]), __uint_as_float(d[4 * r + 2 + e]), s1);
             }
       }
 #pragma unroll
@@ -541,38 +663,13 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
       st0.y = s0 - (dl != nullptr && th.row < wi.rows ? __ldg(dl) : 0.f);
       st1.y = s1 - (dl != nullptr && th.row + 8 < wi.rows ? __ldg(dl + 8) : 0.f);
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t d[32], w[16];
-      tmem_ld_16x256b_x8(dp_addr + 64 * h, d);
-      tmem_wait_ld();
-      if (h == 1) {
-        tc_fence_before();
-        mbar_arrive(sh.bar(C::kBarP));
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const uint32_t* x = p + 4 * (8 * h + r);
-        float a0 = __uint_as_float(x[0]) * (__uint_as_float(d[4 * r + 0]) - st0.y);
-        float a1 = __uint_as_float(x[1]) * (__uint_as_float(d[4 * r + 1]) - st0.y);
-        float b0 = __uint_as_float(x[2]) * (__uint_as_float(d[4 * r + 2]) - st1.y);
-        float b1 = __uint_as_float(x[3]) * (__uint_as_float(d[4 * r + 3]) - st1.y);
-        if (valid < 128) {
-          // keys past the range: whatever their rows held, they add nothing
-          const int col = 64 * h + 8 * r + 2 * th.cq;
-          a0 = col < valid ? a0 : 0.f;
-          b0 = col < valid ? b0 : 0.f;
-          a1 = col + 1 < valid ? a1 : 0.f;
-          b1 = col + 1 < valid ? b1 : 0.f;
-        }
-        w[2 * r] = pack_bf16x2(a0, a1);
-        w[2 * r + 1] = pack_bf16x2(b0, b1);
-      }
-      tmem_st_16x128b_x8(s_addr + 32 * h, w);
+    if (next) {
+      if (now < 128) step(j, now, Yes{}, Yes{});
+      else step(j, now, Yes{}, No{});
+    } else {
+      if (now < 128) step(j, now, No{}, Yes{});
+      else step(j, now, No{}, No{});
     }
-    tmem_wait_st();
-    tc_fence_before();
-    mbar_arrive(sh.bar(C::kBarDs));
   }
   if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
   if (!ok) {
@@ -610,17 +707,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(sh.bar(C::kBarR), 1);
-    for (int s = 0; s < C::kStages; ++s) {
+    for (int s = 0; s < C::kMaxStages; ++s) {
       mbar_init(sh.bar(C::kBarT0 + s), 1);
       mbar_init(sh.bar(C::kBarT1 + s), 1);
       mbar_init(sh.bar(C::kBarAux + s), kAuxThreads);
-      mbar_init(sh.bar(C::kBarE + s), 1);
+      mbar_init(sh.bar(C::kBarE0 + s), 1);
+      mbar_init(sh.bar(C::kBarE1 + s), 1);
     }
     mbar_init(sh.bar(C::kBarS), 1);
-    mbar_init(sh.bar(C::kBarS + 1), 1);
-    mbar_init(sh.bar(C::kBarDp), 1);
-    mbar_init(sh.bar(C::kBarP), 256);
-    mbar_init(sh.bar(C::kBarDs), 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sh.bar(C::kBarDp + i), 1);
+      mbar_init(sh.bar(C::kBarP + i), 256);
+      mbar_init(sh.bar(C::kBarDs + i), 256);
+    }
     mbar_init(sh.bar(C::kBarDone), 1);
     mbar_init(sh.bar(C::kBarDrain), 1);
     *sh.abort_flag = 0;
