@@ -124,6 +124,7 @@ ORL_API int orl_attn_fwd_noalloc(const void* q, const void* k, const void* v, vo
 
 #define ORL_ATTN_BWD_KV 0 /* the item's rows are key rows, its ranges the query rows that read them */
 #define ORL_ATTN_BWD_Q 1  /* the item's rows are query rows, its ranges the key rows they read */
+#define ORL_ATTN_BWD_WHOLE 64 /* segments of at most so many keys take delta from their one tile (field whole) */
 
 /* One backward work item: up to 128 rows of one head. */
 typedef struct orl_attn_bwd_work {
@@ -133,7 +134,7 @@ typedef struct orl_attn_bwd_work {
   int32_t kind;     /* ORL_ATTN_BWD_KV or ORL_ATTN_BWD_Q */
   int32_t range0;   /* first of its ranges */
   int32_t n_ranges; /* 0: the rows' gradients are zero */
-  int32_t n_tiles;  /* 128-row tiles of its ranges */
+  int32_t n_tiles;  /* tiles of its ranges: 128 query rows (kind KV) or 64 key rows (kind Q) */
   int32_t whole;    /* 1: its tiles hold all keys of their queries, so delta is summed from them in fp32 */
 } orl_attn_bwd_work;
 

@@ -18,17 +18,21 @@
 // there - other segments, or NaN in rows no segment owns - enters no product), warps 4-11 hold P and dS: a warp owns 16
 // TMEM lanes, a thread two rows and 32 of their 128 columns each. P and dS go back to TMEM as bf16 and are the A
 // operand of the accumulating MMAs.
-// TMEM columns, kDkv: S^T / P^T [0,128), dP^T / dS^T [128,256), dV [256,256+D), dK [256+D,256+2D) - all 512 at D = 128.
-// While the compute warps work on P(j) the tensor pipe runs dK(j-1) and dP(j); while they work on dS(j), dV(j) and
-// S(j+1). P is handed over in two halves, so dV begins under the second half's exponentials.
-// kDq: S [0,128), dP / dS [128,256) and [256,384) by turns, dQ [384,384+D). One step of the compute warps takes dS(j) from
-// dP(j) and the P(j) in their registers, and P(j+1) from S(j+1): the exponentials (MUFU) of one tile run beside the
-// arithmetic of the other, and S(j+2), dP(j+1) and dQ(j-1) are computed under them.
+//
+// kDkv, tiles of 128 queries. TMEM columns: S^T / P^T [0,128), dP^T / dS^T [128,256), dV [256,256+D), dK [256+D,256+2D):
+// all 512 at D = 128. While the compute warps work on P(j) the tensor pipe runs dK(j-1) and dP(j); while they work on
+// dS(j), dV(j) and S(j+1). P is handed over in two halves, so dV begins under the second half's exponentials.
+// kDq, tiles of 64 keys. TMEM columns: S [0,64), dP [64,192) and dS [192,256) two each by turns, dQ [256,256+D), q
+// [384,..) and dO [448,..) as bf16 A operands: with q and dO out of shared memory a 64-column MMA takes 32 clocks instead
+// of the 48 that reading both operands costs, and the keys' ring has six stages. One step of the compute warps takes
+// dS(u) from dP(u) and the P(u) in their registers, and P(u+1) from S(u+1); S(u+2), dP(u+2) and dQ(u-1) are computed
+// under it. (With 128-key tiles and three key stages, all that fits beside q and dO, a step waited for its keys: 2700
+// clocks per 128 keys.)
 //
 // delta from the forward's bf16 o carries o's rounding. Over many keys that is lost in the rounding of dS, but over a few
 // keys dS is a small difference of large terms (two keys: dq 0.0040 off in the 2-norm instead of 0.0024; 32 keys and
-// more: the same). Where a tile holds all keys of its queries, delta = sum_j P dP - dL is therefore taken from the
-// tile itself in fp32.
+// more: the same). Where a tile holds all keys of its queries (at most 64), delta = sum_j P dP - dL is therefore taken
+// from the tile itself in fp32.
 //
 // Every mbarrier wait is bounded as in the forward: a stuck pipeline sets the error word and winds down.
 #include <cuda.h>
@@ -38,6 +42,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <mutex>
+#include <initializer_list>
 #include <new>
 #include <type_traits>
 #include <vector>
@@ -53,51 +58,71 @@ static_assert(sizeof(BwdWork) == 32, "backward work item layout");
 constexpr int kDkv = ORL_ATTN_BWD_KV, kDq = ORL_ATTN_BWD_Q;
 constexpr float kLog2e = 1.4426950408889634f;
 
+constexpr int kDkvRows = 128, kDqRows = 64;             // rows of a streamed tile
+constexpr int kWholeKeys = ORL_ATTN_BWD_WHOLE;          // segments of so few keys take delta from their tile
+static_assert(kWholeKeys <= kDqRows, "a whole segment is one tile");
+
 template <int D>
 struct BwdCfg {
   static constexpr int kChunks = D / 64;              // 128-byte swizzle columns per row
   static constexpr int kTileBytes = 128 * D * 2;      // one 128-row bf16 tile
   static constexpr int kChunkBytes = 128 * 128;       // one 128-row x 64-column chunk
-  // Resident tiles R0, R1 (K, V or q, dO); rings of streamed tiles T0 (q or K) and T1 (dO or V). kDq has S of tile
-  // j + 2 issued before dQ of tile j, so K needs three stages; at D = 128 that is all the shared memory there is.
-  __host__ __device__ static constexpr int stages0(bool dkv) { return D == 64 ? 4 : dkv ? 2 : 3; }
+  // kDkv: resident tiles K, V; rings of streamed tiles T1 = dO and T0 = q (S of tile j + 1 is issued before dK of tile
+  // j, so q is loaded two tiles ahead of its release). The last stage of T0 holds column sums in whole items.
+  static constexpr int kStages0 = D == 64 ? 4 : 3;
   static constexpr int kStages1 = D == 64 ? 4 : 2;
-  static constexpr int kMaxStages = 4;
   static constexpr int kROff = 0;
   static constexpr int kT1Off = 2 * kTileBytes;
   static constexpr int kT0Off = kT1Off + kStages1 * kTileBytes;
-  // kDkv: (lse2, delta) of the 128 streamed rows per stage, and column sums per warp (both after its last T0 stage)
+  static constexpr int kRedOff = kT0Off + (kStages0 - 1) * kTileBytes;
+  static constexpr int kStatOff = kT0Off + kStages0 * kTileBytes;
   static constexpr int kStatBytes = 2 * 4 * 36 * 4;   // lse2, delta: four groups of 32 columns, padded (see stat_at)
-  static constexpr int kStatOff = kT0Off + stages0(true) * kTileBytes;
-  static constexpr int kRedOff = kStatOff + kMaxStages * kStatBytes;
-  static constexpr int kDkvEnd = kRedOff + 8 * 128 * 4;
-  static constexpr int kDqEnd = kT0Off + stages0(false) * kTileBytes;
-  static constexpr int kValidOff = kDkvEnd > kDqEnd ? kDkvEnd : kDqEnd;   // int per stage: rows inside the range
-  static constexpr int kBarOff = kValidOff + 16;
-  static constexpr int kBarR = 0;                       // resident tiles landed
-  static constexpr int kBarT0 = 1;                      // streamed tiles landed, per stage
+  // kDq: a ring of pairs of 64-row tiles K, V
+  static constexpr int kHalfBytes = kTileBytes / 2;
+  static constexpr int kHalfChunk = kChunkBytes / 2;
+  static constexpr int kPairStages = D == 64 ? 8 : 6;
+  static constexpr int kMaxStages = 8;
+  static constexpr int kValidOff = kStatOff + 2 * kStatBytes;   // kDq, int per stage: keys inside the range
+  static constexpr int kBarOff = kValidOff + 4 * kMaxStages;
+  static constexpr int kBarR = 0;                       // kDkv: resident tiles landed
+  static constexpr int kBarQ = 1;                       // kDq: q and dO in TMEM
+  static constexpr int kBarT0 = 2;                      // streamed tiles landed, per stage (kDq: the pair)
   static constexpr int kBarT1 = kBarT0 + kMaxStages;
-  static constexpr int kBarAux = kBarT1 + kMaxStages;   // statistics and zeroed rows ready, per T0 stage
+  static constexpr int kBarAux = kBarT1 + kStages1;     // streamed tiles landed and prepared, per T0 stage
   static constexpr int kBarE0 = kBarAux + kMaxStages;   // stage free
   static constexpr int kBarE1 = kBarE0 + kMaxStages;
-  static constexpr int kBarS = kBarE1 + kMaxStages;     // S computed
+  static constexpr int kBarS = kBarE1 + kStages1;       // S computed
   static constexpr int kBarDp = kBarS + 1;              // dP computed (kDq: two buffers)
-  static constexpr int kBarP = kBarDp + 2;              // kDkv: half of P stored (two); kDq: S read
-  // dS stored. kDq: two by turns, since dS(j + 1) may be complete before the issuing thread has seen dS(j)
+  static constexpr int kBarP = kBarDp + 2;              // kDkv: half of P stored (two); kDq: S(u + 1) and dP(u) read
+  // dS stored. kDq: two by turns, since dS(u + 1) may be complete before the issuing thread has seen dS(u)
   static constexpr int kBarDs = kBarP + 2;
   static constexpr int kBarDone = kBarDs + 2;
   static constexpr int kBarDrain = kBarDone + 1;
   static constexpr int kNumBars = kBarDrain + 1;
-  static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
+  static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColDv = 256, kColDk = 256 + D;       // kDkv (S at 0, dP at 128)
-  static constexpr uint32_t kColDp = 128, kColDq = 384;           // kDq (S at 0; dP at 128 and 256)
+  static constexpr uint32_t kColDp = 64, kColDs = 192, kColDq = 256, kColQ = 384, kColDo = 448;   // kDq (S at 0)
+  static_assert(kPairStages * 2 * kHalfBytes <= kStatOff && kPairStages <= kMaxStages && kStages0 <= kMaxStages, "rings");
+  static_assert(kStatOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
 // Where the statistic of streamed row c lies: a thread of the compute warps needs columns 8r + 2 cq + {0, 1}, here 32
 // consecutive floats of group cq (eight 16-byte loads); groups 36 floats apart fall into different banks.
 __device__ __forceinline__ int stat_at(int c) { return 36 * ((c >> 1) & 3) + 2 * (c >> 3) + (c & 1); }
+
+// position in a ring of n stages: stage s, parity ph of its current use
+struct Ring {
+  int n, s = 0, ph = 0;
+  __device__ explicit Ring(int n_) : n(n_) {}
+  __device__ void next() {
+    if (++s == n) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+};
 
 constexpr int kBwdThreads = 384;
 constexpr int kAuxThreads = 64;
@@ -123,7 +148,8 @@ struct BwdShared {
   __device__ uint32_t bar(int i) const { return bar0 + 8u * i; }
 };
 
-// the tiles of an item's ranges in order: each range cut into 128-row tiles, the last one of a range shorter
+// the tiles of an item's ranges in order: each range cut into tiles of kRows rows, the last one of a range shorter
+template <int kRows>
 struct TileWalk {
   const int2* ranges;
   int left;              // ranges not yet begun
@@ -139,50 +165,56 @@ struct TileWalk {
       rest = r.y;
     }
     first = row;
-    const int n = min(128, rest);
-    row += 128;
-    rest -= 128;
+    const int n = min(kRows, rest);
+    row += kRows;
+    rest -= kRows;
     return n;
   }
 };
 
 // ---------------------------------------------------------------------------------------------- TMA producer
+// rows [y, y + 64 boxes) of head columns x0.. into a tile of that many 64-row boxes
+template <int D, int kBoxes>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x0, int y,
+                                          uint64_t pol) {
+  constexpr int kBox = 64 * 128;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b)
+      tma_load_2d(dst + (c * kBoxes + b) * kBox, map, bar, x0 + 64 * c, y + 64 * b, pol);
+}
+
 template <int D>
-__device__ __forceinline__ void bwd_producer(const BwdShared& sh, const CUtensorMap* r0, const CUtensorMap* r1,
-                                             const CUtensorMap* t0, const CUtensorMap* t1, const BwdWork& wi,
-                                             const int2* ranges, int* err) {
+__device__ __forceinline__ void bwd_produce_dkv(const BwdShared& sh, const CUtensorMap* tm_q, const CUtensorMap* tm_k,
+                                                const CUtensorMap* tm_v, const CUtensorMap* tm_do, const BwdWork& wi,
+                                                const int2* ranges, int* err) {
   using C = BwdCfg<D>;
-  const uint64_t pol_r = policy_evict_first();
-  const uint64_t pol_t = policy_evict_last();
+  const uint64_t pol_r = policy_evict_first(), pol_t = policy_evict_last();
   const int x0 = wi.head * D;
   mbar_expect_tx(sh.bar(C::kBarR), 2 * C::kTileBytes);
-  for (int c = 0; c < C::kChunks; ++c) {
-    tma_load_2d(sh.sbase + C::kROff + c * C::kChunkBytes, r0, sh.bar(C::kBarR), x0 + 64 * c, wi.row0, pol_r);
-    tma_load_2d(sh.sbase + C::kROff + C::kTileBytes + c * C::kChunkBytes, r1, sh.bar(C::kBarR), x0 + 64 * c, wi.row0,
-                pol_r);
-  }
-  const int n0 = C::stages0(wi.kind == kDkv);
-  auto stream = [&](int j, int y, int stages, int off, int bar_full, int bar_empty, const CUtensorMap* map) {
-    const int s = j % stages;
-    if (j >= stages && !mbar_wait(sh.bar(bar_empty + s), ((j / stages) - 1) & 1, sh.abort_flag)) return false;
-    mbar_expect_tx(sh.bar(bar_full + s), C::kTileBytes);
-    for (int c = 0; c < C::kChunks; ++c)
-      tma_load_2d(sh.sbase + off + s * C::kTileBytes + c * C::kChunkBytes, map, sh.bar(bar_full + s), x0 + 64 * c, y,
-                  pol_t);
-    return true;
-  };
-  TileWalk walk(ranges, wi.n_ranges);
+  load_tile<D, 2>(sh.sbase + C::kROff, tm_k, sh.bar(C::kBarR), x0, wi.row0, pol_r);
+  load_tile<D, 2>(sh.sbase + C::kROff + C::kTileBytes, tm_v, sh.bar(C::kBarR), x0, wi.row0, pol_r);
+  TileWalk<kDkvRows> walk(ranges, wi.n_ranges);
+  const int n0 = C::kStages0 - wi.whole;
+  Ring a(n0), b(C::kStages1);
   int issued0 = 0, issued1 = 0;
-  for (int j = 0; j < wi.n_tiles; ++j) {
+  for (int j = 0; j < wi.n_tiles; ++j, a.next(), b.next()) {
     int y = 0;
     walk.next(y);
-    bool ok = stream(j, y, n0, C::kT0Off, C::kBarT0, C::kBarE0, t0);
-    if (ok) issued0 = j + 1;
-    ok = ok && stream(j, y, C::kStages1, C::kT1Off, C::kBarT1, C::kBarE1, t1);
+    bool ok = j < n0 || mbar_wait(sh.bar(C::kBarE0 + a.s), a.ph ^ 1, sh.abort_flag);
+    if (ok) {
+      mbar_expect_tx(sh.bar(C::kBarT0 + a.s), C::kTileBytes);
+      load_tile<D, 2>(sh.sbase + C::kT0Off + a.s * C::kTileBytes, tm_q, sh.bar(C::kBarT0 + a.s), x0, y, pol_t);
+      issued0 = j + 1;
+      ok = j < C::kStages1 || mbar_wait(sh.bar(C::kBarE1 + b.s), b.ph ^ 1, sh.abort_flag);
+    }
     if (!ok) {
       atomicOr(err, kErrTimeoutLoad);
       break;
     }
+    mbar_expect_tx(sh.bar(C::kBarT1 + b.s), C::kTileBytes);
+    load_tile<D, 2>(sh.sbase + C::kT1Off + b.s * C::kTileBytes, tm_do, sh.bar(C::kBarT1 + b.s), x0, y, pol_t);
     issued1 = j + 1;
   }
   if (*sh.abort_flag) {
@@ -195,16 +227,42 @@ __device__ __forceinline__ void bwd_producer(const BwdShared& sh, const CUtensor
   }
 }
 
-// ---------------------------------------------------------------------------------------------- tile preparation
-// 64 threads (t = 0..63). Per streamed tile: the number of its rows inside the range; in kDkv the statistics of its
-// query rows (lse2 = +inf past the end, so P = 0 there); zeros over the shared-memory rows past the end. In kDq only
-// T0 (K) needs them: the columns of S and dP past the end are masked, but dS K sums over K's rows.
 template <int D>
-__device__ __forceinline__ void bwd_aux(const BwdShared& sh, const BwdWork& wi, const int2* ranges,
-                                        const float2* __restrict__ stats, const float* __restrict__ dlse, long long nq,
-                                        int t, int* err) {
+__device__ __forceinline__ void bwd_produce_dq(const BwdShared& sh, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
+                                               const BwdWork& wi, const int2* ranges, int* err) {
   using C = BwdCfg<D>;
-  const bool dkv = wi.kind == kDkv;
+  const uint64_t pol = policy_evict_last();
+  const int x0 = wi.head * D;
+  TileWalk<kDqRows> walk(ranges, wi.n_ranges);
+  Ring a(C::kPairStages);
+  int issued = 0;
+  for (int u = 0; u < wi.n_tiles; ++u, a.next()) {
+    int y = 0;
+    walk.next(y);
+    if (u >= C::kPairStages && !mbar_wait(sh.bar(C::kBarE0 + a.s), a.ph ^ 1, sh.abort_flag)) {
+      atomicOr(err, kErrTimeoutLoad);
+      break;
+    }
+    const uint32_t dst = sh.sbase + a.s * 2 * C::kHalfBytes, bar = sh.bar(C::kBarT0 + a.s);
+    mbar_expect_tx(bar, 2 * C::kHalfBytes);
+    load_tile<D, 1>(dst, tm_k, bar, x0, y, pol);
+    load_tile<D, 1>(dst + C::kHalfBytes, tm_v, bar, x0, y, pol);
+    issued = u + 1;
+  }
+  if (*sh.abort_flag)
+    for (int u = issued > C::kPairStages ? issued - C::kPairStages : 0; u < issued; ++u)
+      bwd_drain_wait(sh.bar(C::kBarT0 + u % C::kPairStages), (u / C::kPairStages) & 1, err);
+}
+
+// ---------------------------------------------------------------------------------------------- tile preparation
+// 64 threads (t = 0..63) wait for each streamed tile and hand it on prepared, so that the issuing thread has one wait
+// for it. kDkv: the statistics of its query rows (lse2 = +inf past the end, so P = 0 there) into one of two slots, zeros
+// over the shared-memory rows past the end.
+template <int D>
+__device__ __forceinline__ void bwd_prepare_dkv(const BwdShared& sh, const BwdWork& wi, const int2* ranges,
+                                                const float2* __restrict__ stats, const float* __restrict__ dlse,
+                                                long long nq, int t, int* err) {
+  using C = BwdCfg<D>;
   const float2* st = stats + static_cast<long long>(wi.head) * nq;
   const float* dl = dlse == nullptr ? nullptr : dlse + static_cast<long long>(wi.head) * nq;
   // (lse2, delta) of a query row; where the tile gives sum_j P dP itself, its other term -dL
@@ -213,158 +271,214 @@ __device__ __forceinline__ void bwd_aux(const BwdShared& sh, const BwdWork& wi, 
     if (wi.whole) x.y = dl == nullptr ? 0.f : -__ldg(dl + row);
     return x;
   };
-  const int n0 = C::stages0(dkv);
-  TileWalk walk(ranges, wi.n_ranges);
-  for (int j = 0; j < wi.n_tiles; ++j) {
-    const int s = j % n0, s1 = j % C::kStages1;
+  TileWalk<kDkvRows> walk(ranges, wi.n_ranges);
+  const int n0 = C::kStages0 - wi.whole;
+  Ring a(n0), b(C::kStages1), free(n0);                  // free: two tiles behind, whose dK released the slot
+  for (int j = 0; j < wi.n_tiles; ++j, a.next(), b.next()) {
     int row = 0;
     const int valid = walk.next(row);
-    float2 a = make_float2(INFINITY, 0.f), b = a;
-    if (dkv) {
-      if (t < valid) a = row_stats(row + t);
-      if (t + 64 < valid) b = row_stats(row + t + 64);
-    }
+    float2 x = make_float2(INFINITY, 0.f), y = x;
+    if (t < valid) x = row_stats(row + t);
+    if (t + 64 < valid) y = row_stats(row + t + 64);
     bool ok = true;
-    if (j >= n0) ok = mbar_wait(sh.bar(C::kBarE0 + s), ((j / n0) - 1) & 1, sh.abort_flag);
-    if (ok && valid < 128) {
-      ok = mbar_wait(sh.bar(C::kBarT0 + s), (j / n0) & 1, sh.abort_flag);
-      if (ok && dkv) ok = mbar_wait(sh.bar(C::kBarT1 + s1), (j / C::kStages1) & 1, sh.abort_flag);
+    if (j >= 2) {
+      ok = mbar_wait(sh.bar(C::kBarE0 + free.s), free.ph, sh.abort_flag);
+      free.next();
     }
+    ok = ok && mbar_wait(sh.bar(C::kBarT0 + a.s), a.ph, sh.abort_flag) &&
+         mbar_wait(sh.bar(C::kBarT1 + b.s), b.ph, sh.abort_flag);
     if (!ok) {
       if (t == 0) atomicOr(err, kErrTimeoutLoad);
       return;
     }
-    if (dkv) {
-      float* dst = reinterpret_cast<float*>(sh.smem + C::kStatOff + s * C::kStatBytes);
-      dst[stat_at(t)] = a.x;
-      dst[stat_at(t + 64)] = b.x;
-      dst[144 + stat_at(t)] = a.y;
-      dst[144 + stat_at(t + 64)] = b.y;
-    }
-    if (t == 0) *reinterpret_cast<int*>(sh.smem + C::kValidOff + 4 * s) = valid;
-    if (valid < 128) {
-      for (int c = 0; c < (dkv ? 2 : 1) * C::kChunks; ++c) {    // T0's chunks, then T1's
-        uint8_t* chunk = sh.smem + (c < C::kChunks ? C::kT0Off + s * C::kTileBytes + c * C::kChunkBytes
-                                                   : C::kT1Off + s1 * C::kTileBytes + (c - C::kChunks) * C::kChunkBytes);
+    float* dst = reinterpret_cast<float*>(sh.smem + C::kStatOff + (j & 1) * C::kStatBytes);
+    dst[stat_at(t)] = x.x;
+    dst[stat_at(t + 64)] = y.x;
+    dst[144 + stat_at(t)] = x.y;
+    dst[144 + stat_at(t + 64)] = y.y;
+    if (valid < kDkvRows) {
+      for (int c = 0; c < 2 * C::kChunks; ++c) {         // T0's chunks, then T1's
+        uint8_t* chunk = sh.smem + (c < C::kChunks ? C::kT0Off + a.s * C::kTileBytes + c * C::kChunkBytes
+                                                   : C::kT1Off + b.s * C::kTileBytes + (c - C::kChunks) * C::kChunkBytes);
         for (int o = valid * 128 + t * 16; o < C::kChunkBytes; o += kAuxThreads * 16)
           *reinterpret_cast<uint4*>(chunk + o) = make_uint4(0u, 0u, 0u, 0u);
       }
       fence_async_smem();
     }
-    mbar_arrive(sh.bar(C::kBarAux + s));
+    mbar_arrive(sh.bar(C::kBarAux + a.s));
+  }
+}
+
+// kDq: the number of keys inside the range, zeros over K's rows past it (the columns of S and dP past the end are masked,
+// but dS K sums over K's rows)
+template <int D>
+__device__ __forceinline__ void bwd_prepare_dq(const BwdShared& sh, const BwdWork& wi, const int2* ranges, int t,
+                                               int* err) {
+  using C = BwdCfg<D>;
+  TileWalk<kDqRows> walk(ranges, wi.n_ranges);
+  Ring a(C::kPairStages);
+  for (int u = 0; u < wi.n_tiles; ++u, a.next()) {
+    int row = 0;
+    const int valid = walk.next(row);
+    if (!mbar_wait(sh.bar(C::kBarT0 + a.s), a.ph, sh.abort_flag)) {
+      if (t == 0) atomicOr(err, kErrTimeoutLoad);
+      return;
+    }
+    if (t == 0) *reinterpret_cast<int*>(sh.smem + C::kValidOff + 4 * a.s) = valid;
+    if (valid < kDqRows) {
+      uint8_t* k = sh.smem + a.s * 2 * C::kHalfBytes;
+      for (int c = 0; c < C::kChunks; ++c)
+        for (int o = valid * 128 + t * 16; o < C::kHalfChunk; o += kAuxThreads * 16)
+          *reinterpret_cast<uint4*>(k + c * C::kHalfChunk + o) = make_uint4(0u, 0u, 0u, 0u);
+      fence_async_smem();
+    }
+    mbar_arrive(sh.bar(C::kBarAux + a.s));
   }
 }
 
 // ---------------------------------------------------------------------------------------------- MMA issuer
+// Descriptors are built once per tile and stepped by a constant: building one per MMA costs the issuing thread more
+// (67 clocks measured per MMA) than the MMA takes (64 clocks at N = 128), stepping them 20. A wait costs it about 80
+// clocks even when there is nothing to wait for, so waits for tiles stand before those for the compute warps.
+
+__device__ __forceinline__ void bwd_mma_end(const BwdShared& sh, bool ok, int bar_done, int bar_drain, int* err) {
+  if (ok) {
+    mma_commit(sh.bar(bar_done));
+  } else {
+    atomicOr(err, kErrTimeoutMma);
+    mma_commit(sh.bar(bar_drain));
+    bwd_drain_wait(sh.bar(bar_drain), 0, err);
+  }
+}
+
 template <int D>
-struct BwdMma {
+__device__ __forceinline__ void bwd_mma_dkv(const BwdShared& sh, uint32_t tmem, const BwdWork& wi, int* err) {
   using C = BwdCfg<D>;
-  static constexpr uint32_t kIdescS = idesc_bf16(128, 128, false, false);
-  static constexpr uint32_t kIdescA = idesc_bf16(128, D, false, true);
-  // Descriptors are built once per tile and stepped by a constant: building one per MMA costs the issuing thread more
-  // (67 clocks measured per MMA) than the MMA takes (64 clocks at N = 128), stepping them 20.
-  static __device__ __forceinline__ uint64_t k_major(uint32_t tile) { return smem_desc_sw128(tile, 16, 1024); }
-  static __device__ __forceinline__ uint64_t mn_major(uint32_t tile) { return smem_desc_sw128(tile, C::kChunkBytes, 1024); }
-  // D[col] = R (resident tile, K-major descriptor) * T (streamed tile, K-major)^T
-  static __device__ __forceinline__ void product(uint32_t d, uint64_t r, uint64_t t) {
+  constexpr uint32_t kIdescS = idesc_bf16(128, 128, false, false);
+  constexpr uint32_t kIdescA = idesc_bf16(128, D, false, true);
+  constexpr uint64_t kStep = C::kTileBytes >> 4;         // descriptor step from one tile to the next
+  const int n = wi.n_tiles;
+  auto wait = [&](int bar, int phase) { return mbar_wait(sh.bar(bar), phase & 1, sh.abort_flag); };
+  const uint64_t k0 = smem_desc_sw128(sh.sbase + C::kROff, 16, 1024), v0 = k0 + kStep;
+  const uint64_t q0 = smem_desc_sw128(sh.sbase + C::kT0Off, 16, 1024), o0 = smem_desc_sw128(sh.sbase + C::kT1Off, 16, 1024);
+  const uint64_t qt0 = smem_desc_sw128(sh.sbase + C::kT0Off, C::kChunkBytes, 1024);     // the same tiles MN-major
+  const uint64_t ot0 = smem_desc_sw128(sh.sbase + C::kT1Off, C::kChunkBytes, 1024);
+  // D[col] = R * T^T, both K-major
+  auto product = [&](uint32_t d, uint64_t r, uint64_t t) {
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       const uint64_t off = ((kk >> 2) * C::kChunkBytes + (kk & 3) * 32) >> 4;
       mma_ss(d, r + off, t + off, kIdescS, kk > 0 ? 1u : 0u);
     }
-  }
-  // D[col] (+)= A (bf16 in TMEM, 128 x 128) * T (streamed tile, MN-major), A's columns [16 kLo, 16 kHi)
-  template <int kLo, int kHi>
-  static __device__ __forceinline__ void accumulate(uint32_t d, uint32_t a, uint64_t t, bool acc) {
+  };
+  // D[col] (+)= A * T, A bf16 in TMEM, T MN-major; 16-row steps [lo, hi) of the contraction
+  auto accumulate = [&](uint32_t d, uint32_t a, uint64_t t, int lo, int hi, bool acc) {
 #pragma unroll
-    for (int kk = kLo; kk < kHi; ++kk)
-      mma_ts(d, a + kk * 8, t + ((kk * 2048) >> 4), kIdescA, (acc || kk > 0) ? 1u : 0u);
+    for (int kk = 0; kk < 8; ++kk)
+      if (kk >= lo && kk < hi) mma_ts(d, a + kk * 8, t + ((kk * 2048) >> 4), kIdescA, (acc || kk > 0) ? 1u : 0u);
+  };
+  Ring a(C::kStages0 - wi.whole), b(C::kStages1);        // tile j; nx: tile j + 1
+  Ring nx(a.n);
+  nx.next();
+  bool ok = wait(C::kBarR, 0) && wait(C::kBarAux, 0);
+  if (ok) {
+    tc_fence_after();
+    product(tmem, k0, q0);
+    mma_commit(sh.bar(C::kBarS));
   }
-};
+  for (int j = 0; ok && j < n; ++j) {
+    // dP overwrites dS of tile j - 1, whose dK MMA was issued before
+    product(tmem + 128, v0, o0 + b.s * kStep);
+    mma_commit(sh.bar(C::kBarDp));
+    ok = wait(C::kBarP, j);
+    if (!ok) break;
+    tc_fence_after();
+    accumulate(tmem + C::kColDv, tmem, ot0 + b.s * kStep, 0, 4, j > 0);
+    if (j + 1 < n) ok = wait(C::kBarAux + nx.s, nx.ph);
+    ok = ok && wait(C::kBarP + 1, j);
+    if (!ok) break;
+    tc_fence_after();
+    accumulate(tmem + C::kColDv, tmem, ot0 + b.s * kStep, 4, 8, true);
+    if (j + 1 < n) {                                     // over P of this tile, whose dV MMA was issued before
+      product(tmem, k0, q0 + nx.s * kStep);
+      mma_commit(sh.bar(C::kBarS));
+    }
+    mma_commit(sh.bar(C::kBarE1 + b.s));
+    ok = wait(C::kBarDs, j);
+    if (!ok) break;
+    tc_fence_after();
+    accumulate(tmem + C::kColDk, tmem + 128, qt0 + a.s * kStep, 0, 8, j > 0);
+    mma_commit(sh.bar(C::kBarE0 + a.s));
+    a.next();
+    b.next();
+    nx.next();
+  }
+  bwd_mma_end(sh, ok, C::kBarDone, C::kBarDrain, err);
+}
 
 template <int D>
-__device__ __forceinline__ void bwd_mma(const BwdShared& sh, uint32_t tmem, const BwdWork& wi, int* err) {
+__device__ __forceinline__ void bwd_mma_dq(const BwdShared& sh, uint32_t tmem, const BwdWork& wi, int* err) {
   using C = BwdCfg<D>;
-  using M = BwdMma<D>;
+  constexpr uint32_t kIdescS = idesc_bf16(128, 64, false, false);
+  constexpr uint32_t kIdescA = idesc_bf16(128, D, false, true);
+  constexpr uint64_t kStep = (2 * C::kHalfBytes) >> 4;
   const int n = wi.n_tiles;
-  const bool dkv = wi.kind == kDkv;
-  const int n0 = C::stages0(dkv);
-  const uint64_t r0 = M::k_major(sh.sbase + C::kROff), r1 = M::k_major(sh.sbase + C::kROff + C::kTileBytes);
   auto wait = [&](int bar, int phase) { return mbar_wait(sh.bar(bar), phase & 1, sh.abort_flag); };
-  auto tile0 = [&](int j) { return sh.sbase + C::kT0Off + (j % n0) * C::kTileBytes; };
-  auto tile1 = [&](int j) { return sh.sbase + C::kT1Off + (j % C::kStages1) * C::kTileBytes; };
-  // The tiles a product needs are waited for well before its operand from the compute warps is: a wait costs about 90
-  // clocks even when the tile is there, and behind P or dS it would be on the critical path.
-  auto ready0 = [&](int j) {                           // T0 of tile j, prepared
-    const int s = j % n0, ph = j / n0;
-    return wait(C::kBarT0 + s, ph) && wait(C::kBarAux + s, ph);
+  const uint64_t k0 = smem_desc_sw128(sh.sbase, 16, 1024), v0 = k0 + (C::kHalfBytes >> 4);
+  const uint64_t kt0 = smem_desc_sw128(sh.sbase, C::kHalfChunk, 1024);                  // K MN-major
+  // D[col] = A * T^T: A = q or dO in TMEM, T K-major
+  auto product = [&](uint32_t d, uint32_t a, uint64_t t) {
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+      mma_ts(d, a + kk * 8, t + (((kk >> 2) * C::kHalfChunk + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
   };
-  auto ready1 = [&](int j) { return wait(C::kBarT1 + j % C::kStages1, j / C::kStages1); };
-  auto issue_s = [&](int j) {
-    M::product(tmem, r0, M::k_major(tile0(j)));
+  Ring a(C::kPairStages), nx(C::kPairStages);            // tile u; the next tile whose S and dP are to be issued
+  // S over that of tile x - 1, which has been read; dP over that of tile x - 2, likewise
+  auto issue = [&](int x) {
+    product(tmem, tmem + C::kColQ, k0 + nx.s * kStep);
     mma_commit(sh.bar(C::kBarS));
+    product(tmem + C::kColDp + 64 * (x & 1), tmem + C::kColDo, v0 + nx.s * kStep);
+    mma_commit(sh.bar(C::kBarDp + (x & 1)));
+    nx.next();
   };
-  bool ok = wait(C::kBarR, 0) && ready0(0) && ready1(0);
-  if (ok) issue_s(0);
-  if (dkv) {
-    for (int j = 0; ok && j < n; ++j) {
-      // dP overwrites dS of tile j - 1, whose dK MMA was issued before
-      M::product(tmem + 128, r1, M::k_major(tile1(j)));
-      mma_commit(sh.bar(C::kBarDp));
-      ok = wait(C::kBarP, j);
-      if (!ok) break;
-      tc_fence_after();
-      M::template accumulate<0, 4>(tmem + C::kColDv, tmem, M::mn_major(tile1(j)), j > 0);
-      if (j + 1 < n) ok = ready0(j + 1);
-      ok = ok && wait(C::kBarP + 1, j);
-      if (!ok) break;
-      tc_fence_after();
-      M::template accumulate<4, 8>(tmem + C::kColDv, tmem, M::mn_major(tile1(j)), true);
-      if (j + 1 < n) issue_s(j + 1);                   // over P of this tile, whose dV MMA was issued before
-      mma_commit(sh.bar(C::kBarE1 + j % C::kStages1));
-      if (j + 1 < n) ok = ready1(j + 1);
-      ok = ok && wait(C::kBarDs, j);
-      if (!ok) break;
-      tc_fence_after();
-      M::template accumulate<0, 8>(tmem + C::kColDk, tmem + 128, M::mn_major(tile0(j)), j > 0);
-      mma_commit(sh.bar(C::kBarE0 + j % n0));
-    }
-  } else {
-    // dP of tile j into its buffer, over dS of tile j - 2, whose dQ MMA was issued before
-    auto issue_dp = [&](int j) {
-      M::product(tmem + C::kColDp + 128 * (j & 1), r1, M::k_major(tile1(j)));
-      mma_commit(sh.bar(C::kBarDp + (j & 1)));
-      mma_commit(sh.bar(C::kBarE1 + j % C::kStages1));
-    };
-    if (ok) issue_dp(0);
-    if (ok && n > 1) ok = ready0(1) && wait(C::kBarP, 0) && ready1(1);          // S of tile 0 read
-    if (ok && n > 1) issue_s(1);
-    for (int j = 0; ok && j < n; ++j) {
-      if (j + 1 < n) issue_dp(j + 1);
-      if (j + 2 < n) {
-        ok = ready0(j + 2) && wait(C::kBarP, j + 1);
-        if (!ok) break;
-        tc_fence_after();
-        issue_s(j + 2);
-        ok = ready1(j + 2);
-      }
-      ok = ok && wait(C::kBarDs + (j & 1), j >> 1);
-      if (!ok) break;
-      tc_fence_after();
-      M::template accumulate<0, 8>(tmem + C::kColDq, tmem + C::kColDp + 128 * (j & 1), M::mn_major(tile0(j)), j > 0);
-      mma_commit(sh.bar(C::kBarE0 + j % n0));
-    }
-  }
+  bool ok = wait(C::kBarQ, 0) && wait(C::kBarAux, 0);
   if (ok) {
-    mma_commit(sh.bar(C::kBarDone));
-  } else {
-    atomicOr(err, kErrTimeoutMma);
-    mma_commit(sh.bar(C::kBarDrain));
-    bwd_drain_wait(sh.bar(C::kBarDrain), 0, err);
+    tc_fence_after();
+    issue(0);
+    if (n > 1) ok = wait(C::kBarAux + nx.s, nx.ph) && wait(C::kBarP, 0);
   }
+  if (ok && n > 1) {
+    tc_fence_after();
+    issue(1);
+  }
+  for (int u = 0; ok && u < n; ++u) {
+    if (u + 2 < n) {
+      ok = wait(C::kBarAux + nx.s, nx.ph) && wait(C::kBarP, u + 1);
+      if (!ok) break;
+      tc_fence_after();
+      issue(u + 2);
+    }
+    ok = wait(C::kBarDs + (u & 1), u >> 1);
+    if (!ok) break;
+    tc_fence_after();
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      mma_ts(tmem + C::kColDq, tmem + C::kColDs + 32 * (u & 1) + kk * 8, kt0 + a.s * kStep + ((kk * 2048) >> 4), kIdescA,
+             (u > 0 || kk > 0) ? 1u : 0u);
+    mma_commit(sh.bar(C::kBarE0 + a.s));
+    a.next();
+  }
+  bwd_mma_end(sh, ok, C::kBarDone, C::kBarDrain, err);
 }
 
 // ---------------------------------------------------------------------------------------------- P and dS
+// after an mbarrier wait of a whole warp: its lanes leave the wait's loop one by one, and the TMEM accesses that follow
+// are warp-wide (without the __syncwarp a warp that had not come together corrupted its tiles now and then)
+__device__ __forceinline__ void tc_after_wait() {
+  __syncwarp();
+  tc_fence_after();
+}
+
 // Thread layout of the .16x256b / .16x128b TMEM shapes: warp sw owns lanes 32 (sw % 4) + 16 (sw / 4) + [0, 16); its
 // thread holds the rows lane / 4 and lane / 4 + 8 of that block, register 4r + 2i + e of a 64-column load: row i,
 // column 8r + 2 (lane % 4) + e.
@@ -414,11 +528,11 @@ __device__ __forceinline__ void bwd_zero(const BwdThread& th, const BwdWork& wi,
   }
 }
 
-// Adds sum_j P dP over the tile's key rows to the delta of each of its query columns (stage s): rows of a thread, lanes
+// Adds sum_j P dP over the tile's key rows to the delta of each of its query columns (in a slot): rows of a thread, lanes
 // of a warp by shuffles, the eight warps through shared memory.
 template <int D>
 __device__ __forceinline__ void bwd_column_delta(const BwdShared& sh, uint32_t dp_addr, const BwdThread& th, int rows,
-                                              const uint32_t (&p)[64], int s) {
+                                              const uint32_t (&p)[64], int slot) {
   using C = BwdCfg<D>;
   const int t = threadIdx.x - 128;                    // 0..255
   float* red = reinterpret_cast<float*>(sh.smem + C::kRedOff);
@@ -447,7 +561,7 @@ __device__ __forceinline__ void bwd_column_delta(const BwdShared& sh, uint32_t d
     float a = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) a += red[128 * w + t];
-    reinterpret_cast<float*>(sh.smem + C::kStatOff + s * C::kStatBytes)[144 + stat_at(t)] += a;
+    reinterpret_cast<float*>(sh.smem + C::kStatOff + slot * C::kStatBytes)[144 + stat_at(t)] += a;
   }
   asm volatile("bar.sync 1, 256;" ::: "memory");
 }
@@ -459,21 +573,20 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
   using C = BwdCfg<D>;
   const float scale_log2 = scale * kLog2e;
   const uint32_t s_addr = tmem + th.lane_off, dp_addr = s_addr + 128;
-  constexpr int n0 = C::stages0(true);
+  Ring a(C::kStages0 - wi.whole);
   bool ok = true;
   uint32_t p[64];                               // scores, then P in fp32
-  for (int j = 0; j < wi.n_tiles; ++j) {
-    const int s = j % n0;
-    ok = mbar_wait(sh.bar(C::kBarAux + s), (j / n0) & 1, sh.abort_flag);
+  for (int j = 0; j < wi.n_tiles; ++j, a.next()) {
+    ok = mbar_wait(sh.bar(C::kBarAux + a.s), a.ph, sh.abort_flag);
     if (!ok) break;
     // statistics of columns 8r + 2 cq + {0, 1}, two r per load, read before the wait for S (dP)
-    const float4* st = reinterpret_cast<const float4*>(sh.smem + C::kStatOff + s * C::kStatBytes) + 9 * th.cq;
+    const float4* st = reinterpret_cast<const float4*>(sh.smem + C::kStatOff + (j & 1) * C::kStatBytes) + 9 * th.cq;
     float4 c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = st[i];
     ok = mbar_wait(sh.bar(C::kBarS), j & 1, sh.abort_flag);
     if (!ok) break;
-    tc_fence_after();
+    tc_after_wait();
     tmem_ld_16x256b_x8(s_addr, p);
     tmem_ld_16x256b_x8(s_addr + 64, p + 32);
     tmem_wait_ld();
@@ -503,8 +616,8 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
     }
     ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
     if (!ok) break;
-    tc_fence_after();
-    if (wi.whole) bwd_column_delta<D>(sh, dp_addr, th, wi.rows, p, s);
+    tc_after_wait();
+    if (wi.whole) bwd_column_delta<D>(sh, dp_addr, th, wi.rows, p, j & 1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = st[36 + i];
 #pragma unroll
@@ -536,124 +649,102 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
     atomicOr(err, kErrTimeoutSoftmax);
     return;
   }
-  tc_fence_after();
+  tc_after_wait();
   bwd_store<D>(tmem + C::kColDv, th, wi, 1.f, dv, heads);
   bwd_store<D>(tmem + C::kColDk, th, wi, scale, dk, heads);
 }
 
 template <int D>
 __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tmem, const BwdThread& th,
-                                               const BwdWork& wi, float scale, const float2* __restrict__ stats,
-                                               const float* __restrict__ dlse, long long nq, __nv_bfloat16* __restrict__ dq, int heads, int* err) {
+                                               const BwdWork& wi, float scale, const __nv_bfloat16* __restrict__ q,
+                                               const __nv_bfloat16* __restrict__ dout,
+                                               const float2* __restrict__ stats, const float* __restrict__ dlse,
+                                               long long nq, __nv_bfloat16* __restrict__ dq, int heads, int* err) {
   using C = BwdCfg<D>;
+  {
+    // q (first four warps) and dO rows into TMEM, one row per thread; rows past the block are zeros
+    const int sw = (threadIdx.x >> 5) - 4, r = 32 * (sw & 3) + (threadIdx.x & 31);
+    const __nv_bfloat16* src = (sw < 4 ? q : dout) + ((static_cast<long long>(wi.row0) + r) * heads + wi.head) * D;
+    const uint32_t dst = tmem + (sw < 4 ? C::kColQ : C::kColDo) + (static_cast<uint32_t>(32 * (sw & 3)) << 16);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      uint32_t w[32];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 x = r < wi.rows ? __ldg(reinterpret_cast<const uint4*>(src + 64 * c) + i) : make_uint4(0u, 0u, 0u, 0u);
+        w[4 * i] = x.x;
+        w[4 * i + 1] = x.y;
+        w[4 * i + 2] = x.z;
+        w[4 * i + 3] = x.w;
+      }
+      tmem_st32(dst + 32 * c, w);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(sh.bar(C::kBarQ));
+  }
   const float scale_log2 = scale * kLog2e;
   const float2* st = stats + static_cast<long long>(wi.head) * nq + wi.row0 + th.row;
   float2 st0 = th.row < wi.rows ? __ldg(st) : make_float2(INFINITY, 0.f);
   float2 st1 = th.row + 8 < wi.rows ? __ldg(st + 8) : make_float2(INFINITY, 0.f);
   const uint32_t s_addr = tmem + th.lane_off;
-  constexpr int n0 = C::stages0(false);
-  uint32_t p[64];                               // P of the current tile, fp32
-  auto prob = [&](const uint32_t* x, uint32_t* y) {
-    y[0] = __float_as_uint(ex2(fmaf(__uint_as_float(x[0]), scale_log2, -st0.x)));
-    y[1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[1]), scale_log2, -st0.x)));
-    y[2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[2]), scale_log2, -st1.x)));
-    y[3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[3]), scale_log2, -st1.x)));
-  };
-  auto valid_of = [&](int j) { return *reinterpret_cast<const volatile int*>(sh.smem + C::kValidOff + 4 * (j % n0)); };
-  auto wait_s = [&](int j) {
-    return mbar_wait(sh.bar(C::kBarAux + j % n0), (j / n0) & 1, sh.abort_flag) &&
-           mbar_wait(sh.bar(C::kBarS), j & 1, sh.abort_flag);
-  };
-  // dS of tile j over its dP, 32 keys at a time (the next 32 keys' loads in flight); kNext: P of tile j + 1 from its S
-  // in the same sweep; kMask: a tile whose last keys are past the range, which add nothing whatever their rows held
-  auto step = [&](int j, int valid, auto next, auto mask) {
-    constexpr bool kNext = decltype(next)::value, kMask = decltype(mask)::value;
-    const uint32_t dp_addr = tmem + C::kColDp + 128 * (j & 1) + th.lane_off;
-    uint32_t d[2][16], s[64];
-    if (kNext) {
-      tmem_ld_16x256b_x8(s_addr, s);
-      tmem_ld_16x256b_x8(s_addr + 64, s + 32);
-    }
-    tmem_ld_16x256b_x4(dp_addr, d[0]);
+  uint32_t p[32];                               // P of the current tile, fp32
+  auto prob = [&](const uint32_t (&s)[32]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int b = i & 1;
-      tmem_wait_ld();
-      if (i == 0 && kNext) {
-        tc_fence_before();
-        mbar_arrive(sh.bar(C::kBarP));          // S of tile j + 1 is in registers
-      }
-      if (i < 3) tmem_ld_16x256b_x4(dp_addr + 32 * (i + 1), d[b ^ 1]);
-      uint32_t w[8];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        uint32_t* x = p + 16 * i + 4 * r;
-        const uint32_t* g = d[b] + 4 * r;
-        float a0 = __uint_as_float(x[0]) * (__uint_as_float(g[0]) - st0.y);
-        float a1 = __uint_as_float(x[1]) * (__uint_as_float(g[1]) - st0.y);
-        float b0 = __uint_as_float(x[2]) * (__uint_as_float(g[2]) - st1.y);
-        float b1 = __uint_as_float(x[3]) * (__uint_as_float(g[3]) - st1.y);
-        if (kMask) {
-          const int col = 32 * i + 8 * r + 2 * th.cq;
-          a0 = col < valid ? a0 : 0.f;
-          b0 = col < valid ? b0 : 0.f;
-          a1 = col + 1 < valid ? a1 : 0.f;
-          b1 = col + 1 < valid ? b1 : 0.f;
-        }
-        w[2 * r] = pack_bf16x2(a0, a1);
-        w[2 * r + 1] = pack_bf16x2(b0, b1);
-        if (kNext) prob(s + 16 * i + 4 * r, x);
-      }
-      // words [16 i, 16 i + 16) lie over dP columns that are in registers already
-      tmem_st_16x128b_x4(dp_addr + 16 * i, w);
-    }
-    tmem_wait_st();
-    tc_fence_before();
-    mbar_arrive(sh.bar(C::kBarDs + (j & 1)));
+    for (int i = 0; i < 32; ++i)
+      p[i] = __float_as_uint(ex2(fmaf(__uint_as_float(s[i]), scale_log2, (i & 2) ? -st1.x : -st0.x)));
   };
-  using Yes = std::true_type;
-  using No = std::false_type;
+  Ring a(C::kPairStages);
+  auto wait_s = [&](int u) {                    // S of tile u and the number of its keys
+    return mbar_wait(sh.bar(C::kBarAux + a.s), a.ph, sh.abort_flag) && mbar_wait(sh.bar(C::kBarS), u & 1, sh.abort_flag);
+  };
   bool ok = wait_s(0);
   int valid = 0;
   if (ok) {
-    tc_fence_after();
-    valid = valid_of(0);
-    tmem_ld_16x256b_x8(s_addr, p);
-    tmem_ld_16x256b_x8(s_addr + 64, p + 32);
+    tc_after_wait();
+    valid = *reinterpret_cast<const volatile int*>(sh.smem + C::kValidOff + 4 * a.s);
+    uint32_t s[32];
+    tmem_ld_16x256b_x8(s_addr, s);
     tmem_wait_ld();
     tc_fence_before();
     mbar_arrive(sh.bar(C::kBarP));
-#pragma unroll
-    for (int r = 0; r < 16; ++r) prob(p + 4 * r, p + 4 * r);
+    prob(s);
   }
-  for (int j = 0; ok && j < wi.n_tiles; ++j) {
-    const bool next = j + 1 < wi.n_tiles;
+  for (int u = 0; ok && u < wi.n_tiles; ++u) {
+    const bool next = u + 1 < wi.n_tiles;
     const int now = valid;
     if (next) {
-      ok = wait_s(j + 1);
+      a.next();
+      ok = wait_s(u + 1);
       if (!ok) break;
-      valid = valid_of(j + 1);
+      valid = *reinterpret_cast<const volatile int*>(sh.smem + C::kValidOff + 4 * a.s);
     }
-    ok = mbar_wait(sh.bar(C::kBarDp + (j & 1)), (j >> 1) & 1, sh.abort_flag);
+    ok = mbar_wait(sh.bar(C::kBarDp + (u & 1)), (u >> 1) & 1, sh.abort_flag);
+    // dS of this tile goes over that of tile u - 2: its dQ was issued before S(u + 1), or is waited for at the end
+    if (ok && !next && u >= 2)
+      ok = mbar_wait(sh.bar(C::kBarE0 + (u - 2) % C::kPairStages), ((u - 2) / C::kPairStages) & 1, sh.abort_flag);
     if (!ok) break;
-    tc_fence_after();
+    tc_after_wait();
+    uint32_t s[32], d[32], w[16];
+    tmem_ld_16x256b_x8(s_addr + C::kColDp + 64 * (u & 1), d);
+    // read in the last step too, where nothing uses it: a load under a condition ended up outside its wait
+    tmem_ld_16x256b_x8(s_addr, s);
+    tmem_wait_ld();
+    if (next) {
+      tc_fence_before();
+      mbar_arrive(sh.bar(C::kBarP));
+    }
     if (wi.whole) {
       // all keys of these queries are here: delta = sum_j P dP - dL, a quad of threads per row
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t d[16];
-        tmem_ld_16x256b_x4(tmem + C::kColDp + th.lane_off + 32 * i, d);
-        tmem_wait_ld();
+      for (int r = 0; r < 8; ++r)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (32 * i + 8 * r + 2 * th.cq + e < now) {
-              s0 = fmaf(__uint_as_float(p[16 * i + 4 * r + e]), __uint_as_float(d[4 * r + e]), s0);
-              s1 = fmaf(__uint_as_float(p[16 * i + 4 * r + 2 + e]), __uint_as_float(d[4 * r + 2 + e]), s1);
-            }
-      }
+        for (int e = 0; e < 2; ++e)
+          if (8 * r + 2 * th.cq + e < now) {
+            s0 = fmaf(__uint_as_float(p[4 * r + e]), __uint_as_float(d[4 * r + e]), s0);
+            s1 = fmaf(__uint_as_float(p[4 * r + 2 + e]), __uint_as_float(d[4 * r + 2 + e]), s1);
+          }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
         s0 += __shfl_xor_sync(0xffffffffu, s0, o);
@@ -663,20 +754,35 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
       st0.y = s0 - (dl != nullptr && th.row < wi.rows ? __ldg(dl) : 0.f);
       st1.y = s1 - (dl != nullptr && th.row + 8 < wi.rows ? __ldg(dl + 8) : 0.f);
     }
-    if (next) {
-      if (now < 128) step(j, now, Yes{}, Yes{});
-      else step(j, now, Yes{}, No{});
-    } else {
-      if (now < 128) step(j, now, No{}, Yes{});
-      else step(j, now, No{}, No{});
+    if (now < kDqRows) {
+      // keys past the range add nothing, whatever their rows held
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (8 * r + 2 * th.cq + e >= now) {
+            p[4 * r + e] = p[4 * r + 2 + e] = 0u;
+            d[4 * r + e] = d[4 * r + 2 + e] = 0u;
+          }
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float y = (r & 1) ? st1.y : st0.y;
+      w[r] = pack_bf16x2(__uint_as_float(p[2 * r]) * (__uint_as_float(d[2 * r]) - y),
+                         __uint_as_float(p[2 * r + 1]) * (__uint_as_float(d[2 * r + 1]) - y));
+    }
+    tmem_st_16x128b_x8(s_addr + C::kColDs + 32 * (u & 1), w);
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(sh.bar(C::kBarDs + (u & 1)));
+    if (next) prob(s);
   }
   if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
   if (!ok) {
     atomicOr(err, kErrTimeoutSoftmax);
     return;
   }
-  tc_fence_after();
+  tc_after_wait();
   bwd_store<D>(tmem + C::kColDq, th, wi, scale, dq, heads);
 }
 
@@ -684,6 +790,7 @@ template <int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                    const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ dout,
                     const BwdWork* __restrict__ work, const int2* __restrict__ ranges,
                     const float2* __restrict__ stats, const float* __restrict__ dlse, __nv_bfloat16* __restrict__ dq,
                     __nv_bfloat16* __restrict__ dk,
@@ -692,10 +799,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   using C = BwdCfg<D>;
   // a grid sized by an upper bound (work list planned on the device): CTAs past the planned count have no item
   if (n_items_dev != nullptr && static_cast<int>(blockIdx.x) >= __ldg(n_items_dev)) return;
-  extern __shared__ uint8_t smem_raw[];
+  // the tiles need a 1024-byte boundary, which dynamic shared memory without static shared memory before it has
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   BwdShared sh;
-  sh.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  sh.smem = smem_raw;
   sh.sbase = smem_u32(sh.smem);
+  if (sh.sbase & 1023u) {
+    if (threadIdx.x == 0) atomicOr(err, kErrPlan);
+    return;
+  }
   sh.bar0 = sh.sbase + C::kBarOff;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sh.smem + C::kBarOff + C::kNumBars * 8);
   sh.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -707,11 +819,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(sh.bar(C::kBarR), 1);
+    mbar_init(sh.bar(C::kBarQ), 256);
     for (int s = 0; s < C::kMaxStages; ++s) {
       mbar_init(sh.bar(C::kBarT0 + s), 1);
-      mbar_init(sh.bar(C::kBarT1 + s), 1);
       mbar_init(sh.bar(C::kBarAux + s), kAuxThreads);
       mbar_init(sh.bar(C::kBarE0 + s), 1);
+    }
+    for (int s = 0; s < C::kStages1; ++s) {
+      mbar_init(sh.bar(C::kBarT1 + s), 1);
       mbar_init(sh.bar(C::kBarE1 + s), 1);
     }
     mbar_init(sh.bar(C::kBarS), 1);
@@ -741,13 +856,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (wi.n_tiles > 0) {
       if (warp == 0) {
         if (elect_one()) {
-          if (dkv) bwd_producer<D>(sh, &tm_k, &tm_v, &tm_q, &tm_do, wi, rg, err);
-          else bwd_producer<D>(sh, &tm_q, &tm_do, &tm_k, &tm_v, wi, rg, err);
+          if (dkv) bwd_produce_dkv<D>(sh, &tm_q, &tm_k, &tm_v, &tm_do, wi, rg, err);
+          else bwd_produce_dq<D>(sh, &tm_k, &tm_v, wi, rg, err);
         }
       } else if (warp == 1) {
-        if (elect_one()) bwd_mma<D>(sh, tmem, wi, err);
+        if (elect_one()) {
+          if (dkv) bwd_mma_dkv<D>(sh, tmem, wi, err);
+          else bwd_mma_dq<D>(sh, tmem, wi, err);
+        }
+      } else if (dkv) {
+        bwd_prepare_dkv<D>(sh, wi, rg, stats, dlse, nq, threadIdx.x - 64, err);
       } else {
-        bwd_aux<D>(sh, wi, rg, stats, dlse, nq, threadIdx.x - 64, err);
+        bwd_prepare_dq<D>(sh, wi, rg, threadIdx.x - 64, err);
       }
     }
   } else {
@@ -763,7 +883,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     } else if (dkv) {
       bwd_compute_dkv<D>(sh, tmem, th, wi, scale, dk, dv, heads, err);
     } else {
-      bwd_compute_dq<D>(sh, tmem, th, wi, scale, stats, dlse, nq, dq, heads, err);
+      bwd_compute_dq<D>(sh, tmem, th, wi, scale, q, dout, stats, dlse, nq, dq, heads, err);
     }
   }
 
@@ -839,10 +959,10 @@ static int launch_attn_bwd(const void* q, const void* k, const void* v, const vo
   CUtensorMap mq, mk, mv, mdo;
   const long long w = static_cast<long long>(heads) * D;
   int rc;
-  if ((rc = make_rows_map(&mq, q, rq, w, w, 128)) != ORL_OK) return rc;
-  if ((rc = make_rows_map(&mdo, dout, rq, w, w, 128)) != ORL_OK) return rc;
-  if ((rc = make_rows_map(&mk, k, rk, w, w, 128)) != ORL_OK) return rc;
-  if ((rc = make_rows_map(&mv, v, rk, w, w, 128)) != ORL_OK) return rc;
+  if ((rc = make_rows_map(&mq, q, rq, w, w, 64)) != ORL_OK) return rc;
+  if ((rc = make_rows_map(&mdo, dout, rq, w, w, 64)) != ORL_OK) return rc;
+  if ((rc = make_rows_map(&mk, k, rk, w, w, 64)) != ORL_OK) return rc;
+  if ((rc = make_rows_map(&mv, v, rk, w, w, 64)) != ORL_OK) return rc;
   static std::mutex mu;
   static bool attr_set[kMaxDevices] = {};
   static int launch_regs = 0;
@@ -870,7 +990,8 @@ static int launch_attn_bwd(const void* q, const void* k, const void* v, const vo
     if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
   }
   attn_bwd_kernel<D><<<n_items, kBwdThreads, C::kSmemBytes, stream>>>(
-      mq, mk, mv, mdo, work, ranges, stats, dlse, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
+      mq, mk, mv, mdo, static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(dout), work, ranges,
+      stats, dlse, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
       static_cast<__nv_bfloat16*>(dv), nq, heads, scale, err, n_items_dev);
   return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
 }
@@ -927,7 +1048,7 @@ static int plan_bwd(const int32_t* q_start, const int32_t* q_len, const int32_t*
     cut(at, q_start[i], kDq, 0, 0, 0, false);
     plan.ranges.push_back({k_start[i], k_len[i]});
     cut(q_start[i], static_cast<long long>(q_start[i]) + q_len[i], kDq, static_cast<int>(plan.ranges.size()) - 1, 1,
-        (k_len[i] + 127) / 128, k_len[i] > 0 && k_len[i] <= 128);
+        (k_len[i] + kDqRows - 1) / kDqRows, k_len[i] > 0 && k_len[i] <= kWholeKeys);
     at = static_cast<long long>(q_start[i]) + q_len[i];
   }
   cut(at, nq, kDq, 0, 0, 0, false);
@@ -944,20 +1065,20 @@ static int plan_bwd(const int32_t* q_start, const int32_t* q_len, const int32_t*
     const int range0 = static_cast<int>(plan.ranges.size());
     int n = 0;
     long long tiles = 0;
-    bool whole = cuts[c + 1] - cuts[c] <= 128;            // every reader's keys are exactly this block
+    bool whole = cuts[c + 1] - cuts[c] <= kWholeKeys;     // every reader's keys are exactly this block
     for (int i = 0; i < n_seg; ++i)
       if (q_len[i] > 0 && k_len[i] > 0 && k_start[i] <= cuts[c] &&
           static_cast<long long>(k_start[i]) + k_len[i] >= cuts[c + 1]) {
         plan.ranges.push_back({q_start[i], q_len[i]});
-        tiles += (q_len[i] + 127) / 128;
+        tiles += (q_len[i] + kDkvRows - 1) / kDkvRows;
         whole = whole && k_start[i] == cuts[c] && k_len[i] == cuts[c + 1] - cuts[c];
         ++n;
       }
     if (tiles > 0x7fffffffLL || plan.ranges.size() > 0x7ffffff0u) return ORL_ERR_CAPACITY;
     cut(cuts[c], cuts[c + 1], kDkv, range0, n, static_cast<int>(tiles), whole && n > 0);
   }
-  // longest first; a dkv tile has four products and a dq tile three. Blocks of one head and segment stay adjacent.
-  auto cost = [](const Block& b) { return static_cast<long long>(b.n_tiles) * (b.kind == kDkv ? 4 : 3); };
+  // longest first: a dkv tile of 128 rows takes about three times a dq tile of 64
+  auto cost = [](const Block& b) { return static_cast<long long>(b.n_tiles) * (b.kind == kDkv ? 3 : 1); };
   std::vector<int> order(blocks.size());
   for (size_t i = 0; i < order.size(); ++i) order[i] = static_cast<int>(i);
   std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return cost(blocks[a]) > cost(blocks[b]); });
@@ -1058,10 +1179,10 @@ __global__ void __launch_bounds__(1024)
     const int lq = static_cast<int>(q1 - q0), lk = static_cast<int>(k1 - k0);
     s_row[i] = static_cast<int>(k0);
     s_len[i] = lk;
-    s_tiles[i] = (lq + 127) >> 7;
+    s_tiles[i] = (lq + kDkvRows - 1) / kDkvRows;
     s_row[n_seg + i] = static_cast<int>(q0);
     s_len[n_seg + i] = lq;
-    s_tiles[n_seg + i] = (lk + 127) >> 7;
+    s_tiles[n_seg + i] = (lk + kDqRows - 1) / kDqRows;
     ranges[i] = make_int2(static_cast<int>(q0), lq);
     ranges[n_seg + i] = make_int2(static_cast<int>(k0), lk);
   }
@@ -1084,7 +1205,7 @@ __global__ void __launch_bounds__(1024)
     return;
   }
   auto is_dkv = [&](int g) { return g < n_seg || (g >= 2 * n_seg && g < 2 * n_seg + 2); };
-  auto cost = [&](int g) { return static_cast<long long>(s_tiles[g]) * (is_dkv(g) ? 4 : 3); };
+  auto cost = [&](int g) { return static_cast<long long>(s_tiles[g]) * (is_dkv(g) ? 3 : 1); };
   auto items = [&](int g) { return heads * ((s_len[g] + 127) >> 7); };
   for (int g = t; g < n_grp; g += blockDim.x) {
     if (s_len[g] == 0) continue;
@@ -1132,7 +1253,7 @@ __global__ void __launch_bounds__(1024)
     w.n_tiles = s_tiles[g];
     // the segment's keys fit one tile (a dkv block is then the whole segment)
     const int keys = g < 2 * n_seg ? s_len[g % n_seg] : 0;
-    w.whole = w.n_tiles > 0 && keys > 0 && keys <= 128 ? 1 : 0;
+    w.whole = w.n_tiles > 0 && keys > 0 && keys <= kWholeKeys ? 1 : 0;
     work[1 + it] = w;
   }
   if (t == 0) work[0].row0 = n;

@@ -353,6 +353,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         atomicOr(err, kErrTimeoutSoftmax);
         break;
       }
+      __syncwarp();                          // lanes leave the wait one by one; the TMEM loads are warp-wide
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + (static_cast<uint32_t>(32 * (warp - 4)) << 16);
 #pragma unroll 1
