@@ -22,12 +22,11 @@
 // kDkv, tiles of 128 queries. TMEM columns: S^T / P^T [0,128), dP^T / dS^T [128,256), dV [256,256+D), dK [256+D,256+2D):
 // all 512 at D = 128. While the compute warps work on P(j) the tensor pipe runs dK(j-1) and dP(j); while they work on
 // dS(j), dV(j) and S(j+1). P is handed over in two halves, so dV begins under the second half's exponentials.
-// kDq, tiles of 64 keys. TMEM columns: S [0,64), dP [64,192) and dS [192,256) two each by turns, dQ [256,256+D), q
-// [384,..) and dO [448,..) as bf16 A operands: with q and dO out of shared memory a 64-column MMA takes 32 clocks instead
-// of the 48 that reading both operands costs, and the keys' ring has six stages. One step of the compute warps takes
-// dS(u) from dP(u) and the P(u) in their registers, and P(u+1) from S(u+1); S(u+2), dP(u+2) and dQ(u-1) are computed
-// under it. (With 128-key tiles and three key stages, all that fits beside q and dO, a step waited for its keys: 2700
-// clocks per 128 keys.)
+// kDq, tiles of 64 keys, taken by turns by two groups of four compute warps: a step (loads, exponentials, dS) is mostly
+// latency, and each group's hides in the other's. TMEM columns, per group: S [0,128), dP [128,256), dS [256,320) (bf16);
+// dQ [320,320+D), q [448,..) as a bf16 A operand: from TMEM a 64-column MMA takes 32 clocks instead of the 48 that reading
+// both operands from shared memory costs (dO has no TMEM left). S and dP of a group's next tile are issued once it has
+// read them, dQ when dS is there.
 //
 // delta from the forward's bf16 o carries o's rounding. Over many keys that is lost in the rounding of dS, but over a few
 // keys dS is a small difference of large terms (two keys: dq 0.0040 off in the 2-norm instead of 0.0024; 32 keys and
@@ -77,33 +76,32 @@ struct BwdCfg {
   static constexpr int kRedOff = kT0Off + (kStages0 - 1) * kTileBytes;
   static constexpr int kStatOff = kT0Off + kStages0 * kTileBytes;
   static constexpr int kStatBytes = 2 * 4 * 36 * 4;   // lse2, delta: four groups of 32 columns, padded (see stat_at)
-  // kDq: a ring of pairs of 64-row tiles K, V
+  // kDq: dO resident, a ring of pairs of 64-row tiles K, V
+  static constexpr int kPairOff = kTileBytes;
   static constexpr int kHalfBytes = kTileBytes / 2;
   static constexpr int kHalfChunk = kChunkBytes / 2;
   static constexpr int kPairStages = D == 64 ? 8 : 6;
   static constexpr int kMaxStages = 8;
-  static constexpr int kValidOff = kStatOff + 2 * kStatBytes;   // kDq, int per stage: keys inside the range
-  static constexpr int kBarOff = kValidOff + 4 * kMaxStages;
-  static constexpr int kBarR = 0;                       // kDkv: resident tiles landed
-  static constexpr int kBarQ = 1;                       // kDq: q and dO in TMEM
+  static constexpr int kBarOff = kStatOff + 2 * kStatBytes;
+  static constexpr int kBarR = 0;                       // resident tiles landed
+  static constexpr int kBarQ = 1;                       // kDq: q in TMEM
   static constexpr int kBarT0 = 2;                      // streamed tiles landed, per stage (kDq: the pair)
   static constexpr int kBarT1 = kBarT0 + kMaxStages;
   static constexpr int kBarAux = kBarT1 + kStages1;     // streamed tiles landed and prepared, per T0 stage
   static constexpr int kBarE0 = kBarAux + kMaxStages;   // stage free
   static constexpr int kBarE1 = kBarE0 + kMaxStages;
-  static constexpr int kBarS = kBarE1 + kStages1;       // S computed
-  static constexpr int kBarDp = kBarS + 1;              // dP computed (kDq: two buffers)
-  static constexpr int kBarP = kBarDp + 2;              // kDkv: half of P stored (two); kDq: S(u + 1) and dP(u) read
-  // dS stored. kDq: two by turns, since dS(u + 1) may be complete before the issuing thread has seen dS(u)
-  static constexpr int kBarDs = kBarP + 2;
+  static constexpr int kBarS = kBarE1 + kStages1;       // S computed; kDq: S and dP, per group
+  static constexpr int kBarDp = kBarS + 2;              // kDkv: dP computed
+  static constexpr int kBarP = kBarDp + 1;              // kDkv: half of P stored (two); kDq: S and dP read, per group
+  static constexpr int kBarDs = kBarP + 2;              // dS stored; kDq: per group
   static constexpr int kBarDone = kBarDs + 2;
   static constexpr int kBarDrain = kBarDone + 1;
   static constexpr int kNumBars = kBarDrain + 1;
   static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColDv = 256, kColDk = 256 + D;       // kDkv (S at 0, dP at 128)
-  static constexpr uint32_t kColDp = 64, kColDs = 192, kColDq = 256, kColQ = 384, kColDo = 448;   // kDq (S at 0)
-  static_assert(kPairStages * 2 * kHalfBytes <= kStatOff && kPairStages <= kMaxStages && kStages0 <= kMaxStages, "rings");
+  static constexpr uint32_t kColDp = 128, kColDs = 256, kColDq = 320, kColQ = 448;                // kDq (S at 0)
+  static_assert(kPairOff + kPairStages * 2 * kHalfBytes <= kStatOff && kPairStages <= kMaxStages && kStages0 <= kMaxStages, "rings");
   static_assert(kStatOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
@@ -229,10 +227,13 @@ __device__ __forceinline__ void bwd_produce_dkv(const BwdShared& sh, const CUten
 
 template <int D>
 __device__ __forceinline__ void bwd_produce_dq(const BwdShared& sh, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
-                                               const BwdWork& wi, const int2* ranges, int* err) {
+                                               const CUtensorMap* tm_do, const BwdWork& wi, const int2* ranges,
+                                               int* err) {
   using C = BwdCfg<D>;
   const uint64_t pol = policy_evict_last();
   const int x0 = wi.head * D;
+  mbar_expect_tx(sh.bar(C::kBarR), C::kTileBytes);
+  load_tile<D, 2>(sh.sbase + C::kROff, tm_do, sh.bar(C::kBarR), x0, wi.row0, policy_evict_first());
   TileWalk<kDqRows> walk(ranges, wi.n_ranges);
   Ring a(C::kPairStages);
   int issued = 0;
@@ -243,15 +244,17 @@ __device__ __forceinline__ void bwd_produce_dq(const BwdShared& sh, const CUtens
       atomicOr(err, kErrTimeoutLoad);
       break;
     }
-    const uint32_t dst = sh.sbase + a.s * 2 * C::kHalfBytes, bar = sh.bar(C::kBarT0 + a.s);
+    const uint32_t dst = sh.sbase + C::kPairOff + a.s * 2 * C::kHalfBytes, bar = sh.bar(C::kBarT0 + a.s);
     mbar_expect_tx(bar, 2 * C::kHalfBytes);
     load_tile<D, 1>(dst, tm_k, bar, x0, y, pol);
     load_tile<D, 1>(dst + C::kHalfBytes, tm_v, bar, x0, y, pol);
     issued = u + 1;
   }
-  if (*sh.abort_flag)
+  if (*sh.abort_flag) {
+    bwd_drain_wait(sh.bar(C::kBarR), 0, err);
     for (int u = issued > C::kPairStages ? issued - C::kPairStages : 0; u < issued; ++u)
       bwd_drain_wait(sh.bar(C::kBarT0 + u % C::kPairStages), (u / C::kPairStages) & 1, err);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- tile preparation
@@ -309,8 +312,7 @@ __device__ __forceinline__ void bwd_prepare_dkv(const BwdShared& sh, const BwdWo
   }
 }
 
-// kDq: the number of keys inside the range, zeros over K's rows past it (the columns of S and dP past the end are masked,
-// but dS K sums over K's rows)
+// kDq: zeros over K's rows past the range (the columns of S and dP past the end are masked, but dS K sums over K's rows)
 template <int D>
 __device__ __forceinline__ void bwd_prepare_dq(const BwdShared& sh, const BwdWork& wi, const int2* ranges, int t,
                                                int* err) {
@@ -324,9 +326,8 @@ __device__ __forceinline__ void bwd_prepare_dq(const BwdShared& sh, const BwdWor
       if (t == 0) atomicOr(err, kErrTimeoutLoad);
       return;
     }
-    if (t == 0) *reinterpret_cast<int*>(sh.smem + C::kValidOff + 4 * a.s) = valid;
     if (valid < kDqRows) {
-      uint8_t* k = sh.smem + a.s * 2 * C::kHalfBytes;
+      uint8_t* k = sh.smem + C::kPairOff + a.s * 2 * C::kHalfBytes;
       for (int c = 0; c < C::kChunks; ++c)
         for (int o = valid * 128 + t * 16; o < C::kHalfChunk; o += kAuxThreads * 16)
           *reinterpret_cast<uint4*>(k + c * C::kHalfChunk + o) = make_uint4(0u, 0u, 0u, 0u);
@@ -424,39 +425,42 @@ __device__ __forceinline__ void bwd_mma_dq(const BwdShared& sh, uint32_t tmem, c
   constexpr uint64_t kStep = (2 * C::kHalfBytes) >> 4;
   const int n = wi.n_tiles;
   auto wait = [&](int bar, int phase) { return mbar_wait(sh.bar(bar), phase & 1, sh.abort_flag); };
-  const uint64_t k0 = smem_desc_sw128(sh.sbase, 16, 1024), v0 = k0 + (C::kHalfBytes >> 4);
-  const uint64_t kt0 = smem_desc_sw128(sh.sbase, C::kHalfChunk, 1024);                  // K MN-major
-  // D[col] = A * T^T: A = q or dO in TMEM, T K-major
-  auto product = [&](uint32_t d, uint32_t a, uint64_t t) {
+  const uint64_t o0 = smem_desc_sw128(sh.sbase + C::kROff, 16, 1024);
+  const uint64_t k0 = smem_desc_sw128(sh.sbase + C::kPairOff, 16, 1024), v0 = k0 + (C::kHalfBytes >> 4);
+  const uint64_t kt0 = smem_desc_sw128(sh.sbase + C::kPairOff, C::kHalfChunk, 1024);    // K MN-major
+  Ring a(C::kPairStages), nx(C::kPairStages);            // tile u; the next tile whose S and dP are to be issued
+  // S = q K^T and dP = dO V^T of tile x into its group's columns
+  auto issue = [&](int x) {
+    const uint32_t d = tmem + 64 * (x & 1);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk)
-      mma_ts(d, a + kk * 8, t + (((kk >> 2) * C::kHalfChunk + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
-  };
-  Ring a(C::kPairStages), nx(C::kPairStages);            // tile u; the next tile whose S and dP are to be issued
-  // S over that of tile x - 1, which has been read; dP over that of tile x - 2, likewise
-  auto issue = [&](int x) {
-    product(tmem, tmem + C::kColQ, k0 + nx.s * kStep);
-    mma_commit(sh.bar(C::kBarS));
-    product(tmem + C::kColDp + 64 * (x & 1), tmem + C::kColDo, v0 + nx.s * kStep);
-    mma_commit(sh.bar(C::kBarDp + (x & 1)));
+      mma_ts(d, tmem + C::kColQ + kk * 8, k0 + nx.s * kStep + (((kk >> 2) * C::kHalfChunk + (kk & 3) * 32) >> 4), kIdescS,
+             kk > 0 ? 1u : 0u);
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+      mma_ss(d + C::kColDp, o0 + (((kk >> 2) * C::kChunkBytes + (kk & 3) * 32) >> 4),
+             v0 + nx.s * kStep + (((kk >> 2) * C::kHalfChunk + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
+    mma_commit(sh.bar(C::kBarS + (x & 1)));
     nx.next();
   };
-  bool ok = wait(C::kBarQ, 0) && wait(C::kBarAux, 0);
-  if (ok) {
+  // tile x may be issued once tile x - 2 has been read
+  auto ready = [&](int x) {
+    return wait(C::kBarAux + nx.s, nx.ph) && (x < 2 || wait(C::kBarP + (x & 1), (x >> 1) - 1));
+  };
+  bool ok = wait(C::kBarQ, 0) && wait(C::kBarR, 0);
+  for (int x = 0; ok && x < 3 && x < n; ++x) {
+    ok = ready(x);
+    if (!ok) break;
     tc_fence_after();
-    issue(0);
-    if (n > 1) ok = wait(C::kBarAux + nx.s, nx.ph) && wait(C::kBarP, 0);
-  }
-  if (ok && n > 1) {
-    tc_fence_after();
-    issue(1);
+    issue(x);
   }
   for (int u = 0; ok && u < n; ++u) {
-    if (u + 2 < n) {
-      ok = wait(C::kBarAux + nx.s, nx.ph) && wait(C::kBarP, u + 1);
+    // the other group reads its tile u + 1 before this one has dS of tile u
+    if (u + 3 < n) {
+      ok = ready(u + 3);
       if (!ok) break;
       tc_fence_after();
-      issue(u + 2);
+      issue(u + 3);
     }
     ok = wait(C::kBarDs + (u & 1), u >> 1);
     if (!ok) break;
@@ -656,126 +660,123 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
 
 template <int D>
 __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tmem, const BwdThread& th,
-                                               const BwdWork& wi, float scale, const __nv_bfloat16* __restrict__ q,
-                                               const __nv_bfloat16* __restrict__ dout,
-                                               const float2* __restrict__ stats, const float* __restrict__ dlse,
-                                               long long nq, __nv_bfloat16* __restrict__ dq, int heads, int* err) {
+                                               const BwdWork& wi, const int2* ranges, float scale,
+                                               const __nv_bfloat16* __restrict__ q, const float2* __restrict__ stats,
+                                               const float* __restrict__ dlse, long long nq,
+                                               __nv_bfloat16* __restrict__ dq, int heads, int* err) {
   using C = BwdCfg<D>;
+  const int sw = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
+  const int grp = sw >> 2;                      // tiles grp, grp + 2, ...
+  const uint32_t lanes = static_cast<uint32_t>(32 * (sw & 3)) << 16;
   {
-    // q (first four warps) and dO rows into TMEM, one row per thread; rows past the block are zeros
-    const int sw = (threadIdx.x >> 5) - 4, r = 32 * (sw & 3) + (threadIdx.x & 31);
-    const __nv_bfloat16* src = (sw < 4 ? q : dout) + ((static_cast<long long>(wi.row0) + r) * heads + wi.head) * D;
-    const uint32_t dst = tmem + (sw < 4 ? C::kColQ : C::kColDo) + (static_cast<uint32_t>(32 * (sw & 3)) << 16);
+    // q rows into TMEM, one row per thread, half of its columns per group; rows past the block are zeros
+    constexpr int kWords = D / 4;
+    const int r = 32 * (sw & 3) + lane;
+    const __nv_bfloat16* src = q + ((static_cast<long long>(wi.row0) + r) * heads + wi.head) * D + grp * (D / 2);
+    uint32_t w[kWords];
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-      uint32_t w[32];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 x = r < wi.rows ? __ldg(reinterpret_cast<const uint4*>(src + 64 * c) + i) : make_uint4(0u, 0u, 0u, 0u);
-        w[4 * i] = x.x;
-        w[4 * i + 1] = x.y;
-        w[4 * i + 2] = x.z;
-        w[4 * i + 3] = x.w;
-      }
-      tmem_st32(dst + 32 * c, w);
+    for (int i = 0; i < kWords / 4; ++i) {
+      const uint4 x = r < wi.rows ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0u, 0u, 0u, 0u);
+      w[4 * i] = x.x;
+      w[4 * i + 1] = x.y;
+      w[4 * i + 2] = x.z;
+      w[4 * i + 3] = x.w;
     }
+    if constexpr (D == 128) tmem_st32(tmem + C::kColQ + kWords * grp + lanes, w);
+    else tmem_st16(tmem + C::kColQ + kWords * grp + lanes, w);
     tmem_wait_st();
     tc_fence_before();
     mbar_arrive(sh.bar(C::kBarQ));
   }
   const float scale_log2 = scale * kLog2e;
-  const float2* st = stats + static_cast<long long>(wi.head) * nq + wi.row0 + th.row;
-  float2 st0 = th.row < wi.rows ? __ldg(st) : make_float2(INFINITY, 0.f);
-  float2 st1 = th.row + 8 < wi.rows ? __ldg(st + 8) : make_float2(INFINITY, 0.f);
-  const uint32_t s_addr = tmem + th.lane_off;
-  uint32_t p[32];                               // P of the current tile, fp32
-  auto prob = [&](const uint32_t (&s)[32]) {
+  // this thread's four rows: lane / 4 + 8 i of its warp's 32 TMEM lanes, i = 2 h + (register pair) of 16-lane block h
+  float lse2[4], delta[4];
+  const int row = 32 * (sw & 3) + (lane >> 2);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      p[i] = __float_as_uint(ex2(fmaf(__uint_as_float(s[i]), scale_log2, (i & 2) ? -st1.x : -st0.x)));
-  };
-  Ring a(C::kPairStages);
-  auto wait_s = [&](int u) {                    // S of tile u and the number of its keys
-    return mbar_wait(sh.bar(C::kBarAux + a.s), a.ph, sh.abort_flag) && mbar_wait(sh.bar(C::kBarS), u & 1, sh.abort_flag);
-  };
-  bool ok = wait_s(0);
-  int valid = 0;
-  if (ok) {
-    tc_after_wait();
-    valid = *reinterpret_cast<const volatile int*>(sh.smem + C::kValidOff + 4 * a.s);
-    uint32_t s[32];
-    tmem_ld_16x256b_x8(s_addr, s);
-    tmem_wait_ld();
-    tc_fence_before();
-    mbar_arrive(sh.bar(C::kBarP));
-    prob(s);
+  for (int i = 0; i < 4; ++i) {
+    const int r = row + 8 * i;
+    const float2 x = r < wi.rows ? __ldg(stats + static_cast<long long>(wi.head) * nq + wi.row0 + r)
+                                 : make_float2(INFINITY, 0.f);
+    lse2[i] = x.x;
+    delta[i] = x.y;
   }
-  for (int u = 0; ok && u < wi.n_tiles; ++u) {
-    const bool next = u + 1 < wi.n_tiles;
-    const int now = valid;
-    if (next) {
-      a.next();
-      ok = wait_s(u + 1);
-      if (!ok) break;
-      valid = *reinterpret_cast<const volatile int*>(sh.smem + C::kValidOff + 4 * a.s);
-    }
-    ok = mbar_wait(sh.bar(C::kBarDp + (u & 1)), (u >> 1) & 1, sh.abort_flag);
-    // dS of this tile goes over that of tile u - 2: its dQ was issued before S(u + 1), or is waited for at the end
-    if (ok && !next && u >= 2)
-      ok = mbar_wait(sh.bar(C::kBarE0 + (u - 2) % C::kPairStages), ((u - 2) / C::kPairStages) & 1, sh.abort_flag);
+  const uint32_t s_addr = tmem + 64 * grp + lanes, dp_addr = s_addr + C::kColDp, ds_addr = tmem + C::kColDs + 32 * grp + lanes;
+  constexpr uint32_t kBlock = 16u << 16;        // TMEM lane offset of the second 16-lane block
+  TileWalk<kDqRows> walk(ranges, wi.n_ranges);
+  int skip = 0;
+  if (grp == 1) walk.next(skip);
+  Ring before(C::kPairStages);                  // stage of this group's previous tile
+  if (grp == 1) before.next();
+  bool ok = true;
+  for (int u = grp; u < wi.n_tiles; u += 2) {
+    const int valid = walk.next(skip);
+    walk.next(skip);
+    ok = mbar_wait(sh.bar(C::kBarS + grp), (u >> 1) & 1, sh.abort_flag);
     if (!ok) break;
     tc_after_wait();
-    uint32_t s[32], d[32], w[16];
-    tmem_ld_16x256b_x8(s_addr + C::kColDp + 64 * (u & 1), d);
-    // read in the last step too, where nothing uses it: a load under a condition ended up outside its wait
-    tmem_ld_16x256b_x8(s_addr, s);
+    uint32_t p[2][32], d[2][32];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) tmem_ld_16x256b_x8(s_addr + h * kBlock, p[h]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) tmem_ld_16x256b_x8(dp_addr + h * kBlock, d[h]);
     tmem_wait_ld();
-    if (next) {
-      tc_fence_before();
-      mbar_arrive(sh.bar(C::kBarP));
+    tc_fence_before();
+    mbar_arrive(sh.bar(C::kBarP + grp));
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        p[h][i] = __float_as_uint(ex2(fmaf(__uint_as_float(p[h][i]), scale_log2, -lse2[2 * h + ((i >> 1) & 1)])));
+    if (valid < kDqRows) {
+      // keys past the range add nothing, whatever their rows held
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (8 * (i >> 2) + 2 * th.cq + (i & 1) >= valid) p[h][i] = d[h][i] = 0u;
     }
     if (wi.whole) {
       // all keys of these queries are here: delta = sum_j P dP - dL, a quad of threads per row
-      float s0 = 0.f, s1 = 0.f;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (8 * r + 2 * th.cq + e < now) {
-            s0 = fmaf(__uint_as_float(p[4 * r + e]), __uint_as_float(d[4 * r + e]), s0);
-            s1 = fmaf(__uint_as_float(p[4 * r + 2 + e]), __uint_as_float(d[4 * r + 2 + e]), s1);
-          }
+        for (int i = 0; i < 32; ++i) {
+          float& x = sum[2 * h + ((i >> 1) & 1)];
+          x = fmaf(__uint_as_float(p[h][i]), __uint_as_float(d[h][i]), x);
+        }
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-        s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+      for (int i = 0; i < 4; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+        const int r = row + 8 * i;
+        delta[i] = sum[i];
+        if (dlse != nullptr && r < wi.rows)
+          delta[i] -= __ldg(dlse + static_cast<long long>(wi.head) * nq + wi.row0 + r);
       }
-      const float* dl = dlse == nullptr ? nullptr : dlse + static_cast<long long>(wi.head) * nq + wi.row0 + th.row;
-      st0.y = s0 - (dl != nullptr && th.row < wi.rows ? __ldg(dl) : 0.f);
-      st1.y = s1 - (dl != nullptr && th.row + 8 < wi.rows ? __ldg(dl + 8) : 0.f);
     }
-    if (now < kDqRows) {
-      // keys past the range add nothing, whatever their rows held
+    uint32_t w[2][16];
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (8 * r + 2 * th.cq + e >= now) {
-            p[4 * r + e] = p[4 * r + 2 + e] = 0u;
-            d[4 * r + e] = d[4 * r + 2 + e] = 0u;
-          }
+      for (int r = 0; r < 16; ++r) {
+        const float y = delta[2 * h + (r & 1)];
+        w[h][r] = pack_bf16x2(__uint_as_float(p[h][2 * r]) * (__uint_as_float(d[h][2 * r]) - y),
+                              __uint_as_float(p[h][2 * r + 1]) * (__uint_as_float(d[h][2 * r + 1]) - y));
+      }
+    if (u >= 2) {
+      // dS goes over that of tile u - 2: its dQ is done when its stage is free
+      ok = mbar_wait(sh.bar(C::kBarE0 + before.s), before.ph, sh.abort_flag);
+      if (!ok) break;
+      before.next();
+      before.next();
+      tc_after_wait();
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float y = (r & 1) ? st1.y : st0.y;
-      w[r] = pack_bf16x2(__uint_as_float(p[2 * r]) * (__uint_as_float(d[2 * r]) - y),
-                         __uint_as_float(p[2 * r + 1]) * (__uint_as_float(d[2 * r + 1]) - y));
-    }
-    tmem_st_16x128b_x8(s_addr + C::kColDs + 32 * (u & 1), w);
+    tmem_st_16x128b_x8(ds_addr, w[0]);
+    tmem_st_16x128b_x8(ds_addr + kBlock, w[1]);
     tmem_wait_st();
     tc_fence_before();
-    mbar_arrive(sh.bar(C::kBarDs + (u & 1)));
-    if (next) prob(s);
+    mbar_arrive(sh.bar(C::kBarDs + grp));
   }
   if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
   if (!ok) {
@@ -790,7 +791,7 @@ template <int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                    const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ dout,
+                    const __nv_bfloat16* __restrict__ q,
                     const BwdWork* __restrict__ work, const int2* __restrict__ ranges,
                     const float2* __restrict__ stats, const float* __restrict__ dlse, __nv_bfloat16* __restrict__ dq,
                     __nv_bfloat16* __restrict__ dk,
@@ -829,12 +830,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(sh.bar(C::kBarT1 + s), 1);
       mbar_init(sh.bar(C::kBarE1 + s), 1);
     }
-    mbar_init(sh.bar(C::kBarS), 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(sh.bar(C::kBarDp + i), 1);
-      mbar_init(sh.bar(C::kBarP + i), 256);
-      mbar_init(sh.bar(C::kBarDs + i), 256);
+      mbar_init(sh.bar(C::kBarS + i), 1);
+      mbar_init(sh.bar(C::kBarP + i), dkv ? 256 : 128);
+      mbar_init(sh.bar(C::kBarDs + i), dkv ? 256 : 128);
     }
+    mbar_init(sh.bar(C::kBarDp), 1);
     mbar_init(sh.bar(C::kBarDone), 1);
     mbar_init(sh.bar(C::kBarDrain), 1);
     *sh.abort_flag = 0;
@@ -857,7 +858,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (warp == 0) {
         if (elect_one()) {
           if (dkv) bwd_produce_dkv<D>(sh, &tm_q, &tm_k, &tm_v, &tm_do, wi, rg, err);
-          else bwd_produce_dq<D>(sh, &tm_k, &tm_v, wi, rg, err);
+          else bwd_produce_dq<D>(sh, &tm_k, &tm_v, &tm_do, wi, rg, err);
         }
       } else if (warp == 1) {
         if (elect_one()) {
@@ -883,7 +884,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     } else if (dkv) {
       bwd_compute_dkv<D>(sh, tmem, th, wi, scale, dk, dv, heads, err);
     } else {
-      bwd_compute_dq<D>(sh, tmem, th, wi, scale, q, dout, stats, dlse, nq, dq, heads, err);
+      bwd_compute_dq<D>(sh, tmem, th, wi, rg, scale, q, stats, dlse, nq, dq, heads, err);
     }
   }
 
@@ -990,8 +991,7 @@ static int launch_attn_bwd(const void* q, const void* k, const void* v, const vo
     if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
   }
   attn_bwd_kernel<D><<<n_items, kBwdThreads, C::kSmemBytes, stream>>>(
-      mq, mk, mv, mdo, static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(dout), work, ranges,
-      stats, dlse, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
+      mq, mk, mv, mdo, static_cast<const __nv_bfloat16*>(q), work, ranges, stats, dlse, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
       static_cast<__nv_bfloat16*>(dv), nq, heads, scale, err, n_items_dev);
   return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
 }
