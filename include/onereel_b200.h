@@ -261,22 +261,18 @@ ORL_API int orl_linear(const void* x, long long ldx, const void* w, long long ld
                        const void* residual, long long ldr, void* y, void* z, long long m, long long n, long long k,
                        int act, int* err_dev, void* stream);
 
-/* dz = gate * dy * act'(z) [m, n] (NULL: not written), dbias = column sums of dz, dgate = column sums of dy * act(z)
- * (bf16 [n], NULL: not computed). dy has row stride lddy; z may be NULL without activation and gate. Deterministic.
- * scratch: device fp32, orl_linear_dz_scratch elements, needed for dbias or dgate. */
-ORL_API int orl_linear_dz(const void* dy, long long lddy, const void* z, const void* gate, int act, void* dz,
-                          void* dbias, void* dgate, float* scratch, long long m, long long n, void* stream);
+/* Gradients of orl_linear from the gradient dy [m, n] (row stride lddy) of y, the forward's inputs and its z (may be
+ * NULL without activation and gate): dz = gate * dy * act'(z), dx = dz w [m, k], dw = dz^T x [n, k], dbias = column sums
+ * of dz, dgate = column sums of dy * act(z) (bf16; NULL: not computed). The residual's gradient is dy itself.
+ * Deterministic. dz: scratch [m, n] bf16, needed for dx or dw when z is given; scratch: device fp32,
+ * orl_linear_bwd_scratch elements, needed for dbias or dgate. */
+ORL_API int orl_linear_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w, long long ldw,
+                           const void* z, const void* gate, int act, void* dz, void* dx, void* dw, void* dbias,
+                           void* dgate, float* scratch, long long m, long long n, long long k, int* err_dev,
+                           void* stream);
 
-/* fp32 elements of scratch orl_linear_dz needs. */
-ORL_API long long orl_linear_dz_scratch(long long m, long long n);
-
-/* dx [m, k] = dz [m, n] w [n, k] */
-ORL_API int orl_linear_dx(const void* dz, long long lddz, const void* w, long long ldw, void* dx, long long m,
-                          long long n, long long k, int* err_dev, void* stream);
-
-/* dw [n, k] = dz [m, n]^T x [m, k] */
-ORL_API int orl_linear_dw(const void* dz, long long lddz, const void* x, long long ldx, void* dw, long long m,
-                          long long n, long long k, int* err_dev, void* stream);
+/* fp32 elements of scratch orl_linear_bwd needs. */
+ORL_API long long orl_linear_bwd_scratch(long long m, long long n);
 
 /* ---------------------------------------------------------------- frame memory (src/onereel/frame_memory.py) */
 

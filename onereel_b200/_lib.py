@@ -88,10 +88,9 @@ SIGNATURES = {
     'orl_rope_rows': (c_int, [c_vp, c_vp, c_ll, c_int, c_int, c_vp, c_vp, c_ll, c_int, c_vp]),
     'orl_linear': (c_int, [c_vp, c_ll, c_vp, c_ll, c_vp, c_vp, c_vp, c_ll, c_vp, c_vp, c_ll, c_ll, c_ll, c_int, c_vp,
                            c_vp]),
-    'orl_linear_dz': (c_int, [c_vp, c_ll, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_ll, c_ll, c_vp]),
-    'orl_linear_dz_scratch': (c_ll, [c_ll, c_ll]),
-    'orl_linear_dx': (c_int, [c_vp, c_ll, c_vp, c_ll, c_vp, c_ll, c_ll, c_ll, c_vp, c_vp]),
-    'orl_linear_dw': (c_int, [c_vp, c_ll, c_vp, c_ll, c_vp, c_ll, c_ll, c_ll, c_vp, c_vp]),
+    'orl_linear_bwd': (c_int, [c_vp, c_ll, c_vp, c_ll, c_vp, c_ll, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                               c_ll, c_ll, c_ll, c_vp, c_vp]),
+    'orl_linear_bwd_scratch': (c_ll, [c_ll, c_ll]),
     'orl_frame_pool': (c_int, [c_vp, c_int, c_ll, c_int, c_vp, c_vp, c_int, c_vp, c_ll, c_vp]),
     'orl_frame_select_scratch': (c_ll, [c_int, c_int, c_int]),
     'orl_frame_select': (c_int, [c_vp, c_ll, c_ll, c_int, c_int, c_int, c_vp, c_int, c_int, c_int, c_vp, c_ll, c_vp,

@@ -53,6 +53,29 @@ def _err_word(device: torch.device) -> torch.Tensor:
     return _ERR[key]
 
 
+def _stream(dev: torch.device) -> int:
+    """the current stream of dev as the C ABI takes it (without building a torch.cuda.Stream: the small calls' host
+    time is of the order of their kernels')"""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+class _Device:
+    """`with _Device(dev)`: dev current, as torch.cuda.device, for free where it already is"""
+    __slots__ = ('index', 'back')
+
+    def __init__(self, dev: torch.device):
+        self.index = dev.index
+
+    def __enter__(self):
+        self.back = torch._C._cuda_getDevice()
+        if self.back != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.back != self.index:
+            torch.cuda.set_device(self.back)
+
+
 def check(device=None) -> None:
     """synchronise and raise if a kernel on `device` (default: every device used) set a bit in its error word (a
     bounded wait that ran out, or cu_seqlens the device planner rejected)"""
@@ -95,6 +118,12 @@ def _host_list(x) -> list[int]:
 
 
 def _check_inputs(q, k, v):
+    good = torch.bfloat16
+    if (q.__class__ is k.__class__ is v.__class__ is torch.Tensor and q.dtype is k.dtype is v.dtype is good and
+            q.is_cuda and q.dim() == 3 and q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and
+            k.device == v.device == q.device and k.shape == v.shape and k.dim() == 3 and
+            q.shape[1:] == k.shape[1:] and q.shape[2] in (64, 128)):
+        return
     for name, x in (('q', q), ('k', k), ('v', v)):
         if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.bfloat16):
             raise TypeError(f'{name} must be a bf16 CUDA tensor (the B200 path has no fallback), got '
@@ -173,7 +202,7 @@ def attend(q, k, v, q_start, q_len, k_start, k_len, out=None, lse=None, scale=No
     if lse is True:
         lse = torch.empty(H, Nq, dtype=torch.float32, device=dev)
     scale = Dh ** -0.5 if scale is None else float(scale)
-    s = stream if stream is not None else torch.cuda.current_stream(dev).cuda_stream
+    s = stream if stream is not None else _stream(dev)
     global LAUNCHES
     LAUNCHES += 1
     L.check(L.lib().orl_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
@@ -229,8 +258,8 @@ def _attend_cu(q, k, v, cu_q, cu_k, lse, own_scratch=False):
     dev = q.device
     n_seg = cu_q.numel() - 1
     need = L.check(L.lib().orl_attn_fwd_cu_capacity(Nq, n_seg, H), 'orl_attn_fwd_cu_capacity')
-    stream = torch.cuda.current_stream(dev)
-    key = (dev.index, stream.cuda_stream)
+    stream = _stream(dev)
+    key = (dev.index, stream)
     work = None if own_scratch else _CU_WORK.get(key)
     if own_scratch:
         work = torch.empty(need * L.WORK_DTYPE.itemsize, dtype=torch.uint8, device=dev)
@@ -242,7 +271,7 @@ def _attend_cu(q, k, v, cu_q, cu_k, lse, own_scratch=False):
                                     None if lse_t is None else lse_t.data_ptr(), Nq, k.shape[0], H, Dh, Dh ** -0.5,
                                     cu_q.data_ptr(), cu_k.data_ptr(), n_seg, work.data_ptr(),
                                     work.numel() // L.WORK_DTYPE.itemsize, _err_word(dev).data_ptr(),
-                                    stream.cuda_stream), 'orl_attn_fwd_cu')
+                                    stream), 'orl_attn_fwd_cu')
     return out, lse_t
 
 
@@ -277,8 +306,13 @@ def _plan_bwd(q_start, q_len, k_start, k_len, heads: int, nq: int, nk: int, devi
     return res
 
 
-def _grad_buffers(q, k, v, out, lse, dout, dlse):
-    """the checked, contiguous gradient inputs, the gradient tensors and the statistics scratch of a backward call"""
+def _aligned(x):
+    """x contiguous and 16-byte aligned (an incoming gradient may be any view)"""
+    x = x if x.is_contiguous() else x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _check_grad_inputs(q, out, lse, dout, dlse):
     Nq, H, Dh = q.shape
     for name, x, shape, dtype in (('out', out, q.shape, torch.bfloat16), ('dout', dout, q.shape, torch.bfloat16),
                                   ('lse', lse, (H, Nq), torch.float32), ('dlse', dlse, (H, Nq), torch.float32)):
@@ -288,17 +322,21 @@ def _grad_buffers(q, k, v, out, lse, dout, dlse):
             raise TypeError(f'{name} must be a {dtype} tensor on {q.device}')
         if tuple(x.shape) != tuple(shape):
             raise ValueError(f'{name} must have shape {tuple(shape)}, got {tuple(x.shape)}')
-    def c(x):                                    # contiguous and 16-byte aligned (a gradient may be any view)
-        x = x.contiguous()
-        return x if x.data_ptr() % 16 == 0 else x.clone()
-    dlse = None if dlse is None else c(dlse)
-    stats = torch.empty(2 * H * Nq, dtype=torch.float32, device=q.device)
-    return c(out), lse.contiguous(), c(dout), dlse, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), stats
 
 
-def _bwd_pointers(q, k, v, out, lse, dout, dlse, dq, dk, dv):
-    return [x.data_ptr() for x in (q, k, v, out, dout, lse)] + [None if dlse is None else dlse.data_ptr()] + \
-        [x.data_ptr() for x in (dq, dk, dv)]
+def _bwd_args(q, k, v, out, lse, dout, dlse, extra: int = 0):
+    """((dq, dk, dv), the C call's tensor arguments and sizes, addresses of the statistics scratch and of `extra` bytes
+    more, what keeps them alive)"""
+    out, dout, lse = _aligned(out), _aligned(dout), _aligned(lse)
+    dlse = None if dlse is None else _aligned(dlse)
+    Nq, H, Dh = q.shape
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    stats = (8 * H * Nq + 15) // 16 * 16
+    scratch = torch.empty(stats + extra, dtype=torch.uint8, device=q.device)
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
+            None if dlse is None else dlse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), Nq, k.shape[0], H, Dh)
+    at = scratch.data_ptr()
+    return (dq, dk, dv), args, at, at + stats, (out, dout, lse, dlse, scratch)
 
 
 def attend_grad(q, k, v, out, lse, dout, q_start, q_len, k_start, k_len, dlse=None, scale=None):
@@ -306,31 +344,30 @@ def attend_grad(q, k, v, out, lse, dout, q_start, q_len, k_start, k_len, dlse=No
     of lse. Query ranges must not overlap; key ranges may, and a shared key row's gradient is the sum over its readers.
     Rows of no segment get zeros."""
     _check_inputs(q, k, v)
-    Nq, H, Dh = q.shape
+    _check_grad_inputs(q, out, lse, dout, dlse)
+    return _attend_grad(q, k, v, out, lse, dout, q_start, q_len, k_start, k_len, dlse, scale)
+
+
+def _attend_grad(q, k, v, out, lse, dout, q_start, q_len, k_start, k_len, dlse, scale=None):
     dev = q.device
-    with torch.cuda.device(dev):
-        out, lse, dout, dlse, dq, dk, dv, stats = _grad_buffers(q, k, v, out, lse, dout, dlse)
-        work, ranges, n = _plan_bwd(q_start, q_len, k_start, k_len, H, Nq, k.shape[0], dev)
-        L.check(L.lib().orl_attn_bwd(*_bwd_pointers(q, k, v, out, lse, dout, dlse, dq, dk, dv), Nq, k.shape[0], H, Dh,
-                                     Dh ** -0.5 if scale is None else float(scale), work.data_ptr(), n,
-                                     ranges.data_ptr(), stats.data_ptr(), _err_word(dev).data_ptr(),
-                                     torch.cuda.current_stream(dev).cuda_stream), 'orl_attn_bwd')
-    return dq, dk, dv
+    with _Device(dev):
+        grads, args, stats, _, keep = _bwd_args(q, k, v, out, lse, dout, dlse)
+        work, ranges, n = _plan_bwd(q_start, q_len, k_start, k_len, q.shape[1], q.shape[0], k.shape[0], dev)
+        L.check(L.lib().orl_attn_bwd(*args, q.shape[2] ** -0.5 if scale is None else float(scale), work.data_ptr(), n,
+                                     ranges.data_ptr(), stats, _err_word(dev).data_ptr(), _stream(dev)), 'orl_attn_bwd')
+    return grads
 
 
 def _attend_cu_grad(q, k, v, out, lse, dout, dlse, cu_q, cu_k):
     """attend_grad for cu_seqlens on the device, planned there (orl_attn_bwd_cu)"""
-    Nq, H, Dh = q.shape
-    Nk, dev, n_seg = k.shape[0], q.device, cu_q.numel() - 1
-    with torch.cuda.device(dev):
-        out, lse, dout, dlse, dq, dk, dv, stats = _grad_buffers(q, k, v, out, lse, dout, dlse)
-        need = L.check(L.lib().orl_attn_bwd_cu_scratch(Nq, Nk, n_seg, H), 'orl_attn_bwd_cu_scratch')
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-        L.check(L.lib().orl_attn_bwd_cu(*_bwd_pointers(q, k, v, out, lse, dout, dlse, dq, dk, dv), Nq, Nk, H, Dh,
-                                        Dh ** -0.5, cu_q.data_ptr(), cu_k.data_ptr(), n_seg, scratch.data_ptr(), need,
-                                        stats.data_ptr(), _err_word(dev).data_ptr(),
-                                        torch.cuda.current_stream(dev).cuda_stream), 'orl_attn_bwd_cu')
-    return dq, dk, dv
+    dev, n_seg = q.device, cu_q.numel() - 1
+    with _Device(dev):
+        need = L.check(L.lib().orl_attn_bwd_cu_scratch(q.shape[0], k.shape[0], n_seg, q.shape[1]),
+                       'orl_attn_bwd_cu_scratch')
+        grads, args, stats, scratch, keep = _bwd_args(q, k, v, out, lse, dout, dlse, need)
+        L.check(L.lib().orl_attn_bwd_cu(*args, q.shape[2] ** -0.5, cu_q.data_ptr(), cu_k.data_ptr(), n_seg, scratch,
+                                        need, stats, _err_word(dev).data_ptr(), _stream(dev)), 'orl_attn_bwd_cu')
+    return grads
 
 
 class _Ranges(torch.autograd.Function):
@@ -338,7 +375,7 @@ class _Ranges(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, segments):
-        with torch.cuda.device(q.device):
+        with _Device(q.device):
             out, lse = attend(q, k, v, *segments, lse=True)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.segments = segments
@@ -352,7 +389,7 @@ class _Ranges(torch.autograd.Function):
             return None, None, None, None
         q, k, v, out, lse = ctx.saved_tensors
         dout = torch.zeros_like(out) if dout is None else dout
-        return *attend_grad(q, k, v, out, lse, dout, *ctx.segments, dlse=dlse), None
+        return *_attend_grad(q, k, v, out, lse, dout, *ctx.segments, dlse), None
 
 
 class _Varlen(torch.autograd.Function):
@@ -360,7 +397,7 @@ class _Varlen(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k):
-        with torch.cuda.device(q.device):
+        with _Device(q.device):
             out, lse = _attend_cu(q, k, v, cu_q, cu_k, lse=True, own_scratch=True)
         ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
         ctx.set_materialize_grads(False)

@@ -602,60 +602,54 @@ extern "C" int orl_linear(const void* x, long long ldx, const void* w, long long
                             stream);
 }
 
-extern "C" long long orl_linear_dz_scratch(long long m, long long n) {
+extern "C" long long orl_linear_bwd_scratch(long long m, long long n) {
   if (check_linear(m, n, 8) != ORL_OK) return ORL_ERR_ARG;
   return 2ll * dz_strips(static_cast<int>(m), static_cast<int>(n)) * n;
 }
 
-extern "C" int orl_linear_dz(const void* dy, long long lddy, const void* z, const void* gate, int act, void* dz,
-                             void* dbias, void* dgate, float* scratch, long long m, long long n, void* stream_ptr) {
-  int rc = check_linear(m, n, 8);
+extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w,
+                              long long ldw, const void* z, const void* gate, int act, void* dz, void* dx, void* dw,
+                              void* dbias, void* dgate, float* scratch, long long m, long long n, long long k,
+                              int* err_dev, void* stream_ptr) {
+  int rc = check_linear(m, n, k);
   if (rc != ORL_OK) return rc;
-  if (act < ORL_ACT_NONE || act > ORL_ACT_SILU || (m > 0 && dy == nullptr) || lddy < n) return ORL_ERR_ARG;
+  if (act < ORL_ACT_NONE || act > ORL_ACT_SILU || err_dev == nullptr || lddy < n) return ORL_ERR_ARG;
+  if (m > 0 && (dy == nullptr || (dw != nullptr && x == nullptr))) return ORL_ERR_ARG;
+  if ((dw != nullptr && ldx < k) || (dx != nullptr && (w == nullptr || ldw < k))) return ORL_ERR_ARG;
+  // an activation's slope, a gate and a gate's gradient need z; with z, dz is not dy and needs room
   if ((act != ORL_ACT_NONE || gate != nullptr || dgate != nullptr) && z == nullptr && m > 0) return ORL_ERR_ARG;
-  if ((dbias != nullptr || dgate != nullptr) && scratch == nullptr) return ORL_ERR_ARG;
-  if (lddy & 7) return ORL_ERR_ALIGN;
-  for (const void* p : {dy, z, gate, static_cast<const void*>(dz)})
+  const bool products = dx != nullptr || dw != nullptr, sums = dbias != nullptr || dgate != nullptr;
+  if ((z != nullptr && products && dz == nullptr && m > 0) || (sums && scratch == nullptr)) return ORL_ERR_ARG;
+  if ((lddy & 7) || (dw != nullptr && (ldx & 7)) || (dx != nullptr && (ldw & 7))) return ORL_ERR_ALIGN;
+  for (const void* p : {dy, x, w, z, gate, static_cast<const void*>(dz), static_cast<const void*>(dx),
+                        static_cast<const void*>(dw)})
     if (!lin_aligned(p)) return ORL_ERR_ALIGN;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  const int strips = dz_strips(static_cast<int>(m), static_cast<int>(n));
-  float* part_b = dbias != nullptr ? scratch : nullptr;
-  float* part_g = dgate != nullptr ? scratch + static_cast<long long>(strips) * n : nullptr;
-  const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(strips));
-  linear_dz_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(dy), lddy,
-                                             static_cast<const __nv_bfloat16*>(z),
-                                             static_cast<const __nv_bfloat16*>(gate), act, static_cast<int>(m),
-                                             static_cast<int>(n), static_cast<__nv_bfloat16*>(dz), part_b, part_g);
-  if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
-  if (part_b != nullptr && (rc = column_sum(part_b, strips, static_cast<int>(n), n, dbias, stream)) != ORL_OK) return rc;
-  if (part_g != nullptr) return column_sum(part_g, strips, static_cast<int>(n), n, dgate, stream);
+  const int mm = static_cast<int>(m), nn = static_cast<int>(n), kk = static_cast<int>(k);
+  if (sums || (z != nullptr && products)) {
+    const int strips = dz_strips(mm, nn);
+    float* part_b = dbias != nullptr ? scratch : nullptr;
+    float* part_g = dgate != nullptr ? scratch + static_cast<long long>(strips) * n : nullptr;
+    const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(strips));
+    linear_dz_kernel<<<grid, 256, 0, stream>>>(
+        static_cast<const __nv_bfloat16*>(dy), lddy, static_cast<const __nv_bfloat16*>(z),
+        static_cast<const __nv_bfloat16*>(gate), act, mm, nn,
+        z != nullptr && products ? static_cast<__nv_bfloat16*>(dz) : nullptr, part_b, part_g);
+    if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
+    if (part_b != nullptr && (rc = column_sum(part_b, strips, nn, n, dbias, stream)) != ORL_OK) return rc;
+    if (part_g != nullptr && (rc = column_sum(part_g, strips, nn, n, dgate, stream)) != ORL_OK) return rc;
+  }
+  const void* g = z != nullptr ? dz : dy;
+  const long long ldg = z != nullptr ? n : lddy;
+  if (dx != nullptr && m > 0) {
+    const Epilogue ep{nullptr, nullptr, nullptr, 0, static_cast<__nv_bfloat16*>(dx), nullptr, ORL_ACT_NONE};
+    if ((rc = gemm<false, true>(g, ldg, w, ldw, mm, kk, nn, ep, err_dev, stream)) != ORL_OK) return rc;
+  }
+  if (dw != nullptr) {
+    if (m == 0)
+      return cudaMemsetAsync(dw, 0, 2 * static_cast<size_t>(n) * k, stream) == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
+    const Epilogue ep{nullptr, nullptr, nullptr, 0, static_cast<__nv_bfloat16*>(dw), nullptr, ORL_ACT_NONE};
+    return gemm<true, true>(g, ldg, x, ldx, nn, kk, mm, ep, err_dev, stream);
+  }
   return ORL_OK;
-}
-
-extern "C" int orl_linear_dx(const void* dz, long long lddz, const void* w, long long ldw, void* dx, long long m,
-                             long long n, long long k, int* err_dev, void* stream_ptr) {
-  const int rc = check_linear(m, n, k);
-  if (rc != ORL_OK) return rc;
-  if (w == nullptr || err_dev == nullptr || lddz < n || ldw < k || (m > 0 && (dz == nullptr || dx == nullptr)))
-    return ORL_ERR_ARG;
-  if ((lddz & 7) || (ldw & 7) || !lin_aligned(dz) || !lin_aligned(w) || !lin_aligned(dx)) return ORL_ERR_ALIGN;
-  if (m == 0) return ORL_OK;
-  const Epilogue ep{nullptr, nullptr, nullptr, 0, static_cast<__nv_bfloat16*>(dx), nullptr, ORL_ACT_NONE};
-  return gemm<false, true>(dz, lddz, w, ldw, static_cast<int>(m), static_cast<int>(k), static_cast<int>(n), ep, err_dev,
-                           static_cast<cudaStream_t>(stream_ptr));
-}
-
-extern "C" int orl_linear_dw(const void* dz, long long lddz, const void* x, long long ldx, void* dw, long long m,
-                             long long n, long long k, int* err_dev, void* stream_ptr) {
-  const int rc = check_linear(m, n, k);
-  if (rc != ORL_OK) return rc;
-  if (dw == nullptr || err_dev == nullptr || lddz < n || ldx < k || (m > 0 && (dz == nullptr || x == nullptr)))
-    return ORL_ERR_ARG;
-  if ((lddz & 7) || (ldx & 7) || !lin_aligned(dz) || !lin_aligned(x) || !lin_aligned(dw)) return ORL_ERR_ALIGN;
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (m == 0)
-    return cudaMemsetAsync(dw, 0, 2 * static_cast<size_t>(n) * k, stream) == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
-  const Epilogue ep{nullptr, nullptr, nullptr, 0, static_cast<__nv_bfloat16*>(dw), nullptr, ORL_ACT_NONE};
-  return gemm<true, true>(dz, lddz, x, ldx, static_cast<int>(n), static_cast<int>(k), static_cast<int>(m), ep, err_dev,
-                          stream);
 }

@@ -11,7 +11,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
-from onereel_b200.attention import _err_word
+from onereel_b200.attention import _Device, _err_word, _stream
 
 ACTIVATIONS = {None: 0, 'gelu_tanh': 1, 'silu': 2}
 
@@ -87,7 +87,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
 def _forward(x, w, b, gate, residual, act, keep):
     """(y, z or None): the kernel call; keep: also store z = x w^T + bias"""
     M, N, K, dev = x.shape[0], w.shape[0], x.shape[1], x.device
-    with torch.cuda.device(dev):
+    with _Device(dev):
         x, w = _rows(x), _rows(w)
         b, gate = (None if t is None else _vector(t) for t in (b, gate))
         residual = None if residual is None else _rows(residual)
@@ -95,7 +95,7 @@ def _forward(x, w, b, gate, residual, act, keep):
         z = torch.empty_like(y) if keep else None
         L.check(L.lib().orl_linear(x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ptr(b), _ptr(gate), _ptr(residual),
                                    0 if residual is None else _ld(residual), y.data_ptr(), _ptr(z), M, N, K, act,
-                                   _err_word(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
+                                   _err_word(dev).data_ptr(), _stream(dev)),
                 'orl_linear')
     return y, z
 
@@ -116,30 +116,19 @@ class _Linear(torch.autograd.Function):
         x, w, gate, z = ctx.saved_tensors
         need = ctx.needs_input_grad
         (M, K), N, dev = x.shape, w.shape[0], x.device
-        with torch.cuda.device(dev):
-            stream, err = torch.cuda.current_stream(dev).cuda_stream, _err_word(dev).data_ptr()
-            d = _rows(dy)
-            dx = dw = db = dgate = None
-            gv = None if gate is None else _vector(gate)
-            dz = d if z is None else torch.empty(M, N, dtype=torch.bfloat16, device=dev)
-            if need[2]:
-                db = torch.empty(N, dtype=torch.bfloat16, device=dev)
-            if need[3]:
-                dgate = torch.empty(N, dtype=torch.bfloat16, device=dev)
-            if db is not None or dgate is not None or (z is not None and (need[0] or need[1])):
-                scratch = torch.empty(L.check(L.lib().orl_linear_dz_scratch(M, N), 'orl_linear_dz_scratch'),
-                                      dtype=torch.float32, device=dev)
-                L.check(L.lib().orl_linear_dz(d.data_ptr(), _ld(d), _ptr(z), _ptr(gv), ctx.act,
-                                              None if z is None else dz.data_ptr(), _ptr(db), _ptr(dgate),
-                                              scratch.data_ptr(), M, N, stream), 'orl_linear_dz')
-            if need[0]:
-                wr = _rows(w)
-                dx = torch.empty(M, K, dtype=torch.bfloat16, device=dev)
-                L.check(L.lib().orl_linear_dx(dz.data_ptr(), _ld(dz), wr.data_ptr(), _ld(wr), dx.data_ptr(), M, N, K,
-                                              err, stream), 'orl_linear_dx')
-            if need[1]:
-                xr = _rows(x)
-                dw = torch.empty(N, K, dtype=torch.bfloat16, device=dev)
-                L.check(L.lib().orl_linear_dw(dz.data_ptr(), _ld(dz), xr.data_ptr(), _ld(xr), dw.data_ptr(), M, N, K,
-                                              err, stream), 'orl_linear_dw')
+        with _Device(dev):
+            d, xr, wr = _rows(dy), _rows(x), _rows(w)
+            new = lambda *shape: torch.empty(*shape, dtype=torch.bfloat16, device=dev)
+            dx = new(M, K) if need[0] else None
+            dw = new(N, K) if need[1] else None
+            db = new(N) if need[2] else None
+            dgate = new(N) if need[3] else None
+            # scratch: the partial column sums, then dz where it is not dy itself
+            sums = 4 * L.check(L.lib().orl_linear_bwd_scratch(M, N), 'orl_linear_bwd_scratch')
+            scratch = torch.empty(sums + (0 if z is None else 2 * M * N), dtype=torch.uint8, device=dev)
+            at = scratch.data_ptr()
+            L.check(L.lib().orl_linear_bwd(d.data_ptr(), _ld(d), xr.data_ptr(), _ld(xr), wr.data_ptr(), _ld(wr), _ptr(z),
+                                           None if gate is None else _vector(gate).data_ptr(), ctx.act,
+                                           None if z is None else at + sums, _ptr(dx), _ptr(dw), _ptr(db), _ptr(dgate),
+                                           at, M, N, K, _err_word(dev).data_ptr(), _stream(dev)), 'orl_linear_bwd')
         return dx, dw, db, dgate, dy if need[4] else None, None

@@ -8,6 +8,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
+from onereel_b200.attention import _Device, _stream
 
 
 def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int,
@@ -21,14 +22,19 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
     if not (x.is_cuda and x.dtype == torch.bfloat16):
         raise TypeError('qk_norm_rope: x must be a bf16 CUDA tensor (no fallback)')
     x = x.contiguous()
-    rows, hidden = x.shape
-    Dh = hidden // heads
+    rows = x.shape[0]
     w = weight.to(device=x.device, dtype=torch.bfloat16).contiguous()
-    c = cos.to(device=x.device, dtype=torch.float32).reshape(rows, -1).contiguous()
-    s = sin.to(device=x.device, dtype=torch.float32).reshape(rows, -1).contiguous()
+    c, s = _table(cos, rows, x.device), _table(sin, rows, x.device)
     if (out is None and row_map is None and torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)):
         return _QkNormRope.apply(x, w, c, s, heads, float(eps), int(per_head), int(sin_shift))
     return _forward(x, w, c, s, heads, eps, per_head, sin_shift, out, row_map)
+
+
+def _table(t, rows: int, device):
+    """a rotary table as the kernels read it: fp32 [rows, D], contiguous"""
+    if t.dtype is torch.float32 and t.device == device and t.dim() == 2 and t.shape[0] == rows and t.is_contiguous():
+        return t
+    return t.to(device=device, dtype=torch.float32).reshape(rows, -1).contiguous()
 
 
 def _forward(x, w, c, s, heads, eps, per_head, sin_shift, out=None, row_map=None):
@@ -39,7 +45,7 @@ def _forward(x, w, c, s, heads, eps, per_head, sin_shift, out=None, row_map=None
     L.check(L.lib().orl_qk_norm_rope(x.data_ptr(), out.data_ptr(), w.data_ptr(), c.data_ptr(), s.data_ptr(), rows,
                                      heads, Dh, int(per_head), float(eps), int(sin_shift), c.shape[1],
                                      None if rm is None else rm.data_ptr(),
-                                     torch.cuda.current_stream(x.device).cuda_stream), 'orl_qk_norm_rope')
+                                     _stream(x.device)), 'orl_qk_norm_rope')
     return out
 
 
@@ -49,7 +55,7 @@ class _QkNormRope(torch.autograd.Function):
     def forward(ctx, x, w, c, s, heads, eps, per_head, sin_shift):
         ctx.save_for_backward(x, w, c, s)
         ctx.args = heads, eps, per_head, sin_shift
-        with torch.cuda.device(x.device):
+        with _Device(x.device):
             return _forward(x, w, c, s, heads, eps, per_head, sin_shift)
 
     @staticmethod
@@ -70,7 +76,7 @@ def qk_norm_rope_grad(x, weight, cos, sin, dy, heads: int, eps: float, per_head:
         raise ValueError(f'qk_norm_rope: dy must have shape {(rows, heads, hidden // heads)}, got {tuple(dy.shape)}')
     dy = dy.contiguous()
     dy = dy if dy.data_ptr() % 16 == 0 else dy.clone()
-    with torch.cuda.device(x.device):
+    with _Device(x.device):
         n = L.check(L.lib().orl_qk_norm_rope_bwd_scratch(rows, heads, hidden // heads, int(per_head)),
                     'orl_qk_norm_rope_bwd_scratch')
         scratch = torch.empty(n, dtype=torch.float32, device=x.device)
@@ -78,7 +84,7 @@ def qk_norm_rope_grad(x, weight, cos, sin, dy, heads: int, eps: float, per_head:
         L.check(L.lib().orl_qk_norm_rope_bwd(x.data_ptr(), dy.data_ptr(), weight.data_ptr(), cos.data_ptr(),
                                              sin.data_ptr(), dx.data_ptr(), dw.data_ptr(), scratch.data_ptr(), rows,
                                              heads, hidden // heads, int(per_head), float(eps), int(sin_shift),
-                                             cos.shape[1], torch.cuda.current_stream(x.device).cuda_stream),
+                                             cos.shape[1], _stream(x.device)),
                 'orl_qk_norm_rope_bwd')
     return dx, dw
 
@@ -91,6 +97,6 @@ def rotate_rows(x: torch.Tensor, rows: torch.Tensor, cos: torch.Tensor, sin: tor
         return x
     H, Dh = x.shape[1:]
     L.check(L.lib().orl_rope_rows(x.data_ptr(), rows.data_ptr(), Nr, H, Dh, cos.data_ptr(), sin.data_ptr(),
-                                  cos.shape[1], int(sin_shift), torch.cuda.current_stream(x.device).cuda_stream),
+                                  cos.shape[1], int(sin_shift), _stream(x.device)),
             'orl_rope_rows')
     return x

@@ -30,18 +30,16 @@ def test_linear_refuses(h):
 
 
 def test_linear_gradients_refuse(h):
-    ok = [P, 32, P, P, 1, P, P, P, P, 5, 32, None]
-    call = lambda **at: h.orl_linear_dz(*with_(ok, **at))
-    assert call(a0=None) == -1 and call(a2=None) == -1 and call(a4=7) == -1 and call(a8=None) == -1
-    assert call(a1=24) == -1 and call(a1=36) == -2 and call(a10=30) == -2
-    assert h.orl_linear_dz_scratch(-1, 8) == -1 and h.orl_linear_dz_scratch(5, 12) == -1
-    # one partial row per strip for each of the two sums
-    assert h.orl_linear_dz_scratch(5, 32) == 2 * 32 and h.orl_linear_dz_scratch(1000, 32) == 2 * 125 * 32
-    for f in (h.orl_linear_dx, h.orl_linear_dw):
-        ok2 = [P, 32, P, 64, P, 5, 32, 64, P, None]
-        call2 = lambda **at: f(*with_(ok2, **at))
-        assert call2(a0=None) == -1 and call2(a2=None) == -1 and call2(a4=None) == -1 and call2(a8=None) == -1
-        assert call2(a1=24) == -1 and call2(a3=56) == -1 and call2(a3=68) == -2 and call2(a7=60) == -2
+    ok = [P, 32, P, 64, P, 64, P, P, 1, P, P, P, P, P, P, 5, 32, 64, P, None]
+    call = lambda **at: h.orl_linear_bwd(*with_(ok, **at))
+    assert call(a0=None) == -1 and call(a2=None) == -1 and call(a4=None) == -1 and call(a18=None) == -1
+    assert call(a6=None) == -1 and call(a9=None) == -1 and call(a14=None) == -1 and call(a8=7) == -1
+    assert call(a1=24) == -1 and call(a3=56) == -1 and call(a5=56) == -1 and call(a15=-1) == -1 and call(a16=0) == -1
+    assert call(a1=36) == -2 and call(a3=68) == -2 and call(a5=68) == -2 and call(a16=30) == -2 and call(a17=60) == -2
+    assert call(a10=P + 8) == -2 and call(a6=P + 4) == -2
+    assert h.orl_linear_bwd_scratch(-1, 8) == -1 and h.orl_linear_bwd_scratch(5, 12) == -1
+    # one partial row per strip of eight rows or more, for each of the two sums
+    assert h.orl_linear_bwd_scratch(5, 32) == 2 * 32 and h.orl_linear_bwd_scratch(1000, 32) == 2 * 125 * 32
 
 
 def test_norm_rope_gradient_refuses(h):
