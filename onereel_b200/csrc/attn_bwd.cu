@@ -495,13 +495,19 @@ struct BwdThread {
         lane_off(static_cast<uint32_t>(32 * (sw & 3) + 16 * (sw >> 2)) << 16) {}
 };
 
-// rows of an accumulator scaled to bf16: tile row r of the item -> dst row row0 + r, columns head * D ..
+// Gradient rows go out through shared memory (the tiles there are done with): written as bf16 pairs at a pitch that
+// spreads a warp's eight rows over all banks, then one bulk copy per row of D values. (Stored from the registers, 4 bytes
+// per lane, they cost a block 4 us.)
 template <int D>
-__device__ __forceinline__ void bwd_store(uint32_t acc, const BwdThread& th, const BwdWork& wi, float f,
-                                          __nv_bfloat16* __restrict__ dst, int heads) {
-  const bool v0 = th.row < wi.rows, v1 = th.row + 8 < wi.rows;
-  __nv_bfloat16* o0 = dst + (static_cast<long long>(wi.row0) + th.row) * heads * D + wi.head * D + 2 * th.cq;
-  __nv_bfloat16* o1 = o0 + 8ll * heads * D;
+struct BwdOut {
+  static constexpr int kPitch = 2 * D + 16;             // bytes
+  static constexpr int kBytes = 128 * kPitch;
+};
+
+// accumulator columns times f into staging slot i
+template <int D>
+__device__ __forceinline__ void bwd_stage(const BwdShared& sh, uint32_t acc, const BwdThread& th, float f, int i) {
+  uint8_t* row = sh.smem + i * BwdOut<D>::kBytes + th.row * BwdOut<D>::kPitch + 4 * th.cq;
 #pragma unroll
   for (int ch = 0; ch < D / 64; ++ch) {
     uint32_t o[32];
@@ -509,14 +515,27 @@ __device__ __forceinline__ void bwd_store(uint32_t acc, const BwdThread& th, con
     tmem_wait_ld();
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      const int col = 64 * ch + 8 * r;
-      if (v0)
-        *reinterpret_cast<uint32_t*>(o0 + col) =
-            pack_bf16x2(__uint_as_float(o[4 * r + 0]) * f, __uint_as_float(o[4 * r + 1]) * f);
-      if (v1)
-        *reinterpret_cast<uint32_t*>(o1 + col) =
-            pack_bf16x2(__uint_as_float(o[4 * r + 2]) * f, __uint_as_float(o[4 * r + 3]) * f);
+      uint8_t* at = row + 128 * ch + 16 * r;
+      *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(__uint_as_float(o[4 * r + 0]) * f, __uint_as_float(o[4 * r + 1]) * f);
+      *reinterpret_cast<uint32_t*>(at + 8 * BwdOut<D>::kPitch) =
+          pack_bf16x2(__uint_as_float(o[4 * r + 2]) * f, __uint_as_float(o[4 * r + 3]) * f);
     }
+  }
+}
+
+// the n staged tensors' rows to dst[0..n): 256 threads, one row copy each while there are rows
+template <int D>
+__device__ __forceinline__ void bwd_flush(const BwdShared& sh, const BwdWork& wi, int n, __nv_bfloat16* dst0,
+                                          __nv_bfloat16* dst1, int heads) {
+  fence_async_smem();
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  const int t = threadIdx.x - 128, i = t >> 7, r = t & 127;
+  if (i < n && r < wi.rows) {
+    __nv_bfloat16* dst = i == 0 ? dst0 : dst1;
+    bulk_store(dst + ((static_cast<long long>(wi.row0) + r) * heads + wi.head) * D,
+               sh.sbase + i * BwdOut<D>::kBytes + r * BwdOut<D>::kPitch, 2 * D);
+    bulk_commit();
+    bulk_wait_read<0>();                                // shared memory outlives the copies
   }
 }
 
@@ -654,8 +673,10 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
     return;
   }
   tc_after_wait();
-  bwd_store<D>(tmem + C::kColDv, th, wi, 1.f, dv, heads);
-  bwd_store<D>(tmem + C::kColDk, th, wi, scale, dk, heads);
+  static_assert(2 * BwdOut<D>::kBytes <= C::kStatOff, "staging");
+  bwd_stage<D>(sh, tmem + C::kColDv, th, 1.f, 0);
+  bwd_stage<D>(sh, tmem + C::kColDk, th, scale, 1);
+  bwd_flush<D>(sh, wi, 2, dv, dk, heads);
 }
 
 template <int D>
@@ -784,7 +805,8 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
     return;
   }
   tc_after_wait();
-  bwd_store<D>(tmem + C::kColDq, th, wi, scale, dq, heads);
+  bwd_stage<D>(sh, tmem + C::kColDq, th, scale, 0);
+  bwd_flush<D>(sh, wi, 1, dq, dq, heads);
 }
 
 template <int D>
@@ -815,6 +837,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 32 * 2) {
+    tma_prefetch_map(&tm_q);
+    tma_prefetch_map(&tm_k);
+    tma_prefetch_map(&tm_v);
+    tma_prefetch_map(&tm_do);
+  }
   const BwdWork wi = work[blockIdx.x];
   const bool dkv = wi.kind == kDkv;
 
@@ -1149,9 +1177,11 @@ extern "C" int orl_attn_bwd(const void* q, const void* k, const void* v, const v
 }
 
 // ------------------------------------------------------------------------------------------------ device plan
-// orl_attn_bwd_cu: cu_seqlens on the device, the work list planned there (one block). Keys of different segments do
+// orl_attn_bwd_cu: cu_seqlens on the device, the work list planned there. Keys of different segments do
 // not overlap, so a segment's key rows have one query range and its query rows one key range: ranges[i] = segment
 // i's query range, ranges[n_seg + i] its key range. Rows before the first and after the last segment get zeros.
+// Every block ranks the segments for itself and writes its share of the items (one block took 30 us to write the 12000
+// items of two scenes of 22000 rows and 16 heads).
 // Scratch: a 32-byte header (slot 0: item count), the items, then the ranges.
 namespace orl {
 
@@ -1183,8 +1213,10 @@ __global__ void __launch_bounds__(1024)
     s_row[n_seg + i] = static_cast<int>(q0);
     s_len[n_seg + i] = lq;
     s_tiles[n_seg + i] = (lk + kDqRows - 1) / kDqRows;
-    ranges[i] = make_int2(static_cast<int>(q0), lq);
-    ranges[n_seg + i] = make_int2(static_cast<int>(k0), lk);
+    if (blockIdx.x == 0) {
+      ranges[i] = make_int2(static_cast<int>(q0), lq);
+      ranges[n_seg + i] = make_int2(static_cast<int>(k0), lk);
+    }
   }
   if (t < 4) {
     const int32_t* cu = t < 2 ? cu_k : cu_q;
@@ -1198,7 +1230,7 @@ __global__ void __launch_bounds__(1024)
   }
   __syncthreads();
   if (bad) {
-    if (t == 0) {
+    if (t == 0 && blockIdx.x == 0) {
       work[0].row0 = 0;
       atomicOr(err, kErrPlan);
     }
@@ -1227,13 +1259,13 @@ __global__ void __launch_bounds__(1024)
   __syncthreads();
   const int n = total, m = n_ranked;
   if (static_cast<long long>(n) + 1 > capacity) {
-    if (t == 0) {
+    if (t == 0 && blockIdx.x == 0) {
       work[0].row0 = 0;
       atomicOr(err, kErrPlan);
     }
     return;
   }
-  for (int it = t; it < n; it += blockDim.x) {
+  for (int it = blockIdx.x * blockDim.x + t; it < n; it += gridDim.x * blockDim.x) {
     int lo = 0, hi = m - 1;                 // first rank whose items end after it
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -1256,7 +1288,7 @@ __global__ void __launch_bounds__(1024)
     w.whole = w.n_tiles > 0 && keys > 0 && keys <= kWholeKeys ? 1 : 0;
     work[1 + it] = w;
   }
-  if (t == 0) work[0].row0 = n;
+  if (t == 0 && blockIdx.x == 0) work[0].row0 = n;
 }
 
 }  // namespace orl
@@ -1300,7 +1332,8 @@ extern "C" int orl_attn_bwd_cu(const void* q, const void* k, const void* v, cons
   }
   BwdWork* work = static_cast<BwdWork*>(scratch_dev);
   int2* ranges = reinterpret_cast<int2*>(work + 1 + items);
-  attn_bwd_plan_kernel<<<1, 1024, smem, stream>>>(cu_q_dev, cu_k_dev, n_seg, heads, nq, nk, work, ranges, 1 + items,
+  const int blocks = static_cast<int>(std::min<long long>(64, (items + 1023) / 1024));
+  attn_bwd_plan_kernel<<<blocks, 1024, smem, stream>>>(cu_q_dev, cu_k_dev, n_seg, heads, nq, nk, work, ranges, 1 + items,
                                                   err_dev);
   if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
   auto launch = head_dim == 64 ? launch_attn_bwd<64> : launch_attn_bwd<128>;
