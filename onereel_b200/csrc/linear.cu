@@ -9,7 +9,10 @@
 // accumulators, warps 4-7 drain the other: bias, activation, gate, residual and the bf16 stores run under the next
 // tile's MMAs. kCtas = 2: a cluster of two CTAs owns a 256 x 256 tile (tcgen05 cta_group::2): each holds half of A's
 // rows and half of B's, so an SM reads 64 bytes of shared memory per clock where a 128 x 256 tile of its own would read
-// 96 and fill as much again. Rows and columns past the ends are zeros (TMA fill) and are not stored.
+// 96 and fill as much again. Its epilogue moves 32-row x 64-column pieces through shared memory: the residual comes in
+// and y (and z) go out by TMA, whole 128-byte lines at a time (stored from the registers, a row per lane, the epilogue of
+// 9540 x 2048 -> 8192 with z took longer than the product: 319 us instead of 222). kCtas = 1 serves problems too small
+// for that, down to a few rows. Rows and columns past the ends are zeros (TMA fill) and are not stored.
 // Every mbarrier wait is bounded (ptx.cuh).
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -28,27 +31,33 @@ namespace orl {
 
 // ------------------------------------------------------------------------------------------------ activations
 // With t = 1 / (1 + exp(-a)): silu a = z, gelu_tanh a = 2 sqrt(2 / pi) (z + 0.044715 z^3) (tanh(u) = 2 sigmoid(2u) - 1);
-// act = z t in both.
-constexpr float kLog2eF = 1.4426950408889634f;
+// act = z t in both, act' = t + z a' t (1 - t). z^2 is capped where t has long been 0 or 1, so that a and a' stay finite.
+constexpr float kMinusLog2e = -1.4426950408889634f;
 constexpr float kGelu = 1.5957691216057308f;          // 2 sqrt(2 / pi)
 constexpr float kGelu3 = 0.044715f;
 
-__device__ __forceinline__ float sigmoid(float a) { return __fdividef(1.0f, 1.0f + ex2(-a * kLog2eF)); }
+template <int kAct>
+__device__ __forceinline__ float gate_of(float z, float z2) {
+  const float a = kAct == ORL_ACT_GELU_TANH ? z * fmaf(kMinusLog2e * kGelu * kGelu3, z2, kMinusLog2e * kGelu)
+                                            : z * kMinusLog2e;
+  return __fdividef(1.0f, 1.0f + ex2(a));
+}
 
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == ORL_ACT_GELU_TANH) return z * sigmoid(kGelu * (z + kGelu3 * z * z * z));
-  if (act == ORL_ACT_SILU) return z * sigmoid(z);
-  return z;
+template <int kAct>
+__device__ __forceinline__ float activate(float z) {
+  if (kAct == ORL_ACT_NONE) return z;
+  return z * gate_of<kAct>(z, fminf(z * z, 1e4f));
 }
 
 // act(z) and act'(z)
-__device__ __forceinline__ float2 activate_slope(float z, int act) {
-  if (act == ORL_ACT_NONE) return make_float2(z, 1.0f);
-  const bool gelu = act == ORL_ACT_GELU_TANH;
-  const float t = sigmoid(gelu ? kGelu * (z + kGelu3 * z * z * z) : z);
-  const float da = gelu ? kGelu * (1.0f + 3.0f * kGelu3 * z * z) : 1.0f;
-  const float s = t * (1.0f - t);                     // 0 far out, where z^2 may be infinite
-  return make_float2(z * t, s == 0.0f ? t : t + z * da * s);
+template <int kAct>
+__device__ __forceinline__ float2 activate_slope(float z) {
+  if (kAct == ORL_ACT_NONE) return make_float2(z, 1.0f);
+  const float z2 = fminf(z * z, 1e4f);
+  const float t = gate_of<kAct>(z, z2);
+  const float s = fmaf(-t, t, t);                      // t (1 - t): 0 far out
+  const float d = kAct == ORL_ACT_GELU_TANH ? fmaf(3.0f * kGelu * kGelu3, z2, kGelu) * s : s;
+  return make_float2(z * t, fmaf(z, d, t));
 }
 
 __device__ __forceinline__ void unpack8(uint4 r, float (&f)[8]) {
@@ -76,36 +85,46 @@ struct Epilogue {
   int act;
 };
 
-// eight columns n0.. of one row: f = products in, y out
-__device__ __forceinline__ void finish8(const Epilogue& ep, long long row, int n0, int n, float (&f)[8]) {
-  const long long at = row * n + n0;
+// eight columns n0.. of a row: f = products in, y out, z = their bf16 sums with the bias; res: the residual's values or
+// null
+__device__ __forceinline__ void finish8(const Epilogue& ep, int n0, float (&f)[8], uint4& z, const uint4* res) {
   float t[8];
   if (ep.bias != nullptr) {
     unpack8(__ldg(reinterpret_cast<const uint4*>(ep.bias + n0)), t);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] += t[i];
   }
-  if (ep.z != nullptr) *reinterpret_cast<uint4*>(ep.z + at) = pack8(f);
-  if (ep.act != ORL_ACT_NONE) {
+  z = pack8(f);
+  if (ep.act == ORL_ACT_GELU_TANH) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = activate(f[i], ep.act);
+    for (int i = 0; i < 8; ++i) f[i] = activate<ORL_ACT_GELU_TANH>(f[i]);
+  } else if (ep.act == ORL_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = activate<ORL_ACT_SILU>(f[i]);
   }
   if (ep.gate != nullptr) {
     unpack8(__ldg(reinterpret_cast<const uint4*>(ep.gate + n0)), t);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] *= t[i];
   }
-  if (ep.residual != nullptr) {
-    unpack8(*reinterpret_cast<const uint4*>(ep.residual + row * ep.ldr + n0), t);
+  if (res != nullptr) {
+    unpack8(*res, t);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] += t[i];
   }
-  *reinterpret_cast<uint4*>(ep.y + at) = pack8(f);
+}
+
+// the same with its loads and stores straight from memory
+__device__ __forceinline__ void finish8_global(const Epilogue& ep, long long row, int n0, int n, float (&f)[8]) {
+  uint4 z, r;
+  if (ep.residual != nullptr) r = *reinterpret_cast<const uint4*>(ep.residual + row * ep.ldr + n0);
+  finish8(ep, n0, f, z, ep.residual != nullptr ? &r : nullptr);
+  if (ep.z != nullptr) *reinterpret_cast<uint4*>(ep.z + row * n + n0) = z;
+  *reinterpret_cast<uint4*>(ep.y + row * n + n0) = pack8(f);
 }
 
 // ------------------------------------------------------------------------------------------------ matrix product
 
-constexpr int kGemmThreads = 256;
 constexpr int kBk = 64;                                // contraction depth of a stage: one 128-byte swizzle row
 
 template <int kCtas, int BN>
@@ -115,18 +134,28 @@ struct GemmCfg {
   static constexpr int kABytes = 128 * kBk * 2;
   static constexpr int kBBytes = kBRows * kBk * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = (196 * 1024) / kStageBytes;
-  static constexpr int kBarOff = kStages * kStageBytes;
+  // kCtas = 2: eight epilogue warps, two per 32 rows that take pieces by turns (with four, bias, gelu and z of a 256 x 256
+  // tile at k = 2048 took longer than its product); staging of two pieces each: y (the residual first) and z, or y twice
+  static constexpr bool kStaged = kCtas == 2;
+  static constexpr int kEpiWarps = kStaged ? 8 : 4;
+  static constexpr int kThreads = 128 + 32 * kEpiWarps;
+  static constexpr int kPiece = 32 * 128;
+  static constexpr int kStagingBytes = kStaged ? kEpiWarps * 2 * kPiece : 0;
+  static constexpr int kStages = (224 * 1024 - kStagingBytes) / kStageBytes;
+  static constexpr int kStagingOff = kStages * kStageBytes;
+  static constexpr int kBarOff = kStagingOff + kStagingBytes;
   static constexpr int kBarFull = 0;
   static constexpr int kBarEmpty = kStages;
   static constexpr int kBarAccFull = 2 * kStages;      // + accumulator
   static constexpr int kBarAccEmpty = kBarAccFull + 2;
-  static constexpr int kBarDrain = kBarAccEmpty + 2;
+  static constexpr int kBarRes = kBarAccEmpty + 2;     // residual piece landed, per epilogue warp and buffer
+  static constexpr int kBarDrain = kBarRes + 2 * kEpiWarps;
   static constexpr int kNumBars = kBarDrain + 1;
   static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
   static constexpr uint32_t kTmemCols = 2 * BN;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
-  static_assert(kTmemCols == 128 || kTmemCols == 256 || kTmemCols == 512, "TMEM allocation size");
+  static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32 && kTmemCols <= 512, "TMEM allocation size");
+  static_assert(kStageBytes % 1024 == 0 && (!kStaged || BN % 64 == 0), "tile alignment");
 };
 
 struct GemmShape {
@@ -204,9 +233,10 @@ __device__ __forceinline__ int2 tile_at(const GemmShape& g, int t) {
 }
 
 template <int kCtas, int BN, bool kAmn, bool kBmn>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(GemmCfg<kCtas, BN>::kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                const __grid_constant__ GemmShape g, const __grid_constant__ Epilogue ep, int* __restrict__ err) {
+                const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_z,
+                const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ GemmShape g, const __grid_constant__ Epilogue ep, int* __restrict__ err) {
   using C = GemmCfg<kCtas, BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -228,8 +258,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(sh.bar(C::kBarAccFull + i), 1);
-      mbar_init(sh.bar(C::kBarAccEmpty + i), 4 * kCtas);
+      mbar_init(sh.bar(C::kBarAccEmpty + i), C::kEpiWarps * kCtas);
     }
+    for (int i = 0; i < 2 * C::kEpiWarps; ++i) mbar_init(sh.bar(C::kBarRes + i), 1);
     mbar_init(sh.bar(C::kBarDrain), 1);
     *sh.abort_flag = 0;
     fence_mbar_init();
@@ -343,36 +374,104 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue: one row per thread
-    int n = 0;
-    for (int t = cluster; t < n_tiles; t += n_clusters, ++n) {
+    const int ew = warp - 4;
+    const uint32_t lanes = static_cast<uint32_t>(32 * (ew & 3)) << 16;
+    const bool res = ep.residual != nullptr, two = ep.z == nullptr;    // two: both pieces are y's, by turns
+    uint8_t* staging = smem + C::kStagingOff + ew * 2 * C::kPiece;
+    const uint32_t staging_s = sh.sbase + C::kStagingOff + ew * 2 * C::kPiece;
+    int n = 0, piece = 0;                                              // pieces done by this warp
+    bool ok = true;
+    for (int t = cluster; ok && t < n_tiles; t += n_clusters, ++n) {
       const int buf = n & 1;
       const int2 at = tile_at(g, t);
-      const long long row = static_cast<long long>(at.x) * C::kTileM + 128 * rank + 32 * (warp - 4) + lane;
+      const int row0 = at.x * C::kTileM + 128 * rank + 32 * (ew & 3);
       const int n0 = at.y * BN;
-      if (!mbar_wait(sh.bar(C::kBarAccFull + buf), (n >> 1) & 1, sh.abort_flag)) {
-        atomicOr(err, kErrTimeoutSoftmax);
-        break;
-      }
-      __syncwarp();                          // lanes leave the wait one by one; the TMEM loads are warp-wide
-      tc_fence_after();
-      const uint32_t acc = tmem + buf * BN + (static_cast<uint32_t>(32 * (warp - 4)) << 16);
+      const uint32_t acc = tmem + buf * BN + lanes;
+      if constexpr (C::kStaged) {
+        // piece p goes into buffer b: free once the store that used it last has read it; then its residual comes in
+        auto prepare = [&](int p, int c) {
+          const int b = two ? p & 1 : 0;
+          if (lane == 0) {
+            if (two) bulk_wait_read<1>();
+            else bulk_wait_read<0>();
+            if (res) {
+              mbar_expect_tx(sh.bar(C::kBarRes + 2 * ew + b), C::kPiece);
+              tma_load_2d(staging_s + b * C::kPiece, &tm_r, sh.bar(C::kBarRes + 2 * ew + b), n0 + c, row0,
+                          policy_evict_first());
+            }
+          }
+          __syncwarp();
+        };
+        const int half = ew >> 2;                // this warp's pieces: half, half + 2, ...
+        const int n_pieces = row0 < g.m ? (min(BN, g.n - n0) + 63) / 64 : 0;
+        if (half < n_pieces) prepare(piece, 64 * half);
+        ok = mbar_wait(sh.bar(C::kBarAccFull + buf), (n >> 1) & 1, sh.abort_flag);
+        __syncwarp();                            // lanes leave the wait one by one; the TMEM loads are warp-wide
+        if (ok) tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        if (n0 + c >= g.n) break;
-        uint32_t v[32];
-        tmem_ld32(acc + c, v);
-        tmem_wait_ld();
-        if (row < g.m) {
+        for (int i = half; ok && i < n_pieces; i += 2, ++piece) {
+          const int b = two ? piece & 1 : 0;
+          uint32_t v[64];
+          tmem_ld32(acc + 64 * i, *reinterpret_cast<uint32_t(*)[32]>(v));
+          tmem_ld32(acc + 64 * i + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+          tmem_wait_ld();
+          if (res) {
+            ok = mbar_wait(sh.bar(C::kBarRes + 2 * ew + b), (two ? piece >> 1 : piece) & 1, sh.abort_flag);
+            if (!ok) break;
+          }
+          uint8_t* y = staging + b * C::kPiece + lane * 128;
+          uint8_t* z = staging + C::kPiece + lane * 128;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (n0 + c + 8 * i < g.n) {
-              float f[8];
+          for (int c = 0; c < 8; ++c) {
+            const int col = n0 + 64 * i + 8 * c;
+            uint4* dst = reinterpret_cast<uint4*>(y + ((c ^ (lane & 7)) << 4));      // the 128-byte swizzle
+            float f[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[8 * i + e]);
-              finish8(ep, row, n0 + c + 8 * i, g.n, f);
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[8 * c + e]);
+            uint4 zz;
+            const uint4 r = res ? *dst : make_uint4(0u, 0u, 0u, 0u);
+            finish8(ep, min(col, g.n - 8), f, zz, res ? &r : nullptr);               // columns past the end: not stored
+            *dst = pack8(f);
+            if (!two) *reinterpret_cast<uint4*>(z + ((c ^ (lane & 7)) << 4)) = zz;
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tm_y, staging_s + b * C::kPiece, n0 + 64 * i, row0);
+            if (!two) tma_store_2d(&tm_z, staging_s + C::kPiece, n0 + 64 * i, row0);
+            bulk_commit();
+          }
+          if (i + 2 < n_pieces) prepare(piece + 1, 64 * (i + 2));
+        }
+        // the loop's waits may have been left by some lanes before others
+        __syncwarp();
+      } else {
+        ok = mbar_wait(sh.bar(C::kBarAccFull + buf), (n >> 1) & 1, sh.abort_flag);
+        __syncwarp();
+        if (ok) tc_fence_after();
+        const long long row = row0 + lane;
+#pragma unroll 1
+        for (int c = 0; ok && c < BN; c += 32) {
+          if (n0 + c >= g.n) break;
+          uint32_t v[32];
+          tmem_ld32(acc + c, v);
+          tmem_wait_ld();
+          if (row < g.m) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (n0 + c + 8 * i < g.n) {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[8 * i + e]);
+                finish8_global(ep, row, n0 + c + 8 * i, g.n, f);
+              }
             }
           }
         }
+      }
+      if (!ok) {
+        atomicOr(err, kErrTimeoutSoftmax);
+        break;
       }
       tc_fence_before();
       __syncwarp();
@@ -380,6 +479,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (kCtas == 2) mbar_arrive_leader(sh.bar(C::kBarAccEmpty + buf));
         else mbar_arrive(sh.bar(C::kBarAccEmpty + buf));
       }
+    }
+    if (C::kStaged && lane == 0) {
+      if (!ok && res) {                          // a residual piece may be in flight: it lands before shared memory goes
+        const unsigned long long t0 = global_ns();
+        while (!mbar_try_wait(sh.bar(C::kBarRes + 2 * ew + (two ? piece & 1 : 0)), (two ? piece >> 1 : piece) & 1))
+          if (global_ns() - t0 > kWaitLimitNs) {
+            atomicOr(err, kErrTimeoutDrain);
+            break;
+          }
+      }
+      bulk_wait_read<0>();
     }
   }
 
@@ -395,27 +505,27 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
 // ------------------------------------------------------------------------------------------------ few rows
 // m <= kRowsMax rows: the weight is read once and little else happens, so tensor-core tiles would leave most SMs idle
-// (n / 64 CTAs). One warp per output column pair streams their weight rows with 16-byte loads; x is in shared memory.
+// (n / 64 CTAs). A block of eight warps takes eight output columns; the warps split the depth and read their parts of the
+// eight weight rows with 16-byte loads, all of them in flight at once; sums meet in shared memory.
 constexpr int kRowsMax = 4;
-constexpr int kRowsWarps = 8;
 
 template <int M>
-__global__ void __launch_bounds__(32 * kRowsWarps) linear_rows_kernel(const __nv_bfloat16* __restrict__ x,
-                                                                      long long ldx,
-                                                                      const __nv_bfloat16* __restrict__ w,
-                                                                      long long ldw, int n, int k, Epilogue ep) {
+__global__ void __launch_bounds__(256) linear_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx,
+                                                          const __nv_bfloat16* __restrict__ w, long long ldw, int n,
+                                                          int k, Epilogue ep) {
+  __shared__ float part[M * 8][9];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = 8 * (blockIdx.x * kRowsWarps + warp);
-  if (n0 >= n) return;                                  // n is a multiple of 8
+  const int n0 = 8 * blockIdx.x;                        // n is a multiple of 8
+  const __nv_bfloat16* w0 = w + static_cast<long long>(n0) * ldw;
   float acc[M][8];
 #pragma unroll
   for (int r = 0; r < M; ++r)
 #pragma unroll
     for (int c = 0; c < 8; ++c) acc[r][c] = 0.f;
-  for (int e = 8 * lane; e < k; e += 256) {
+  for (int e = 256 * warp + 8 * lane; e < k; e += 2048) {
     uint4 wr[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) wr[c] = __ldcs(reinterpret_cast<const uint4*>(w + (n0 + c) * ldw + e));
+    for (int c = 0; c < 8; ++c) wr[c] = __ldcs(reinterpret_cast<const uint4*>(w0 + c * ldw + e));
     float xf[M][8];
 #pragma unroll
     for (int r = 0; r < M; ++r) unpack8(__ldg(reinterpret_cast<const uint4*>(x + r * ldx + e)), xf[r]);
@@ -432,12 +542,23 @@ __global__ void __launch_bounds__(32 * kRowsWarps) linear_rows_kernel(const __nv
 #pragma unroll
   for (int r = 0; r < M; ++r)
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
+    for (int c = 0; c < 8; ++c) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc[r][c] += __shfl_xor_sync(0xffffffffu, acc[r][c], o);
+      if (lane == 0) part[8 * r + c][warp] = acc[r][c];
+    }
+  __syncthreads();
+  const int r = threadIdx.x;
+  if (r < M) {
+    float f[8];
 #pragma unroll
-  for (int r = 0; r < M; ++r)
-    if (lane == r) finish8(ep, r, n0, n, acc[r]);
+    for (int c = 0; c < 8; ++c) {
+      f[c] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[c] += part[8 * r + c][i];
+    }
+    finish8_global(ep, r, n0, n, f);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ dz and column sums
@@ -445,9 +566,10 @@ __global__ void __launch_bounds__(32 * kRowsWarps) linear_rows_kernel(const __nv
 // 256 columns (8 per thread, 32 threads across) and a strip of rows (8 at a time); its sums are one partial row.
 constexpr int kDzBlocks = 1184;                          // at most, over rows and columns: 8 per SM
 
-__global__ void __launch_bounds__(256) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, long long lddy,
+template <int kAct, bool kGateGrad>
+__global__ void __launch_bounds__(256, 4) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, long long lddy,
                                                         const __nv_bfloat16* __restrict__ z,
-                                                        const __nv_bfloat16* __restrict__ gate, int act, int m, int n,
+                                                        const __nv_bfloat16* __restrict__ gate, int m, int n,
                                                         __nv_bfloat16* __restrict__ dz, float* __restrict__ part_b,
                                                         float* __restrict__ part_g) {
   __shared__ float red[8][257];
@@ -462,26 +584,42 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const __nv_bfloat16* __r
   }
   if (on && gate != nullptr) unpack8(__ldg(reinterpret_cast<const uint4*>(gate + col)), gf);
   if (on) {
-    for (int r = 8 * blockIdx.y + ty; r < m; r += 8 * gridDim.y) {
-      const long long at = static_cast<long long>(r) * n + col;
-      float d[8], h[8];
-      unpack8(*reinterpret_cast<const uint4*>(dy + r * lddy + col), d);
-      if (z != nullptr) {
-        unpack8(*reinterpret_cast<const uint4*>(z + at), h);
+    const int stride = 8 * gridDim.y;
+    const bool slope = z != nullptr;
+    for (int r0 = 8 * blockIdx.y + ty; r0 < m; r0 += 2 * stride) {
+      uint4 rd[2], rz[2];                                // two rows' loads in flight
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 a = activate_slope(h[i], act);
-          sg[i] += d[i] * a.x;
-          d[i] *= gf[i] * a.y;
+      for (int u = 0; u < 2; ++u) {
+        const int r = r0 + u * stride;
+        rd[u] = rz[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < m) {
+          rd[u] = __ldcs(reinterpret_cast<const uint4*>(dy + r * lddy + col));
+          if (slope) rz[u] = __ldcs(reinterpret_cast<const uint4*>(z + static_cast<long long>(r) * n + col));
         }
       }
-      if (dz != nullptr) *reinterpret_cast<uint4*>(dz + at) = pack8(d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sb[i] += d[i];
+      for (int u = 0; u < 2; ++u) {
+        const int r = r0 + u * stride;
+        float d[8];
+        unpack8(rd[u], d);
+        if (slope) {
+          float h[8];
+          unpack8(rz[u], h);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 a = activate_slope<kAct>(h[i]);
+            if (kGateGrad) sg[i] += d[i] * a.x;
+            d[i] *= gf[i] * a.y;
+          }
+        }
+        if (dz != nullptr && r < m) *reinterpret_cast<uint4*>(dz + static_cast<long long>(r) * n + col) = pack8(d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sb[i] += d[i];
+      }
     }
   }
 #pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
+  for (int which = 0; which < (kGateGrad ? 2 : 1); ++which) {
     float* part = which == 0 ? part_b : part_g;
     if (part == nullptr) continue;
     __syncthreads();
@@ -516,6 +654,12 @@ static int launch_gemm(const void* a, long long lda, const void* b, long long ld
   if (rc != ORL_OK) return rc;
   rc = kBmn ? make_rows_map(&mb, b, g.k, g.n, ldb, kBk) : make_rows_map(&mb, b, g.n, g.k, ldb, C::kBRows);
   if (rc != ORL_OK) return rc;
+  CUtensorMap my = ma, mz = ma, mr = ma;                 // used where there is a z, a residual
+  if (C::kStaged) {
+    if ((rc = make_rows_map(&my, ep.y, g.m, g.n, g.n, 32)) != ORL_OK) return rc;
+    if (ep.z != nullptr && (rc = make_rows_map(&mz, ep.z, g.m, g.n, g.n, 32)) != ORL_OK) return rc;
+    if (ep.residual != nullptr && (rc = make_rows_map(&mr, ep.residual, g.m, g.n, ep.ldr, 32)) != ORL_OK) return rc;
+  }
   auto kernel = gemm_kernel<kCtas, BN, kAmn, kBmn>;
   static std::mutex mu;
   static int clusters[kMaxDevices] = {};                 // clusters resident at once
@@ -526,7 +670,7 @@ static int launch_gemm(const void* a, long long lda, const void* b, long long ld
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kCtas;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -545,18 +689,22 @@ static int launch_gemm(const void* a, long long lda, const void* b, long long ld
     most = clusters[dev];
   }
   cfg.gridDim = dim3(static_cast<unsigned>(kCtas * std::min(most, g.tiles_m * g.tiles_n)));
-  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, g, ep, err) == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, my, mz, mr, g, ep, err) == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
 }
 
-// Tile choice: the pair's 256 x 256 tile reads the least shared memory per MMA, but needs enough tiles to occupy the 74
-// pairs; below that, 128 x 64 tiles spread the work (and the streaming of the weight) over more SMs.
+// Tile choice: the largest tile that still occupies the GPU. The pair's 256 x 256 tile reads the least shared memory per
+// MMA, 256 x 128 has twice the tiles; below that one CTA takes 128 x 64, or 128 x 32 where few rows leave the streaming of
+// the weight to too few SMs.
 template <bool kAmn, bool kBmn>
 static int gemm(const void* a, long long lda, const void* b, long long ldb, int m, int n, int k, const Epilogue& ep,
                 int* err, cudaStream_t stream) {
   GemmShape g{m, n, k, 0, 0};
-  const long long big = (static_cast<long long>(m) + 255) / 256 * ((n + 255) / 256);
-  if (big >= 64) return launch_gemm<2, 256, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
-  return launch_gemm<1, 64, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
+  auto tiles = [&](int tm, int tn) { return (static_cast<long long>(m) + tm - 1) / tm * ((n + tn - 1) / tn); };
+  if (m > 128 && tiles(256, 256) >= 60) return launch_gemm<2, 256, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
+  if (m > 128 && tiles(256, 128) >= 48) return launch_gemm<2, 128, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
+  if (kBmn || tiles(128, 64) >= 100) return launch_gemm<1, 64, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
+  if constexpr (!kBmn) return launch_gemm<1, 32, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
+  return ORL_ERR_UNSUPPORTED;
 }
 
 static bool lin_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -588,13 +736,13 @@ extern "C" int orl_linear(const void* x, long long ldx, const void* w, long long
   const Epilogue ep{bf(bias), bf(gate), bf(residual), ldr, static_cast<__nv_bfloat16*>(y),
                     static_cast<__nv_bfloat16*>(z), act};
   if (m <= kRowsMax) {
-    const unsigned grid = static_cast<unsigned>((n / 8 + kRowsWarps - 1) / kRowsWarps);
+    const unsigned grid = static_cast<unsigned>(n / 8);
     const int nn = static_cast<int>(n), kk = static_cast<int>(k);
     switch (m) {
-      case 1: linear_rows_kernel<1><<<grid, 32 * kRowsWarps, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
-      case 2: linear_rows_kernel<2><<<grid, 32 * kRowsWarps, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
-      case 3: linear_rows_kernel<3><<<grid, 32 * kRowsWarps, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
-      default: linear_rows_kernel<4><<<grid, 32 * kRowsWarps, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep);
+      case 1: linear_rows_kernel<1><<<grid, 256, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
+      case 2: linear_rows_kernel<2><<<grid, 256, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
+      case 3: linear_rows_kernel<3><<<grid, 256, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep); break;
+      default: linear_rows_kernel<4><<<grid, 256, 0, stream>>>(bf(x), ldx, bf(w), ldw, nn, kk, ep);
     }
     return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
   }
@@ -631,9 +779,12 @@ extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, lon
     float* part_b = dbias != nullptr ? scratch : nullptr;
     float* part_g = dgate != nullptr ? scratch + static_cast<long long>(strips) * n : nullptr;
     const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(strips));
-    linear_dz_kernel<<<grid, 256, 0, stream>>>(
+    auto kernel = act == ORL_ACT_GELU_TANH ? (part_g ? linear_dz_kernel<ORL_ACT_GELU_TANH, true> : linear_dz_kernel<ORL_ACT_GELU_TANH, false>)
+                  : act == ORL_ACT_SILU    ? (part_g ? linear_dz_kernel<ORL_ACT_SILU, true> : linear_dz_kernel<ORL_ACT_SILU, false>)
+                                           : (part_g ? linear_dz_kernel<ORL_ACT_NONE, true> : linear_dz_kernel<ORL_ACT_NONE, false>);
+    kernel<<<grid, 256, 0, stream>>>(
         static_cast<const __nv_bfloat16*>(dy), lddy, static_cast<const __nv_bfloat16*>(z),
-        static_cast<const __nv_bfloat16*>(gate), act, mm, nn,
+        static_cast<const __nv_bfloat16*>(gate), mm, nn,
         z != nullptr && products ? static_cast<__nv_bfloat16*>(dz) : nullptr, part_b, part_g);
     if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
     if (part_b != nullptr && (rc = column_sum(part_b, strips, nn, n, dbias, stream)) != ORL_OK) return rc;

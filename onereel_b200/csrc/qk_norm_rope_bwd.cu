@@ -19,6 +19,7 @@
 namespace orl {
 
 constexpr int kNrBlocks = 592;             // at most: 148 SMs x 4 blocks of 256 threads
+constexpr int kNrRows = 2;                 // rows in flight per thread
 
 // tpr threads per row (hidden / 8, rounded up to whole warps), blockDim.x / tpr rows at a time
 __global__ void __launch_bounds__(1024) qk_norm_rope_bwd_kernel(
@@ -26,7 +27,7 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_bwd_kernel(
     const float* __restrict__ cos_t, const float* __restrict__ sin_t, __nv_bfloat16* __restrict__ dx,
     float* __restrict__ part, long long rows, int hidden, int head_dim, int per_head, float eps, int sin_shift,
     long long rope_ld, int tpr) {
-  __shared__ float2 red[2][32];
+  __shared__ float2 red[2][kNrRows][32];
   extern __shared__ float wsum[];          // [blockDim.x][8] at the end
   const int t = threadIdx.x, lane_row = t / tpr, tr = t % tpr;
   const int n_lanes = blockDim.x / tpr;
@@ -48,71 +49,96 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_bwd_kernel(
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
   const float inv_n = 1.0f / (per_head ? head_dim : hidden);
+  const int wpr = tpr >> 5;
+  const long long step = static_cast<long long>(gridDim.x) * n_lanes;
   int turn = 0;
-  for (long long row0 = static_cast<long long>(blockIdx.x) * n_lanes; row0 < rows;
-       row0 += static_cast<long long>(gridDim.x) * n_lanes, turn ^= 1) {
-    const long long row = row0 + lane_row;
-    const bool on = active && row < rows;
-    uint4 rx = make_uint4(0u, 0u, 0u, 0u), ry = rx;
-    float4 c0 = make_float4(0.f, 0.f, 0.f, 0.f), c1 = c0, s0 = c0, s1 = c0;
-    if (on) {
-      rx = __ldcs(reinterpret_cast<const uint4*>(x + row * hidden + e));
-      ry = __ldcs(reinterpret_cast<const uint4*>(dy + row * hidden + e));
-      const float4* cr = reinterpret_cast<const float4*>(cos_t + row * rope_ld + d);
-      const float4* sr = reinterpret_cast<const float4*>(sin_t + row * rope_ld + d);
-      c0 = __ldg(cr);
-      c1 = __ldg(cr + 1);
-      s0 = __ldg(sr);
-      s1 = __ldg(sr + 1);
-    }
-    const float c[4] = {c0.x, c0.z, c1.x, c1.z};
-    const float s[4] = {sin_shift ? s0.y : s0.x, sin_shift ? s0.w : s0.z, sin_shift ? s1.y : s1.x,
-                        sin_shift ? s1.w : s1.z};
-    const uint32_t ax[4] = {rx.x, rx.y, rx.z, rx.w}, ay[4] = {ry.x, ry.y, ry.z, ry.w};
-    float v[8], u[8];
-    float2 sum = make_float2(0.f, 0.f);    // x^2, w u x
+  for (long long row0 = static_cast<long long>(blockIdx.x) * n_lanes; row0 < rows; row0 += kNrRows * step, turn ^= 1) {
+    // the rows' loads are all in flight before anything is reduced; the rows stay packed meanwhile
+    uint4 rx[kNrRows], ry[kNrRows];
+    float c[kNrRows][4], s[kNrRows][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ax[i]));
-      const float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ay[i]));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-      u[2 * i] = g.x * c[i] + g.y * s[i];
-      u[2 * i + 1] = g.y * c[i] - g.x * s[i];
-      sum.x += f.x * f.x + f.y * f.y;
-      sum.y += w[2 * i] * u[2 * i] * f.x + w[2 * i + 1] * u[2 * i + 1] * f.y;
+    for (int k = 0; k < kNrRows; ++k) {
+      const long long row = row0 + k * step + lane_row;
+      rx[k] = ry[k] = make_uint4(0u, 0u, 0u, 0u);
+      float4 c0 = make_float4(0.f, 0.f, 0.f, 0.f), c1 = c0, s0 = c0, s1 = c0;
+      if (active && row < rows) {
+        rx[k] = __ldcs(reinterpret_cast<const uint4*>(x + row * hidden + e));
+        ry[k] = __ldcs(reinterpret_cast<const uint4*>(dy + row * hidden + e));
+        const float4* cr = reinterpret_cast<const float4*>(cos_t + row * rope_ld + d);
+        const float4* sr = reinterpret_cast<const float4*>(sin_t + row * rope_ld + d);
+        c0 = __ldg(cr);
+        c1 = __ldg(cr + 1);
+        s0 = __ldg(sr);
+        s1 = __ldg(sr + 1);
+      }
+      c[k][0] = c0.x, c[k][1] = c0.z, c[k][2] = c1.x, c[k][3] = c1.z;
+      s[k][0] = sin_shift ? s0.y : s0.x, s[k][1] = sin_shift ? s0.w : s0.z;
+      s[k][2] = sin_shift ? s1.y : s1.x, s[k][3] = sin_shift ? s1.w : s1.z;
     }
-    // per head: its head_dim / 8 consecutive lanes; whole row: its warps, through shared memory (two buffers by turns,
-    // so that one barrier per row is enough)
-    for (int o = per_head ? (head_dim >> 4) : 16; o > 0; o >>= 1) {
-      sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
-      sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
-    }
-    if (!per_head && tpr > 32) {
-      if ((t & 31) == 0) red[turn][t >> 5] = sum;
-      __syncthreads();
-      const int wpr = tpr >> 5;
-      sum = make_float2(0.f, 0.f);
-      for (int i = 0; i < wpr; ++i) {
-        const float2 p = red[turn][lane_row * wpr + i];
-        sum.x += p.x;
-        sum.y += p.y;
+    // pair i of row k: x, u = R^T dy
+    auto pair = [&](int k, int i, float2& v, float2& u) {
+      const uint32_t ax = i == 0 ? rx[k].x : i == 1 ? rx[k].y : i == 2 ? rx[k].z : rx[k].w;
+      const uint32_t ay = i == 0 ? ry[k].x : i == 1 ? ry[k].y : i == 2 ? ry[k].z : ry[k].w;
+      v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ax));
+      const float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ay));
+      u = make_float2(g.x * c[k][i] + g.y * s[k][i], g.y * c[k][i] - g.x * s[k][i]);
+    };
+    float2 sum[kNrRows];                   // x^2, w u x
+#pragma unroll
+    for (int k = 0; k < kNrRows; ++k) {
+      sum[k] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 v, u;
+        pair(k, i, v, u);
+        sum[k].x += v.x * v.x + v.y * v.y;
+        sum[k].y += w[2 * i] * u.x * v.x + w[2 * i + 1] * u.y * v.y;
       }
     }
-    const float inv = rsqrtf(sum.x * inv_n + eps);
-    const float back = inv * inv * inv * inv_n * sum.y;
-    uint4 packed;
-    uint32_t* o = &packed.x;
+    // per head: its head_dim / 8 consecutive lanes; whole row: its warps, through shared memory (two buffers by turns,
+    // so that one barrier per turn is enough)
+    for (int o = per_head ? (head_dim >> 4) : 16; o > 0; o >>= 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = u[2 * i] * inv, b = u[2 * i + 1] * inv;
-      acc[2 * i] += a * v[2 * i];
-      acc[2 * i + 1] += b * v[2 * i + 1];
-      const __nv_bfloat162 r = __floats2bfloat162_rn(a * w[2 * i] - v[2 * i] * back,
-                                                     b * w[2 * i + 1] - v[2 * i + 1] * back);
-      o[i] = *reinterpret_cast<const uint32_t*>(&r);
+      for (int k = 0; k < kNrRows; ++k) {
+        sum[k].x += __shfl_xor_sync(0xffffffffu, sum[k].x, o);
+        sum[k].y += __shfl_xor_sync(0xffffffffu, sum[k].y, o);
+      }
     }
-    if (on) *reinterpret_cast<uint4*>(dx + row * hidden + e) = packed;
+    if (!per_head && tpr > 32) {
+      if ((t & 31) == 0) {
+#pragma unroll
+        for (int k = 0; k < kNrRows; ++k) red[turn][k][t >> 5] = sum[k];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kNrRows; ++k) {
+        sum[k] = make_float2(0.f, 0.f);
+        for (int i = 0; i < wpr; ++i) {
+          const float2 p = red[turn][k][lane_row * wpr + i];
+          sum[k].x += p.x;
+          sum[k].y += p.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kNrRows; ++k) {
+      const long long row = row0 + k * step + lane_row;
+      const float inv = rsqrtf(sum[k].x * inv_n + eps);
+      const float back = inv * inv * inv * inv_n * sum[k].y;
+      uint4 packed;
+      uint32_t* o = &packed.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 v, u;
+        pair(k, i, v, u);
+        const float a = u.x * inv, b = u.y * inv;
+        acc[2 * i] += a * v.x;
+        acc[2 * i + 1] += b * v.y;
+        const __nv_bfloat162 r = __floats2bfloat162_rn(a * w[2 * i] - v.x * back, b * w[2 * i + 1] - v.y * back);
+        o[i] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+      if (active && row < rows) *reinterpret_cast<uint4*>(dx + row * hidden + e) = packed;
+    }
   }
   // this block's partial row: its row lanes, and the heads of a per-head weight, added in order
 #pragma unroll
