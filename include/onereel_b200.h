@@ -189,6 +189,13 @@ ORL_API int orl_pack(const orl_copy_run* runs_dev, int n_runs, long long total_v
              const void* const* src_bases, void* const* dst_bases, const int32_t* seg_len_dev, int n_seg,
              int32_t* cu_out_dev, int* err_dev, void* stream);
 
+/* Gradient of a pack (the torch.cat copies' backward): for every plane p < planes (<= 3) and row i < n_rows of row_bytes,
+ * dst[p] row i = the sum of the bf16 rows rows_dev[offsets_dev[i] .. offsets_dev[i + 1]) of src[p], in that order, in
+ * fp32; zeros where there are none. offsets_dev [n_rows + 1], rows_dev: device int32. src and dst: HOST arrays of
+ * device pointers. */
+ORL_API int orl_row_sum(const void* const* src, void* const* dst, int planes, const int32_t* offsets_dev,
+                        const int32_t* rows_dev, long long n_rows, long long row_bytes, void* stream);
+
 /* Log-sum-exp merge of two partial attention results over disjoint key sets (hunyuan15.py:274-276, ring.py:63-70):
  * o1 [n, heads, head_dim] bf16 (in/out) with its lse1 [heads, ld_lse1] fp32 (in/out), o2 / lse2 [heads, ld_lse2]
  * the second part; rows [0, n) of each. head_dim a multiple of 32. */

@@ -219,6 +219,11 @@ def _shared_rotation(ctx, plan, device):
     return res
 
 
+def _rotate_with(rows, cos, sin):
+    """rotate of scene.attend_plan for a _shared_rotation"""
+    return lambda packed, back: rotate_rows(packed, rows, cos, -sin if back else sin)
+
+
 class _RankPlan:
     """everything one rank needs for a scene-path layer: the pieces, the near / far segment plans (or the LSE
     overlap's local / remote plans), the receive-buffer layout"""
@@ -363,6 +368,10 @@ class Processor:
         H, Dh = q.shape[1:]
         lse_overlap = ctx.overlap == 'lse'
         plan = self._plan(H, Dh, q.device, lse_overlap)
+        if D.world() == 1 and A._wants_grad(q, k, v, eq, ek, ev) and plan.near is not None and plan.near.segs:
+            # one GPU: every key is local. The same values, differentiable (several ranks: no gradients)
+            rot = _shared_rotation(ctx, plan.near, k.device) if _move_active(ctx) else None
+            return S.attend_plan(plan.near, q, k, v, eq, ek, ev, None if rot is None else _rotate_with(*rot))
         _mark('start')
         ex = comm.kv_exchange(ctx.exchange, ctx.layout, ctx.own, ctx.T, k, v) if D.world() > 1 else None
         if ex is not None and ex.remote_index != plan.remote_index:

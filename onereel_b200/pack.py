@@ -56,6 +56,36 @@ class RunTable:
                                  s), 'orl_pack')
 
 
+class RowSum:
+    """the gradient of a pack: for each of n_rows source rows, the sum of its copies among the packed rows
+    (orl_row_sum). source / packed: int arrays, packed row packed[i] is a copy of source row source[i]."""
+
+    def __init__(self, source, packed, n_rows: int, device):
+        source, packed = np.asarray(source, np.int64), np.asarray(packed, np.int64)
+        if source.size and (source.min() < 0 or source.max() >= n_rows):
+            raise ValueError('source row out of range')
+        order = np.argsort(source, kind='stable')
+        offsets = np.searchsorted(source[order], np.arange(n_rows + 1))
+        self.n_rows, self.n_packed = n_rows, int(packed.max()) + 1 if packed.size else 0
+        self.offsets = torch.from_numpy(offsets.astype(np.int32)).to(device)
+        self.rows = torch.from_numpy(packed[order].astype(np.int32)).to(device)
+
+    def run(self, parts):
+        """parts: packed gradients [n, H, D] bf16, contiguous -> one [n_rows, H, D] each"""
+        dev = parts[0].device
+        for p in parts:
+            if p.shape[0] < self.n_packed or not p.is_contiguous() or p.dtype != torch.bfloat16:
+                raise ValueError('packed gradients must be contiguous bf16 with a row per packed row')
+        out = [p.new_empty(self.n_rows, *p.shape[1:]) for p in parts]
+        if self.n_rows:
+            arr = L.c_vp * len(parts)
+            L.check(L.lib().orl_row_sum(arr(*(p.data_ptr() for p in parts)), arr(*(o.data_ptr() for o in out)), len(parts),
+                                        self.offsets.data_ptr(), self.rows.data_ptr() if self.rows.numel() else None,
+                                        self.n_rows, row_bytes(out[0]), torch.cuda.current_stream(dev).cuda_stream),
+                    'orl_row_sum')
+        return out
+
+
 def row_bytes(x: torch.Tensor) -> int:
     return x.stride(0) * x.element_size()
 

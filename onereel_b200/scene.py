@@ -22,9 +22,10 @@ from dataclasses import dataclass, field
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from onereel_b200 import attention as A
-from onereel_b200.pack import RunTable
+from onereel_b200.pack import RowSum, RunTable
 
 # source ids of row runs
 VIDEO, TEXT, REMOTE = 0, 1, 2
@@ -178,6 +179,7 @@ class ScenePlan:
     cu_k: list = field(default_factory=list)
     cu_k_dev: torch.Tensor = None
     lk_dev: torch.Tensor = None
+    _row_sums: dict = field(default_factory=dict)
 
     def __post_init__(self):
         rb = self.row_bytes
@@ -214,6 +216,21 @@ class ScenePlan:
         dst = [0, 0, 0, kp.data_ptr(), 0, 0, 0, vp.data_ptr()]
         self.kv_table.run(src, dst, n_planes=2, seg_len_dev=self.lk_dev, cu_out=self.cu_k_dev)
         return kp, vp
+
+
+    def row_sums(self, source: int, n_rows: int) -> RowSum:
+        """the gradient of the pack for the n_rows rows of one source: which packed rows are their copies"""
+        key = (source, n_rows)
+        if key not in self._row_sums:
+            tok, at, row = [np.zeros(0, np.int64)], [np.zeros(0, np.int64)], 0
+            for s in self.segs:
+                for src, lo, hi in s.kv:
+                    if src == source:
+                        tok.append(np.arange(lo, hi))
+                        at.append(np.arange(row, row + hi - lo))
+                    row += hi - lo
+            self._row_sums[key] = RowSum(np.concatenate(tok), np.concatenate(at), n_rows, self.device)
+        return self._row_sums[key]
 
 
 # Optional launch timing for benchmarks: when TIMING is a list, every attend_segments call appends (start, end) CUDA
@@ -260,3 +277,55 @@ def attend_segments(plan: ScenePlan, q, eq, kp, vp, ov, ot, lse_v=None, lse_t=No
         e1.record(cur)
         H, Dh = launches[0][0].shape[1:]
         TIMING.append((e0, e1, sum(4.0 * a * b * H * Dh for x in launches for a, b in zip(x[4], x[6]))))
+
+
+class _PlanAttention(torch.autograd.Function):
+    """attend_segments of a plan on one GPU, differentiable: the backward pass packs K / V again, takes the packed
+    gradients of all segments in one call and sums every source row's copies"""
+
+    @staticmethod
+    def forward(ctx, plan, rotate, q, k, v, eq, ek, ev):
+        H = q.shape[1]
+        lse = lambda x: None if x is None else torch.empty(H, x.shape[0], dtype=torch.float32, device=x.device)
+        kp, vp = _packed_kv(plan, rotate, k, v, ek, ev)
+        ov, ot, lse_v, lse_t = torch.empty_like(q), None if eq is None else torch.zeros_like(eq), lse(q), lse(eq)
+        attend_segments(plan, q, eq, kp, vp, ov, ot, lse_v, lse_t)
+        ctx.plan, ctx.rotate = plan, rotate
+        ctx.save_for_backward(q, k, v, eq, ek, ev, ov, ot, lse_v, lse_t)
+        return ov, ot
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dov, dot):
+        plan, rotate = ctx.plan, ctx.rotate
+        q, k, v, eq, ek, ev, ov, ot, lse_v, lse_t = ctx.saved_tensors
+        kp, vp = _packed_kv(plan, rotate, k, v, ek, ev)
+        first = [s.q[1] + (0 if s.q[0] == VIDEO else q.shape[0]) for s in plan.segs]
+        if eq is None:
+            Q, out, lse, dout = q, ov, lse_v, dov
+        else:
+            Q, out, dout = torch.cat([q, eq]), torch.cat([ov, ot]), torch.cat([dov, dot])
+            lse = torch.cat([lse_v, lse_t], 1)
+        dQ, dk, dv = A.attend_grad(Q, kp, vp, out, lse, dout, first, plan.lq, plan.cu_k[:-1], plan.lk)
+        if rotate is not None:
+            rotate(dk, True)
+        grads = plan.row_sums(VIDEO, k.shape[0]).run([dk, dv])
+        text = [None, None] if ek is None else plan.row_sums(TEXT, ek.shape[0]).run([dk, dv])
+        deq = None if eq is None else dQ[q.shape[0]:]
+        return None, None, dQ[:q.shape[0]], *grads, deq, *text
+
+
+def _packed_kv(plan, rotate, k, v, ek, ev):
+    kp, vp = plan.pack_kv(k, v, ek, ev)
+    if rotate is not None:
+        rotate(kp, False)
+    return kp, vp
+
+
+def attend_plan(plan: ScenePlan, q, k, v, eq=None, ek=None, ev=None, rotate=None):
+    """(video outputs, text outputs or None) of a plan whose keys are all local: pack_kv and attend_segments with the same
+    values, differentiable in q, k, v and the text rows eq, ek, ev. rotate(packed keys, back): rotates rows of the packed
+    keys in place, back = True by the opposite angles."""
+    if any(src == REMOTE for s in plan.segs for src, _, _ in s.kv):
+        raise ValueError('attend_plan: the plan reads keys of other ranks')
+    return _PlanAttention.apply(plan, rotate, q, k, v, eq, ek, ev)

@@ -119,6 +119,8 @@ class Processor:
                 scenes = [(j, (lo * T, hi * T)) for j, (lo, hi) in enumerate(lay.ranges)]
                 plan = self.ctx._cache[key] = S.ScenePlan(S.scene_segments(lay, T, None, scenes, set(), (0, L)),
                                                           H * Dh * 2, H, q.device)
+            if D.world() == 1 and A._wants_grad(q, k, v):
+                return S.attend_plan(plan, q, k, v)[0]
             o = torch.empty_like(q)
             _attend(plan, q, None, k, v, None, None, o, None)
             return o

@@ -60,3 +60,50 @@ def test_python_refuses_cpu_tensors():
         linear(x, x)
     with pytest.raises(TypeError):
         qk_norm_rope(x, x[0], x, x, 1, 1e-6, True, 0)
+
+
+def test_row_sum_refuses_and_plans(h):
+    import ctypes
+
+    import numpy as np
+
+    from onereel_b200 import _lib as L
+    from onereel_b200.pack import RowSum
+    arr = L.c_vp * 2
+    src, dst, odd = arr(P, P), arr(P, P), arr(P, P + 8)
+    call = lambda s, d, planes, off, rows, n, rb: h.orl_row_sum(s, d, planes, off, rows, n, rb, None)
+    assert call(src, dst, 4, P, P, 5, 64) == -1 and call(src, dst, 0, P, P, 5, 64) == -1
+    assert call(src, dst, 2, None, P, 5, 64) == -1 and call(src, dst, 2, P, P, -1, 64) == -1
+    assert call(src, dst, 2, P, P, 5, 0) == -1 and call(arr(P, None), dst, 2, P, P, 5, 64) == -1
+    assert call(src, dst, 2, P, P, 5, 24) == -2 and call(src, odd, 2, P, P, 5, 64) == -2
+    assert call(src, dst, 2, P, P, 0, 64) == 0
+    s = RowSum([3, 0, 3, 1], [0, 1, 2, 3], 5, 'cpu')
+    assert s.offsets.tolist() == [0, 1, 2, 2, 4, 4] and s.rows.tolist() == [1, 3, 0, 2] and s.n_packed == 4
+    with pytest.raises(ValueError):
+        RowSum([5], [0], 5, 'cpu')
+    with pytest.raises(ValueError):
+        RowSum([-1], [0], 5, 'cpu')
+    with pytest.raises(ValueError):
+        s.run([torch.zeros(3, 1, 8, dtype=torch.bfloat16)])
+
+
+def test_plan_row_sums_cover_every_copy():
+    """the copies that a scene plan's pack makes: every packed row is counted once, for its own source row"""
+    import numpy as np
+
+    from onereel_b200 import scene as S
+    from onereel_b200.layout import SceneLayout
+    lay = SceneLayout([3, 2, 4], halo=1, extra={0: [5], 2: [0]})
+    T, counts = 5, [2, 0, 3]
+    L = lay.n_frames * T
+    scenes = [(j, (lo * T, hi * T)) for j, (lo, hi) in enumerate(lay.ranges)]
+    segs = S.scene_segments(lay, T, counts, scenes, {0, 1, 2}, (0, L))
+    plan = S.ScenePlan(segs, 64, 1, 'cpu')
+    video, text = plan.row_sums(S.VIDEO, L), plan.row_sums(S.TEXT, sum(counts))
+    packed = [(src, r) for s in segs for src, lo, hi in s.kv for r in range(lo, hi)]
+    for rs, source, n in ((video, S.VIDEO, L), (text, S.TEXT, sum(counts))):
+        off, rows = rs.offsets.tolist(), rs.rows.tolist()
+        assert len(off) == n + 1
+        for i in range(n):
+            assert rows[off[i]:off[i + 1]] == [p for p, x in enumerate(packed) if x == (source, i)]
+    assert len(video.rows) + len(text.rows) == plan.n_keys
