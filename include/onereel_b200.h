@@ -124,7 +124,7 @@ ORL_API int orl_attn_fwd_noalloc(const void* q, const void* k, const void* v, vo
 
 #define ORL_ATTN_BWD_KV 0 /* the item's rows are key rows, its ranges the query rows that read them */
 #define ORL_ATTN_BWD_Q 1  /* the item's rows are query rows, its ranges the key rows they read */
-#define ORL_ATTN_BWD_WHOLE 64 /* segments of at most so many keys take delta from their one tile (field whole) */
+#define ORL_ATTN_BWD_WHOLE 64 /* segments of at most so many keys are one tile (field whole) */
 
 /* One backward work item: up to 128 rows of one head. */
 typedef struct orl_attn_bwd_work {
@@ -135,11 +135,12 @@ typedef struct orl_attn_bwd_work {
   int32_t range0;   /* first of its ranges */
   int32_t n_ranges; /* 0: the rows' gradients are zero */
   int32_t n_tiles;  /* tiles of its ranges: 128 query rows (kind KV) or 64 key rows (kind Q) */
-  int32_t whole;    /* 1: its tiles hold all keys of their queries, so delta is summed from them in fp32 */
+  int32_t whole;    /* kind Q, 1: its one tile holds all keys of its queries */
 } orl_attn_bwd_work;
 
 /* Work list of a backward call for segments given as in orl_attn_plan_ranges (key ranges may overlap, query ranges
- * may not) over nq query and nk key rows; rows of no segment get zero gradients. Returns the item count and stores
+ * may not) over nq query and nk key rows; rows of no segment get zero gradients. Items of kind Q come first: those of
+ * kind KV wait for what they publish, so a list without them ends in a timeout. Returns the item count and stores
  * the number of ranges (pairs first row, rows); if a buffer is NULL or too small returns -(items + 1000). */
 ORL_API int orl_attn_bwd_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start,
                               const int32_t* k_len, int n_seg, int heads, long long nq, long long nk,
@@ -148,7 +149,7 @@ ORL_API int orl_attn_bwd_plan(const int32_t* q_start, const int32_t* q_len, cons
 
 /* dq [nq, heads, head_dim], dk / dv [nk, heads, head_dim] bf16 from the forward's inputs, out and lse [heads, nq], the
  * gradient dout of out and, unless NULL, dlse [heads, nq] of lse. work_dev / ranges_dev: the plan in device memory.
- * stats_dev: scratch of 2 * heads * nq floats, 16-byte aligned. */
+ * stats_dev: scratch of 3 * heads * nq + 4 floats, 16-byte aligned. */
 ORL_API int orl_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
                          const float* lse, const float* dlse, void* dq, void* dk, void* dv, long long nq, long long nk,
                          int heads, int head_dim, float scale, const orl_attn_bwd_work* work_dev, int n_items,

@@ -331,7 +331,7 @@ def _bwd_args(q, k, v, out, lse, dout, dlse, extra: int = 0):
     dlse = None if dlse is None else _aligned(dlse)
     Nq, H, Dh = q.shape
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    stats = (8 * H * Nq + 15) // 16 * 16
+    stats = (12 * H * Nq + 31) // 16 * 16
     scratch = torch.empty(stats + extra, dtype=torch.uint8, device=q.device)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
             None if dlse is None else dlse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), Nq, k.shape[0], H, Dh)

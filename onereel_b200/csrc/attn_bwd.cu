@@ -28,10 +28,14 @@
 // both operands from shared memory costs (dO has no TMEM left). S and dP of a group's next tile are issued once it has
 // read them, dQ when dS is there.
 //
-// delta from the forward's bf16 o carries o's rounding. Over many keys that is lost in the rounding of dS, but over a few
-// keys dS is a small difference of large terms (two keys: dq 0.0040 off in the 2-norm instead of 0.0024; 32 keys and
-// more: the same). Where a tile holds all keys of its queries (at most 64), delta = sum_j P dP - dL is therefore taken
-// from the tile itself in fp32.
+// delta. do . o~ with the forward's bf16 o~ (P rounded, then o rounded) is off by some e_i, the same for all keys of query
+// i. In dq_i it adds e_i sum_j P k, one more error of the size of dS's roundings. In the dk it adds up: sum_j dS_ij should
+// be 0 and becomes -e_i, so that sums of dk over keys - the gradient of a key bias - came out twice as far from float64 as
+// with exact attention. So the kDq blocks, which see all keys of their queries, also sum P dP in fp32 and publish
+// delta_i = sum_j P dP - dL; the kDkv blocks wait for it. Items are drawn by a ticket with the kDq items first: whoever
+// holds a kDkv item knows that every kDq item is being computed or done, and kDq items wait for nothing. Where one tile
+// holds all keys of its queries (at most 64: then dS is a small difference of large terms; two keys: dq 0.0040 off in
+// the 2-norm instead of 0.0024) a kDq block uses its own sum as well.
 //
 // Every mbarrier wait is bounded as in the forward: a stuck pipeline sets the error word and winds down.
 #include <cuda.h>
@@ -67,13 +71,12 @@ struct BwdCfg {
   static constexpr int kTileBytes = 128 * D * 2;      // one 128-row bf16 tile
   static constexpr int kChunkBytes = 128 * 128;       // one 128-row x 64-column chunk
   // kDkv: resident tiles K, V; rings of streamed tiles T1 = dO and T0 = q (S of tile j + 1 is issued before dK of tile
-  // j, so q is loaded two tiles ahead of its release). The last stage of T0 holds column sums in whole items.
+  // j, so q is loaded two tiles ahead of its release).
   static constexpr int kStages0 = D == 64 ? 4 : 3;
   static constexpr int kStages1 = D == 64 ? 4 : 2;
   static constexpr int kROff = 0;
   static constexpr int kT1Off = 2 * kTileBytes;
   static constexpr int kT0Off = kT1Off + kStages1 * kTileBytes;
-  static constexpr int kRedOff = kT0Off + (kStages0 - 1) * kTileBytes;
   static constexpr int kStatOff = kT0Off + kStages0 * kTileBytes;
   static constexpr int kStatBytes = 2 * 4 * 36 * 4;   // lse2, delta: four groups of 32 columns, padded (see stat_at)
   // kDq: dO resident, a ring of pairs of 64-row tiles K, V
@@ -194,7 +197,7 @@ __device__ __forceinline__ void bwd_produce_dkv(const BwdShared& sh, const CUten
   load_tile<D, 2>(sh.sbase + C::kROff, tm_k, sh.bar(C::kBarR), x0, wi.row0, pol_r);
   load_tile<D, 2>(sh.sbase + C::kROff + C::kTileBytes, tm_v, sh.bar(C::kBarR), x0, wi.row0, pol_r);
   TileWalk<kDkvRows> walk(ranges, wi.n_ranges);
-  const int n0 = C::kStages0 - wi.whole;
+  const int n0 = C::kStages0;
   Ring a(n0), b(C::kStages1);
   int issued0 = 0, issued1 = 0;
   for (int j = 0; j < wi.n_tiles; ++j, a.next(), b.next()) {
@@ -258,33 +261,48 @@ __device__ __forceinline__ void bwd_produce_dq(const BwdShared& sh, const CUtens
 }
 
 // ---------------------------------------------------------------------------------------------- tile preparation
+constexpr uint32_t kDeltaPending = 0x7fd1d1d1u;          // a NaN no arithmetic gives
+__device__ __forceinline__ uint32_t load_relaxed(const float* p) {
+  uint32_t v;
+  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // 64 threads (t = 0..63) wait for each streamed tile and hand it on prepared, so that the issuing thread has one wait
 // for it. kDkv: the statistics of its query rows (lse2 = +inf past the end, so P = 0 there) into one of two slots, zeros
 // over the shared-memory rows past the end.
 template <int D>
 __device__ __forceinline__ void bwd_prepare_dkv(const BwdShared& sh, const BwdWork& wi, const int2* ranges,
-                                                const float2* __restrict__ stats, const float* __restrict__ dlse,
+                                                const float2* __restrict__ stats, const float* __restrict__ delta,
                                                 long long nq, int t, int* err) {
   using C = BwdCfg<D>;
-  const float2* st = stats + static_cast<long long>(wi.head) * nq;
-  const float* dl = dlse == nullptr ? nullptr : dlse + static_cast<long long>(wi.head) * nq;
-  // (lse2, delta) of a query row; where the tile gives sum_j P dP itself, its other term -dL
-  auto row_stats = [&](long long row) {
-    float2 x = __ldg(st + row);
-    if (wi.whole) x.y = dl == nullptr ? 0.f : -__ldg(dl + row);
+  const long long h0 = static_cast<long long>(wi.head) * nq;
+  // (lse2, delta) of a query row, once its kDq block has published it
+  auto row_stats = [&](long long row, bool& ok) {
+    float2 x = __ldg(stats + h0 + row);
+    const unsigned long long t0 = global_ns();
+    uint32_t bits = load_relaxed(delta + h0 + row);
+    while (ok && bits == kDeltaPending) {
+      if (*sh.abort_flag || global_ns() - t0 > kWaitLimitNs) {
+        *sh.abort_flag = 1;
+        ok = false;
+      }
+      bits = load_relaxed(delta + h0 + row);
+    }
+    x.y = __uint_as_float(bits);
     return x;
   };
   TileWalk<kDkvRows> walk(ranges, wi.n_ranges);
-  const int n0 = C::kStages0 - wi.whole;
+  const int n0 = C::kStages0;
   Ring a(n0), b(C::kStages1), free(n0);                  // free: two tiles behind, whose dK released the slot
   for (int j = 0; j < wi.n_tiles; ++j, a.next(), b.next()) {
     int row = 0;
     const int valid = walk.next(row);
     float2 x = make_float2(INFINITY, 0.f), y = x;
-    if (t < valid) x = row_stats(row + t);
-    if (t + 64 < valid) y = row_stats(row + t + 64);
     bool ok = true;
-    if (j >= 2) {
+    if (t < valid) x = row_stats(row + t, ok);
+    if (t + 64 < valid) y = row_stats(row + t + 64, ok);
+    if (ok && j >= 2) {
       ok = mbar_wait(sh.bar(C::kBarE0 + free.s), free.ph, sh.abort_flag);
       free.next();
     }
@@ -378,7 +396,7 @@ __device__ __forceinline__ void bwd_mma_dkv(const BwdShared& sh, uint32_t tmem, 
     for (int kk = 0; kk < 8; ++kk)
       if (kk >= lo && kk < hi) mma_ts(d, a + kk * 8, t + ((kk * 2048) >> 4), kIdescA, (acc || kk > 0) ? 1u : 0u);
   };
-  Ring a(C::kStages0 - wi.whole), b(C::kStages1);        // tile j; nx: tile j + 1
+  Ring a(C::kStages0), b(C::kStages1);        // tile j; nx: tile j + 1
   Ring nx(a.n);
   nx.next();
   bool ok = wait(C::kBarR, 0) && wait(C::kBarAux, 0);
@@ -551,44 +569,6 @@ __device__ __forceinline__ void bwd_zero(const BwdThread& th, const BwdWork& wi,
   }
 }
 
-// Adds sum_j P dP over the tile's key rows to the delta of each of its query columns (in a slot): rows of a thread, lanes
-// of a warp by shuffles, the eight warps through shared memory.
-template <int D>
-__device__ __forceinline__ void bwd_column_delta(const BwdShared& sh, uint32_t dp_addr, const BwdThread& th, int rows,
-                                              const uint32_t (&p)[64], int slot) {
-  using C = BwdCfg<D>;
-  const int t = threadIdx.x - 128;                    // 0..255
-  float* red = reinterpret_cast<float*>(sh.smem + C::kRedOff);
-  const float m0 = th.row < rows ? 1.f : 0.f, m1 = th.row + 8 < rows ? 1.f : 0.f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t d[32];
-    tmem_ld_16x256b_x8(dp_addr + 64 * h, d);
-    tmem_wait_ld();
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const uint32_t* x = p + 4 * (8 * h + r);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        // rows past the range may hold anything: they are not multiplied in
-        float a = m0 != 0.f ? __uint_as_float(x[e]) * __uint_as_float(d[4 * r + e]) : 0.f;
-        if (m1 != 0.f) a = fmaf(__uint_as_float(x[2 + e]), __uint_as_float(d[4 * r + 2 + e]), a);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-        if ((t & 31) < 4) red[128 * (t >> 5) + 64 * h + 8 * r + 2 * th.cq + e] = a;
-      }
-    }
-  }
-  asm volatile("bar.sync 1, 256;" ::: "memory");
-  if (t < 128) {
-    float a = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) a += red[128 * w + t];
-    reinterpret_cast<float*>(sh.smem + C::kStatOff + slot * C::kStatBytes)[144 + stat_at(t)] += a;
-  }
-  asm volatile("bar.sync 1, 256;" ::: "memory");
-}
-
 template <int D>
 __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tmem, const BwdThread& th,
                                                 const BwdWork& wi, float scale, __nv_bfloat16* __restrict__ dk,
@@ -596,7 +576,7 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
   using C = BwdCfg<D>;
   const float scale_log2 = scale * kLog2e;
   const uint32_t s_addr = tmem + th.lane_off, dp_addr = s_addr + 128;
-  Ring a(C::kStages0 - wi.whole);
+  Ring a(C::kStages0);
   bool ok = true;
   uint32_t p[64];                               // scores, then P in fp32
   for (int j = 0; j < wi.n_tiles; ++j, a.next()) {
@@ -640,7 +620,6 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
     ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
     if (!ok) break;
     tc_after_wait();
-    if (wi.whole) bwd_column_delta<D>(sh, dp_addr, th, wi.rows, p, j & 1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = st[36 + i];
 #pragma unroll
@@ -679,12 +658,17 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
   bwd_flush<D>(sh, wi, 2, dv, dk, heads);
 }
 
+__device__ __forceinline__ float quad_add(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 1);
+  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+}
+
 template <int D>
 __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tmem, const BwdThread& th,
                                                const BwdWork& wi, const int2* ranges, float scale,
                                                const __nv_bfloat16* __restrict__ q, const float2* __restrict__ stats,
-                                               const float* __restrict__ dlse, long long nq,
-                                               __nv_bfloat16* __restrict__ dq, int heads, int* err) {
+                                               const float* __restrict__ dlse, float* __restrict__ delta_out,
+                                               long long nq, __nv_bfloat16* __restrict__ dq, int heads, int* err) {
   using C = BwdCfg<D>;
   const int sw = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
   const int grp = sw >> 2;                      // tiles grp, grp + 2, ...
@@ -711,7 +695,7 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
   }
   const float scale_log2 = scale * kLog2e;
   // this thread's four rows: lane / 4 + 8 i of its warp's 32 TMEM lanes, i = 2 h + (register pair) of 16-lane block h
-  float lse2[4], delta[4];
+  float lse2[4], delta[4], dl[4], pdp[4];      // pdp: this thread's part of sum_j P dP
   const int row = 32 * (sw & 3) + (lane >> 2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -720,6 +704,8 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
                                  : make_float2(INFINITY, 0.f);
     lse2[i] = x.x;
     delta[i] = x.y;
+    dl[i] = dlse != nullptr && r < wi.rows ? __ldg(dlse + static_cast<long long>(wi.head) * nq + wi.row0 + r) : 0.f;
+    pdp[i] = 0.f;
   }
   const uint32_t s_addr = tmem + 64 * grp + lanes, dp_addr = s_addr + C::kColDp, ds_addr = tmem + C::kColDs + 32 * grp + lanes;
   constexpr uint32_t kBlock = 16u << 16;        // TMEM lane offset of the second 16-lane block
@@ -756,25 +742,18 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
         for (int i = 0; i < 32; ++i)
           if (8 * (i >> 2) + 2 * th.cq + (i & 1) >= valid) p[h][i] = d[h][i] = 0u;
     }
-    if (wi.whole) {
-      // all keys of these queries are here: delta = sum_j P dP - dL, a quad of threads per row
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float& x = sum[2 * h + ((i >> 1) & 1)];
-          x = fmaf(__uint_as_float(p[h][i]), __uint_as_float(d[h][i]), x);
-        }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        const int r = row + 8 * i;
-        delta[i] = sum[i];
-        if (dlse != nullptr && r < wi.rows)
-          delta[i] -= __ldg(dlse + static_cast<long long>(wi.head) * nq + wi.row0 + r);
+      for (int i = 0; i < 32; ++i) {
+        float& x = sum[2 * h + ((i >> 1) & 1)];
+        x = fmaf(__uint_as_float(p[h][i]), __uint_as_float(d[h][i]), x);
       }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (wi.whole) delta[i] = quad_add(sum[i]) - dl[i];
+      pdp[i] += sum[i];
     }
     uint32_t w[2][16];
 #pragma unroll
@@ -799,6 +778,30 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
     tc_fence_before();
     mbar_arrive(sh.bar(C::kBarDs + grp));
   }
+  if (ok) {
+    // both groups' sums meet in shared memory; group 0 publishes the rows' delta
+    float* meet = reinterpret_cast<float*>(sh.smem + C::kStatOff);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pdp[i] = quad_add(pdp[i]);
+      if (grp == 1 && th.cq == 0) meet[row + 8 * i] = pdp[i];
+    }
+  }
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  if (ok && grp == 0 && th.cq == 0) {
+    const float* meet = reinterpret_cast<const float*>(sh.smem + C::kStatOff);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row + 8 * i;
+      if (r >= wi.rows) continue;
+      const float x = pdp[i] + meet[r] - dl[i];
+      const uint32_t bits = x == x ? __float_as_uint(x) : 0x7fffffffu;      // any NaN but the pending mark
+      asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(delta_out + static_cast<long long>(wi.head) * nq +
+                                                               wi.row0 + r),
+                   "r"(bits)
+                   : "memory");
+    }
+  }
   if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
   if (!ok) {
     atomicOr(err, kErrTimeoutSoftmax);
@@ -815,13 +818,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                     const __nv_bfloat16* __restrict__ q,
                     const BwdWork* __restrict__ work, const int2* __restrict__ ranges,
-                    const float2* __restrict__ stats, const float* __restrict__ dlse, __nv_bfloat16* __restrict__ dq,
+                    const float2* __restrict__ stats, float* __restrict__ delta, int* __restrict__ ticket,
+                    const float* __restrict__ dlse, __nv_bfloat16* __restrict__ dq,
                     __nv_bfloat16* __restrict__ dk,
                     __nv_bfloat16* __restrict__ dv, long long nq, int heads, float scale, int* __restrict__ err,
                     const int* __restrict__ n_items_dev) {
   using C = BwdCfg<D>;
-  // a grid sized by an upper bound (work list planned on the device): CTAs past the planned count have no item
-  if (n_items_dev != nullptr && static_cast<int>(blockIdx.x) >= __ldg(n_items_dev)) return;
   // the tiles need a 1024-byte boundary, which dynamic shared memory without static shared memory before it has
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   BwdShared sh;
@@ -843,7 +845,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tma_prefetch_map(&tm_v);
     tma_prefetch_map(&tm_do);
   }
-  const BwdWork wi = work[blockIdx.x];
+  volatile int* drawn = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  if (threadIdx.x == 0) *drawn = atomicAdd(ticket, 1);
+  __syncthreads();
+  const int item = *drawn;
+  // a grid sized by an upper bound (work list planned on the device): CTAs past the planned count have no item
+  if (n_items_dev != nullptr && item >= __ldg(n_items_dev)) return;
+  const BwdWork wi = work[item];
   const bool dkv = wi.kind == kDkv;
 
   if (threadIdx.x == 0) {
@@ -894,7 +902,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           else bwd_mma_dq<D>(sh, tmem, wi, err);
         }
       } else if (dkv) {
-        bwd_prepare_dkv<D>(sh, wi, rg, stats, dlse, nq, threadIdx.x - 64, err);
+        bwd_prepare_dkv<D>(sh, wi, rg, stats, delta, nq, threadIdx.x - 64, err);
       } else {
         bwd_prepare_dq<D>(sh, wi, rg, threadIdx.x - 64, err);
       }
@@ -912,7 +920,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     } else if (dkv) {
       bwd_compute_dkv<D>(sh, tmem, th, wi, scale, dk, dv, heads, err);
     } else {
-      bwd_compute_dq<D>(sh, tmem, th, wi, rg, scale, q, stats, dlse, nq, dq, heads, err);
+      bwd_compute_dq<D>(sh, tmem, th, wi, rg, scale, q, stats, dlse, delta, nq, dq, heads, err);
     }
   }
 
@@ -925,7 +933,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 }
 
 // ---------------------------------------------------------------------------------------------- row statistics
-// stats[h][row] = (lse * log2 e, sum_d dO o - dL). Memory bound: dO and o are read once, 16 bytes per thread, D / 8
+// stats[h][row] = (lse * log2 e, sum_d dO o - dL), and delta[h][row] marked as pending, the ticket as undrawn. Memory bound: dO and o are read once, 16 bytes per thread, D / 8
 // lanes per (row, head); a block covers 32 rows x 8 heads and writes its pairs through shared memory, so that the
 // head-major statistics are written in runs of 32 rows.
 template <int D>
@@ -933,7 +941,9 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const __nv_bfloat16
                                                              const __nv_bfloat16* __restrict__ dout,
                                                              const float* __restrict__ lse,
                                                              const float* __restrict__ dlse,
-                                                             float2* __restrict__ stats, long long nq, int heads) {
+                                                             float2* __restrict__ stats, float* __restrict__ pending,
+                                                             int* __restrict__ ticket, long long nq, int heads) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *ticket = 0;
   constexpr int kLanes = D / 8;                 // lanes per (row, head)
   constexpr int kPer = 256 / kLanes;            // (row, head) pairs per pass: 8 heads x kPer / 8 rows
   __shared__ float delta[8][33];
@@ -970,6 +980,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const __nv_bfloat16
     float d = delta[t >> 5][t & 31];
     if (dlse != nullptr) d -= dlse[at];
     stats[at] = make_float2(lse[at] * kLog2e, d);
+    pending[at] = __uint_as_float(kDeltaPending);
   }
 }
 
@@ -979,7 +990,7 @@ template <int D>
 static int launch_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
                            const float* lse, const float* dlse, void* dq, void* dk, void* dv, long long nq,
                            long long nk, int heads, float scale, const BwdWork* work, int n_items, const int2* ranges,
-                           float2* stats, int* err, cudaStream_t stream, const int* n_items_dev) {
+                           float* scratch, int* err, cudaStream_t stream, const int* n_items_dev) {
   using C = BwdCfg<D>;
   // an empty side has no tiles to load: its maps only need a valid address
   if (nk == 0) k = v = q;
@@ -1011,15 +1022,17 @@ static int launch_attn_bwd(const void* q, const void* k, const void* v, const vo
   }
   // as in the forward: a build with another register count could leave the split's increase waiting, so it never runs
   if (launch_regs != kBwdLaunchRegs) return ORL_ERR_UNSUPPORTED;
-  if (nq > 0) {
-    const dim3 grid(static_cast<unsigned>((nq + 31) / 32), static_cast<unsigned>((heads + 7) / 8));
-    attn_bwd_stats_kernel<D><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(out),
-                                                       static_cast<const __nv_bfloat16*>(dout), lse, dlse, stats, nq,
-                                                       heads);
-    if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
-  }
+  // scratch: the ticket (16 bytes), the pairs, delta
+  int* ticket = reinterpret_cast<int*>(scratch);
+  float2* stats = reinterpret_cast<float2*>(scratch + 4);
+  float* delta = scratch + 4 + 2 * static_cast<long long>(heads) * nq;
+  const dim3 grid(static_cast<unsigned>(std::max<long long>(1, (nq + 31) / 32)), static_cast<unsigned>((heads + 7) / 8));
+  attn_bwd_stats_kernel<D><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(out),
+                                                     static_cast<const __nv_bfloat16*>(dout), lse, dlse, stats, delta,
+                                                     ticket, nq, heads);
+  if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
   attn_bwd_kernel<D><<<n_items, kBwdThreads, C::kSmemBytes, stream>>>(
-      mq, mk, mv, mdo, static_cast<const __nv_bfloat16*>(q), work, ranges, stats, dlse, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
+      mq, mk, mv, mdo, static_cast<const __nv_bfloat16*>(q), work, ranges, stats, delta, ticket, dlse, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
       static_cast<__nv_bfloat16*>(dv), nq, heads, scale, err, n_items_dev);
   return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
 }
@@ -1033,8 +1046,8 @@ static int check_bwd(const void* q, const void* k, const void* v, const void* ou
     return ORL_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return ORL_ERR_UNSUPPORTED;
   if (static_cast<long long>(heads) * head_dim > 0x7fffffffLL) return ORL_ERR_ARG;
-  if (nq > 0 && (q == nullptr || out == nullptr || dout == nullptr || lse == nullptr || dq == nullptr ||
-                 stats == nullptr))
+  if (stats == nullptr) return ORL_ERR_ARG;
+  if (nq > 0 && (q == nullptr || out == nullptr || dout == nullptr || lse == nullptr || dq == nullptr))
     return ORL_ERR_ARG;
   if (nk > 0 && (k == nullptr || v == nullptr || dk == nullptr || dv == nullptr)) return ORL_ERR_ARG;
   for (const void* p : {q, k, v, out, dout, static_cast<const void*>(dq), static_cast<const void*>(dk),
@@ -1093,23 +1106,23 @@ static int plan_bwd(const int32_t* q_start, const int32_t* q_len, const int32_t*
     const int range0 = static_cast<int>(plan.ranges.size());
     int n = 0;
     long long tiles = 0;
-    bool whole = cuts[c + 1] - cuts[c] <= kWholeKeys;     // every reader's keys are exactly this block
     for (int i = 0; i < n_seg; ++i)
       if (q_len[i] > 0 && k_len[i] > 0 && k_start[i] <= cuts[c] &&
           static_cast<long long>(k_start[i]) + k_len[i] >= cuts[c + 1]) {
         plan.ranges.push_back({q_start[i], q_len[i]});
         tiles += (q_len[i] + kDkvRows - 1) / kDkvRows;
-        whole = whole && k_start[i] == cuts[c] && k_len[i] == cuts[c + 1] - cuts[c];
         ++n;
       }
     if (tiles > 0x7fffffffLL || plan.ranges.size() > 0x7ffffff0u) return ORL_ERR_CAPACITY;
-    cut(cuts[c], cuts[c + 1], kDkv, range0, n, static_cast<int>(tiles), whole && n > 0);
+    cut(cuts[c], cuts[c + 1], kDkv, range0, n, static_cast<int>(tiles), false);
   }
-  // longest first: a dkv tile of 128 rows takes about three times a dq tile of 64
-  auto cost = [](const Block& b) { return static_cast<long long>(b.n_tiles) * (b.kind == kDkv ? 3 : 1); };
+  // the queries' items first (the keys' wait for their delta), longest first
   std::vector<int> order(blocks.size());
   for (size_t i = 0; i < order.size(); ++i) order[i] = static_cast<int>(i);
-  std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return cost(blocks[a]) > cost(blocks[b]); });
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) {
+    const Block &x = blocks[a], &y = blocks[b];
+    return x.kind != y.kind ? x.kind == kDq : x.n_tiles > y.n_tiles;
+  });
   if (static_cast<long long>(blocks.size()) * heads > 0x3fffffffLL) return ORL_ERR_CAPACITY;
   plan.items.reserve(blocks.size() * heads);
   for (size_t lo = 0; lo < order.size();) {
@@ -1172,7 +1185,7 @@ extern "C" int orl_attn_bwd(const void* q, const void* k, const void* v, const v
   if (n_items == 0) return ORL_OK;
   auto launch = head_dim == 64 ? launch_attn_bwd<64> : launch_attn_bwd<128>;
   return launch(q, k, v, out, dout, lse, dlse, dq, dk, dv, nq, nk, heads, scale, work_dev, n_items,
-                reinterpret_cast<const int2*>(ranges_dev), reinterpret_cast<float2*>(stats_dev), err_dev,
+                reinterpret_cast<const int2*>(ranges_dev), stats_dev, err_dev,
                 static_cast<cudaStream_t>(stream_ptr), nullptr);
 }
 
@@ -1237,7 +1250,8 @@ __global__ void __launch_bounds__(1024)
     return;
   }
   auto is_dkv = [&](int g) { return g < n_seg || (g >= 2 * n_seg && g < 2 * n_seg + 2); };
-  auto cost = [&](int g) { return static_cast<long long>(s_tiles[g]) * (is_dkv(g) ? 3 : 1); };
+  // the queries' items first (the keys' wait for their delta), longest first
+  auto cost = [&](int g) { return static_cast<long long>(s_tiles[g]) + (is_dkv(g) ? 0 : 1ll << 32); };
   auto items = [&](int g) { return heads * ((s_len[g] + 127) >> 7); };
   for (int g = t; g < n_grp; g += blockDim.x) {
     if (s_len[g] == 0) continue;
@@ -1283,9 +1297,8 @@ __global__ void __launch_bounds__(1024)
     w.range0 = g < 2 * n_seg ? g : 0;
     w.n_ranges = s_tiles[g] > 0 ? 1 : 0;
     w.n_tiles = s_tiles[g];
-    // the segment's keys fit one tile (a dkv block is then the whole segment)
-    const int keys = g < 2 * n_seg ? s_len[g % n_seg] : 0;
-    w.whole = w.n_tiles > 0 && keys > 0 && keys <= kWholeKeys ? 1 : 0;
+    const int keys = g >= n_seg && g < 2 * n_seg ? s_len[g - n_seg] : 0;
+    w.whole = keys > 0 && keys <= kWholeKeys ? 1 : 0;
     work[1 + it] = w;
   }
   if (t == 0 && blockIdx.x == 0) work[0].row0 = n;
@@ -1338,5 +1351,5 @@ extern "C" int orl_attn_bwd_cu(const void* q, const void* k, const void* v, cons
   if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
   auto launch = head_dim == 64 ? launch_attn_bwd<64> : launch_attn_bwd<128>;
   return launch(q, k, v, out, dout, lse, dlse, dq, dk, dv, nq, nk, heads, scale, work + 1, static_cast<int>(items),
-                ranges, reinterpret_cast<float2*>(stats_dev), err_dev, stream, reinterpret_cast<const int*>(work));
+                ranges, stats_dev, err_dev, stream, reinterpret_cast<const int*>(work));
 }

@@ -58,14 +58,8 @@ def test_plan_covers_every_row_once(lib, ci, heads):
             assert got == want
         tile = 128 if w['kind'] == 0 else 64
         assert w['n_tiles'] == sum((x + tile - 1) // tile for _, x in got)
-        # a tile holds all keys of its queries: the block's own rows, or the one range that its rows read
-        if w['kind'] == 0:
-            readers = [(k0, lk) for q0, lq, k0, lk in segs if lq > 0 and k0 <= rows[0] < k0 + lk]
-            whole = bool(readers) and w['rows'] <= 64 and all(x == (w['row0'], w['rows']) for x in readers)
-        else:
-            whole = bool(got) and 0 < got[0][1] <= 64
-        assert w['whole'] == whole
-        cost.append(w['n_tiles'] * (3 if w['kind'] == 0 else 1))
+        assert w['whole'] == (w['kind'] == 1 and bool(got) and 0 < got[0][1] <= 64)     # one tile holds all its keys
+        cost.append((w['kind'], w['n_tiles']))                          # queries first, longest first
     assert (seen[0, :, :nk] == 1).all() and (seen[1, :, :nq] == 1).all()
     assert cost == sorted(cost, reverse=True)
 

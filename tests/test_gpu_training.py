@@ -210,7 +210,9 @@ def test_fused_block_trains():
 
 
 def test_backward_captures_while_an_eager_graph_lives():
-    """a training step captured into a graph with an eager graph of the same leaves alive, then replayed on new inputs"""
+    """a training step captured into a graph with an eager graph of the same tensors alive, then replayed on new inputs.
+    The step takes fresh leaves of its tensors: with the eager graph's own leaves, torch's engine waits for the stream
+    that built them, which invalidates a capture whatever the operators are (F.linear alone does it too)."""
     from onereel_b200 import attention as A
     from onereel_b200.linear import linear
     H, D, n = 2, 64, 96
@@ -219,11 +221,15 @@ def test_backward_captures_while_an_eager_graph_lives():
     g = rand(n, H, D, seed=3)
     cu = A.cu_seqlens([40, 56])
 
-    def step():
+    def out(x, w):
         q, k, v = (t.contiguous().view(n, H, D) for t in linear(x, w).chunk(3, -1))
-        return torch.autograd.grad(A.varlen(q, k, v, cu, cu, 56, 56), (x, w), g)
+        return A.varlen(q, k, v, cu, cu, 56, 56)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, w)]
+        return torch.autograd.grad(out(*leaves), leaves, g)
     step()
-    alive = A.varlen(*(t.contiguous().view(n, H, D) for t in linear(x, w).chunk(3, -1)), cu, cu, 56, 56)
+    alive = out(x, w)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         res = step()
