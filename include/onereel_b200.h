@@ -220,11 +220,11 @@ ORL_API int orl_qk_norm_rope(const void* x, void* y, const void* weight, const f
 
 /* Gradients of orl_qk_norm_rope (without a row map): dx [rows, heads * head_dim] bf16 and dweight (bf16, the weight's
  * size) from the gradient dy of y and the forward's x, weight and tables. Deterministic. scratch: device fp32,
- * orl_qk_norm_rope_bwd_scratch elements. heads * head_dim at most 8192. */
+ * orl_qk_norm_rope_bwd_scratch elements; err_dev: as in orl_attn_fwd. heads * head_dim at most 8192. */
 ORL_API int orl_qk_norm_rope_bwd(const void* x, const void* dy, const void* weight, const float* cos_t,
                                  const float* sin_t, void* dx, void* dweight, float* scratch, long long rows,
                                  int heads, int head_dim, int per_head, float eps, int sin_shift, long long rope_ld,
-                                 void* stream);
+                                 int* err_dev, void* stream);
 
 /* fp32 elements of scratch orl_qk_norm_rope_bwd needs. */
 ORL_API long long orl_qk_norm_rope_bwd_scratch(long long rows, int heads, int head_dim, int per_head);
@@ -273,14 +273,14 @@ ORL_API int orl_linear(const void* x, long long ldx, const void* w, long long ld
  * NULL without activation and gate): dz = gate * dy * act'(z), dx = dz w [m, k], dw = dz^T x [n, k], dbias = column sums
  * of dz, dgate = column sums of dy * act(z) (bf16; NULL: not computed). The residual's gradient is dy itself.
  * Deterministic. dz: scratch [m, n] bf16, needed for dx or dw when z is given; scratch: device fp32,
- * orl_linear_bwd_scratch elements, needed for dbias or dgate. */
+ * orl_linear_bwd_scratch elements, needed for dbias, dgate or, with at most four rows, dx. */
 ORL_API int orl_linear_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w, long long ldw,
                            const void* z, const void* gate, int act, void* dz, void* dx, void* dw, void* dbias,
                            void* dgate, float* scratch, long long m, long long n, long long k, int* err_dev,
                            void* stream);
 
 /* fp32 elements of scratch orl_linear_bwd needs. */
-ORL_API long long orl_linear_bwd_scratch(long long m, long long n);
+ORL_API long long orl_linear_bwd_scratch(long long m, long long n, long long k);
 
 /* ---------------------------------------------------------------- frame memory (src/onereel/frame_memory.py) */
 

@@ -84,14 +84,14 @@ SIGNATURES = {
     'orl_lse_merge_acc': (c_int, [c_vp, c_vp, c_vp, c_vp, c_ll, c_ll, c_ll, c_int, c_int, c_vp]),
     'orl_qk_norm_rope': (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_ll, c_int, c_int, c_int, c_float, c_int, c_ll, c_vp,
                                  c_vp]),
-    'orl_qk_norm_rope_bwd': (c_int, [c_vp] * 8 + [c_ll, c_int, c_int, c_int, c_float, c_int, c_ll, c_vp]),
+    'orl_qk_norm_rope_bwd': (c_int, [c_vp] * 8 + [c_ll, c_int, c_int, c_int, c_float, c_int, c_ll, c_vp, c_vp]),
     'orl_qk_norm_rope_bwd_scratch': (c_ll, [c_ll, c_int, c_int, c_int]),
     'orl_rope_rows': (c_int, [c_vp, c_vp, c_ll, c_int, c_int, c_vp, c_vp, c_ll, c_int, c_vp]),
     'orl_linear': (c_int, [c_vp, c_ll, c_vp, c_ll, c_vp, c_vp, c_vp, c_ll, c_vp, c_vp, c_ll, c_ll, c_ll, c_int, c_vp,
                            c_vp]),
     'orl_linear_bwd': (c_int, [c_vp, c_ll, c_vp, c_ll, c_vp, c_ll, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                c_ll, c_ll, c_ll, c_vp, c_vp]),
-    'orl_linear_bwd_scratch': (c_ll, [c_ll, c_ll]),
+    'orl_linear_bwd_scratch': (c_ll, [c_ll, c_ll, c_ll]),
     'orl_frame_pool': (c_int, [c_vp, c_int, c_ll, c_int, c_vp, c_vp, c_int, c_vp, c_ll, c_vp]),
     'orl_frame_select_scratch': (c_ll, [c_int, c_int, c_int]),
     'orl_frame_select': (c_int, [c_vp, c_ll, c_ll, c_int, c_int, c_int, c_vp, c_int, c_int, c_int, c_vp, c_ll, c_vp,

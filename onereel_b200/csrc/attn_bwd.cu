@@ -313,10 +313,10 @@ __device__ __forceinline__ void bwd_prepare_dkv(const BwdShared& sh, const BwdWo
       return;
     }
     float* dst = reinterpret_cast<float*>(sh.smem + C::kStatOff + (j & 1) * C::kStatBytes);
-    dst[stat_at(t)] = x.x;
-    dst[stat_at(t + 64)] = y.x;
-    dst[144 + stat_at(t)] = x.y;
-    dst[144 + stat_at(t + 64)] = y.y;
+    dst[stat_at(t)] = -x.x;                              // negated, as they are added
+    dst[stat_at(t + 64)] = -y.x;
+    dst[144 + stat_at(t)] = -x.y;
+    dst[144 + stat_at(t + 64)] = -y.y;
     if (valid < kDkvRows) {
       for (int c = 0; c < 2 * C::kChunks; ++c) {         // T0's chunks, then T1's
         uint8_t* chunk = sh.smem + (c < C::kChunks ? C::kT0Off + a.s * C::kTileBytes + c * C::kChunkBytes
@@ -495,11 +495,15 @@ __device__ __forceinline__ void bwd_mma_dq(const BwdShared& sh, uint32_t tmem, c
 
 // ---------------------------------------------------------------------------------------------- P and dS
 // after an mbarrier wait of a whole warp: its lanes leave the wait's loop one by one, and the TMEM accesses that follow
-// are warp-wide (without the __syncwarp a warp that had not come together corrupted its tiles now and then)
+// need them together
 __device__ __forceinline__ void tc_after_wait() {
   __syncwarp();
   tc_fence_after();
 }
+
+// two consecutive fp32 values of a fragment (one row, two columns) as a pair for the f32x2 instructions, which halve the
+// issue slots of the arithmetic around the exponentials
+__device__ __forceinline__ F2 f2_of(const uint32_t* x) { return f2(__uint_as_float(x[0]), __uint_as_float(x[1])); }
 
 // Thread layout of the .16x256b / .16x128b TMEM shapes: warp sw owns lanes 32 (sw % 4) + 16 (sw / 4) + [0, 16); its
 // thread holds the rows lane / 4 and lane / 4 + 8 of that block, register 4r + 2i + e of a 64-column load: row i,
@@ -576,6 +580,7 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
   using C = BwdCfg<D>;
   const float scale_log2 = scale * kLog2e;
   const uint32_t s_addr = tmem + th.lane_off, dp_addr = s_addr + 128;
+  const F2 sc = f2(scale_log2, scale_log2);
   Ring a(C::kStages0);
   bool ok = true;
   uint32_t p[64];                               // scores, then P in fp32
@@ -599,12 +604,10 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const float4 c4 = c[4 * h + (r >> 1)];
-        const float l0 = (r & 1) ? c4.z : c4.x, l1 = (r & 1) ? c4.w : c4.y;
+        const F2 l = (r & 1) ? f2(c4.z, c4.w) : f2(c4.x, c4.y);
         uint32_t* x = p + 4 * (8 * h + r);
-        const float a0 = ex2(fmaf(__uint_as_float(x[0]), scale_log2, -l0));
-        const float a1 = ex2(fmaf(__uint_as_float(x[1]), scale_log2, -l1));
-        const float b0 = ex2(fmaf(__uint_as_float(x[2]), scale_log2, -l0));
-        const float b1 = ex2(fmaf(__uint_as_float(x[3]), scale_log2, -l1));
+        const float2 u = f2_split(ffma2(f2_of(x), sc, l)), v = f2_split(ffma2(f2_of(x + 2), sc, l));
+        const float a0 = ex2(u.x), a1 = ex2(u.y), b0 = ex2(v.x), b1 = ex2(v.y);
         x[0] = __float_as_uint(a0);
         x[1] = __float_as_uint(a1);
         x[2] = __float_as_uint(b0);
@@ -630,14 +633,12 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const float4 c4 = c[4 * h + (r >> 1)];
-        const float l0 = (r & 1) ? c4.z : c4.x, l1 = (r & 1) ? c4.w : c4.y;
+        const F2 l = (r & 1) ? f2(c4.z, c4.w) : f2(c4.x, c4.y);
         const uint32_t* x = p + 4 * (8 * h + r);
-        const float a0 = __uint_as_float(x[0]) * (__uint_as_float(d[4 * r + 0]) - l0);
-        const float a1 = __uint_as_float(x[1]) * (__uint_as_float(d[4 * r + 1]) - l1);
-        const float b0 = __uint_as_float(x[2]) * (__uint_as_float(d[4 * r + 2]) - l0);
-        const float b1 = __uint_as_float(x[3]) * (__uint_as_float(d[4 * r + 3]) - l1);
-        w[2 * r] = pack_bf16x2(a0, a1);
-        w[2 * r + 1] = pack_bf16x2(b0, b1);
+        const float2 u = f2_split(fmul2(f2_of(x), fadd2(f2_of(d + 4 * r), l)));
+        const float2 v = f2_split(fmul2(f2_of(x + 2), fadd2(f2_of(d + 4 * r + 2), l)));
+        w[2 * r] = pack_bf16x2(u.x, u.y);
+        w[2 * r + 1] = pack_bf16x2(v.x, v.y);
       }
       // dS words of half h go over the dP columns [32 h, 32 h + 32), which half 0 has loaded
       tmem_st_16x128b_x8(dp_addr + 32 * h, w);
@@ -742,27 +743,31 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
         for (int i = 0; i < 32; ++i)
           if (8 * (i >> 2) + 2 * th.cq + (i & 1) >= valid) p[h][i] = d[h][i] = 0u;
     }
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    // d <- P dP and its row sums, two columns per instruction
+    F2 sum[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
+    F2 t[2][16];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float& x = sum[2 * h + ((i >> 1) & 1)];
-        x = fmaf(__uint_as_float(p[h][i]), __uint_as_float(d[h][i]), x);
+      for (int r = 0; r < 16; ++r) {
+        t[h][r] = fmul2(f2_of(&p[h][2 * r]), f2_of(&d[h][2 * r]));
+        F2& x = sum[2 * h + (r & 1)];
+        x = fadd2(x, t[h][r]);
       }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (wi.whole) delta[i] = quad_add(sum[i]) - dl[i];
-      pdp[i] += sum[i];
+      const float2 x = f2_split(sum[i]);
+      if (wi.whole) delta[i] = quad_add(x.x + x.y) - dl[i];
+      pdp[i] += x.x + x.y;
     }
     uint32_t w[2][16];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float y = delta[2 * h + (r & 1)];
-        w[h][r] = pack_bf16x2(__uint_as_float(p[h][2 * r]) * (__uint_as_float(d[h][2 * r]) - y),
-                              __uint_as_float(p[h][2 * r + 1]) * (__uint_as_float(d[h][2 * r + 1]) - y));
+        const float y = -delta[2 * h + (r & 1)];
+        const float2 ds = f2_split(ffma2(f2(y, y), f2_of(&p[h][2 * r]), t[h][r]));      // P dP - delta P
+        w[h][r] = pack_bf16x2(ds.x, ds.y);
       }
     if (u >= 2) {
       // dS goes over that of tile u - 2: its dQ is done when its stage is free

@@ -561,6 +561,108 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(const __nv_bfloat16* _
   }
 }
 
+// Their gradients, likewise bound by the weight-sized tensor: dx [m, k] = dz w reads w once (a block takes 256 columns of a
+// strip of w's rows, its sums are one partial row of m k values), dw [n, k] = dz^T x writes dw once.
+constexpr int kRowsDxBlocks = 592;                       // at most, over columns and strips: 4 per SM
+
+template <int M>
+__global__ void __launch_bounds__(256) linear_rows_dx_kernel(const __nv_bfloat16* __restrict__ dz, long long lddz,
+                                                             const __nv_bfloat16* __restrict__ w, long long ldw, int n,
+                                                             int k, float* __restrict__ part) {
+  __shared__ float red[8][M][257];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = 256 * blockIdx.x + 8 * lane;
+  const int per = (n + gridDim.y - 1) / gridDim.y, lo = blockIdx.y * per, hi = min(n, lo + per);
+  float acc[M][8];
+#pragma unroll
+  for (int r = 0; r < M; ++r)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[r][i] = 0.f;
+  if (col < k) {
+    for (int j0 = lo + warp; j0 < hi; j0 += 32) {
+      uint4 wr[4];                                       // four rows' loads in flight
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        wr[u] = j0 + 8 * u < hi ? __ldcs(reinterpret_cast<const uint4*>(w + (j0 + 8 * u) * ldw + col))
+                                : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = min(j0 + 8 * u, hi - 1);
+        float wf[8];
+        unpack8(wr[u], wf);
+#pragma unroll
+        for (int r = 0; r < M; ++r) {
+          const float g = j0 + 8 * u < hi ? __bfloat162float(dz[r * lddz + j]) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[r][i] = fmaf(g, wf[i], acc[r][i]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < M; ++r)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[warp][r][8 * lane + i] = acc[r][i];
+  __syncthreads();
+  const int c = 256 * blockIdx.x + threadIdx.x;
+  if (c < k) {
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+      float a = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a += red[i][r][threadIdx.x];
+      part[(static_cast<long long>(blockIdx.y) * M + r) * k + c] = a;
+    }
+  }
+}
+
+template <int M>
+__global__ void __launch_bounds__(256) linear_rows_dw_kernel(const __nv_bfloat16* __restrict__ dz, long long lddz,
+                                                             const __nv_bfloat16* __restrict__ x, long long ldx, int n,
+                                                             int k, __nv_bfloat16* __restrict__ dw) {
+  // one 16-byte vector of a row of dw per thread; a block's rows follow each other
+  const int vecs = k / 8;
+  const long long total = static_cast<long long>(n) * vecs;
+  for (long long v = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; v < total;
+       v += static_cast<long long>(gridDim.x) * 256) {
+    const int j = static_cast<int>(v / vecs), c = 8 * static_cast<int>(v - static_cast<long long>(j) * vecs);
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+      const float g = __bfloat162float(dz[r * lddz + j]);
+      float xf[8];
+      unpack8(__ldg(reinterpret_cast<const uint4*>(x + r * ldx + c)), xf);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = fmaf(g, xf[i], f[i]);
+    }
+    __stcs(reinterpret_cast<uint4*>(dw) + v, pack8(f));
+  }
+}
+
+static int rows_dx_strips(int n, int k) {
+  return std::max(1, std::min((n + 63) / 64, kRowsDxBlocks / std::max(1, (k + 255) / 256)));
+}
+
+template <int M>
+static int rows_gradients(const void* dz, long long lddz, const void* x, long long ldx, const void* w, long long ldw,
+                          void* dx, void* dw, float* scratch, int n, int k, cudaStream_t stream) {
+  auto bf = [](const void* p) { return static_cast<const __nv_bfloat16*>(p); };
+  if (dx != nullptr) {
+    const int strips = rows_dx_strips(n, k);
+    linear_rows_dx_kernel<M><<<dim3((k + 255) / 256, strips), 256, 0, stream>>>(bf(dz), lddz, bf(w), ldw, n, k, scratch);
+    if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
+    const int rc = column_sum(scratch, strips, M * k, static_cast<long long>(M) * k, dx, stream);
+    if (rc != ORL_OK) return rc;
+  }
+  if (dw != nullptr) {
+    const long long blocks = std::min<long long>(8 * 148, (static_cast<long long>(n) * (k / 8) + 255) / 256);
+    linear_rows_dw_kernel<M><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(bf(dz), lddz, bf(x), ldx, n, k,
+                                                                               static_cast<__nv_bfloat16*>(dw));
+    if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
+  }
+  return ORL_OK;
+}
+
 // ------------------------------------------------------------------------------------------------ dz and column sums
 // dz = gate * dy * act'(z), with the column sums of dz (bias) and of dy * act(z) (gate). Memory bound. A block covers
 // 256 columns (8 per thread, 32 threads across) and a strip of rows (8 at a time); its sums are one partial row.
@@ -750,9 +852,12 @@ extern "C" int orl_linear(const void* x, long long ldx, const void* w, long long
                             stream);
 }
 
-extern "C" long long orl_linear_bwd_scratch(long long m, long long n) {
-  if (check_linear(m, n, 8) != ORL_OK) return ORL_ERR_ARG;
-  return 2ll * dz_strips(static_cast<int>(m), static_cast<int>(n)) * n;
+extern "C" long long orl_linear_bwd_scratch(long long m, long long n, long long k) {
+  if (check_linear(m, n, k) != ORL_OK) return ORL_ERR_ARG;
+  const long long sums = 2ll * dz_strips(static_cast<int>(m), static_cast<int>(n)) * n;
+  // few rows: the partial rows of dx, which follow the column sums on the stream and may take their place
+  const long long rows = m <= kRowsMax ? m * k * rows_dx_strips(static_cast<int>(n), static_cast<int>(k)) : 0;
+  return std::max(sums, rows);
 }
 
 extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w,
@@ -767,7 +872,9 @@ extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, lon
   // an activation's slope, a gate and a gate's gradient need z; with z, dz is not dy and needs room
   if ((act != ORL_ACT_NONE || gate != nullptr || dgate != nullptr) && z == nullptr && m > 0) return ORL_ERR_ARG;
   const bool products = dx != nullptr || dw != nullptr, sums = dbias != nullptr || dgate != nullptr;
-  if ((z != nullptr && products && dz == nullptr && m > 0) || (sums && scratch == nullptr)) return ORL_ERR_ARG;
+  if ((z != nullptr && products && dz == nullptr && m > 0) ||
+      ((sums || (dx != nullptr && m <= kRowsMax)) && scratch == nullptr))
+    return ORL_ERR_ARG;
   if ((lddy & 7) || (dw != nullptr && (ldx & 7)) || (dx != nullptr && (ldw & 7))) return ORL_ERR_ALIGN;
   for (const void* p : {dy, x, w, z, gate, static_cast<const void*>(dz), static_cast<const void*>(dx),
                         static_cast<const void*>(dw)})
@@ -792,6 +899,10 @@ extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, lon
   }
   const void* g = z != nullptr ? dz : dy;
   const long long ldg = z != nullptr ? n : lddy;
+  if (m > 0 && m <= kRowsMax) {
+    auto run = m == 1 ? rows_gradients<1> : m == 2 ? rows_gradients<2> : m == 3 ? rows_gradients<3> : rows_gradients<4>;
+    return run(g, ldg, x, ldx, w, ldw, dx, dw, scratch, nn, kk, stream);
+  }
   if (dx != nullptr && m > 0) {
     const Epilogue ep{nullptr, nullptr, nullptr, 0, static_cast<__nv_bfloat16*>(dx), nullptr, ORL_ACT_NONE};
     if ((rc = gemm<false, true>(g, ldg, w, ldw, mm, kk, nn, ep, err_dev, stream)) != ORL_OK) return rc;

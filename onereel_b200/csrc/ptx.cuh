@@ -359,6 +359,17 @@ __device__ __forceinline__ F2 fadd2(F2 a, F2 b) {
   return d;
 }
 
+__device__ __forceinline__ F2 fmul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 ffma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+
 __device__ __forceinline__ bool elect_one() {
   uint32_t pred = 0;
   asm volatile(

@@ -123,8 +123,8 @@ class _Linear(torch.autograd.Function):
             dw = new(N, K) if need[1] else None
             db = new(N) if need[2] else None
             dgate = new(N) if need[3] else None
-            # scratch: the partial column sums, then dz where it is not dy itself
-            sums = 4 * L.check(L.lib().orl_linear_bwd_scratch(M, N), 'orl_linear_bwd_scratch')
+            # scratch: partial sums, then dz where it is not dy itself
+            sums = 4 * L.check(L.lib().orl_linear_bwd_scratch(M, N, K), 'orl_linear_bwd_scratch')
             scratch = torch.empty(sums + (0 if z is None else 2 * M * N), dtype=torch.uint8, device=dev)
             at = scratch.data_ptr()
             L.check(L.lib().orl_linear_bwd(d.data_ptr(), _ld(d), xr.data_ptr(), _ld(xr), wr.data_ptr(), _ld(wr), _ptr(z),

@@ -8,7 +8,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
-from onereel_b200.attention import _Device, _stream
+from onereel_b200.attention import _Device, _err_word, _stream
 
 
 def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int,
@@ -84,7 +84,7 @@ def qk_norm_rope_grad(x, weight, cos, sin, dy, heads: int, eps: float, per_head:
         L.check(L.lib().orl_qk_norm_rope_bwd(x.data_ptr(), dy.data_ptr(), weight.data_ptr(), cos.data_ptr(),
                                              sin.data_ptr(), dx.data_ptr(), dw.data_ptr(), scratch.data_ptr(), rows,
                                              heads, hidden // heads, int(per_head), float(eps), int(sin_shift),
-                                             cos.shape[1], _stream(x.device)),
+                                             cos.shape[1], _err_word(x.device).data_ptr(), _stream(x.device)),
                 'orl_qk_norm_rope_bwd')
     return dx, dw
 

@@ -37,15 +37,17 @@ def test_linear_gradients_refuse(h):
     assert call(a1=24) == -1 and call(a3=56) == -1 and call(a5=56) == -1 and call(a15=-1) == -1 and call(a16=0) == -1
     assert call(a1=36) == -2 and call(a3=68) == -2 and call(a5=68) == -2 and call(a16=30) == -2 and call(a17=60) == -2
     assert call(a10=P + 8) == -2 and call(a6=P + 4) == -2
-    assert h.orl_linear_bwd_scratch(-1, 8) == -1 and h.orl_linear_bwd_scratch(5, 12) == -1
+    assert h.orl_linear_bwd_scratch(-1, 8, 8) == -1 and h.orl_linear_bwd_scratch(5, 12, 8) == -1
     # one partial row per strip of eight rows or more, for each of the two sums
-    assert h.orl_linear_bwd_scratch(5, 32) == 2 * 32 and h.orl_linear_bwd_scratch(1000, 32) == 2 * 125 * 32
+    assert h.orl_linear_bwd_scratch(5, 32, 64) == 2 * 32 and h.orl_linear_bwd_scratch(1000, 32, 64) == 2 * 125 * 32
+    # few rows: a partial dx per strip of 64 rows of the weight or more
+    assert h.orl_linear_bwd_scratch(3, 640, 512) == 10 * 3 * 512
 
 
 def test_norm_rope_gradient_refuses(h):
-    ok = [P] * 8 + [10, 2, 64, 1, 1e-6, 0, 64, None]
+    ok = [P] * 8 + [10, 2, 64, 1, 1e-6, 0, 64, P, None]
     call = lambda **at: h.orl_qk_norm_rope_bwd(*with_(ok, **at))
-    assert all(call(**{f'a{i}': None}) == -1 for i in range(8))
+    assert all(call(**{f'a{i}': None}) == -1 for i in (*range(8), 15))
     assert call(a8=-1) == -1 and call(a9=0) == -1 and call(a10=60) == -1 and call(a13=2) == -1 and call(a14=32) == -1
     assert call(a9=200) == -3 and call(a10=96, a14=96) == -3 and call(a14=66) == -2 and call(a1=P + 4) == -2
     assert h.orl_qk_norm_rope_bwd_scratch(10, 2, 64, 1) == 2 * 64       # 8 rows of 32 threads share a block
