@@ -47,6 +47,17 @@ def reference(x, w, cos, sin, dy, heads, eps, per_head, shift):
 @pytest.mark.parametrize('heads,dh,per_head', [(16, 128, True), (12, 128, False), (4, 64, True), (3, 64, False),
                                                (1, 64, False), (1, 8, True), (64, 128, False)])
 def test_gradients(rows, heads, dh, per_head):
+    check_gradients(rows, heads, dh, per_head)
+
+
+@pytest.mark.parametrize('rows', [1, 149, 2003])
+@pytest.mark.parametrize('heads,dh,per_head', [(40, 128, False), (40, 128, True), (13, 96, False), (60, 40, False),
+                                               (3, 256, True), (5, 24, False), (1, 8192, False), (9, 256, False)])
+def test_gradients_of_rows_over_several_warps_and_odd_heads(rows, heads, dh, per_head):
+    check_gradients(rows, heads, dh, per_head)
+
+
+def check_gradients(rows, heads, dh, per_head):
     from onereel_b200.rope import qk_norm_rope
     shift = 0 if per_head else 1
     x, w, cos, sin, dy = make(rows, heads, dh, per_head, seed=rows)
