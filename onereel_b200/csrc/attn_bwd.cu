@@ -99,7 +99,8 @@ struct BwdCfg {
   static constexpr int kBarDs = kBarP + 2;              // dS stored; kDq: per group
   static constexpr int kBarDone = kBarDs + 2;
   static constexpr int kBarDrain = kBarDone + 1;
-  static constexpr int kNumBars = kBarDrain + 1;
+  static constexpr int kBarDrain1 = kBarDrain + 1;      // kDq: of the thread that issues S and dP
+  static constexpr int kNumBars = kBarDrain1 + 1;
   static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColDv = 256, kColDk = 256 + D;       // kDkv (S at 0, dP at 128)
@@ -268,8 +269,8 @@ __device__ __forceinline__ uint32_t load_relaxed(const float* p) {
   return v;
 }
 
-// 64 threads (t = 0..63) wait for each streamed tile and hand it on prepared, so that the issuing thread has one wait
-// for it. kDkv: the statistics of its query rows (lse2 = +inf past the end, so P = 0 there) into one of two slots, zeros
+// 64 threads (kDq: 32) wait for each streamed tile and hand it on prepared, so that the issuing thread has one wait for it.
+// kDkv: the statistics of its query rows (lse2 = +inf past the end, so P = 0 there) into one of two slots, zeros
 // over the shared-memory rows past the end.
 template <int D>
 __device__ __forceinline__ void bwd_prepare_dkv(const BwdShared& sh, const BwdWork& wi, const int2* ranges,
@@ -347,7 +348,7 @@ __device__ __forceinline__ void bwd_prepare_dq(const BwdShared& sh, const BwdWor
     if (valid < kDqRows) {
       uint8_t* k = sh.smem + C::kPairOff + a.s * 2 * C::kHalfBytes;
       for (int c = 0; c < C::kChunks; ++c)
-        for (int o = valid * 128 + t * 16; o < C::kHalfChunk; o += kAuxThreads * 16)
+        for (int o = valid * 128 + t * 16; o < C::kHalfChunk; o += 32 * 16)
           *reinterpret_cast<uint4*>(k + c * C::kHalfChunk + o) = make_uint4(0u, 0u, 0u, 0u);
       fence_async_smem();
     }
@@ -435,52 +436,50 @@ __device__ __forceinline__ void bwd_mma_dkv(const BwdShared& sh, uint32_t tmem, 
   bwd_mma_end(sh, ok, C::kBarDone, C::kBarDrain, err);
 }
 
+// kDq has two issuing threads, one for S and dP and one for dQ. One thread for all three was never waiting for anything but
+// its own instructions (900 clocks of waits that were met and of issuing per 64 keys, in which the MMAs take 450 at D = 64
+// and 900 at D = 128). What orders them is what the compute warps have read and written.
 template <int D>
-__device__ __forceinline__ void bwd_mma_dq(const BwdShared& sh, uint32_t tmem, const BwdWork& wi, int* err) {
+__device__ __forceinline__ void bwd_mma_dq_scores(const BwdShared& sh, uint32_t tmem, const BwdWork& wi, int* err) {
   using C = BwdCfg<D>;
   constexpr uint32_t kIdescS = idesc_bf16(128, 64, false, false);
-  constexpr uint32_t kIdescA = idesc_bf16(128, D, false, true);
   constexpr uint64_t kStep = (2 * C::kHalfBytes) >> 4;
-  const int n = wi.n_tiles;
   auto wait = [&](int bar, int phase) { return mbar_wait(sh.bar(bar), phase & 1, sh.abort_flag); };
   const uint64_t o0 = smem_desc_sw128(sh.sbase + C::kROff, 16, 1024);
   const uint64_t k0 = smem_desc_sw128(sh.sbase + C::kPairOff, 16, 1024), v0 = k0 + (C::kHalfBytes >> 4);
-  const uint64_t kt0 = smem_desc_sw128(sh.sbase + C::kPairOff, C::kHalfChunk, 1024);    // K MN-major
-  Ring a(C::kPairStages), nx(C::kPairStages);            // tile u; the next tile whose S and dP are to be issued
-  // S = q K^T and dP = dO V^T of tile x into its group's columns
-  auto issue = [&](int x) {
-    const uint32_t d = tmem + 64 * (x & 1);
+  Ring a(C::kPairStages);
+  bool ok = wait(C::kBarQ, 0) && wait(C::kBarR, 0);
+  for (int u = 0; ok && u < wi.n_tiles; ++u, a.next()) {
+    // into the columns of tile u - 2 once that has been read
+    ok = wait(C::kBarAux + a.s, a.ph) && (u < 2 || wait(C::kBarP + (u & 1), (u >> 1) - 1));
+    if (!ok) break;
+    tc_fence_after();
+    const uint32_t d = tmem + 64 * (u & 1);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk)
-      mma_ts(d, tmem + C::kColQ + kk * 8, k0 + nx.s * kStep + (((kk >> 2) * C::kHalfChunk + (kk & 3) * 32) >> 4), kIdescS,
+      mma_ts(d, tmem + C::kColQ + kk * 8, k0 + a.s * kStep + (((kk >> 2) * C::kHalfChunk + (kk & 3) * 32) >> 4), kIdescS,
              kk > 0 ? 1u : 0u);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk)
       mma_ss(d + C::kColDp, o0 + (((kk >> 2) * C::kChunkBytes + (kk & 3) * 32) >> 4),
-             v0 + nx.s * kStep + (((kk >> 2) * C::kHalfChunk + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
-    mma_commit(sh.bar(C::kBarS + (x & 1)));
-    nx.next();
-  };
-  // tile x may be issued once tile x - 2 has been read
-  auto ready = [&](int x) {
-    return wait(C::kBarAux + nx.s, nx.ph) && (x < 2 || wait(C::kBarP + (x & 1), (x >> 1) - 1));
-  };
-  bool ok = wait(C::kBarQ, 0) && wait(C::kBarR, 0);
-  for (int x = 0; ok && x < 3 && x < n; ++x) {
-    ok = ready(x);
-    if (!ok) break;
-    tc_fence_after();
-    issue(x);
+             v0 + a.s * kStep + (((kk >> 2) * C::kHalfChunk + (kk & 3) * 32) >> 4), kIdescS, kk > 0 ? 1u : 0u);
+    mma_commit(sh.bar(C::kBarS + (u & 1)));
   }
-  for (int u = 0; ok && u < n; ++u) {
-    // the other group reads its tile u + 1 before this one has dS of tile u
-    if (u + 3 < n) {
-      ok = ready(u + 3);
-      if (!ok) break;
-      tc_fence_after();
-      issue(u + 3);
-    }
-    ok = wait(C::kBarDs + (u & 1), u >> 1);
+  if (!ok) atomicOr(err, kErrTimeoutMma);
+  mma_commit(sh.bar(C::kBarDrain1));
+  bwd_drain_wait(sh.bar(C::kBarDrain1), 0, err);
+}
+
+template <int D>
+__device__ __forceinline__ void bwd_mma_dq_acc(const BwdShared& sh, uint32_t tmem, const BwdWork& wi, int* err) {
+  using C = BwdCfg<D>;
+  constexpr uint32_t kIdescA = idesc_bf16(128, D, false, true);
+  constexpr uint64_t kStep = (2 * C::kHalfBytes) >> 4;
+  const uint64_t kt0 = smem_desc_sw128(sh.sbase + C::kPairOff, C::kHalfChunk, 1024);    // K MN-major
+  Ring a(C::kPairStages);
+  bool ok = true;
+  for (int u = 0; u < wi.n_tiles; ++u, a.next()) {
+    ok = mbar_wait(sh.bar(C::kBarDs + (u & 1)), (u >> 1) & 1, sh.abort_flag);
     if (!ok) break;
     tc_fence_after();
 #pragma unroll
@@ -488,7 +487,6 @@ __device__ __forceinline__ void bwd_mma_dq(const BwdShared& sh, uint32_t tmem, c
       mma_ts(tmem + C::kColDq, tmem + C::kColDs + 32 * (u & 1) + kk * 8, kt0 + a.s * kStep + ((kk * 2048) >> 4), kIdescA,
              (u > 0 || kk > 0) ? 1u : 0u);
     mma_commit(sh.bar(C::kBarE0 + a.s));
-    a.next();
   }
   bwd_mma_end(sh, ok, C::kBarDone, C::kBarDrain, err);
 }
@@ -708,6 +706,7 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
     dl[i] = dlse != nullptr && r < wi.rows ? __ldg(dlse + static_cast<long long>(wi.head) * nq + wi.row0 + r) : 0.f;
     pdp[i] = 0.f;
   }
+  const F2 sc = f2(scale_log2, scale_log2);
   const uint32_t s_addr = tmem + 64 * grp + lanes, dp_addr = s_addr + C::kColDp, ds_addr = tmem + C::kColDs + 32 * grp + lanes;
   constexpr uint32_t kBlock = 16u << 16;        // TMEM lane offset of the second 16-lane block
   TileWalk<kDqRows> walk(ranges, wi.n_ranges);
@@ -733,8 +732,12 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        p[h][i] = __float_as_uint(ex2(fmaf(__uint_as_float(p[h][i]), scale_log2, -lse2[2 * h + ((i >> 1) & 1)])));
+      for (int r = 0; r < 16; ++r) {
+        const float l = -lse2[2 * h + (r & 1)];
+        const float2 x = f2_split(ffma2(f2_of(&p[h][2 * r]), sc, f2(l, l)));
+        p[h][2 * r] = __float_as_uint(ex2(x.x));
+        p[h][2 * r + 1] = __float_as_uint(ex2(x.y));
+      }
     if (valid < kDqRows) {
       // keys past the range add nothing, whatever their rows held
 #pragma unroll
@@ -864,7 +867,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(sh.bar(C::kBarQ), 256);
     for (int s = 0; s < C::kMaxStages; ++s) {
       mbar_init(sh.bar(C::kBarT0 + s), 1);
-      mbar_init(sh.bar(C::kBarAux + s), kAuxThreads);
+      mbar_init(sh.bar(C::kBarAux + s), dkv ? kAuxThreads : 32);
       mbar_init(sh.bar(C::kBarE0 + s), 1);
     }
     for (int s = 0; s < C::kStages1; ++s) {
@@ -879,6 +882,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(sh.bar(C::kBarDp), 1);
     mbar_init(sh.bar(C::kBarDone), 1);
     mbar_init(sh.bar(C::kBarDrain), 1);
+    mbar_init(sh.bar(C::kBarDrain1), 1);
     *sh.abort_flag = 0;
     fence_mbar_init();
   }
@@ -904,12 +908,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       } else if (warp == 1) {
         if (elect_one()) {
           if (dkv) bwd_mma_dkv<D>(sh, tmem, wi, err);
-          else bwd_mma_dq<D>(sh, tmem, wi, err);
+          else bwd_mma_dq_scores<D>(sh, tmem, wi, err);
         }
       } else if (dkv) {
         bwd_prepare_dkv<D>(sh, wi, rg, stats, delta, nq, threadIdx.x - 64, err);
-      } else {
+      } else if (warp == 2) {
         bwd_prepare_dq<D>(sh, wi, rg, threadIdx.x - 64, err);
+      } else if (elect_one()) {
+        bwd_mma_dq_acc<D>(sh, tmem, wi, err);
       }
     }
   } else {
