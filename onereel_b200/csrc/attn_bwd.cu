@@ -13,29 +13,35 @@
 // S and dP are computed twice (seven products of the size of S instead of five). In exchange nothing is added across
 // CTAs: no atomics, no fp32 dQ in memory, the same bits on every run.
 //
-// A CTA is the forward's: warp 0 streams tiles by TMA, warp 1 owns TMEM and issues the MMAs, warps 2-3 prepare each
-// tile (row statistics of streamed queries; zeros in the shared-memory rows past a range's end, so that what lies
-// there - other segments, or NaN in rows no segment owns - enters no product), warps 4-11 hold P and dS: a warp owns 16
-// TMEM lanes, a thread two rows and 32 of their 128 columns each. P and dS go back to TMEM as bf16 and are the A
-// operand of the accumulating MMAs.
+// A CTA has the forward's roles: warp 0 streams tiles by TMA, warp 1 owns TMEM and issues MMAs (kDq: those of S and dP;
+// warp 3 those of dQ), warps 2-3 (kDq: warp 2) prepare each tile (row statistics of streamed queries; zeros in the
+// shared-memory rows past a range's end, so that what lies there - other segments, or NaN in rows no segment owns -
+// enters no product), warps 4-11 hold P and dS as fragments of two rows of a 16-lane block each and write them back to
+// TMEM as bf16, the A operand of the accumulating MMAs.
 //
 // kDkv, tiles of 128 queries. TMEM columns: S^T / P^T [0,128), dP^T / dS^T [128,256), dV [256,256+D), dK [256+D,256+2D):
 // all 512 at D = 128. While the compute warps work on P(j) the tensor pipe runs dK(j-1) and dP(j); while they work on
 // dS(j), dV(j) and S(j+1). P is handed over in two halves, so dV begins under the second half's exponentials.
 // kDq, tiles of 64 keys, taken by turns by two groups of four compute warps: a step (loads, exponentials, dS) is mostly
 // latency, and each group's hides in the other's. TMEM columns, per group: S [0,128), dP [128,256), dS [256,320) (bf16);
-// dQ [320,320+D), q [448,..) as a bf16 A operand: from TMEM a 64-column MMA takes 32 clocks instead of the 48 that reading
-// both operands from shared memory costs (dO has no TMEM left). S and dP of a group's next tile are issued once it has
-// read them, dQ when dS is there.
+// dQ [320,320+D), q [448,..) as a bf16 A operand: from TMEM a 64-column MMA takes 32 clocks instead of the 48 that
+// reading both operands from shared memory costs (dO has no TMEM left). S and dP of a group's next tile are issued once
+// it has read them, dQ when dS is there.
 //
-// delta. do . o~ with the forward's bf16 o~ (P rounded, then o rounded) is off by some e_i, the same for all keys of query
-// i. In dq_i it adds e_i sum_j P k, one more error of the size of dS's roundings. In the dk it adds up: sum_j dS_ij should
-// be 0 and becomes -e_i, so that sums of dk over keys - the gradient of a key bias - came out twice as far from float64 as
-// with exact attention. So the kDq blocks, which see all keys of their queries, also sum P dP in fp32 and publish
-// delta_i = sum_j P dP - dL; the kDkv blocks wait for it. Items are drawn by a ticket with the kDq items first: whoever
-// holds a kDkv item knows that every kDq item is being computed or done, and kDq items wait for nothing. Where one tile
-// holds all keys of its queries (at most 64: then dS is a small difference of large terms; two keys: dq 0.0040 off in
-// the 2-norm instead of 0.0024) a kDq block uses its own sum as well.
+// delta. do . o~ with the forward's bf16 o~ (P rounded, then o rounded) is off by some e_i, the same for all keys of
+// query i. In dq_i it adds e_i sum_j P k, one more error of the size of dS's roundings. In the dk it adds up: sum_j dS_ij
+// should be 0 and becomes -e_i, so that sums of dk over keys - the gradient of a key bias - came out twice as far from
+// float64 as with exact attention. So the kDq blocks, which see all keys of their queries, also sum P dP in fp32 and
+// publish delta_i = sum_j P dP - dL; the kDkv blocks wait for it. Items are drawn by a ticket with the kDq items first:
+// whoever holds a kDkv item knows that every kDq item is being computed or done, and kDq items wait for nothing. Where
+// one tile holds all keys of its queries (at most 64: then dS is a small difference of large terms; two keys: dq 0.0040
+// off in the 2-norm instead of 0.0024) a kDq block uses its own sum as well.
+//
+// What bounds it (figures: forward excluded, 5 products of useful work). 16 heads of 128, 22516 x 48212 rows in segments
+// of up to 14438 keys: 6.7 ms, 0.90 PFLOP/s useful and 1.26 computed, with the clock down at 1.7 GHz under the power cap:
+// the seven products run at 0.92 of the rate at which a library product is sustained under that cap. 16 heads of 64,
+// 3 x 2048 rows: 273 us; a tile costs the compute warps as much as at D = 128 (exponentials, TMEM loads and barriers of
+// some 1200 clocks per 64 keys), in which its MMAs take 450.
 //
 // Every mbarrier wait is bounded as in the forward: a stuck pipeline sets the error word and winds down.
 #include <cuda.h>
@@ -105,7 +111,8 @@ struct BwdCfg {
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColDv = 256, kColDk = 256 + D;       // kDkv (S at 0, dP at 128)
   static constexpr uint32_t kColDp = 128, kColDs = 256, kColDq = 320, kColQ = 448;                // kDq (S at 0)
-  static_assert(kPairOff + kPairStages * 2 * kHalfBytes <= kStatOff && kPairStages <= kMaxStages && kStages0 <= kMaxStages, "rings");
+  static_assert(kPairOff + kPairStages * 2 * kHalfBytes <= kStatOff, "ring of pairs");
+  static_assert(kPairStages <= kMaxStages && kStages0 <= kMaxStages, "rings");
   static_assert(kStatOff % 16 == 0 && kBarOff % 8 == 0, "alignment");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
@@ -969,9 +976,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 }
 
 // ---------------------------------------------------------------------------------------------- row statistics
-// stats[h][row] = (lse * log2 e, sum_d dO o - dL), and delta[h][row] marked as pending, the ticket as undrawn. Memory bound: dO and o are read once, 16 bytes per thread, D / 8
-// lanes per (row, head); a block covers 32 rows x 8 heads and writes its pairs through shared memory, so that the
-// head-major statistics are written in runs of 32 rows.
+// stats[h][row] = (lse * log2 e, sum_d dO o - dL), and delta[h][row] marked as pending, the ticket as undrawn. Memory
+// bound: dO and o are read once, 16 bytes per thread, D / 8 lanes per (row, head); a block covers 32 rows x 8 heads and
+// writes its pairs through shared memory, so that the head-major statistics are written in runs of 32 rows.
 template <int D>
 __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const __nv_bfloat16* __restrict__ out,
                                                              const __nv_bfloat16* __restrict__ dout,
@@ -1068,7 +1075,8 @@ static int launch_attn_bwd(const void* q, const void* k, const void* v, const vo
                                                      ticket, nq, heads);
   if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
   attn_bwd_kernel<D><<<n_items, kBwdThreads, C::kSmemBytes, stream>>>(
-      mq, mk, mv, mdo, static_cast<const __nv_bfloat16*>(q), work, ranges, stats, delta, ticket, dlse, static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
+      mq, mk, mv, mdo, static_cast<const __nv_bfloat16*>(q), work, ranges, stats, delta, ticket, dlse,
+      static_cast<__nv_bfloat16*>(dq), static_cast<__nv_bfloat16*>(dk),
       static_cast<__nv_bfloat16*>(dv), nq, heads, scale, err, n_items_dev);
   return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
 }
