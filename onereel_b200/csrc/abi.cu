@@ -27,9 +27,9 @@ extern "C" int orl_error_bits_describe(int bits, char* buf, int cap) {
   if (buf == nullptr || cap <= 0) return ORL_ERR_ARG;
   buf[0] = 0;
   const struct { int bit; const char* what; } names[] = {
-      {orl::kErrTimeoutLoad, "producer timed out waiting for a free K/V stage"},
-      {orl::kErrTimeoutMma, "MMA warp timed out waiting for a tile or for P"},
-      {orl::kErrTimeoutSoftmax, "softmax warps timed out waiting for S or O"},
+      {orl::kErrTimeoutLoad, "a load did not arrive or its stage (K/V in attention) was not freed in time"},
+      {orl::kErrTimeoutMma, "MMA warp timed out waiting for a tile, an accumulator, P or dS"},
+      {orl::kErrTimeoutSoftmax, "softmax (or epilogue) warps timed out waiting for S, O or an accumulator"},
       {orl::kErrTimeoutDrain, "wind-down timed out waiting for in-flight copies"},
       {orl::kErrTimeoutPack, "pack kernel timed out waiting for a bulk copy"},
       {orl::kErrPlan, "cu_seqlens rejected on the device (decreasing or outside the tensors): nothing computed"},

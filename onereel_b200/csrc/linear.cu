@@ -6,14 +6,19 @@
 // gemm_kernel computes C = A B^T over operands whose contraction dimension is contiguous (K-major) or not (MN-major:
 // the tcgen05 descriptors read such tiles transposed), so dx and dw need no transposed copies. Persistent and warp
 // specialised: warp 0 streams 64-deep A and B tiles by TMA into a ring, warp 1 issues the MMAs into one of two TMEM
-// accumulators, warps 4-7 drain the other: bias, activation, gate, residual and the bf16 stores run under the next
-// tile's MMAs. kCtas = 2: a cluster of two CTAs owns a 256 x 256 tile (tcgen05 cta_group::2): each holds half of A's
+// accumulators, four or eight warps drain the other: bias, activation, gate, residual and the bf16 stores run under the
+// next tile's MMAs. kCtas = 2: a cluster of two CTAs owns a 256 x 256 tile (tcgen05 cta_group::2): each holds half of A's
 // rows and half of B's, so an SM reads 64 bytes of shared memory per clock where a 128 x 256 tile of its own would read
 // 96 and fill as much again. Its epilogue moves 32-row x 64-column pieces through shared memory: the residual comes in
 // and y (and z) go out by TMA, whole 128-byte lines at a time (stored from the registers, a row per lane, the epilogue of
 // 9540 x 2048 -> 8192 with z took longer than the product: 319 us instead of 222). kCtas = 1 serves problems too small
 // for that, down to a few rows. Rows and columns past the ends are zeros (TMA fill) and are not stored.
 // Every mbarrier wait is bounded (ptx.cuh).
+//
+// Measured (device time): 22260 x 8192 -> 2048 with bias, gate and residual 520 us, 1.43 PFLOP/s, 0.88 of a library
+// product's burst rate; 9540 x 2048 -> 8192 with gelu 238 us keeping z, dx 234, dw 219, dz and db 99 + 4. Few rows: 1 x 2048
+// -> 24576 19.4 us, 0.79 of the memory's copy rate; 77 x 2048 -> 8192 11.4 us (the weight alone 5.4), where neither the
+// memory nor the tensor pipe is busy: a block's chain of loads, products and epilogue is.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
