@@ -279,3 +279,47 @@ def test_few_keys_keep_their_precision(lk, D):
     for t, n in zip(got, ('dq', 'dk', 'dv')):
         rel = ((t.double() - want[n][0]).norm() / want[n][0].norm()).item()
         assert rel < tol, (n, rel)
+
+
+@pytest.mark.parametrize('D', [64, 128])
+def test_calls_on_two_streams_at_once(D):
+    """backward passes that share the GPU (each one's key blocks wait for its own query blocks) give the bits of one alone"""
+    from onereel_b200 import attention as A
+    H, n = 6, 2500
+    q, k, v, dout, _ = inputs(n, n, H, D, seed=21)
+    seg = ([0, 900], [900, n - 900], [0, 700], [1500, n - 700])
+    out, lse = A.attend(q, k, v, *seg, lse=True)
+    want = A.attend_grad(q, k, v, out, lse, dout, *seg)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(A.attend_grad(q, k, v, out, lse, dout, *seg))
+    torch.cuda.synchronize()
+    A.check()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def test_one_tensor_in_every_place_and_gradients_of_some():
+    """q, k and v one leaf: its gradient is the three roles' sum; gradients asked of v alone; a broadcast dout"""
+    from onereel_b200 import attention as A
+    H, n, D = 2, 200, 64
+    x = rand(n, H, D, seed=30)
+    cu = A.cu_seqlens([n])
+    leaves = [x.clone().requires_grad_() for _ in range(3)]
+    parts = torch.autograd.grad(A.varlen(*leaves, cu, cu, n, n).sum(), leaves)
+    one = x.clone().requires_grad_()
+    (g,) = torch.autograd.grad(A.varlen(one, one, one, cu, cu, n, n).sum(), one)
+    # autograd adds the three in some order and rounds each sum
+    total = sum(p.double() for p in parts)
+    assert (g.double() - total).abs().max().item() <= 2.0 ** -7 * sum(p.double().abs() for p in parts).max().item()
+    v = x.clone().requires_grad_()
+    (gv,) = torch.autograd.grad(A.varlen(x, x, v, cu, cu, n, n).sum(), v)
+    assert torch.equal(gv, parts[2])
+    # Elementwise bounds, not the norm's two roundings: here s_ii = |x_i|^2 / 8 is about 8 where the others are about 1, so
+    # P_ii is near 1 and dS_ii = P_ii (dP_ii - delta_i) a difference of sums over 64 elements of size 1 that nearly
+    # cancel: out's rounding alone moves delta_i by u |sum_d o_id| / sqrt(3), some 0.02, against dS of a few tenths.
+    want = attention_grads(x, x, x, torch.ones_like(x), [0], [n], [0], [n])
+    for p, name in zip(parts, ('dq', 'dk', 'dv')):
+        assert ((p.double() - want[name][0]).abs() <= want[name][1]).all(), name

@@ -231,3 +231,21 @@ def test_refusals():
         linear(x, w, residual=x)
     with pytest.raises(ValueError):
         linear(x, w, gate=x[:1, :8])
+
+
+@pytest.mark.parametrize('act', [None, 'silu'])
+def test_gradient_of_the_residual_alone_and_of_no_rows(act):
+    from onereel_b200.linear import linear
+    g = torch.Generator().manual_seed(5)
+    w = torch.randn(64, 128, generator=g).cuda().bfloat16()
+    x = torch.randn(5, 128, generator=g).cuda().bfloat16()
+    gate = torch.randn(64, generator=g).cuda().bfloat16()
+    residual = torch.randn(5, 64, generator=g).cuda().bfloat16().requires_grad_()
+    dy = torch.randn(5, 64, generator=g).cuda().bfloat16()
+    (dr,) = torch.autograd.grad(linear(x, w, None, act, residual, gate), residual, dy)
+    assert torch.equal(dr, dy)
+    none = torch.empty(0, 128, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    leaf, b, gt = w.clone().requires_grad_(), gate.clone().requires_grad_(), gate.clone().requires_grad_()
+    y = linear(none, leaf, b, act, None, gt)
+    grads = torch.autograd.grad(y, (none, leaf, b, gt), torch.empty_like(y))
+    assert [t.shape for t in grads] == [none.shape, leaf.shape, b.shape, gt.shape] and not any(t.any() for t in grads)
