@@ -16,6 +16,7 @@ synchronises and raises if it is set (tests and benchmarks call it; it costs a d
 """
 from __future__ import annotations
 
+import functools
 from collections import OrderedDict
 
 import numpy as np
@@ -74,6 +75,23 @@ class _Device:
     def __exit__(self, *exc):
         if self.back != self.index:
             torch.cuda.set_device(self.back)
+
+
+def _first_order(backward):
+    """once_differentiable, whose own cost (it enters no_grad and looks every gradient over) is only paid where a second
+    derivative could be asked for: without create_graph the backward pass runs with autograd off"""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_size(name: str, *sizes) -> int:
+    """what the C ABI's size query `name` answers for these sizes"""
+    return L.check(getattr(L.lib(), name)(*sizes), name)
 
 
 def check(device=None) -> None:
@@ -257,7 +275,7 @@ def _attend_cu(q, k, v, cu_q, cu_k, lse, own_scratch=False):
     Nq, H, Dh = q.shape
     dev = q.device
     n_seg = cu_q.numel() - 1
-    need = L.check(L.lib().orl_attn_fwd_cu_capacity(Nq, n_seg, H), 'orl_attn_fwd_cu_capacity')
+    need = _scratch_size('orl_attn_fwd_cu_capacity', Nq, n_seg, H)
     stream = _stream(dev)
     key = (dev.index, stream)
     work = None if own_scratch else _CU_WORK.get(key)
@@ -362,8 +380,7 @@ def _attend_cu_grad(q, k, v, out, lse, dout, dlse, cu_q, cu_k):
     """attend_grad for cu_seqlens on the device, planned there (orl_attn_bwd_cu)"""
     dev, n_seg = q.device, cu_q.numel() - 1
     with _Device(dev):
-        need = L.check(L.lib().orl_attn_bwd_cu_scratch(q.shape[0], k.shape[0], n_seg, q.shape[1]),
-                       'orl_attn_bwd_cu_scratch')
+        need = _scratch_size('orl_attn_bwd_cu_scratch', q.shape[0], k.shape[0], n_seg, q.shape[1])
         grads, args, stats, scratch, keep = _bwd_args(q, k, v, out, lse, dout, dlse, need)
         L.check(L.lib().orl_attn_bwd_cu(*args, q.shape[2] ** -0.5, cu_q.data_ptr(), cu_k.data_ptr(), n_seg, scratch,
                                         need, stats, _err_word(dev).data_ptr(), _stream(dev)), 'orl_attn_bwd_cu')
@@ -383,7 +400,7 @@ class _Ranges(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout, dlse):
         if dout is None and dlse is None:
             return None, None, None, None
@@ -404,7 +421,7 @@ class _Varlen(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout, dlse):
         if dout is None and dlse is None:
             return None, None, None, None, None
@@ -422,7 +439,7 @@ class _PackRows(torch.autograd.Function):
         return pack_rows(parts, parts[0].new_empty(sum(ctx.lengths), *parts[0].shape[1:]))
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         return g.split(ctx.lengths)
 

@@ -10,8 +10,13 @@
 
 namespace orl {
 
-static __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, int rows, int cols,
-                                                                 long long ld, __nv_bfloat16* __restrict__ out) {
+// Two such sums may share a launch: blockIdx.y = 1 takes part1 and out1.
+static __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part0, int rows, int cols,
+                                                                 long long ld, __nv_bfloat16* __restrict__ out0,
+                                                                 const float* __restrict__ part1,
+                                                                 __nv_bfloat16* __restrict__ out1) {
+  const float* part = blockIdx.y == 0 ? part0 : part1;
+  __nv_bfloat16* out = blockIdx.y == 0 ? out0 : out1;
   __shared__ float s[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int c = 32 * blockIdx.x + x;
@@ -34,8 +39,11 @@ static __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __
   if (x == 0 && cc < cols) out[cc] = __float2bfloat16_rn(v);
 }
 
-inline int column_sum(const float* part, int rows, int cols, long long ld, void* out, cudaStream_t stream) {
-  column_sum_kernel<<<(cols + 31) / 32, 1024, 0, stream>>>(part, rows, cols, ld, static_cast<__nv_bfloat16*>(out));
+// part1 / out1: a second sum of the same shape, or NULL
+inline int column_sum(const float* part, int rows, int cols, long long ld, void* out, cudaStream_t stream,
+                      const float* part1 = nullptr, void* out1 = nullptr) {
+  column_sum_kernel<<<dim3((cols + 31) / 32, part1 != nullptr ? 2 : 1), 1024, 0, stream>>>(
+      part, rows, cols, ld, static_cast<__nv_bfloat16*>(out), part1, static_cast<__nv_bfloat16*>(out1));
   return cudaGetLastError() == cudaSuccess ? ORL_OK : ORL_ERR_LAUNCH;
 }
 

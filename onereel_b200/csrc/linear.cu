@@ -899,8 +899,9 @@ extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, lon
         static_cast<const __nv_bfloat16*>(gate), mm, nn,
         z != nullptr && products ? static_cast<__nv_bfloat16*>(dz) : nullptr, part_b, part_g);
     if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
-    if (part_b != nullptr && (rc = column_sum(part_b, strips, nn, n, dbias, stream)) != ORL_OK) return rc;
-    if (part_g != nullptr && (rc = column_sum(part_g, strips, nn, n, dgate, stream)) != ORL_OK) return rc;
+    if (part_b != nullptr) rc = column_sum(part_b, strips, nn, n, dbias, stream, part_g, dgate);
+    else if (part_g != nullptr) rc = column_sum(part_g, strips, nn, n, dgate, stream);
+    if (rc != ORL_OK) return rc;
   }
   const void* g = z != nullptr ? dz : dy;
   const long long ldg = z != nullptr ? n : lddy;

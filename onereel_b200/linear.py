@@ -8,10 +8,9 @@ gave up is reported by onereel_b200.attention.check().
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
-from onereel_b200.attention import _Device, _err_word, _stream
+from onereel_b200.attention import _Device, _err_word, _first_order, _scratch_size, _stream
 
 ACTIVATIONS = {None: 0, 'gelu_tanh': 1, 'silu': 2}
 
@@ -74,14 +73,17 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         _check('gate', gate, None, dev)
         if gate.numel() != N:
             raise ValueError(f'gate must have {N} elements, got {tuple(gate.shape)}')
-    args = [x.reshape(-1, K), weight, bias, None if gate is None else gate.reshape(-1),
-            None if residual is None else residual.reshape(-1, N)]
+    # reshaped only where need be: with gradients each view is one more node of the graph
+    flat = x.dim() == 2
+    args = (x if flat else x.reshape(-1, K), weight, bias,
+            gate if gate is None or gate.dim() == 1 else gate.reshape(-1),
+            residual if residual is None or flat else residual.reshape(-1, N))
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
         y = _Linear.apply(*args, act)
     else:
         y = _forward(*args, act, keep=False)[0]
-    return y.view(shape)
+    return y if flat else y.view(shape)
 
 
 def _forward(x, w, b, gate, residual, act, keep):
@@ -111,7 +113,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, w, gate, z = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -124,7 +126,7 @@ class _Linear(torch.autograd.Function):
             db = new(N) if need[2] else None
             dgate = new(N) if need[3] else None
             # scratch: partial sums, then dz where it is not dy itself
-            sums = 4 * L.check(L.lib().orl_linear_bwd_scratch(M, N, K), 'orl_linear_bwd_scratch')
+            sums = 4 * _scratch_size('orl_linear_bwd_scratch', M, N, K)
             scratch = torch.empty(sums + (0 if z is None else 2 * M * N), dtype=torch.uint8, device=dev)
             at = scratch.data_ptr()
             L.check(L.lib().orl_linear_bwd(d.data_ptr(), _ld(d), xr.data_ptr(), _ld(xr), wr.data_ptr(), _ld(wr), _ptr(z),

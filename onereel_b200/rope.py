@@ -5,10 +5,9 @@ into a Triton kernel)."""
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
-from onereel_b200.attention import _Device, _err_word, _stream
+from onereel_b200.attention import _Device, _err_word, _first_order, _scratch_size, _stream
 
 
 def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int,
@@ -59,7 +58,7 @@ class _QkNormRope(torch.autograd.Function):
             return _forward(x, w, c, s, heads, eps, per_head, sin_shift)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, w, c, s = ctx.saved_tensors
         dx, dw = qk_norm_rope_grad(x, w, c, s, dy, *ctx.args)
@@ -77,8 +76,7 @@ def qk_norm_rope_grad(x, weight, cos, sin, dy, heads: int, eps: float, per_head:
     dy = dy.contiguous()
     dy = dy if dy.data_ptr() % 16 == 0 else dy.clone()
     with _Device(x.device):
-        n = L.check(L.lib().orl_qk_norm_rope_bwd_scratch(rows, heads, hidden // heads, int(per_head)),
-                    'orl_qk_norm_rope_bwd_scratch')
+        n = _scratch_size('orl_qk_norm_rope_bwd_scratch', rows, heads, hidden // heads, int(per_head))
         scratch = torch.empty(n, dtype=torch.float32, device=x.device)
         dx, dw = torch.empty_like(x), torch.empty_like(weight)
         L.check(L.lib().orl_qk_norm_rope_bwd(x.data_ptr(), dy.data_ptr(), weight.data_ptr(), cos.data_ptr(),
