@@ -707,6 +707,7 @@ __global__ void __launch_bounds__(256, 4) linear_dz_kernel(const __nv_bfloat16* 
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int r = r0 + u * stride;
+        if (r >= m) break;                               // no 0 * gate where the gate is infinite
         float d[8];
         unpack8(rd[u], d);
         if (slope) {
@@ -719,7 +720,7 @@ __global__ void __launch_bounds__(256, 4) linear_dz_kernel(const __nv_bfloat16* 
             d[i] *= gf[i] * a.y;
           }
         }
-        if (dz != nullptr && r < m) *reinterpret_cast<uint4*>(dz + static_cast<long long>(r) * n + col) = pack8(d);
+        if (dz != nullptr) *reinterpret_cast<uint4*>(dz + static_cast<long long>(r) * n + col) = pack8(d);
 #pragma unroll
         for (int i = 0; i < 8; ++i) sb[i] += d[i];
       }

@@ -249,3 +249,17 @@ def test_gradient_of_the_residual_alone_and_of_no_rows(act):
     y = linear(none, leaf, b, act, None, gt)
     grads = torch.autograd.grad(y, (none, leaf, b, gt), torch.empty_like(y))
     assert [t.shape for t in grads] == [none.shape, leaf.shape, b.shape, gt.shape] and not any(t.any() for t in grads)
+
+
+def test_infinite_gate_reaches_only_its_own_column():
+    """a row strip's missing second row adds nothing, not 0 * inf, to the column sums"""
+    from onereel_b200.linear import linear
+    g = torch.Generator().manual_seed(6)
+    x, w = (torch.randn(*s, generator=g).cuda().bfloat16() for s in ((9, 64), (64, 64)))
+    b = torch.zeros(64, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    gate = torch.ones(64, device='cuda', dtype=torch.bfloat16)
+    gate[3] = float('inf')
+    (db,) = torch.autograd.grad(linear(x, w, b, None, None, gate), b, torch.ones(9, 64, device='cuda', dtype=torch.bfloat16))
+    want = torch.full_like(db, 9.0)
+    want[3] = float('inf')
+    assert torch.equal(db, want)
