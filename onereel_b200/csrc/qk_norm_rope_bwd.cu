@@ -166,7 +166,9 @@ __global__ void __launch_bounds__(32 * kNrWarps) qk_norm_rope_bwd_kernel(
     };
     // dx and the weight sums of one chunk from its row's (or head's) sums
     auto finish = [&](int c, float sum_xx, float sum_wux) {
-      const float inv = rsqrtf(sum_xx * inv_n + eps);
+      // Over heads, lanes past the row's end have sums of their own, all 0: without their factor of 0 (eps = 0: infinite
+      // times their zeros) they would put NaN into the weight sums that they share with the row's lanes.
+      const float inv = kMode == kHead && kNrChunk * c + 8 * lane >= cols ? 0.f : rsqrtf(sum_xx * inv_n + eps);
       const float back = -inv * inv * inv * inv_n * sum_wux;
       const F2 inv2 = f2(inv, inv), back2 = f2(back, back);
       const int cw = kMode == kHead ? 0 : c;

@@ -121,3 +121,20 @@ def test_refusals():
         qk_norm_rope_grad(x, w, cos, sin, dy.float(), 2, 1e-6, True, 0)
     with pytest.raises(ValueError):
         qk_norm_rope_grad(x, w, cos, sin, dy[:5], 2, 1e-6, True, 0)
+
+
+@pytest.mark.parametrize('heads,dh,per_head', [(5, 64, True), (1, 128, True), (3, 128, True), (1, 8, True), (4, 64, True),
+                                               (5, 24, False), (16, 128, False)])
+@pytest.mark.parametrize('eps', [0.0, 1e-2])
+def test_gradients_without_and_with_a_large_epsilon(heads, dh, per_head, eps):
+    """rows whose elements are not a multiple of a warp's 256 columns: the lanes without elements add nothing, also where
+    only eps stands between their sum of squares (0) and a division by it"""
+    from onereel_b200.rope import qk_norm_rope
+    x, w, cos, sin, dy = make(67, heads, dh, per_head, seed=heads)
+    x.requires_grad_()
+    w.requires_grad_()
+    y = qk_norm_rope(x, w, cos, sin, heads, eps, per_head, 0)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    wx, ww = reference(x, w, cos, sin, dy, heads, eps, per_head, 0)
+    assert_close(dx, wx, 'dx')
+    assert_close(dw, ww, 'dw')
