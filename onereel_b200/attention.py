@@ -17,6 +17,7 @@ synchronises and raises if it is set (tests and benchmarks call it; it costs a d
 from __future__ import annotations
 
 import functools
+import threading
 from collections import OrderedDict
 
 import numpy as np
@@ -43,7 +44,50 @@ def cu_seqlens(lengths, device='cuda') -> torch.Tensor:
 
 # ------------------------------------------------------------------------------------------------ plans and errors
 
-_PLANS: OrderedDict = OrderedDict()
+def _capturing(device) -> bool:
+    """whether the current stream is being captured into a graph"""
+    return torch.device(device).type == 'cuda' and torch.cuda.is_current_stream_capturing()
+
+
+class _Plans:
+    """Device tables by layout (layouts repeat every layer and step), shared by the calling and autograd's threads. Kernels
+    read the tables by address, so an entry's memory outlives its readers: what a captured graph was given stays for good
+    (a replay reads it again), and the others leave half the cache at a time, least recently used first, after their
+    devices have been waited for (no kernel on any stream still reads them)."""
+
+    def __init__(self, limit: int = 512):
+        self.limit = limit
+        self.entries: OrderedDict = OrderedDict()
+        self.held: dict = {}                     # entries given to a captured graph
+        self.lock = threading.Lock()
+
+    def get(self, key, device, build):
+        """the entry of key (on `device`), made by build() where there is none"""
+        capturing = _capturing(device)
+        with self.lock:
+            hit = self.held.get(key)
+            if hit is None:
+                hit = self.entries.get(key)
+                if hit is not None:
+                    self.entries.move_to_end(key)
+                    if capturing:
+                        self.held[key] = hit
+            if hit is not None:
+                return hit
+        entry = build()
+        gone = []
+        with self.lock:
+            entry = self.entries.setdefault(key, entry)
+            if capturing:
+                self.held[key] = entry
+            elif len(self.entries) > self.limit:
+                gone = [self.entries.popitem(last=False) for _ in range(len(self.entries) - self.limit // 2)]
+        for dev in {t.device for _, e in gone for t in e if isinstance(t, torch.Tensor) and t.is_cuda}:
+            torch.cuda.synchronize(dev)
+        return entry
+
+
+_PLANS = _Plans()
 _ERR: dict = {}
 
 
@@ -107,12 +151,12 @@ def check(device=None) -> None:
 
 
 def plan(q_start, q_len, k_start, k_len, heads: int, device) -> tuple[torch.Tensor, int]:
-    """device work list for segments given as (start, length) rows (cached: layouts repeat every layer and step)"""
+    """device work list for segments given as (start, length) rows and its item count (cached)"""
     key = (tuple(q_start), tuple(q_len), tuple(k_start), tuple(k_len), heads, str(device))
-    hit = _PLANS.get(key)
-    if hit is not None:
-        _PLANS.move_to_end(key)
-        return hit
+    return _PLANS.get(key, device, lambda: _make_plan(*key[:4], heads, device))
+
+
+def _make_plan(q_start, q_len, k_start, k_len, heads, device):
     arrs = [np.ascontiguousarray(x, dtype=np.int32) for x in (q_start, q_len, k_start, k_len)]
     n_seg = len(arrs[0])
     need = L.lib().orl_attn_plan_ranges(*(L.i32p(a) for a in arrs), n_seg, heads, None, 0)
@@ -124,11 +168,7 @@ def plan(q_start, q_len, k_start, k_len, heads: int, device) -> tuple[torch.Tens
     work = np.zeros(max(need_n, 1), dtype=L.WORK_DTYPE)
     n = L.check(L.lib().orl_attn_plan_ranges(*(L.i32p(a) for a in arrs), n_seg, heads, work.ctypes.data, len(work)),
                 'orl_attn_plan_ranges')
-    dev = torch.from_numpy(work.view(np.uint8)).to(device)
-    _PLANS[key] = (dev, n)
-    if len(_PLANS) > 512:
-        _PLANS.popitem(last=False)
-    return dev, n
+    return torch.from_numpy(work.view(np.uint8)).to(device), n
 
 
 def _host_list(x) -> list[int]:
@@ -295,17 +335,17 @@ def _attend_cu(q, k, v, cu_q, cu_k, lse, own_scratch=False):
 
 # ------------------------------------------------------------------------------------------------ gradients
 
-_BWD_PLANS: OrderedDict = OrderedDict()
+_BWD_PLANS = _Plans()
 
 
 def _plan_bwd(q_start, q_len, k_start, k_len, heads: int, nq: int, nk: int, device):
     """device work list and ranges of the backward pass for segments given as (start, length) rows (cached like
     `plan`): (items uint8 [32 n], ranges int32 [m, 2], n)"""
     key = (tuple(q_start), tuple(q_len), tuple(k_start), tuple(k_len), heads, nq, nk, str(device))
-    hit = _BWD_PLANS.get(key)
-    if hit is not None:
-        _BWD_PLANS.move_to_end(key)
-        return hit
+    return _BWD_PLANS.get(key, device, lambda: _make_bwd_plan(*key[:4], heads, nq, nk, device))
+
+
+def _make_bwd_plan(q_start, q_len, k_start, k_len, heads, nq, nk, device):
     arrs = [np.ascontiguousarray(x, dtype=np.int32) for x in (q_start, q_len, k_start, k_len)]
     args = [L.i32p(a) for a in arrs] + [len(arrs[0]), heads, nq, nk]
     n_ranges = L.c_int(0)
@@ -317,11 +357,7 @@ def _plan_bwd(q_start, q_len, k_start, k_len, heads: int, nq: int, nk: int, devi
     else:
         work, ranges = np.zeros(1, dtype=L.BWD_WORK_DTYPE), np.zeros((1, 2), dtype=np.int32)
     L.check(n, 'orl_attn_bwd_plan')
-    res = (torch.from_numpy(work.view(np.uint8)).to(device), torch.from_numpy(ranges).to(device), n)
-    _BWD_PLANS[key] = res
-    if len(_BWD_PLANS) > 512:
-        _BWD_PLANS.popitem(last=False)
-    return res
+    return torch.from_numpy(work.view(np.uint8)).to(device), torch.from_numpy(ranges).to(device), n
 
 
 def _aligned(x):

@@ -323,3 +323,33 @@ def test_one_tensor_in_every_place_and_gradients_of_some():
     want = attention_grads(x, x, x, torch.ones_like(x), [0], [n], [0], [n])
     for p, name in zip(parts, ('dq', 'dk', 'dv')):
         assert ((p.double() - want[name][0]).abs() <= want[name][1]).all(), name
+
+
+def test_captured_host_planned_calls_outlive_the_plan_cache(monkeypatch):
+    """forward and backward of overlapping ranges captured after a first call, replayed when the caches have dropped
+    hundreds of layouts since and their memory has been given out again: the replay's own work lists are still there"""
+    from onereel_b200 import attention as A
+    H, D = 2, 64
+    qr, kr = [(0, 90), (90, 250)], [(0, 150), (40, 260)]
+    q, k, v, dout, _ = inputs(250, 260, H, D, seed=60)
+
+    def step():
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        return torch.autograd.grad(A.overlapping_ranges(*leaves, qr, kr), leaves, dout)
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for n in range(1, 700):
+        A.plan([0], [n], [0], [n], H, q.device)
+        A._plan_bwd([0], [n], [0], [n], H, n, n, q.device)
+    key = next(iter(A._BWD_PLANS.held))
+    assert key not in A._BWD_PLANS.entries and len(A._BWD_PLANS.entries) <= A._BWD_PLANS.limit
+    junk = [torch.full((4096,), 7, dtype=torch.int32, device='cuda') for _ in range(600)]
+    with torch.no_grad():
+        q.copy_(rand(250, H, D, seed=70))
+    graph.replay()
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(res, want))
+    A.check()
+    del junk
