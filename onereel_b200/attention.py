@@ -25,7 +25,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
-from onereel_b200.pack import pack_rows
+from onereel_b200.pack import capturing, pack_rows, upload
 
 BACKEND = 'b200'         # 'b200' (also accepted: the reference's 'fa2' | 'fa3' | 'auto', all served by this kernel)
 _BACKENDS = ('b200', 'fa2', 'fa3', 'auto')
@@ -44,11 +44,6 @@ def cu_seqlens(lengths, device='cuda') -> torch.Tensor:
 
 # ------------------------------------------------------------------------------------------------ plans and errors
 
-def _capturing(device) -> bool:
-    """whether the current stream is being captured into a graph"""
-    return torch.device(device).type == 'cuda' and torch.cuda.is_current_stream_capturing()
-
-
 class _Plans:
     """Device tables by layout (layouts repeat every layer and step), shared by the calling and autograd's threads. Kernels
     read the tables by address, so an entry's memory outlives its readers: what a captured graph was given stays for good
@@ -63,24 +58,22 @@ class _Plans:
 
     def get(self, key, device, build):
         """the entry of key (on `device`), made by build() where there is none"""
-        capturing = _capturing(device)
+        taken = capturing(device)
         with self.lock:
             hit = self.held.get(key)
             if hit is None:
                 hit = self.entries.get(key)
                 if hit is not None:
                     self.entries.move_to_end(key)
-                    if capturing:
+                    if taken:
                         self.held[key] = hit
             if hit is not None:
                 return hit
-        entry = build()
+        entry = build()                          # refused in a capture
         gone = []
         with self.lock:
             entry = self.entries.setdefault(key, entry)
-            if capturing:
-                self.held[key] = entry
-            elif len(self.entries) > self.limit:
+            if len(self.entries) > self.limit:
                 gone = [self.entries.popitem(last=False) for _ in range(len(self.entries) - self.limit // 2)]
         for dev in {t.device for _, e in gone for t in e if isinstance(t, torch.Tensor) and t.is_cuda}:
             torch.cuda.synchronize(dev)
@@ -168,7 +161,7 @@ def _make_plan(q_start, q_len, k_start, k_len, heads, device):
     work = np.zeros(max(need_n, 1), dtype=L.WORK_DTYPE)
     n = L.check(L.lib().orl_attn_plan_ranges(*(L.i32p(a) for a in arrs), n_seg, heads, work.ctypes.data, len(work)),
                 'orl_attn_plan_ranges')
-    return torch.from_numpy(work.view(np.uint8)).to(device), n
+    return upload(work.view(np.uint8), device), n
 
 
 def _host_list(x) -> list[int]:
@@ -357,7 +350,7 @@ def _make_bwd_plan(q_start, q_len, k_start, k_len, heads, nq, nk, device):
     else:
         work, ranges = np.zeros(1, dtype=L.BWD_WORK_DTYPE), np.zeros((1, 2), dtype=np.int32)
     L.check(n, 'orl_attn_bwd_plan')
-    return torch.from_numpy(work.view(np.uint8)).to(device), torch.from_numpy(ranges).to(device), n
+    return upload(work.view(np.uint8), device), upload(ranges, device), n
 
 
 def _aligned(x):

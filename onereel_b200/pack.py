@@ -20,6 +20,21 @@ def _err_word(device):
     return word(device)
 
 
+def capturing(device) -> bool:
+    """whether the current stream is being captured into a graph"""
+    return torch.device(device).type == 'cuda' and torch.cuda.is_current_stream_capturing()
+
+
+def upload(table: np.ndarray, device) -> torch.Tensor:
+    """a host table on the device; refused while a graph is captured, which a copy from pageable memory would end with an
+    error that names neither the call nor the way out"""
+    if capturing(device):
+        raise RuntimeError('a table of this layout is not on the device yet, and none can be copied there during a graph '
+                           'capture: run the same calls, both passes, once before capturing them (packed and packed_lse '
+                           'copy a table in every call and cannot be captured)')
+    return torch.from_numpy(table).to(device)
+
+
 class RunTable:
     """a prepared run table on one device: runs_dev (uint8 view of orl_copy_run [n]), total 16-byte vectors"""
     launches = 0          # pack launches issued by this process (benchmark launch accounting)
@@ -36,7 +51,7 @@ class RunTable:
         self.src_slot = [int(x) for x in src_slot]
         self.src_off, self.dst_off = [int(x) for x in src_off], [int(x) for x in dst_off]
         self.nbytes_list = nb.tolist()
-        self.dev = torch.from_numpy(arr.view(np.uint8)).to(device) if n else None
+        self.dev = upload(arr.view(np.uint8), device) if n else None
         self.device = torch.device(device)
 
     def run(self, src_bases, dst_bases, n_planes=1, seg_len_dev=None, cu_out=None, stream=None):
@@ -67,8 +82,8 @@ class RowSum:
         order = np.argsort(source, kind='stable')
         offsets = np.searchsorted(source[order], np.arange(n_rows + 1))
         self.n_rows, self.n_packed = n_rows, int(packed.max()) + 1 if packed.size else 0
-        self.offsets = torch.from_numpy(offsets.astype(np.int32)).to(device)
-        self.rows = torch.from_numpy(packed[order].astype(np.int32)).to(device)
+        self.offsets = upload(offsets.astype(np.int32), device)
+        self.rows = upload(packed[order].astype(np.int32), device)
 
     def run(self, parts):
         """parts: packed gradients [n, H, D] bf16, contiguous -> one [n_rows, H, D] each"""

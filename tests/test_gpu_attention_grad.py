@@ -353,3 +353,22 @@ def test_captured_host_planned_calls_outlive_the_plan_cache(monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(res, want))
     A.check()
     del junk
+
+
+def test_first_use_of_a_layout_in_a_capture_is_refused():
+    """host-planned calls and packs say so instead of ending the capture; the same calls work afterwards"""
+    from onereel_b200 import attention as A
+    H, D = 1, 64
+    q, k, v, dout, _ = inputs(37, 41, H, D, seed=80)
+    leaf = q.clone().requires_grad_()
+    torch.cuda.synchronize()
+    for call in (lambda: A.overlapping_ranges(q, k, v, [(0, 37)], [(3, 41)]), lambda: A.packed([(q, k, v)]),
+                 lambda: A.dense(q[None, :31], k[None, :29], v[None, :29])):
+        with pytest.raises(RuntimeError, match='once before capturing'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        call()
+    (want,) = torch.autograd.grad(A.overlapping_ranges(leaf, k, v, [(0, 37)], [(3, 41)]), leaf, dout)
+    torch.cuda.synchronize()
+    A.check()
+    assert want.shape == q.shape

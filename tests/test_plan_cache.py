@@ -31,9 +31,9 @@ def test_what_a_captured_graph_was_given_stays(monkeypatch):
     from onereel_b200 import attention as A
     c = A._Plans(limit=4)
     first = c.get('a', 'cpu', lambda: (torch.zeros(1), 1))
-    monkeypatch.setattr(A, '_capturing', lambda device: True)
+    monkeypatch.setattr(A, 'capturing', lambda device: True)
     assert c.get('a', 'cpu', None) is first
-    monkeypatch.setattr(A, '_capturing', lambda device: False)
+    monkeypatch.setattr(A, 'capturing', lambda device: False)
     for k in range(50):
         c.get(k, 'cpu', lambda: (torch.zeros(1), 1))
     assert 'a' not in c.entries and c.held['a'] is first
@@ -71,3 +71,16 @@ def test_threads():
     for t in ts:
         t.join()
     assert not errors
+
+
+def test_tables_are_refused_during_a_capture(monkeypatch):
+    """the error comes before the copy that would end the capture, and says what to do"""
+    from onereel_b200 import attention as A, pack
+    monkeypatch.setattr(pack, 'capturing', lambda device: True)
+    monkeypatch.setattr(A, '_PLANS', A._Plans())
+    monkeypatch.setattr(A, '_BWD_PLANS', A._Plans())
+    for call in (lambda: A.plan([0], [3], [0], [4], 1, 'cpu'), lambda: A._plan_bwd([0], [3], [0], [4], 1, 3, 4, 'cpu'),
+                 lambda: pack.RunTable([0], [0], [0], [0], [64], 'cpu'), lambda: pack.RowSum([0], [0], 1, 'cpu')):
+        with pytest.raises(RuntimeError, match='once before capturing'):
+            call()
+    assert not A._PLANS.entries and not A._BWD_PLANS.entries
