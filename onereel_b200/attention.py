@@ -301,12 +301,14 @@ def _check_cu(q, cu_q, cu_k):
 
 def _attend_cu(q, k, v, cu_q, cu_k, lse, own_scratch=False):
     """cu_seqlens on the device: orl_attn_fwd_cu plans the work list on the GPU, no host synchronisation. The
-    scratch is per (device, stream), so calls on one stream reuse it in order; own_scratch: scratch of this call alone
-    (safe in captured graphs that replay side by side)."""
+    scratch is per (device, stream), so calls on one stream reuse it in order; own_scratch, and any call that is being
+    captured: scratch of this call alone (graphs may replay side by side, and after a larger call replaced the stream's
+    scratch)."""
     _check_inputs(q, k, v)
     _check_cu(q, cu_q, cu_k)
     Nq, H, Dh = q.shape
     dev = q.device
+    own_scratch = own_scratch or capturing(dev)
     n_seg = cu_q.numel() - 1
     need = _scratch_size('orl_attn_fwd_cu_capacity', Nq, n_seg, H)
     stream = _stream(dev)

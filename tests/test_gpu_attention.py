@@ -261,3 +261,33 @@ def test_key_split_of_coarse_launches():
     assert (o.float() - o1.float()).abs().max().item() < MAX_ABS
     assert torch.equal(o[sum(lq[:3]):], torch.zeros_like(o[sum(lq[:3]):]))
     assert torch.isinf(l[:, sum(lq[:3]):]).all()
+
+
+def test_captured_varlen_calls_share_no_scratch():
+    """two captured calls with other layouts, replayed side by side on two streams: each gives its eager result, and a
+    capture leaves the streams' scratch alone"""
+    from onereel_b200 import attention as A
+    H, D, n = 4, 64, 1200
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(n, H, D, generator=g).cuda().bfloat16() for _ in range(3))
+    cus = [A.cu_seqlens(x) for x in ([700, 500], [100, 800, 300])]
+    want = [A.varlen(q, k, v, c, c, 800, 800) for c in cus]
+    torch.cuda.synchronize()
+    before = {key: t.data_ptr() for key, t in A._CU_WORK.items()}
+    graphs = []
+    for c in cus:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = A.varlen(q, k, v, c, c, 800, 800)
+        graphs.append((graph, out))
+    assert {key: t.data_ptr() for key, t in A._CU_WORK.items()} == before
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+        torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    A.check()
+    assert all(torch.equal(out, w) for (_, out), w in zip(graphs, want))
