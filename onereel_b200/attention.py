@@ -9,7 +9,7 @@ CUDA tensors with head_dim 64 or 128.
 Gradients: like the reference's FlashAttention calls, `varlen`, `varlen_lse`, `packed`, `packed_lse`,
 `overlapping_ranges` and `dense` are differentiable in q, k and v (also through the log-sum-exp) when autograd is on
 and an input requires a gradient; the backward pass (onereel_b200/csrc/attn_bwd.cu) recomputes the probabilities and is
-deterministic. `attend_grad` is the same computation as a plain call. First derivatives only.
+deterministic. `attend_grad` is the same computation as a plain call. First derivatives in reverse mode only.
 
 Kernel failures: the kernel never hangs; a bounded wait that gives up sets a per-device error word. `check()`
 synchronises and raises if it is set (tests and benchmarks call it; it costs a device sync).
@@ -22,6 +22,7 @@ from collections import OrderedDict
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from onereel_b200 import _lib as L
@@ -476,7 +477,12 @@ class _PackRows(torch.autograd.Function):
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    """whether a call on these tensors (None: not there) has to record a backward pass; refuses tangents of forward-mode
+    differentiation, which a kernel that writes into a fresh tensor would drop"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError('the B200 kernels have no forward-mode derivative (reverse mode only)')
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _attend_ranges(q, k, v, q_start, q_len, k_start, k_len, lse=False):

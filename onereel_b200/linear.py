@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from onereel_b200 import _lib as L
-from onereel_b200.attention import _Device, _err_word, _first_order, _scratch_size, _stream
+from onereel_b200.attention import _Device, _err_word, _first_order, _scratch_size, _stream, _wants_grad
 
 ACTIVATIONS = {None: 0, 'gelu_tanh': 1, 'silu': 2}
 
@@ -53,7 +53,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     x [..., K], weight [N, K], bias [N], gate of N elements (one factor per output feature, e.g. [1, 1, N]), residual
     and the result [..., N]; activation None, 'gelu_tanh' or 'silu'; bf16 CUDA tensors, K and N multiples of 8. Views
     whose rows are strided by multiples of 8 elements are read in place, others are copied. Differentiable in every
-    tensor (first derivatives; deterministic); with an activation or a gate the product is kept for the backward pass."""
+    tensor (first derivatives in reverse mode; deterministic); with an activation or a gate the product is kept for the
+    backward pass."""
     if activation not in ACTIVATIONS:
         raise ValueError(f'unknown activation {activation!r}: one of {sorted(map(str, ACTIVATIONS))}')
     _check('x', x, None, getattr(x, 'device', None))
@@ -79,7 +80,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
             gate if gate is None or gate.dim() == 1 else gate.reshape(-1),
             residual if residual is None or flat else residual.reshape(-1, N))
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+    if _wants_grad(*args):
         y = _Linear.apply(*args, act)
     else:
         y = _forward(*args, act, keep=False)[0]

@@ -7,7 +7,7 @@ from __future__ import annotations
 import torch
 
 from onereel_b200 import _lib as L
-from onereel_b200.attention import _Device, _err_word, _first_order, _scratch_size, _stream
+from onereel_b200.attention import _Device, _err_word, _first_order, _scratch_size, _stream, _wants_grad
 
 
 def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int,
@@ -24,7 +24,7 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
     rows = x.shape[0]
     w = weight.to(device=x.device, dtype=torch.bfloat16).contiguous()
     c, s = _table(cos, rows, x.device), _table(sin, rows, x.device)
-    if (out is None and row_map is None and torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)):
+    if _wants_grad(x, w) and out is None and row_map is None:
         return _QkNormRope.apply(x, w, c, s, heads, float(eps), int(per_head), int(sin_shift))
     return _forward(x, w, c, s, heads, eps, per_head, sin_shift, out, row_map)
 

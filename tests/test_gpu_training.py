@@ -240,3 +240,29 @@ def test_backward_captures_while_an_eager_graph_lives():
     assert all(torch.equal(a, b) for a, b in zip(res, want))
     del alive
     A.check()
+
+
+def test_forward_mode_tangents_are_refused():
+    """every differentiable entry point, with and without an input that requires a gradient"""
+    from torch.autograd import forward_ad
+
+    from onereel_b200 import attention as A
+    from onereel_b200.linear import linear
+    from onereel_b200.rope import qk_norm_rope
+    H, D, n = 2, 64, 10
+    x, w = rand(n, H, D, seed=1), rand(H * D, H * D, seed=2)
+    cos, sin = torch.ones(n, D, device='cuda'), torch.zeros(n, D, device='cuda')
+    cu = A.cu_seqlens([n])
+    calls = [lambda t: A.varlen(t, x, x, cu, cu, n, n), lambda t: A.varlen_lse(x, t, x, cu, cu, n, n),
+             lambda t: A.varlen(x, x, t, [0, n], [0, n], n, n), lambda t: A.packed([(t, x, x)]),
+             lambda t: A.packed_lse([(x, t, x)]), lambda t: A.overlapping_ranges(x, x, t, [(0, n)], [(0, n)]),
+             lambda t: A.dense(t[None], x[None], x[None]), lambda t: linear(t.view(n, -1), w),
+             lambda t: linear(t.view(n, -1), w.requires_grad_()),
+             lambda t: qk_norm_rope(t.view(n, -1), w[0, :D].detach(), cos, sin, H, 1e-6, True, 0)]
+    for call in calls:
+        call(x)
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(NotImplementedError):
+                call(dual)
+    A.check()
