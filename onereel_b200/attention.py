@@ -237,7 +237,7 @@ def _attend_split(q, k, v, q_start, q_len, k_start, k_len, out, lse, scale):
 
 
 def attend(q, k, v, q_start, q_len, k_start, k_len, out=None, lse=None, scale=None, stream=None, split_keys=False):
-    """the kernel call: segment i = q rows q_start[i] + [0, q_len[i]) attending to k / v rows k_start[i] + [0, k_len[i]).
+    """the kernel call, without a backward pass: segment i = q rows q_start[i] + [0, q_len[i]) attending to k / v rows k_start[i] + [0, k_len[i]).
     out [Nq, H, D] bf16 (allocated if None); lse None, True (allocate [H, Nq] fp32) or a tensor. split_keys: allow the
     key split of coarse launches (see SPLIT_WAVES)."""
     _check_inputs(q, k, v)
@@ -264,7 +264,7 @@ def attend(q, k, v, q_start, q_len, k_start, k_len, out=None, lse=None, scale=No
 
 
 def attend_work(q, k, v, work, n_items: int, out, lse=None, scale=None, stream=None):
-    """the kernel call with a caller-held device work list (orl_attn_plan_ranges items, possibly edited on the
+    """the kernel call, without a backward pass, with a caller-held device work list (orl_attn_plan_ranges items, possibly edited on the
     device since: the bounded memory sets each item's key count per head from its selection)"""
     _check_inputs(q, k, v)
     Nq, H, Dh = q.shape
@@ -483,6 +483,39 @@ def _wants_grad(*tensors) -> bool:
                                               for t in tensors):
         raise NotImplementedError('the B200 kernels have no forward-mode derivative (reverse mode only)')
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _NoGradient(torch.autograd.Function):
+    """a value computed outside autograd, handed on; a backward pass that reaches it raises instead of leaving its share out"""
+
+    @staticmethod
+    def forward(ctx, what, value, *inputs):
+        ctx.what = what
+        return value
+
+    @staticmethod
+    def backward(ctx, g):
+        raise NotImplementedError(f'{ctx.what} carries no gradients on the B200 path')
+
+
+def without_gradient(what: str, values, *inputs):
+    """values (a tensor, or a tuple of tensors and None) that a path without a backward pass computed from inputs: as they
+    are, except that a backward pass through them raises where an input asks for a gradient"""
+    if not _wants_grad(*inputs):
+        return values
+    inputs = [x for x in inputs if x is not None]
+    tie = lambda v: v if v is None or v.requires_grad else _NoGradient.apply(what, v, *inputs)
+    return tuple(tie(v) for v in values) if isinstance(values, tuple) else tie(values)
+
+
+def no_gradients(what: str):
+    """decorator of a method on tensors whose results go through without_gradient (those that carry a graph already pass)"""
+    def wrap(method):
+        @functools.wraps(method)
+        def run(self, *tensors, **named):
+            return without_gradient(what, method(self, *tensors, **named), *tensors, *named.values())
+        return run
+    return wrap
 
 
 def _attend_ranges(q, k, v, q_start, q_len, k_start, k_len, lse=False):

@@ -303,6 +303,7 @@ class Processor:
         ehs = attn.to_add_out(ehs.flatten(1, 2)[None].to(hidden_states.dtype))
         return hs, ehs
 
+    @A.no_gradients('the bounded cross-scene memory')
     def memory(self, q, k, v, eq, ek, ev):
         """hunyuan15.py:305-333: bounded cross-scene memory (onereel_b200.memory). One GPU or Ulysses: all tokens of
         the local heads, each rank clusters its own heads. K/V gathering: the rank's scene pieces read their scenes
@@ -358,6 +359,7 @@ class Processor:
             plan = ctx._cache[key] = _RankPlan(ctx, H, Dh, device, lse_overlap)
         return plan
 
+    @A.no_gradients('the gathering scene path')
     def scene(self, q, k, v, eq, ek, ev):
         """hunyuan15.py:212-251: the scenes of this rank's token range. The exchange is posted first; scenes whose keys
         are all local attend while it is in flight; then the others (or, with overlap='lse', the others attend to
@@ -369,7 +371,7 @@ class Processor:
         lse_overlap = ctx.overlap == 'lse'
         plan = self._plan(H, Dh, q.device, lse_overlap)
         if D.world() == 1 and A._wants_grad(q, k, v, eq, ek, ev) and plan.near is not None and plan.near.segs:
-            # one GPU: every key is local. The same values, differentiable (several ranks: no gradients)
+            # one GPU: every key is local. The same values, differentiable (several ranks: a backward pass raises)
             rot = _shared_rotation(ctx, plan.near, k.device) if _move_active(ctx) else None
             return S.attend_plan(plan.near, q, k, v, eq, ek, ev, None if rot is None else _rotate_with(*rot))
         _mark('start')
@@ -424,6 +426,7 @@ class Processor:
                 A.lse_merge(ot[lo:hi], lse_t[:, lo:hi], o2t[lo:hi], l2t[:, lo:hi])
         _mark('far_remote')
 
+    @A.no_gradients('the Ulysses path')
     def ulysses(self, q, k, v, eq, ek, ev):
         """hunyuan15.py:279-303: heads redistributed by all-to-all; every scene on the local heads; text outputs of the
         local heads all-reduced"""

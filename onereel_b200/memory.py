@@ -249,7 +249,7 @@ class MemoryAttention:
         as `frame_plan` describes -> [Sq, H, D] (rows outside the plan's queries are zero)"""
         out = q.new_zeros(q.shape)
         self.run(key, plan, q, k, v, q, k, v, out, out)
-        return out
+        return A.without_gradient('the bounded cross-scene memory', out, q, k, v)
 
     @torch.no_grad()
     def run(self, key, plan: MemoryPlan, q, k, v, eq, ek, ev, ov, ot, remote_k=None, remote_v=None):

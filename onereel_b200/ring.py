@@ -161,4 +161,4 @@ def attention(plan: RingPlan, q, k, v, eq=None, ek=None, ev=None, text_ranges=No
             for w in works:
                 w.wait()
             cur, src = buf, nxt
-    return o.to(q.dtype), (ot.to(eq.dtype) if has_text else None)
+    return A.without_gradient('the ring', (o.to(q.dtype), ot.to(eq.dtype) if has_text else None), q, k, v, eq, ek, ev)

@@ -95,11 +95,12 @@ class Processor:
         if ctx.attn_override is not None:
             qa, ka, va = comm.a2a_heads(q), comm.a2a_heads(k), comm.a2a_heads(v)
             r = ctx.attn_override(self.layer, qa, ka, va)
-            o = comm.a2a_tokens(self.ranges(qa, ka, va) if r is None else r)
+            o = A.without_gradient('the Ulysses path', comm.a2a_tokens(self.ranges(qa, ka, va) if r is None else r), q, k, v)
         elif ctx.memory:
             o = self.memory(q, k, v)
         elif ctx.run_mode == 'ulysses' or D.world() == 1:
-            o = comm.a2a_tokens(self.ranges(comm.a2a_heads(q), comm.a2a_heads(k), comm.a2a_heads(v)))
+            o = A.without_gradient('the Ulysses path', comm.a2a_tokens(
+                self.ranges(comm.a2a_heads(q), comm.a2a_heads(k), comm.a2a_heads(v))), q, k, v)
         elif ctx.run_mode == 'ring':
             o = R.attention(ctx.ring, q, k, v, tag=id(lay.extra))[0]
         else:
@@ -130,6 +131,7 @@ class Processor:
             assert b - a == len(lay.key_frames(j)), 'halo must be contiguous with its scene'
         return A.overlapping_ranges(q, k, v, q_ranges, k_ranges)
 
+    @A.no_gradients('the gathering scene path')
     def scene(self, q, k, v):
         """wan.py:126-152: K/V gathering; scenes whose keys are all local attend while the exchange is in flight"""
         ctx, T, lay = self.ctx, self.ctx.T, self.ctx.layout
@@ -159,6 +161,7 @@ class Processor:
 
 
 
+    @A.no_gradients('the bounded cross-scene memory')
     def memory(self, q, k, v):
         """wan.py:154-173: bounded cross-scene memory (onereel_b200.memory). One GPU / Ulysses: all tokens of the
         local heads; K/V gathering: this rank's scene pieces, with the missing scene frames and every boundary

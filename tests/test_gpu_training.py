@@ -266,3 +266,33 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(NotImplementedError):
                 call(dual)
     A.check()
+
+
+def test_paths_without_gradients_raise_in_the_backward_pass():
+    """bounded memory, Ulysses and the ring, for both models: the same bits as without autograd, and an error where a
+    training step would leave the attention out of its gradients"""
+    from onereel_b200 import hunyuan15 as HY, ring as R, wan
+    from onereel_b200.layout import SceneLayout
+    lay = SceneLayout([3, 2, 4], halo=0)
+    T, H, D, counts = 16, 2, 64, [7, 9, 5]
+    L = lay.n_frames * T
+    x = [rand(n, H, D, seed=i) for i, n in enumerate((L, L, L, *[sum(counts)] * 3))]
+    scale = torch.ones(D, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+
+    def hunyuan(**kw):
+        return HY.Processor(HY.Context(lay, T=T, counts={True: counts}, fwd=1, own=[(0, L)], **kw), 0)
+
+    def wan_(**kw):
+        return wan.Processor(wan.Context(lay, T=T, own=[(0, L)], fwd=1, **kw), 'self', None, 0)
+    calls = [lambda *t: hunyuan(memory=8).memory(*t), lambda *t: hunyuan().ulysses(*t),
+             lambda *t: wan_(memory=8).memory(*t[:3]), lambda *t: wan_().scene(*t[:3]),
+             lambda *t: R.attention(R.RingPlan(lay, 1, T), *t, [(0, 7), (7, 16), (16, 21)], 0)]
+    for call in calls:
+        with torch.no_grad():
+            want = call(*x)
+        got = call(*(t * scale for t in x))
+        pairs = list(zip(got, want)) if isinstance(got, tuple) else [(got, want)]
+        for a, b in pairs:
+            assert torch.equal(a, b)
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(a.float().sum() + scale.float().sum(), scale)

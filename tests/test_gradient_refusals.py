@@ -18,3 +18,36 @@ def test_forward_mode_tangents_are_refused():
                 _wants_grad(t)
     with pytest.raises(NotImplementedError, match='forward-mode'):
         torch.func.jvp(lambda t: t if _wants_grad(t) else t, (x,), (x,))
+
+
+def test_a_path_without_a_backward_pass_raises_in_it():
+    """values and graph-free inference are untouched; backward and grad() through the path raise, also where the rest of the
+    loss has a gradient of its own"""
+    from onereel_b200.attention import no_gradients, without_gradient
+    x, w = torch.randn(3, 4), torch.randn(4, requires_grad=True)
+    q = x * w
+    for values in (q.detach() * 2, (q.detach() * 2, None), (q.detach() * 2, x + 1)):
+        with torch.no_grad():
+            assert without_gradient('this path', values, q, None) is values
+        assert without_gradient('this path', values, x, None) is values
+        tied = without_gradient('this path', values, q, None)
+        one = tied[0] if isinstance(tied, tuple) else tied
+        assert torch.equal(one, q.detach() * 2) and one.requires_grad
+        for t in tied if isinstance(tied, tuple) else (tied,):
+            if t is not None:
+                with pytest.raises(NotImplementedError, match='this path'):
+                    (q.sum() + t.sum()).backward()
+                with pytest.raises(NotImplementedError, match='this path'):
+                    torch.autograd.grad(q.sum() + t.sum(), w)
+        q = x * w
+    kept = x * w                                         # already differentiable: handed on
+    assert without_gradient('this path', kept, q) is kept
+
+    class Path:
+        @no_gradients('this path')
+        def run(self, q, k=None):
+            return q.detach() + 1, None
+    out, none = Path().run(x, k=w)
+    assert none is None and torch.equal(out, x + 1)
+    with pytest.raises(NotImplementedError):
+        out.sum().backward()
