@@ -508,6 +508,29 @@ def without_gradient(what: str, values, *inputs):
     return tuple(tie(v) for v in values) if isinstance(values, tuple) else tie(values)
 
 
+class _Overwritten(torch.autograd.Function):
+    """a tensor that a kernel overwrites: what its old values were saved for refuses them, and a backward pass through the new
+    ones raises"""
+
+    @staticmethod
+    def forward(ctx, what, target, *inputs):
+        ctx.what = what
+        ctx.mark_dirty(target)
+        return target
+
+    @staticmethod
+    def backward(ctx, g):
+        raise NotImplementedError(f'{ctx.what} carries no gradients on the B200 path')
+
+
+def overwrites(what: str, targets, *inputs):
+    """to be called before a kernel overwrites `targets` from inputs: autograd learns of it as of any in-place operation (and
+    refuses the same: leaves, outputs of split)"""
+    if _wants_grad(*targets, *inputs):
+        for t in targets:                        # each tied to all that the kernel reads, one output per node (views need it)
+            _Overwritten.apply(what, t, *(x for x in (*targets, *inputs) if x is not t))
+
+
 def no_gradients(what: str):
     """decorator of a method on tensors whose results go through without_gradient (those that carry a graph already pass)"""
     def wrap(method):
@@ -600,7 +623,9 @@ def dense(q, k, v):
 
 def lse_merge(o1, lse1, o2, lse2):
     """in place: (o1, lse1) <- the merge of two partial results over disjoint keys (hunyuan15.py:274-276,
-    ring.py:63-70). o [n, H, D] bf16 contiguous, lse [H, >= n] fp32 (row stride = its second dimension)."""
+    ring.py:63-70). o [n, H, D] bf16 contiguous, lse [H, >= n] fp32 (row stride = its second dimension). A backward pass
+    through the merged values raises."""
+    overwrites('the log-sum-exp merge', (o1, lse1), o2, lse2)
     n, H, Dh = o1.shape
     s = torch.cuda.current_stream(o1.device).cuda_stream
     L.check(L.lib().orl_lse_merge(o1.data_ptr(), lse1.data_ptr(), o2.data_ptr(), lse2.data_ptr(), n, lse1.stride(0),
@@ -610,7 +635,9 @@ def lse_merge(o1, lse1, o2, lse2):
 
 def lse_merge_acc(acc, lse_acc, part, lse_part):
     """in place: fp32 (acc, lse_acc) <- merged with a bf16 partial result (part, lse_part) over disjoint keys
-    (ring.py:63-70). acc [n, H, D] fp32 / part [n, H, D] bf16 contiguous rows, lse [H, >= n] fp32."""
+    (ring.py:63-70). acc [n, H, D] fp32 / part [n, H, D] bf16 contiguous rows, lse [H, >= n] fp32. A backward pass
+    through the merged values raises."""
+    overwrites('the log-sum-exp merge', (acc, lse_acc), part, lse_part)
     n, H, Dh = acc.shape
     s = torch.cuda.current_stream(acc.device).cuda_stream
     L.check(L.lib().orl_lse_merge_acc(acc.data_ptr(), lse_acc.data_ptr(), part.data_ptr(), lse_part.data_ptr(), n,

@@ -7,7 +7,8 @@ from __future__ import annotations
 import torch
 
 from onereel_b200 import _lib as L
-from onereel_b200.attention import _Device, _err_word, _first_order, _scratch_size, _stream, _wants_grad
+from onereel_b200.attention import (_Device, _err_word, _first_order, _scratch_size, _stream, _wants_grad, overwrites,
+                                    without_gradient)
 
 
 def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int,
@@ -15,7 +16,8 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
                  row_map: torch.Tensor | None = None) -> torch.Tensor:
     """x [rows, heads * D] (or [1, rows, heads * D]) bf16 -> [rows, heads, D] bf16, normalised and rotated; cos / sin
     [rows, D] (any float dtype; converted to fp32 contiguous). out / row_map: write row i to out[row_map[i]].
-    Differentiable in x and weight (first derivatives; the tables get none) unless out or row_map is given."""
+    Differentiable in x and weight (first derivatives; the tables get none); with out or row_map a backward pass through
+    the returned tensor raises."""
     if x.dim() == 3:
         x = x[0]
     if not (x.is_cuda and x.dtype == torch.bfloat16):
@@ -26,7 +28,8 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
     c, s = _table(cos, rows, x.device), _table(sin, rows, x.device)
     if _wants_grad(x, w) and out is None and row_map is None:
         return _QkNormRope.apply(x, w, c, s, heads, float(eps), int(per_head), int(sin_shift))
-    return _forward(x, w, c, s, heads, eps, per_head, sin_shift, out, row_map)
+    y = _forward(x, w, c, s, heads, eps, per_head, sin_shift, out, row_map)
+    return without_gradient('qk_norm_rope with out or row_map', y, x, w)
 
 
 def _table(t, rows: int, device):
@@ -89,10 +92,11 @@ def qk_norm_rope_grad(x, weight, cos, sin, dy, heads: int, eps: float, per_head:
 
 def rotate_rows(x: torch.Tensor, rows: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, sin_shift: int = 0):
     """in place: rows `rows` (int32 CUDA tensor) of x [N, H, D] bf16 rotated by the table rows cos / sin
-    [len(rows), D] fp32 (orl_rope_rows)"""
+    [len(rows), D] fp32 (orl_rope_rows). A backward pass through the rotated values raises."""
     Nr = rows.numel()
     if Nr == 0:
         return x
+    overwrites('rotate_rows', (x,))
     H, Dh = x.shape[1:]
     L.check(L.lib().orl_rope_rows(x.data_ptr(), rows.data_ptr(), Nr, H, Dh, cos.data_ptr(), sin.data_ptr(),
                                   cos.shape[1], int(sin_shift), _stream(x.device)),

@@ -296,3 +296,53 @@ def test_paths_without_gradients_raise_in_the_backward_pass():
             assert torch.equal(a, b)
             with pytest.raises(NotImplementedError):
                 torch.autograd.grad(a.float().sum() + scale.float().sum(), scale)
+
+
+def test_in_place_kernels_raise_in_the_backward_pass():
+    """merging two key parts' results, accumulating one, rotating rows, norm + rope into a buffer: the bits of a call without
+    autograd, and an error in the backward pass where a gradient would come out wrong"""
+    from onereel_b200 import attention as A
+    from onereel_b200.rope import qk_norm_rope, rotate_rows
+    H, D, n, m = 2, 64, 40, 90
+    x = [rand(r, H, D, seed=i) for i, r in enumerate((n, m, m))]
+    cut = lambda t, lo, hi: t[lo:hi].contiguous()
+    cos, sin = torch.full((n, D), 0.6, device='cuda'), torch.full((n, D), 0.8, device='cuda')
+    rows = torch.arange(0, n, 2, dtype=torch.int32, device='cuda')
+
+    def parts(q, k, v):
+        return [A.varlen_lse(q, cut(k, lo, hi), cut(v, lo, hi), [0, n], [0, hi - lo], n, hi - lo)
+                for lo, hi in ((0, 30), (30, m))]
+
+    def merge(q, k, v):
+        (o, l), (o2, l2) = parts(q, k, v)
+        return A.lse_merge(o, l, o2, l2)
+
+    def merge_second_only(q, k, v):
+        with torch.no_grad():
+            o, l = parts(q, k, v)[0]
+        return A.lse_merge(o, l, *parts(q, k, v)[1])
+
+    def accumulate(q, k, v):
+        acc, l = torch.zeros(n, H, D, device='cuda'), torch.full((H, n), -float('inf'), device='cuda')
+        for o2, l2 in parts(q, k, v):
+            A.lse_merge_acc(acc, l, o2, l2)
+        return acc, l
+    calls = [merge, merge_second_only, accumulate, lambda q, k, v: (rotate_rows(q.clone(), rows, cos, sin),),
+             lambda q, k, v: (qk_norm_rope(q.reshape(n, -1), torch.ones(D, device='cuda'), cos, sin, H, 1e-6, True, 0,
+                                           out=torch.empty_like(q)),)]
+    leaves = [t.clone().requires_grad_() for t in x]
+    for call in calls:
+        with torch.no_grad():
+            want = call(*x)
+        got = call(*leaves)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for t in got:
+            with pytest.raises((NotImplementedError, RuntimeError), match='carries no gradients'):
+                torch.autograd.grad(t.float().sum() + sum(y.float().sum() for y in leaves), leaves, retain_graph=True)
+    # the first part's own backward pass does not run on the merged values
+    (o, l), second = parts(*leaves)
+    head = o[:5] * 2
+    A.lse_merge(o, l, *second)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(head.float().sum(), leaves)
+    A.check()

@@ -51,3 +51,32 @@ def test_a_path_without_a_backward_pass_raises_in_it():
     assert none is None and torch.equal(out, x + 1)
     with pytest.raises(NotImplementedError):
         out.sum().backward()
+
+
+def test_overwritten_tensors_raise_in_the_backward_pass():
+    """old values that a node saved are refused, new ones have no gradient; views, second targets and plain targets too;
+    without a wish for gradients nothing is recorded"""
+    from onereel_b200.attention import overwrites
+    w = torch.randn(4, requires_grad=True)
+    a, b = torch.exp(w), torch.zeros(4)                  # exp saves its result
+    overwrites('this kernel', (a, b), torch.ones(4))
+    assert a.requires_grad and b.requires_grad
+    for t in (a, b):
+        with pytest.raises(NotImplementedError, match='this kernel'):
+            torch.autograd.grad(t.sum() + w.sum(), w, retain_graph=True)
+    saved = torch.exp(w)
+    kept = saved * 1
+    overwrites('this kernel', (saved,))
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        kept.sum().backward()
+    base = torch.exp(w)
+    overwrites('this kernel', (base[1:3],))
+    with pytest.raises(NotImplementedError, match='this kernel'):
+        base.sum().backward()
+    plain = torch.zeros(4)
+    overwrites('this kernel', (plain,), torch.ones(4))
+    with torch.no_grad():
+        overwrites('this kernel', (plain, torch.exp(w)), w)
+    assert not plain.requires_grad
+    with pytest.raises(RuntimeError, match='leaf'):
+        overwrites('this kernel', (w,))
