@@ -372,8 +372,13 @@ class Processor:
         plan = self._plan(H, Dh, q.device, lse_overlap)
         if D.world() == 1 and A._wants_grad(q, k, v, eq, ek, ev) and plan.near is not None and plan.near.segs:
             # one GPU: every key is local. The same values, differentiable (several ranks: a backward pass raises)
+            _mark('start')
+            _mark('exchange')
             rot = _shared_rotation(ctx, plan.near, k.device) if _move_active(ctx) else None
-            return S.attend_plan(plan.near, q, k, v, eq, ek, ev, None if rot is None else _rotate_with(*rot))
+            out = S.attend_plan(plan.near, q, k, v, eq, ek, ev, None if rot is None else _rotate_with(*rot))
+            for phase in ('near', 'exchange_wait', 'far', 'text_sync'):
+                _mark(phase)
+            return out
         _mark('start')
         ex = comm.kv_exchange(ctx.exchange, ctx.layout, ctx.own, ctx.T, k, v) if D.world() > 1 else None
         if ex is not None and ex.remote_index != plan.remote_index:

@@ -346,3 +346,20 @@ def test_in_place_kernels_raise_in_the_backward_pass():
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         torch.autograd.grad(head.float().sum(), leaves)
     A.check()
+
+
+def test_phase_marks_with_and_without_gradients(monkeypatch):
+    """the scene path marks the same phases in the same order whether or not it records a backward pass"""
+    from onereel_b200 import hunyuan15 as HY
+    from onereel_b200.layout import SceneLayout
+    lay = SceneLayout([2, 3], halo=1)
+    T, H, D, counts = 16, 2, 64, [3, 4]
+    L = lay.n_frames * T
+    proc = HY.Processor(HY.Context(lay, T=T, counts={True: counts}, fwd=1, own=[(0, L)]), 0)
+    x = [rand(n, H, D, seed=i) for i, n in enumerate((L, L, L, 7, 7, 7))]
+    seen = []
+    for grad in (False, True):
+        monkeypatch.setattr(HY, 'PHASES', [])
+        proc.scene(*(t.clone().requires_grad_(grad) for t in x))
+        seen.append([name for name, _ in HY.PHASES])
+    assert seen[0] == seen[1] and seen[0][0] == 'start' and 'near' in seen[0]
