@@ -263,16 +263,16 @@ ORL_API int orl_peer_gather(const void* const* src, void* const* dst, int planes
 #define ORL_ACT_GELU_TANH 1 /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
 #define ORL_ACT_SILU 2      /* z / (1 + exp(-z)) */
 
-/* z (optional, [m, n]): receives x w^T + bias, which the backward pass of an activation or a gate needs. err_dev: as
- * in orl_attn_fwd. */
+/* z (optional, [m, n]): receives x w^T + bias, which the backward pass of an activation and the gate's gradient need.
+ * err_dev: as in orl_attn_fwd. */
 ORL_API int orl_linear(const void* x, long long ldx, const void* w, long long ldw, const void* bias, const void* gate,
                        const void* residual, long long ldr, void* y, void* z, long long m, long long n, long long k,
                        int act, int* err_dev, void* stream);
 
-/* Gradients of orl_linear from the gradient dy [m, n] (row stride lddy) of y, the forward's inputs and its z (may be
- * NULL without activation and gate): dz = gate * dy * act'(z), dx = dz w [m, k], dw = dz^T x [n, k], dbias = column sums
- * of dz, dgate = column sums of dy * act(z) (bf16; NULL: not computed). The residual's gradient is dy itself.
- * Deterministic. dz: scratch [m, n] bf16, needed for dx or dw when z is given; scratch: device fp32,
+/* Gradients of orl_linear from the gradient dy [m, n] (row stride lddy) of y, the forward's inputs (x for dw, w for dx,
+ * the gate for dx, dw and dbias; NULL where not needed) and its z (may be NULL without activation and dgate):
+ * dz = gate * dy * act'(z), dx = dz w [m, k], dw = dz^T x [n, k], dbias = column sums of dz, dgate = column sums of
+ * dy * act(z) (bf16; NULL: not computed). The residual's gradient is dy itself. Deterministic. dz: scratch [m, n] bf16, needed for dx or dw when z or a gate is given; scratch: device fp32,
  * orl_linear_bwd_scratch elements, needed for dbias, dgate or, with at most four rows, dx. */
 ORL_API int orl_linear_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w, long long ldw,
                            const void* z, const void* gate, int act, void* dz, void* dx, void* dw, void* dbias,

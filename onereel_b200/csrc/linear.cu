@@ -1,6 +1,6 @@
 // Linear layers with their epilogue, bf16 in / fp32 accumulate / bf16 out, for sm_100a:
 //   y = residual + gate * act(x w^T + bias)          x [m, k], w [n, k], bias / gate [n], residual / y [m, n]
-// and their gradients:  dz = gate dy act'(z) (z = x w^T + bias, which the forward keeps), dx = dz w, dw = dz^T x,
+// and their gradients:  dz = gate dy act'(z) (z = x w^T + bias, which the forward keeps for it), dx = dz w, dw = dz^T x,
 // db = sum dz, dgate = sum dy act(z).
 //
 // gemm_kernel computes C = A B^T over operands whose contraction dimension is contiguous (K-major) or not (MN-major:
@@ -719,6 +719,9 @@ __global__ void __launch_bounds__(256, 4) linear_dz_kernel(const __nv_bfloat16* 
             if (kGateGrad) sg[i] += d[i] * a.x;
             d[i] *= gf[i] * a.y;
           }
+        } else if (gate != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] *= gf[i];
         }
         if (dz != nullptr) *reinterpret_cast<uint4*>(dz + static_cast<long long>(r) * n + col) = pack8(d);
 #pragma unroll
@@ -875,10 +878,11 @@ extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, lon
   if (act < ORL_ACT_NONE || act > ORL_ACT_SILU || err_dev == nullptr || lddy < n) return ORL_ERR_ARG;
   if (m > 0 && (dy == nullptr || (dw != nullptr && x == nullptr))) return ORL_ERR_ARG;
   if ((dw != nullptr && ldx < k) || (dx != nullptr && (w == nullptr || ldw < k))) return ORL_ERR_ARG;
-  // an activation's slope, a gate and a gate's gradient need z; with z, dz is not dy and needs room
-  if ((act != ORL_ACT_NONE || gate != nullptr || dgate != nullptr) && z == nullptr && m > 0) return ORL_ERR_ARG;
+  // an activation's slope and a gate's gradient need z; with it or a gate, dz is not dy and needs room
+  if ((act != ORL_ACT_NONE || dgate != nullptr) && z == nullptr && m > 0) return ORL_ERR_ARG;
   const bool products = dx != nullptr || dw != nullptr, sums = dbias != nullptr || dgate != nullptr;
-  if ((z != nullptr && products && dz == nullptr && m > 0) ||
+  const bool own_dz = z != nullptr || gate != nullptr;
+  if ((own_dz && products && dz == nullptr && m > 0) ||
       ((sums || (dx != nullptr && m <= kRowsMax)) && scratch == nullptr))
     return ORL_ERR_ARG;
   if ((lddy & 7) || (dw != nullptr && (ldx & 7)) || (dx != nullptr && (ldw & 7))) return ORL_ERR_ALIGN;
@@ -887,7 +891,7 @@ extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, lon
     if (!lin_aligned(p)) return ORL_ERR_ALIGN;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   const int mm = static_cast<int>(m), nn = static_cast<int>(n), kk = static_cast<int>(k);
-  if (sums || (z != nullptr && products)) {
+  if (sums || (own_dz && products)) {
     const int strips = dz_strips(mm, nn);
     float* part_b = dbias != nullptr ? scratch : nullptr;
     float* part_g = dgate != nullptr ? scratch + static_cast<long long>(strips) * n : nullptr;
@@ -898,14 +902,14 @@ extern "C" int orl_linear_bwd(const void* dy, long long lddy, const void* x, lon
     kernel<<<grid, 256, 0, stream>>>(
         static_cast<const __nv_bfloat16*>(dy), lddy, static_cast<const __nv_bfloat16*>(z),
         static_cast<const __nv_bfloat16*>(gate), mm, nn,
-        z != nullptr && products ? static_cast<__nv_bfloat16*>(dz) : nullptr, part_b, part_g);
+        own_dz && products ? static_cast<__nv_bfloat16*>(dz) : nullptr, part_b, part_g);
     if (cudaGetLastError() != cudaSuccess) return ORL_ERR_LAUNCH;
     if (part_b != nullptr) rc = column_sum(part_b, strips, nn, n, dbias, stream, part_g, dgate);
     else if (part_g != nullptr) rc = column_sum(part_g, strips, nn, n, dgate, stream);
     if (rc != ORL_OK) return rc;
   }
-  const void* g = z != nullptr ? dz : dy;
-  const long long ldg = z != nullptr ? n : lddy;
+  const void* g = own_dz ? dz : dy;
+  const long long ldg = own_dz ? n : lddy;
   if (m > 0 && m <= kRowsMax) {
     auto run = m == 1 ? rows_gradients<1> : m == 2 ? rows_gradients<2> : m == 3 ? rows_gradients<3> : rows_gradients<4>;
     return run(g, ldg, x, ldx, w, ldw, dx, dw, scratch, nn, kk, stream);

@@ -53,8 +53,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     x [..., K], weight [N, K], bias [N], gate of N elements (one factor per output feature, e.g. [1, 1, N]), residual
     and the result [..., N]; activation None, 'gelu_tanh' or 'silu'; bf16 CUDA tensors, K and N multiples of 8. Views
     whose rows are strided by multiples of 8 elements are read in place, others are copied. Differentiable in every
-    tensor (first derivatives in reverse mode; deterministic); with an activation or a gate the product is kept for the
-    backward pass."""
+    tensor (first derivatives in reverse mode; deterministic). Kept for the backward pass is what the wanted gradients need:
+    x for the weight's, the weight for x's, and the product x weight^T + bias (m x n) for the gate's and, under an
+    activation, for all but the residual's."""
     if activation not in ACTIVATIONS:
         raise ValueError(f'unknown activation {activation!r}: one of {sorted(map(str, ACTIVATIONS))}')
     _check('x', x, None, getattr(x, 'device', None))
@@ -107,10 +108,13 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, gate, residual, act):
-        # z is needed for act' and for the gate's gradient; without them dz is dy itself
-        y, z = _forward(x, w, b, gate, residual, act, keep=act != 0 or gate is not None)
-        ctx.save_for_backward(x, w, gate, z)
-        ctx.act = act
+        # Kept is what the wanted gradients are made of: z for act' and for the gate's gradient (without either, dz is dy or
+        # gate dy), x for dw, w for dx.
+        need_x, need_w, need_b, need_gate, _, _ = ctx.needs_input_grad
+        slope = need_x or need_w or need_b
+        y, z = _forward(x, w, b, gate, residual, act, keep=need_gate or (slope and act != 0))
+        ctx.save_for_backward(x if need_w else None, w if need_x else None, gate if slope else None, z)
+        ctx.act, ctx.sizes = act if z is not None else 0, (x.shape[0], *w.shape)
         return y
 
     @staticmethod
@@ -118,20 +122,24 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, gate, z = ctx.saved_tensors
         need = ctx.needs_input_grad
-        (M, K), N, dev = x.shape, w.shape[0], x.device
+        if not any(need[:4]):
+            return None, None, None, None, dy, None
+        (M, N, K), dev = ctx.sizes, dy.device
         with _Device(dev):
-            d, xr, wr = _rows(dy), _rows(x), _rows(w)
+            d, xr, wr = _rows(dy), x if x is None else _rows(x), w if w is None else _rows(w)
             new = lambda *shape: torch.empty(*shape, dtype=torch.bfloat16, device=dev)
             dx = new(M, K) if need[0] else None
             dw = new(N, K) if need[1] else None
             db = new(N) if need[2] else None
             dgate = new(N) if need[3] else None
             # scratch: partial sums, then dz where it is not dy itself
+            own_dz = z is not None or gate is not None
             sums = 4 * _scratch_size('orl_linear_bwd_scratch', M, N, K)
-            scratch = torch.empty(sums + (0 if z is None else 2 * M * N), dtype=torch.uint8, device=dev)
+            scratch = torch.empty(sums + (2 * M * N if own_dz else 0), dtype=torch.uint8, device=dev)
             at = scratch.data_ptr()
-            L.check(L.lib().orl_linear_bwd(d.data_ptr(), _ld(d), xr.data_ptr(), _ld(xr), wr.data_ptr(), _ld(wr), _ptr(z),
+            L.check(L.lib().orl_linear_bwd(d.data_ptr(), _ld(d), _ptr(xr), K if x is None else _ld(xr), _ptr(wr),
+                                           K if w is None else _ld(wr), _ptr(z),
                                            None if gate is None else _vector(gate).data_ptr(), ctx.act,
-                                           None if z is None else at + sums, _ptr(dx), _ptr(dw), _ptr(db), _ptr(dgate),
+                                           at + sums if own_dz else None, _ptr(dx), _ptr(dw), _ptr(db), _ptr(dgate),
                                            at, M, N, K, _err_word(dev).data_ptr(), _stream(dev)), 'orl_linear_bwd')
         return dx, dw, db, dgate, dy if need[4] else None, None

@@ -263,3 +263,31 @@ def test_infinite_gate_reaches_only_its_own_column():
     want = torch.full_like(db, 9.0)
     want[3] = float('inf')
     assert torch.equal(db, want)
+
+
+@pytest.mark.parametrize('m', [3, 150])
+@pytest.mark.parametrize('act,with_gate', [(None, False), (None, True), ('gelu_tanh', False), ('silu', True)])
+def test_frozen_inputs_keep_only_what_the_others_gradients_need(m, act, with_gate):
+    """every set of inputs that want gradients: the bits of the call where all do, and no tensor kept without a use"""
+    from itertools import combinations
+
+    from onereel_b200.linear import linear
+    n, k = 72, 136
+    t = make(m, n, k, residual=True, gate=with_gate, seed=m)
+    dy = rand(m, n, seed=9)
+
+    def grads(names):
+        kept = []
+        d = {a: x.detach().requires_grad_(a in names) for a, x in t.items()}
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: kept.append(tuple(x.shape)) or x, lambda x: x):
+            y = linear(**d, activation=act)
+        return dict(zip(names, torch.autograd.grad(y, [d[a] for a in names], dy))), sorted(kept)
+    full = grads(tuple(t))[0]
+    for size in range(1, len(t) + 1):
+        for names in combinations(t, size):
+            got, kept = grads(names)
+            assert all(torch.equal(got[a], full[a]) for a in names), names
+            slope = any(a in names for a in ('x', 'weight', 'bias'))
+            want = [(m, k)] * ('weight' in names) + [(n, k)] * ('x' in names) + [(n,)] * (with_gate and slope)
+            want += [(m, n)] * ('gate' in names or (act is not None and slope))
+            assert kept == sorted(want), names

@@ -109,3 +109,11 @@ def test_plan_row_sums_cover_every_copy():
         for i in range(n):
             assert rows[off[i]:off[i + 1]] == [p for p, x in enumerate(packed) if x == (source, i)]
     assert len(video.rows) + len(text.rows) == plan.n_keys
+
+
+def test_linear_gradients_without_the_product(h):
+    """z may be left out where no gradient needs it: with a gate and no activation; not for the gate's own gradient"""
+    ok = [P, 32, None, 64, P, 64, None, P, 0, P, P, None, P, None, P, 5, 32, 64, P, None]
+    call = lambda **at: h.orl_linear_bwd(*with_(ok, **at))
+    assert call(a13=P) == -1 and call(a8=1) == -1 and call(a9=None) == -1    # dgate, an activation, no room for dz
+    assert call(a10=P + 8) == -2                                             # past those checks: dx misaligned
