@@ -8,6 +8,8 @@
 //   warp 0      TMA producer: Q tiles once, then K_j / V_j tiles of 128 rows into a ring of shared-memory stages
 //   warp 1      TMEM owner and MMA issuer (one elected thread): S_t = Q_t K_j^T (SS form), O_t += P_t V_j (TS form,
 //               P read from TMEM in two 64-key halves), each committed to an mbarrier
+//   warps 2-3   zero the V rows that the last, ragged tile's PV reads past the segment's end (P is 0 there, but what lies
+//               behind the segment may be NaN or infinite)
 //   warps 4-11  softmax, all eight on one tile at a time (tile 0, then tile 1, per 128-key step): a warp owns 16
 //               TMEM lanes (query rows), a quad of threads one row, 32 of its 128 scores per thread. Loads S,
 //               exponentiates against the running max while reducing the tile max (rescaling O in TMEM only when
@@ -51,7 +53,9 @@ struct AttnCfg {
   static constexpr int kBarP = kBarS + 2;            // + 2 t + half
   static constexpr int kBarDone = kBarP + 4;
   static constexpr int kBarDrain = kBarDone + 1;
-  static constexpr int kNumBars = kBarDrain + 1;
+  static constexpr int kBarTail = kBarDrain + 1;     // a ragged last V tile has landed
+  static constexpr int kBarTailZero = kBarTail + 1;  // its rows past the segment's end are zeros
+  static constexpr int kNumBars = kBarTailZero + 1;
   static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
   static constexpr uint32_t kTmemCols = 512;
   // TMEM columns: S of tile t (128 fp32 columns; its P is 64 bf16x2 columns at the same start), O of tile t
@@ -61,7 +65,8 @@ struct AttnCfg {
 };
 
 constexpr int kThreads = 384;
-// register split: the launch has 384 threads x 168 registers; warpgroup 0 (producer, MMA issuer, two idle warps)
+constexpr int kTailThreads = 64;
+// register split: the launch has 384 threads x 168 registers; warpgroup 0 (producer, MMA issuer, the two tail warps)
 // keeps kRegsLow, the two softmax warpgroups get kRegsHigh (4 x 32 x kRegsLow + 8 x 32 x kRegsHigh = 384 x 168)
 constexpr int kLaunchRegs = 168, kRegsLow = 120, kRegsHigh = 192;
 static_assert(4 * kRegsLow + 8 * kRegsHigh == 12 * kLaunchRegs, "register split must add up to the launch total");
@@ -133,14 +138,32 @@ __device__ __forceinline__ void producer_role(const AttnShared& sh, const CUtens
   }
 }
 
+// ---------------------------------------------------------------------------------------------- tail of V
+// The rows of a ragged last V tile past the segment's end are other segments' or nobody's. P is 0 there, but 0 * NaN would be
+// NaN: they become zeros once the MMA thread has seen the tile land, under the softmax of that tile.
+template <int D>
+__device__ __forceinline__ void tail_role(const AttnShared& sh, int k_len, int n_kv, int t) {
+  using C = AttnCfg<D>;
+  const int first = k_len - 128 * (n_kv - 1), rows = 128 - first;
+  if (rows == 0 || !mbar_wait(sh.bar(C::kBarTail), 0, sh.abort_flag)) return;     // the waiting MMA thread reports it
+  const uint32_t v = sh.sbase + C::kVOff + ((n_kv - 1) % C::kStages) * C::kTileBytes + first * 128;
+  for (int i = t; i < rows * 8 * C::kChunks; i += kTailThreads) {
+    const int chunk = i / (rows * 8), o = i - chunk * rows * 8;
+    smem_zero16(v + chunk * C::kChunkBytes + 16 * o);
+  }
+  fence_async_smem();
+  mbar_arrive(sh.bar(C::kBarTailZero));
+}
+
 // ---------------------------------------------------------------------------------------------- MMA issuer
 // Per 128-key tile j: S_t = Q_t K_j^T (both operands from shared memory) and O_t += P_t V_j (A = P from TMEM,
 // B = V MN-major), P handed over in two 64-key halves so the PV of the first half starts while the softmax warps
 // still exponentiate the second. Issue order: PV_0(j), S_0(j+1), PV_1(j), S_1(j+1): the tensor pipe computes one
 // tile while the softmax warps work on the other.
 template <int D>
-__device__ __forceinline__ void mma_role(const AttnShared& sh, uint32_t tmem, int n_qt, int n_kv, int* err) {
+__device__ __forceinline__ void mma_role(const AttnShared& sh, uint32_t tmem, int n_qt, int n_kv, int k_len, int* err) {
   using C = AttnCfg<D>;
+  const int j_ragged = (k_len & 127) != 0 ? n_kv - 1 : -1;
   constexpr uint32_t kIdescS = idesc_bf16(128, 128, false, false);
   constexpr uint32_t kIdescO = idesc_bf16(128, D, false, true);
   auto issue_s = [&](int t, int s) {
@@ -173,6 +196,10 @@ __device__ __forceinline__ void mma_role(const AttnShared& sh, uint32_t tmem, in
     const bool more = j + 1 < n_kv;
     bool k_next = false;                 // K of tile j + 1 waited for (lazily, before its first S)
     ok = mbar_wait(sh.bar(C::kBarV + s), (j / C::kStages) & 1, sh.abort_flag);
+    if (ok && j == j_ragged) {
+      mbar_arrive(sh.bar(C::kBarTail));
+      ok = mbar_wait(sh.bar(C::kBarTailZero), 0, sh.abort_flag);
+    }
     for (int t = 0; ok && t < n_qt; ++t) {
       for (int half = 0; ok && half < 2; ++half) {
         ok = mbar_wait(sh.bar(C::kBarP + 2 * t + half), j & 1, sh.abort_flag);
@@ -442,6 +469,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 4; ++i) mbar_init(sh.bar(C::kBarP + i), 256);
     mbar_init(sh.bar(C::kBarDone), 1);
     mbar_init(sh.bar(C::kBarDrain), 1);
+    mbar_init(sh.bar(C::kBarTail), 1);
+    mbar_init(sh.bar(C::kBarTailZero), kTailThreads);
     *sh.abort_flag = 0;
     fence_mbar_init();
   }
@@ -460,7 +489,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       if (elect_one() && n_kv > 0) producer_role<D>(sh, &tm_q, &tm_k, &tm_v, wi, n_qt, n_kv, err);
     } else if (warp == 1) {
-      if (elect_one() && n_kv > 0) mma_role<D>(sh, tmem, n_qt, n_kv, err);
+      if (elect_one() && n_kv > 0) mma_role<D>(sh, tmem, n_qt, n_kv, wi.k_len, err);
+    } else if (n_kv > 0) {
+      tail_role<D>(sh, wi.k_len, n_kv, threadIdx.x - 64);
     }
   } else {
     regs_inc<kRegsHigh>();

@@ -132,6 +132,11 @@ __device__ __forceinline__ void bulk_wait() {
   asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// 16 bytes of shared memory (a shared-window address) to zeros
+__device__ __forceinline__ void smem_zero16(uint32_t addr) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");
+}
+
 // Orders this thread's earlier ordinary shared-memory writes before later accesses of the asynchronous proxy (TMA,
 // tcgen05.mma operand reads) that an mbarrier arrival after it releases.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

@@ -199,7 +199,7 @@ class MemoryPlan:
 
     def kv_buffers(self, like: torch.Tensor):
         """persistent packed K / V (zero-initialised once: representative slots beyond a head's count and the spare
-        row are read by the last key tile of a segment and must hold finite values)"""
+        row are loaded, and masked, by the last key tile of a segment)"""
         if self.buffers is None:
             self.buffers = (like.new_zeros(self.n_rows, self.H, self.Dh), like.new_zeros(self.n_rows, self.H, self.Dh))
         return self.buffers

@@ -291,3 +291,56 @@ def test_captured_varlen_calls_share_no_scratch():
     torch.cuda.synchronize()
     A.check()
     assert all(torch.equal(out, w) for (_, out), w in zip(graphs, want))
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+@pytest.mark.parametrize('lk', [[1, 130], [16, 200], [100, 127], [129, 5], [300, 250], [384, 513], [1025, 40]])
+def test_rows_of_other_segments_reach_nothing(lk, bad, D):
+    """NaN or infinity in the keys and values behind a segment (the next segment's, or rows no segment owns), which its last
+    tile loads as well: the segment's rows are the bits that they are with clean neighbours, through every entry point"""
+    from onereel_b200 import attention as A
+    H, lq = 3, [70, 300]
+    g = torch.Generator().manual_seed(lk[0])
+    q, k, v = (torch.randn(n, H, D, generator=g).cuda().bfloat16() for n in (sum(lq), sum(lk) + 90, sum(lk) + 90))
+    cq, ck = A.cu_seqlens(lq), A.cu_seqlens(lk)
+    calls = [lambda *t: A.varlen_lse(*t, cq, ck, 300, max(lk)), lambda *t: A.varlen_lse(*t, cq.tolist(), ck.tolist(), 300, 0),
+             lambda *t: (A.overlapping_ranges(*t, [(0, 70), (70, 370)], [(0, lk[0]), (lk[0], sum(lk))]), None)]
+    for call in calls:
+        want, want_l = call(q, k, v)
+        assert torch.isfinite(want).all()
+        kk, vv = k.clone(), v.clone()
+        kk[sum(lk):] = bad
+        vv[sum(lk):] = bad
+        got, got_l = call(q, kk, vv)
+        assert torch.equal(got, want) and (want_l is None or torch.equal(got_l, want_l))
+        kk[lk[0]:] = bad                             # all of the second segment's too
+        vv[lk[0]:] = bad
+        got, got_l = call(q, kk, vv)
+        assert torch.equal(got[:70], want[:70]) and (want_l is None or torch.equal(got_l[:, :70], want_l[:, :70]))
+    torch.cuda.synchronize()
+    A.check()
+
+
+@pytest.mark.parametrize('D', [64, 128])
+def test_gradients_with_bad_rows_behind_the_segments(D):
+    """NaN in q, k, v and dout rows that no segment owns: values and gradients as with zeros there, zero gradients for them"""
+    from onereel_b200 import attention as A
+    H, lq, lk = 2, [70, 130], [200, 301]
+    g = torch.Generator().manual_seed(11)
+    data = [torch.randn(n, H, D, generator=g).cuda().bfloat16() for n in (300, 600, 600, 300)]
+    cq, ck = (torch.tensor(c, dtype=torch.int32, device='cuda') for c in ([40, 110, 240], [30, 230, 531]))
+    res = []
+    for fill in (0.0, float('nan')):
+        x = [t.clone() for t in data]
+        for t, lo, hi in ((x[0], 40, 240), (x[1], 30, 531), (x[2], 30, 531), (x[3], 40, 240)):
+            t[:lo] = fill
+            t[hi:] = fill
+        leaves = [t.requires_grad_() for t in x[:3]]
+        out = A.varlen(*leaves, cq, ck, 130, 301)
+        grads = torch.autograd.grad(out, leaves, x[3])
+        res.append([out.detach()[40:240], *grads])
+    torch.cuda.synchronize()
+    A.check()
+    for a, b in zip(*res):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
