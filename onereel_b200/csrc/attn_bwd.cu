@@ -43,7 +43,9 @@
 // 3 x 2048 rows: 273 us; a tile costs the compute warps as much as at D = 128 (exponentials, TMEM loads and barriers of
 // some 1200 clocks per 64 keys), in which its MMAs take 450.
 //
-// Every mbarrier wait is bounded as in the forward: a stuck pipeline sets the error word and winds down.
+// Every mbarrier wait is bounded as in the forward: a stuck pipeline sets the error word and winds down. The compute warps'
+// waits have one verdict per warp, and their last barrier one for all eight, so that no warp waits there for another that has
+// given up (0.7 % of the time at D = 128, 2 % at D = 64).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -499,11 +501,20 @@ __device__ __forceinline__ void bwd_mma_dq_acc(const BwdShared& sh, uint32_t tme
 }
 
 // ---------------------------------------------------------------------------------------------- P and dS
-// after an mbarrier wait of a whole warp: its lanes leave the wait's loop one by one, and the TMEM accesses that follow
-// need them together
-__device__ __forceinline__ void tc_after_wait() {
+// whether ok holds for all eight compute warps (each with one verdict of its own, see mbar_wait_warp): all 256
+// threads get here
+__device__ __forceinline__ bool all_compute_warps(bool ok) {
+  uint32_t all;
   __syncwarp();
-  tc_fence_after();
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(ok ? 1u : 0u)
+      : "memory");
+  return all != 0;
 }
 
 // two consecutive fp32 values of a fragment (one row, two columns) as a pair for the f32x2 instructions, which halve the
@@ -550,12 +561,16 @@ __device__ __forceinline__ void bwd_stage(const BwdShared& sh, uint32_t acc, con
   }
 }
 
-// the n staged tensors' rows to dst[0..n): 256 threads, one row copy each while there are rows
+// the n staged tensors' rows to dst[0..n): 256 threads, one row copy each while there are rows; nothing unless all of them
+// got here with ok
 template <int D>
 __device__ __forceinline__ void bwd_flush(const BwdShared& sh, const BwdWork& wi, int n, __nv_bfloat16* dst0,
-                                          __nv_bfloat16* dst1, int heads) {
+                                          __nv_bfloat16* dst1, int heads, bool ok, int* err) {
   fence_async_smem();
-  asm volatile("bar.sync 1, 256;" ::: "memory");
+  if (!all_compute_warps(ok)) {
+    atomicOr(err, kErrTimeoutSoftmax);
+    return;
+  }
   const int t = threadIdx.x - 128, i = t >> 7, r = t & 127;
   if (i < n && r < wi.rows) {
     __nv_bfloat16* dst = i == 0 ? dst0 : dst1;
@@ -590,16 +605,16 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
   bool ok = true;
   uint32_t p[64];                               // scores, then P in fp32
   for (int j = 0; j < wi.n_tiles; ++j, a.next()) {
-    ok = mbar_wait(sh.bar(C::kBarAux + a.s), a.ph, sh.abort_flag);
+    ok = mbar_wait_warp(sh.bar(C::kBarAux + a.s), a.ph, sh.abort_flag);
     if (!ok) break;
     // statistics of columns 8r + 2 cq + {0, 1}, two r per load, read before the wait for S (dP)
     const float4* st = reinterpret_cast<const float4*>(sh.smem + C::kStatOff + (j & 1) * C::kStatBytes) + 9 * th.cq;
     float4 c[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = st[i];
-    ok = mbar_wait(sh.bar(C::kBarS), j & 1, sh.abort_flag);
+    ok = mbar_wait_warp(sh.bar(C::kBarS), j & 1, sh.abort_flag);
     if (!ok) break;
-    tc_after_wait();
+    tc_fence_after();
     tmem_ld_16x256b_x8(s_addr, p);
     tmem_ld_16x256b_x8(s_addr + 64, p + 32);
     tmem_wait_ld();
@@ -625,9 +640,9 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
       tc_fence_before();
       mbar_arrive(sh.bar(C::kBarP + h));
     }
-    ok = mbar_wait(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
+    ok = mbar_wait_warp(sh.bar(C::kBarDp), j & 1, sh.abort_flag);
     if (!ok) break;
-    tc_after_wait();
+    tc_fence_after();
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = st[36 + i];
 #pragma unroll
@@ -652,16 +667,14 @@ __device__ __forceinline__ void bwd_compute_dkv(const BwdShared& sh, uint32_t tm
     tc_fence_before();
     mbar_arrive(sh.bar(C::kBarDs));
   }
-  if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
-  if (!ok) {
-    atomicOr(err, kErrTimeoutSoftmax);
-    return;
-  }
-  tc_after_wait();
+  if (ok) ok = mbar_wait_warp(sh.bar(C::kBarDone), 0, sh.abort_flag);
   static_assert(2 * BwdOut<D>::kBytes <= C::kStatOff, "staging");
-  bwd_stage<D>(sh, tmem + C::kColDv, th, 1.f, 0);
-  bwd_stage<D>(sh, tmem + C::kColDk, th, scale, 1);
-  bwd_flush<D>(sh, wi, 2, dv, dk, heads);
+  if (ok) {
+    tc_fence_after();
+    bwd_stage<D>(sh, tmem + C::kColDv, th, 1.f, 0);
+    bwd_stage<D>(sh, tmem + C::kColDk, th, scale, 1);
+  }
+  bwd_flush<D>(sh, wi, 2, dv, dk, heads, ok, err);
 }
 
 __device__ __forceinline__ float quad_add(float x) {
@@ -725,9 +738,9 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
   for (int u = grp; u < wi.n_tiles; u += 2) {
     const int valid = walk.next(skip);
     walk.next(skip);
-    ok = mbar_wait(sh.bar(C::kBarS + grp), (u >> 1) & 1, sh.abort_flag);
+    ok = mbar_wait_warp(sh.bar(C::kBarS + grp), (u >> 1) & 1, sh.abort_flag);
     if (!ok) break;
-    tc_after_wait();
+    tc_fence_after();
     uint32_t p[2][32], d[2][32];
 #pragma unroll
     for (int h = 0; h < 2; ++h) tmem_ld_16x256b_x8(s_addr + h * kBlock, p[h]);
@@ -806,11 +819,11 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
     }
     if (u >= 2) {
       // dS goes over that of tile u - 2: its dQ is done when its stage is free
-      ok = mbar_wait(sh.bar(C::kBarE0 + before.s), before.ph, sh.abort_flag);
+      ok = mbar_wait_warp(sh.bar(C::kBarE0 + before.s), before.ph, sh.abort_flag);
       if (!ok) break;
       before.next();
       before.next();
-      tc_after_wait();
+      tc_fence_after();
     }
     tmem_st_16x128b_x8(ds_addr, w[0]);
     tmem_st_16x128b_x8(ds_addr + kBlock, w[1]);
@@ -827,7 +840,7 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
       if (grp == 1 && th.cq == 0) meet[row + 8 * i] = pdp[i];
     }
   }
-  asm volatile("bar.sync 1, 256;" ::: "memory");
+  asm volatile("bar.sync 1, 256;" ::: "memory");         // by every compute warp, whatever its verdict
   if (ok && grp == 0 && th.cq == 0) {
     const float* meet = reinterpret_cast<const float*>(sh.smem + C::kStatOff);
 #pragma unroll
@@ -842,14 +855,12 @@ __device__ __forceinline__ void bwd_compute_dq(const BwdShared& sh, uint32_t tme
                    : "memory");
     }
   }
-  if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
-  if (!ok) {
-    atomicOr(err, kErrTimeoutSoftmax);
-    return;
+  if (ok) ok = mbar_wait_warp(sh.bar(C::kBarDone), 0, sh.abort_flag);
+  if (ok) {
+    tc_fence_after();
+    bwd_stage<D>(sh, tmem + C::kColDq, th, scale, 0);
   }
-  tc_after_wait();
-  bwd_stage<D>(sh, tmem + C::kColDq, th, scale, 0);
-  bwd_flush<D>(sh, wi, 1, dq, dq, heads);
+  bwd_flush<D>(sh, wi, 1, dq, dq, heads, ok, err);
 }
 
 template <int D>

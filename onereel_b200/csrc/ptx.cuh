@@ -82,6 +82,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
 }
 
+// The same by all lanes of a warp, with one verdict for all: lanes leave the wait one by one, and near the limit some could see
+// the phase complete and others the limit passed. What follows (TMEM accesses, shuffles, named barriers) is warp-wide.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
 // ------------------------------------------------------------------------------------------------ TMA
 
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {

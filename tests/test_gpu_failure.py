@@ -53,3 +53,38 @@ def test_peer_barrier_times_out_when_a_peer_never_arrives():
     torch.cuda.synchronize()
     assert err.item() == 0
     assert _lib.lib().orl_peer_barrier(ptrs, 2, 2, 3, 20_000_000, err.data_ptr(), s) == -1   # rank outside world
+
+
+def test_attention_backward_winds_down_when_its_wait_runs_out():
+    """a work list without query items: the key items' bounded wait for the rows' delta runs out, every role of the kernel ends
+    and reports it, nothing is stored, and the same call with the whole list runs"""
+    if not torch.cuda.is_available():
+        pytest.skip('needs a B200')
+    from onereel_b200.csrc.build import build
+    build()
+    from onereel_b200 import _lib as L, attention as A
+    for D in (64, 128):
+        H, n = 2, 300
+        g = torch.Generator().manual_seed(D)
+        q, k, v, dout = (torch.randn(n, H, D, generator=g).cuda().bfloat16() for _ in range(4))
+        seg = ([0], [n], [0], [n])
+        out, lse = A.attend(q, k, v, *seg, lse=True)
+        want = A.attend_grad(q, k, v, out, lse, dout, *seg)
+        work, ranges, items = A._plan_bwd(*seg, H, n, n, q.device)
+        table = work.cpu().numpy().view(L.BWD_WORK_DTYPE)
+        keys = torch.from_numpy(table[table['kind'] == 0].copy().view('uint8')).cuda()
+        grads, args, stats, _, keep = A._bwd_args(q, k, v, out, lse, dout, None)
+        for t in grads:
+            t.fill_(7.0)
+        rc = L.lib().orl_attn_bwd(*args, D ** -0.5, keys.data_ptr(), keys.numel() // 32, ranges.data_ptr(), stats,
+                                  A._err_word(q.device).data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and 0 < keys.numel() // 32 < items
+        torch.cuda.synchronize()
+        with pytest.raises(L.OrlError):
+            A.check()
+        assert all((t == 7.0).all() for t in grads)
+        again = A.attend_grad(q, k, v, out, lse, dout, *seg)
+        torch.cuda.synchronize()
+        A.check()
+        assert all(torch.equal(a, b) for a, b in zip(again, want))
+        del keep
