@@ -13,7 +13,7 @@
 // and y (and z) go out by TMA, whole 128-byte lines at a time (stored from the registers, a row per lane, the epilogue of
 // 9540 x 2048 -> 8192 with z took longer than the product: 319 us instead of 222). kCtas = 1 serves problems too small
 // for that, down to a few rows. Rows and columns past the ends are zeros (TMA fill) and are not stored.
-// Every mbarrier wait is bounded (ptx.cuh).
+// Every mbarrier wait is bounded (ptx.cuh); the epilogue warps' have one verdict per warp.
 //
 // Measured (device time): 22260 x 8192 -> 2048 with bias, gate and residual 520 us, 1.43 PFLOP/s, 0.88 of a library
 // product's burst rate; 9540 x 2048 -> 8192 with gelu 238 us keeping z, dx 234, dw 219, dz and db 99 + 4. Few rows: 1 x 2048
@@ -410,8 +410,7 @@ __global__ void __launch_bounds__(GemmCfg<kCtas, BN>::kThreads, 1)
         const int half = ew >> 2;                // this warp's pieces: half, half + 2, ...
         const int n_pieces = row0 < g.m ? (min(BN, g.n - n0) + 63) / 64 : 0;
         if (half < n_pieces) prepare(piece, 64 * half);
-        ok = mbar_wait(sh.bar(C::kBarAccFull + buf), (n >> 1) & 1, sh.abort_flag);
-        __syncwarp();                            // lanes leave the wait one by one; the TMEM loads are warp-wide
+        ok = mbar_wait_warp(sh.bar(C::kBarAccFull + buf), (n >> 1) & 1, sh.abort_flag);
         if (ok) tc_fence_after();
 #pragma unroll 1
         for (int i = half; ok && i < n_pieces; i += 2, ++piece) {
@@ -421,7 +420,7 @@ __global__ void __launch_bounds__(GemmCfg<kCtas, BN>::kThreads, 1)
           tmem_ld32(acc + 64 * i + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
           tmem_wait_ld();
           if (res) {
-            ok = mbar_wait(sh.bar(C::kBarRes + 2 * ew + b), (two ? piece >> 1 : piece) & 1, sh.abort_flag);
+            ok = mbar_wait_warp(sh.bar(C::kBarRes + 2 * ew + b), (two ? piece >> 1 : piece) & 1, sh.abort_flag);
             if (!ok) break;
           }
           uint8_t* y = staging + b * C::kPiece + lane * 128;
@@ -448,11 +447,8 @@ __global__ void __launch_bounds__(GemmCfg<kCtas, BN>::kThreads, 1)
           }
           if (i + 2 < n_pieces) prepare(piece + 1, 64 * (i + 2));
         }
-        // the loop's waits may have been left by some lanes before others
-        __syncwarp();
       } else {
-        ok = mbar_wait(sh.bar(C::kBarAccFull + buf), (n >> 1) & 1, sh.abort_flag);
-        __syncwarp();
+        ok = mbar_wait_warp(sh.bar(C::kBarAccFull + buf), (n >> 1) & 1, sh.abort_flag);
         if (ok) tc_fence_after();
         const long long row = row0 + lane;
 #pragma unroll 1
