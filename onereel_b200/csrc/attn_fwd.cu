@@ -367,7 +367,7 @@ __device__ __forceinline__ void softmax_role(const AttnShared& sh, uint32_t tmem
   uint32_t pb[16];
   for (int j = 0; ok && j < n_kv; ++j) {
     const int valid = wi.k_len - 128 * j;
-    ok = mbar_wait(sh.bar(C::kBarS + 0), j & 1, sh.abort_flag);
+    ok = mbar_wait_warp(sh.bar(C::kBarS + 0), j & 1, sh.abort_flag);
     if (!ok) break;
     tc_fence_after();
     load_s(0, s);
@@ -375,7 +375,7 @@ __device__ __forceinline__ void softmax_role(const AttnShared& sh, uint32_t tmem
     const TileState st0 = tile_front(j, 0, valid, s, pb);
     tile_back(0, st0);
     if (n_qt == 2) {
-      ok = mbar_wait(sh.bar(C::kBarS + 1), j & 1, sh.abort_flag);
+      ok = mbar_wait_warp(sh.bar(C::kBarS + 1), j & 1, sh.abort_flag);
       if (!ok) break;
       tc_fence_after();
       load_s(1, s2);
@@ -384,7 +384,7 @@ __device__ __forceinline__ void softmax_role(const AttnShared& sh, uint32_t tmem
       tile_back(1, st1);
     }
   }
-  if (ok) ok = mbar_wait(sh.bar(C::kBarDone), 0, sh.abort_flag);
+  if (ok) ok = mbar_wait_warp(sh.bar(C::kBarDone), 0, sh.abort_flag);
   if (ok) {
     tc_fence_after();
     for (int t = 0; t < n_qt; ++t) {
