@@ -144,8 +144,9 @@ def check(device=None) -> None:
             raise L.OrlError(f'kernel on cuda:{key} reported: {L.describe_error_bits(bits)}')
 
 
-def plan(q_start, q_len, k_start, k_len, heads: int, device) -> tuple[torch.Tensor, int]:
-    """device work list for segments given as (start, length) rows and its item count (cached)"""
+def plan(q_start, q_len, k_start, k_len, heads: int, device) -> tuple[torch.Tensor, int, int, int]:
+    """for segments given as (start, length) rows: device work list, its item count, and the rows of q and of k / v that the
+    tensors must have for it (cached)"""
     key = (tuple(q_start), tuple(q_len), tuple(k_start), tuple(k_len), heads, str(device))
     return _PLANS.get(key, device, lambda: _make_plan(*key[:4], heads, device))
 
@@ -162,7 +163,8 @@ def _make_plan(q_start, q_len, k_start, k_len, heads, device):
     work = np.zeros(max(need_n, 1), dtype=L.WORK_DTYPE)
     n = L.check(L.lib().orl_attn_plan_ranges(*(L.i32p(a) for a in arrs), n_seg, heads, work.ctypes.data, len(work)),
                 'orl_attn_plan_ranges')
-    return upload(work.view(np.uint8), device), n
+    ends = lambda start, length: max((a + b for a, b, c in zip(start, length, q_len) if b > 0 and c > 0), default=0)
+    return upload(work.view(np.uint8), device), n, ends(q_start, q_len), ends(k_start, k_len)
 
 
 def _host_list(x) -> list[int]:
@@ -243,7 +245,9 @@ def attend(q, k, v, q_start, q_len, k_start, k_len, out=None, lse=None, scale=No
     _check_inputs(q, k, v)
     Nq, H, Dh = q.shape
     dev = q.device
-    work, n = plan(q_start, q_len, k_start, k_len, H, dev)
+    work, n, need_q, need_k = plan(q_start, q_len, k_start, k_len, H, dev)
+    if need_q > Nq or need_k > k.shape[0]:
+        raise ValueError(f'segments reach to row {need_q} of q and {need_k} of k / v, which have {Nq} and {k.shape[0]}')
     if (split_keys and stream is None and n and n < SPLIT_WAVES * _sm_count(dev) and
             max(k_len) >= SPLIT_MIN_KEYS):
         if lse is True:

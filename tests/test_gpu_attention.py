@@ -344,3 +344,19 @@ def test_gradients_with_bad_rows_behind_the_segments(D):
     A.check()
     for a, b in zip(*res):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_segments_outside_the_tensors_are_refused():
+    """host-planned calls whose query or key rows reach past the tensors: an error instead of reads and stores out of range"""
+    from onereel_b200 import attention as A
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(n, 2, 64, generator=g).cuda().bfloat16() for n in (40, 60, 60))
+    for call in (lambda: A.varlen(q, k, v, [0, 41], [0, 60], 41, 60), lambda: A.varlen(q, k, v, [0, 40], [0, 61], 40, 61),
+                 lambda: A.varlen_lse(q, k, v, [20, 41], [0, 60], 21, 60), lambda: A.attend(q, k, v, [39], [2], [0], [1]),
+                 lambda: A.overlapping_ranges(q, k, v, [(0, 40)], [(1, 61)]),
+                 lambda: A.varlen(q.clone().requires_grad_(), k, v, [0, 40], [0, 61], 40, 61)):
+        with pytest.raises(ValueError, match='segments reach'):
+            call()
+    A.varlen(q, k, v, [0, 40], [0, 60], 40, 60)
+    torch.cuda.synchronize()
+    A.check()

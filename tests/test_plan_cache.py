@@ -84,3 +84,11 @@ def test_tables_are_refused_during_a_capture(monkeypatch):
         with pytest.raises(RuntimeError, match='once before capturing'):
             call()
     assert not A._PLANS.entries and not A._BWD_PLANS.entries
+
+
+def test_work_lists_know_the_rows_they_need():
+    """the ends of the segments that have queries, and of their keys; empty ones need nothing"""
+    from onereel_b200 import attention as A
+    for segs, need in ((([0, 9], [5, 3], [4, 0], [6, 30]), (12, 30)), (([7], [2], [50], [0]), (9, 0)),
+                       (([0, 90], [5, 0], [0, 70], [8, 9]), (5, 8)), (([], [], [], []), (0, 0))):
+        assert A.plan(*segs, 2, 'cpu')[2:] == need
