@@ -256,8 +256,8 @@ ORL_API int orl_peer_gather(const void* const* src, void* const* dst, int planes
 /* ---------------------------------------------------------------- linear layers with their epilogue
  * The projections and feed-forward layers around the attention, which the reference runs as separate torch ops:
  * y = residual + gate * act(x w^T + bias), x [m, k] (row stride ldx), w [n, k] (row stride ldw), bias / gate [n],
- * residual [m, n] (row stride ldr), y [m, n], all bf16, accumulated and finished in fp32. n, k and the row strides are
- * multiples of 8 elements, pointers 16-byte aligned; bias, gate, residual may be NULL. */
+ * residual [m, n] (row stride ldr), y [m, n], all bf16, accumulated and finished in fp32. n, k (at most 2^28) and the
+ * row strides are multiples of 8 elements, pointers 16-byte aligned; bias, gate, residual may be NULL. */
 
 #define ORL_ACT_NONE 0
 #define ORL_ACT_GELU_TANH 1 /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
@@ -272,8 +272,9 @@ ORL_API int orl_linear(const void* x, long long ldx, const void* w, long long ld
 /* Gradients of orl_linear from the gradient dy [m, n] (row stride lddy) of y, the forward's inputs (x for dw, w for dx,
  * the gate for dx, dw and dbias; NULL where not needed) and its z (may be NULL without activation and dgate):
  * dz = gate * dy * act'(z), dx = dz w [m, k], dw = dz^T x [n, k], dbias = column sums of dz, dgate = column sums of
- * dy * act(z) (bf16; NULL: not computed). The residual's gradient is dy itself. Deterministic. dz: scratch [m, n] bf16, needed for dx or dw when z or a gate is given; scratch: device fp32,
- * orl_linear_bwd_scratch elements, needed for dbias, dgate or, with at most four rows, dx. */
+ * dy * act(z) (bf16; NULL: not computed). The residual's gradient is dy itself. Deterministic.
+ * dz: scratch [m, n] bf16, needed for dx or dw when z or a gate is given; scratch: device fp32, orl_linear_bwd_scratch
+ * elements, needed for dbias, dgate or, with at most four rows, dx. */
 ORL_API int orl_linear_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w, long long ldw,
                            const void* z, const void* gate, int act, void* dz, void* dx, void* dw, void* dbias,
                            void* dgate, float* scratch, long long m, long long n, long long k, int* err_dev,

@@ -817,7 +817,8 @@ static int gemm(const void* a, long long lda, const void* b, long long ldb, int 
 static bool lin_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static int check_linear(long long m, long long n, long long k) {
-  if (m < 0 || n <= 0 || k <= 0 || m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return ORL_ERR_ARG;
+  // rows and columns are counted in 32 bits, a step of a strip's rows past the end and kRowsMax rows' columns included
+  if (m < 0 || n <= 0 || k <= 0 || m > 0x7fff0000LL || n > (1LL << 28) || k > (1LL << 28)) return ORL_ERR_ARG;
   if ((n & 7) || (k & 7)) return ORL_ERR_ALIGN;
   return ORL_OK;
 }

@@ -117,3 +117,15 @@ def test_linear_gradients_without_the_product(h):
     call = lambda **at: h.orl_linear_bwd(*with_(ok, **at))
     assert call(a13=P) == -1 and call(a8=1) == -1 and call(a9=None) == -1    # dgate, an activation, no room for dz
     assert call(a10=P + 8) == -2                                             # past those checks: dx misaligned
+
+
+def test_linear_refuses_sizes_past_its_counters(h):
+    """4 rows of 2^30 columns and rows up to the last strip's step would wrap 32-bit counters"""
+    fwd = [P, 64, P, 64, P, P, P, 32, P, None, 5, 32, 64, 0, P, None]
+    bwd = [P, 32, P, 64, P, 64, P, P, 1, P, P, P, P, P, P, 5, 32, 64, P, None]
+    big = 2 ** 28 + 8
+    assert h.orl_linear(*with_(fwd, a12=big, a1=big, a3=big)) == -1 and h.orl_linear(*with_(fwd, a11=big, a7=big)) == -1
+    assert h.orl_linear(*with_(fwd, a10=0x7fff0001)) == -1
+    assert h.orl_linear_bwd(*with_(bwd, a15=4, a17=big, a3=big, a5=big)) == -1
+    assert h.orl_linear_bwd_scratch(4, 64, big) == -1 and h.orl_linear_bwd_scratch(0x7fff0001, 64, 64) == -1
+    assert h.orl_linear_bwd_scratch(4, 64, 2 ** 28) == 4 * 2 ** 28      # one strip
