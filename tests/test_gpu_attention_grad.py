@@ -372,3 +372,58 @@ def test_first_use_of_a_layout_in_a_capture_is_refused():
     torch.cuda.synchronize()
     A.check()
     assert want.shape == q.shape
+
+
+@pytest.mark.parametrize('H,D', [(40, 128), (24, 64), (7, 128)])
+def test_many_heads(H, D):
+    from onereel_b200 import attention as A
+    lq, lk = [33, 200], [150, 65]
+    q, k, v, dout, dlse = inputs(sum(lq), sum(lk), H, D, seed=H)
+    segs = (starts(lq), lq, starts(lk), lk)
+    out, lse = A.attend(q, k, v, *segs, lse=True)
+    dq, dk, dv = A.attend_grad(q, k, v, out, lse, dout, *segs, dlse=dlse)
+    check_all(dict(out=out, lse=lse, dq=dq, dk=dk, dv=dv), attention_grads(q, k, v, dout, *segs, dlse=dlse))
+
+
+@pytest.mark.parametrize('n', [1000, 4096])
+def test_many_segments_on_the_device_plan(n):
+    """thousands of short segments, empty ones among them: the device-planned passes give the host-planned bits, which match
+    float64; one segment more than the device plan takes is refused by both passes"""
+    from onereel_b200 import _lib as L, attention as A
+    H, D = 2, 64
+    g = torch.Generator().manual_seed(n)
+    lq = torch.randint(0, 6, (n,), generator=g).tolist()
+    lk = (2 + torch.randint(0, 9, (n,), generator=g)).tolist()
+    lq[3], lk[5], lk[7], lq[n // 2], lk[n // 2] = 0, 0, 300, 260, 200
+    q, k, v, dout, _ = inputs(sum(lq), sum(lk), H, D, seed=n)
+    segs = (starts(lq), lq, starts(lk), lk)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    cq, ck = A.cu_seqlens(lq), A.cu_seqlens(lk)
+    out, lse = A.varlen_lse(*leaves, cq, ck, max(lq), max(lk))
+    got = torch.autograd.grad(out, leaves, dout)
+    plain = [x.detach() for x in leaves]
+    want_o, want_l = A.attend(*plain, *segs, lse=True)
+    host = A.attend_grad(*plain, want_o, want_l, dout, *segs)
+    assert torch.equal(out, want_o) and torch.equal(lse, want_l) and all(torch.equal(a, b) for a, b in zip(got, host))
+    want = attention_grads(*plain, dout, *segs)
+    torch.cuda.synchronize()
+    A.check()
+    for name, t in dict(out=out.detach(), dq=got[0], dk=got[1], dv=got[2]).items():
+        assert ((t.double() - want[name][0]).abs() <= want[name][1]).all(), name
+    if n == 4096:
+        more = torch.zeros(n + 2, dtype=torch.int32, device='cuda')
+        for call in (lambda: A.varlen(q, k, v, more, more, 1, 1),
+                     lambda: A._attend_cu_grad(*plain, want_o, want_l, dout, None, more, more)):
+            with pytest.raises(L.OrlError):
+                call()
+
+
+def test_long_segment():
+    """thousands of rows on both sides: tens of tiles per item in either kind, rows past the last whole tile"""
+    from onereel_b200 import attention as A
+    H, D, lq, lk = 1, 128, [4001, 900], [7003, 12001]
+    q, k, v, dout, dlse = inputs(sum(lq), sum(lk), H, D, seed=90)
+    segs = (starts(lq), lq, starts(lk), lk)
+    out, lse = A.attend(q, k, v, *segs, lse=True)
+    dq, dk, dv = A.attend_grad(q, k, v, out, lse, dout, *segs, dlse=dlse)
+    check_all(dict(out=out, lse=lse, dq=dq, dk=dk, dv=dv), attention_grads(q, k, v, dout, *segs, dlse=dlse))

@@ -291,3 +291,72 @@ def test_frozen_inputs_keep_only_what_the_others_gradients_need(m, act, with_gat
             want = [(m, k)] * ('weight' in names) + [(n, k)] * ('x' in names) + [(n,)] * (with_gate and slope)
             want += [(m, n)] * ('gate' in names or (act is not None and slope))
             assert kept == sorted(want), names
+
+
+@pytest.mark.parametrize('act,residual,gate', [(None, False, False), ('silu', True, True), ('gelu_tanh', True, False)])
+@pytest.mark.parametrize('m,n,k', [(1801, 1504, 1000), (1000, 2056, 1024)])
+def test_middle_tiles(m, n, k, act, residual, gate):
+    """sizes between the one-CTA tiles and 256 x 256: the pair's 256 x 128 tile, in every direction's operand layout at the
+    first size (y: 96 tiles, dx: 64, dw: 48) and with ragged ends"""
+    from onereel_b200 import attention as A
+    from onereel_b200.linear import linear
+    t = make(m, n, k, residual=residual, gate=gate, seed=m)
+    for x in t.values():
+        x.requires_grad_()
+    dy = rand(m, n, seed=8)
+    y = linear(t['x'], t['weight'], t['bias'], act, t.get('residual'), t.get('gate'))
+    grads = dict(zip(t, torch.autograd.grad(y, list(t.values()), dy)))
+    torch.cuda.synchronize()
+    A.check()
+    want = reference(t, act, dy)
+    assert_close(y, want['y'], 'y')
+    for name in t:
+        assert_close(grads[name], want[name], name)
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+@pytest.mark.parametrize('m,n,k', [(3, 72, 136), (77, 200, 1000), (1801, 1504, 1000), (2100, 2056, 520)])
+def test_values_that_are_not_finite_stay_where_they_belong(m, n, k, bad):
+    """a bad element of x or dy reaches its row of y and dx, one of the weight its column, one of the residual itself; what lies
+    around strided operands (here all of it bad) reaches nothing"""
+    from onereel_b200.linear import linear
+    t = make(m, n, k, residual=True, gate=True, seed=m)
+    dy = rand(m, n, seed=9)
+
+    def inside(v):
+        big = torch.full((v.shape[0] + 2, v.shape[1] + 16), bad, dtype=v.dtype, device='cuda')
+        big[1:-1, 8:-8] = v
+        return big[1:-1, 8:-8]
+
+    def grads(d, g):
+        leaves = {a: x.detach().requires_grad_() for a, x in d.items()}
+        y = linear(**leaves, activation='silu')
+        return (y.detach(), *torch.autograd.grad(y, [leaves['x'], leaves['weight'], leaves['bias']], g))
+    clean = grads(t, dy)
+    assert all(torch.isfinite(x).all() for x in clean)
+    wrapped = {a: inside(v) if v.dim() == 2 else v for a, v in t.items()}
+    assert all(torch.equal(a, b) for a, b in zip(grads(wrapped, inside(dy)), clean))
+    row, col = m // 2, n // 3
+
+    def put(name, at):
+        v = t[name].clone()
+        v[at] = bad
+        return {**t, name: v}
+    y, dx, *_ = grads(put('x', (row, 5)), dy)
+    keep = torch.arange(m, device='cuda') != row
+    assert torch.equal(y[keep], clean[0][keep]) and torch.equal(dx[keep], clean[1][keep])
+    assert not torch.isfinite(y[row]).all()
+    y = grads(put('weight', (col, 5)), dy)[0]
+    cols = torch.arange(n, device='cuda') != col
+    assert torch.equal(y[:, cols], clean[0][:, cols]) and not torch.isfinite(y[:, col]).all()
+    y, dx, dw, db = grads(put('residual', (row, col)), dy)
+    want = clean[0].clone()
+    want[row, col] = bad
+    assert torch.equal(y.nan_to_num(nan=123.0), want.nan_to_num(nan=123.0))
+    assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), clean[1:]))
+    g = dy.clone()
+    g[row, col] = bad
+    y, dx, dw, db = grads(t, g)
+    rows = torch.arange(n, device='cuda') != col
+    assert torch.equal(y, clean[0]) and torch.equal(dx[keep], clean[1][keep]) and not torch.isfinite(dx[row]).any()
+    assert torch.equal(dw[rows], clean[2][rows]) and torch.equal(db[rows], clean[3][rows]) and not torch.isfinite(db[col])
