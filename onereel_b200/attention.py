@@ -185,6 +185,8 @@ def _check_inputs(q, k, v):
         if x.dim() != 3 or x.stride(-1) != 1 or x.stride(1) != x.shape[2] or x.stride(0) != x.shape[1] * x.shape[2]:
             raise ValueError(f'{name} must be a contiguous [rows, heads, head_dim] tensor, got {tuple(x.shape)} '
                              f'strides {x.stride()}')
+        if x.device != q.device:
+            raise ValueError(f'{name} is on {x.device}, q on {q.device}')
     if q.shape[1:] != k.shape[1:] or k.shape != v.shape:
         raise ValueError(f'shape mismatch q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}')
     if q.shape[2] not in (64, 128):
