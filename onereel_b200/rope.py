@@ -19,6 +19,8 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
     Differentiable in x and weight (first derivatives; the tables get none); with out or row_map a backward pass through
     the returned tensor raises."""
     if x.dim() == 3:
+        if x.shape[0] != 1:
+            raise ValueError(f'qk_norm_rope: x must be [rows, heads * D] or [1, rows, heads * D], got {tuple(x.shape)}')
         x = x[0]
     if not (x.is_cuda and x.dtype == torch.bfloat16):
         raise TypeError('qk_norm_rope: x must be a bf16 CUDA tensor (no fallback)')
@@ -26,10 +28,29 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
     rows = x.shape[0]
     w = weight.to(device=x.device, dtype=torch.bfloat16).contiguous()
     c, s = _table(cos, rows, x.device), _table(sin, rows, x.device)
+    _check_shapes(x, w, c, s, heads, per_head)
+    if out is not None and not (out.dtype == x.dtype and out.device == x.device and out.is_contiguous() and
+                                (row_map is not None or out.numel() >= x.numel())):
+        raise ValueError(f'qk_norm_rope: out must be contiguous, with {tuple(x.shape)} bf16 elements on {x.device}')
+    if row_map is not None and row_map.numel() != rows:
+        raise ValueError(f'qk_norm_rope: row_map must have {rows} entries, got {row_map.numel()}')
     if _wants_grad(x, w) and out is None and row_map is None:
         return _QkNormRope.apply(x, w, c, s, heads, float(eps), int(per_head), int(sin_shift))
     y = _forward(x, w, c, s, heads, eps, per_head, sin_shift, out, row_map)
     return without_gradient('qk_norm_rope with out or row_map', y, x, w)
+
+
+def _check_shapes(x, w, c, s, heads: int, per_head):
+    """that the kernels, which get addresses and the sizes of x, stay inside the weight and the tables"""
+    hidden = x.shape[-1]
+    if x.dim() != 2 or heads <= 0 or hidden % heads:
+        raise ValueError(f'qk_norm_rope: x must have rows of {heads} equal heads, got {tuple(x.shape)}')
+    dh = hidden // heads
+    if w.numel() != (dh if per_head else hidden):
+        raise ValueError(f'qk_norm_rope: weight must have {dh if per_head else hidden} elements, got {tuple(w.shape)}')
+    if c.shape != s.shape or c.dim() != 2 or c.shape[0] != x.shape[0] or c.shape[1] < dh:
+        raise ValueError(f'qk_norm_rope: cos and sin must be tables [{x.shape[0]}, {dh}], got {tuple(c.shape)} and '
+                         f'{tuple(s.shape)}')
 
 
 def _table(t, rows: int, device):
@@ -71,6 +92,11 @@ class _QkNormRope(torch.autograd.Function):
 def qk_norm_rope_grad(x, weight, cos, sin, dy, heads: int, eps: float, per_head: bool, sin_shift: int):
     """(dx, dweight) of qk_norm_rope (orl_qk_norm_rope_bwd): x [rows, heads * D] and weight bf16, cos / sin fp32
     [rows, D], all contiguous as the forward used them; dy [rows, heads, D] bf16"""
+    for name, t, dtype in (('x', x, torch.bfloat16), ('weight', weight, torch.bfloat16), ('cos', cos, torch.float32),
+                           ('sin', sin, torch.float32)):
+        if t.dtype != dtype or not t.is_cuda or t.device != x.device or not t.is_contiguous():
+            raise TypeError(f'qk_norm_rope: {name} must be a contiguous {dtype} tensor on {x.device}')
+    _check_shapes(x, weight, cos, sin, heads, per_head)
     rows, hidden = x.shape
     if dy.dtype != torch.bfloat16 or dy.device != x.device:
         raise TypeError(f'qk_norm_rope: dy must be bf16 on {x.device}')
