@@ -87,10 +87,11 @@ class RowSum:
 
     def run(self, parts):
         """parts: packed gradients [n, H, D] bf16, contiguous -> one [n_rows, H, D] each"""
-        dev = parts[0].device
+        dev = self.offsets.device
         for p in parts:
-            if p.shape[0] < self.n_packed or not p.is_contiguous() or p.dtype != torch.bfloat16:
-                raise ValueError('packed gradients must be contiguous bf16 with a row per packed row')
+            if (p.shape[0] < self.n_packed or not p.is_contiguous() or p.dtype != torch.bfloat16 or p.device != dev or
+                    p.shape[1:] != parts[0].shape[1:]):
+                raise ValueError('packed gradients must be contiguous bf16, alike, with a row per packed row')
         out = [p.new_empty(self.n_rows, *p.shape[1:]) for p in parts]
         if self.n_rows:
             arr = L.c_vp * len(parts)

@@ -218,6 +218,11 @@ class ScenePlan:
         return kp, vp
 
 
+    def rows_needed(self, source: int) -> int:
+        """rows of a source that the plan reads, as keys or queries"""
+        ends = [hi for s in self.segs for src, lo, hi in (*s.kv, s.q) if src == source and hi > lo]
+        return max(ends, default=0)
+
     def row_sums(self, source: int, n_rows: int) -> RowSum:
         """the gradient of the pack for the n_rows rows of one source: which packed rows are their copies"""
         key = (source, n_rows)
@@ -325,7 +330,22 @@ def _packed_kv(plan, rotate, k, v, ek, ev):
 def attend_plan(plan: ScenePlan, q, k, v, eq=None, ek=None, ev=None, rotate=None):
     """(video outputs, text outputs or None) of a plan whose keys are all local: pack_kv and attend_segments with the same
     values, differentiable in q, k, v and the text rows eq, ek, ev. rotate(packed keys, back): rotates rows of the packed
-    keys in place, back = True by the opposite angles."""
+    keys in place, back = True by the opposite angles. The tensors are contiguous [rows, heads, head_dim], with the rows that
+    the plan reads."""
+    A._check_inputs(q, k, v)
+    given = [(q, VIDEO), (k, VIDEO)]
+    if any(t is not None for t in (eq, ek, ev)):
+        if any(t is None for t in (eq, ek, ev)):
+            raise ValueError('attend_plan: eq, ek and ev come together')
+        A._check_inputs(eq, ek, ev)
+        A._check_inputs(q, ek, ev)
+        given += [(eq, TEXT), (ek, TEXT)]
+    elif plan.rows_needed(TEXT):
+        raise ValueError('attend_plan: the plan reads text rows, and none are given')
+    for t, source in given:
+        if t.shape[0] < plan.rows_needed(source) or t.shape[1] != plan.heads or 2 * t.shape[1] * t.shape[2] != plan.row_bytes:
+            raise ValueError(f'attend_plan: the plan is of {plan.rows_needed(source)} rows of {plan.row_bytes} bytes in '
+                             f'{plan.heads} heads, the tensor {tuple(t.shape)}')
     if any(src == REMOTE for s in plan.segs for src, _, _ in s.kv):
         raise ValueError('attend_plan: the plan reads keys of other ranks')
     return _PlanAttention.apply(plan, rotate, q, k, v, eq, ek, ev)

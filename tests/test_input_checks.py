@@ -50,3 +50,38 @@ def test_norm_rope_refuses_shapes_that_do_not_fit():
                dict(sin=cuda(6, 64, dtype=f32, index=1))):
         with pytest.raises(TypeError):
             qk_norm_rope_grad(**args(**kw), dy=cuda(6, 2, 64))
+
+
+def test_scene_plan_refuses_tensors_that_do_not_fit():
+    """fewer rows than the plan reads, strided or missing tensors, other heads; parts of a pack's gradient that differ"""
+    from onereel_b200 import scene as S
+    from onereel_b200.layout import SceneLayout
+    from onereel_b200.pack import RowSum
+    lay, T, counts, H = SceneLayout([2, 3], halo=1), 8, [3, 4], 2
+    L, E = lay.n_frames * T, sum(counts)
+    scenes = [(j, (lo * T, hi * T)) for j, (lo, hi) in enumerate(lay.ranges)]
+    plan = S.ScenePlan(S.scene_segments(lay, T, counts, scenes, {0, 1}, (0, L)), H * 128, H, 'cpu')
+    assert plan.rows_needed(S.VIDEO) == L and plan.rows_needed(S.TEXT) == E and plan.rows_needed(S.REMOTE) == 0
+    good = [cuda(n, H, 64) for n in (L, L, L, E, E, E)]
+    for i, t in ((0, cuda(L - 1, H, 64)), (1, cuda(L - 1, H, 64)), (2, cuda(L, 64, H).transpose(1, 2)), (3, cuda(E - 1, H, 64)),
+                 (4, cuda(E, H, 128)), (3, None), (5, None)):
+        with pytest.raises(ValueError):
+            S.attend_plan(plan, *(t if i == j else x for j, x in enumerate(good)))
+    with pytest.raises(ValueError):
+        S.attend_plan(plan, *(cuda(x.shape[0] - 1, H, 64) if i in (1, 2) else x for i, x in enumerate(good)))
+    with pytest.raises(ValueError):
+        S.attend_plan(plan, *good[:3])
+    with pytest.raises(ValueError):
+        S.attend_plan(plan, *(cuda(x.shape[0], 2 * H, 64) for x in good))
+    with pytest.raises(TypeError):
+        S.attend_plan(plan, *(x.float() for x in good))
+
+
+def test_row_sum_refuses_parts_that_differ():
+    from onereel_b200.pack import RowSum
+    with torch._subclasses.fake_tensor.unset_fake_temporarily():
+        s = RowSum([0, 1, 1], [0, 1, 2], 2, 'cpu')
+        part = lambda *shape, dtype=BF16: torch.zeros(*shape, dtype=dtype)
+        for parts in ([part(3, 1, 16), part(3, 1, 8)], [part(3, 1, 8), part(2, 1, 8)], [part(3, 1, 8), part(3, 1, 8, dtype=torch.half)]):
+            with pytest.raises(ValueError, match='alike'):
+                s.run(parts)
