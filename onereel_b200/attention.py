@@ -488,7 +488,11 @@ def _wants_grad(*tensors) -> bool:
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
                                               for t in tensors):
         raise NotImplementedError('the B200 kernels have no forward-mode derivative (reverse mode only)')
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class _NoGradient(torch.autograd.Function):

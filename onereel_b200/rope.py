@@ -37,7 +37,7 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
     if _wants_grad(x, w) and out is None and row_map is None:
         return _QkNormRope.apply(x, w, c, s, heads, float(eps), int(per_head), int(sin_shift))
     y = _forward(x, w, c, s, heads, eps, per_head, sin_shift, out, row_map)
-    return without_gradient('qk_norm_rope with out or row_map', y, x, w)
+    return y if out is None and row_map is None else without_gradient('qk_norm_rope with out or row_map', y, x, w)
 
 
 def _check_shapes(x, w, c, s, heads: int, per_head):
@@ -85,7 +85,7 @@ class _QkNormRope(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy):
         x, w, c, s = ctx.saved_tensors
-        dx, dw = qk_norm_rope_grad(x, w, c, s, dy, *ctx.args)
+        dx, dw = _grad(x, w, c, s, dy, *ctx.args)
         return dx, dw, None, None, None, None, None, None
 
 
@@ -102,6 +102,11 @@ def qk_norm_rope_grad(x, weight, cos, sin, dy, heads: int, eps: float, per_head:
         raise TypeError(f'qk_norm_rope: dy must be bf16 on {x.device}')
     if dy.shape != (rows, heads, hidden // heads):
         raise ValueError(f'qk_norm_rope: dy must have shape {(rows, heads, hidden // heads)}, got {tuple(dy.shape)}')
+    return _grad(x, weight, cos, sin, dy, heads, eps, per_head, sin_shift)
+
+
+def _grad(x, weight, cos, sin, dy, heads, eps, per_head, sin_shift):
+    rows, hidden = x.shape
     dy = dy.contiguous()
     dy = dy if dy.data_ptr() % 16 == 0 else dy.clone()
     with _Device(x.device):
