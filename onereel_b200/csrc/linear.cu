@@ -15,10 +15,14 @@
 // for that, down to a few rows. Rows and columns past the ends are zeros (TMA fill) and are not stored.
 // Every mbarrier wait is bounded (ptx.cuh); the epilogue warps' have one verdict per warp.
 //
-// Measured (device time): 22260 x 8192 -> 2048 with bias, gate and residual 520 us, 1.43 PFLOP/s, 0.88 of a library
-// product's burst rate; 9540 x 2048 -> 8192 with gelu 238 us keeping z, dx 234, dw 219, dz and db 99 + 4. Few rows: 1 x 2048
-// -> 24576 19.4 us, 0.79 of the memory's copy rate; 77 x 2048 -> 8192 11.4 us (the weight alone 5.4), where neither the
-// memory nor the tensor pipe is busy: a block's chain of loads, products and epilogue is.
+// Measured (device time): 22260 x 8192 -> 2048 with bias, gate and residual 490 to 520 us a launch by itself, 1.43 to 1.52
+// PFLOP/s, 0.88 to 0.93 of a library product's burst rate; 610 us (1.22 PFLOP/s) in a row, under the power cap. 9540 x 2048
+// -> 8192 with gelu 238 us keeping z, dx 234, dw 219, dz and db 99 + 4. Few rows: 1 x 2048 -> 24576 19.4 us, 0.79 of the
+// memory's copy rate; 77 x 2048 -> 8192 11.4 us (the weight alone 5.4), where neither the memory nor the tensor pipe is
+// busy: a block's chain of loads, products and epilogue is.
+//
+// Rounded to bf16 are the outputs, z and dz: dz as the operand of two tensor-core products, z because it is m n values to
+// store and read again (act' and act of the rounded z move dz and dgate by half a step of z at most).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -801,7 +805,15 @@ static int launch_gemm(const void* a, long long lda, const void* b, long long ld
 
 // Tile choice: the largest tile that still occupies the GPU. The pair's 256 x 256 tile reads the least shared memory per
 // MMA, 256 x 128 has twice the tiles; below that one CTA takes 128 x 64, or 128 x 32 where few rows leave the streaming of
-// the weight to too few SMs.
+// the weight to too few SMs. Measured on both sides (us, k = 2048 unless given, events resolve 2 us):
+//   256 x 256 from 60 tiles on: 300 x 8192 (64 tiles) 25 against 27 with 256 x 128, 1800 x 2048 (64) 23 and 23; below,
+//     1001 x 2048 (32) 20 against 16, 1537 x 2048 (56) 23 and 23, 1001 x 2048 for dw of depth 1001 (32) 16 against 12.
+//   256 x 128 from 48 on: 513 x 2048 (48) 16 against 18 with 128 x 64, 2000 x 1024 at k = 8192 (64) 41 against 53; below,
+//     300 x 2048 (32) 14 against 12, 1024 x 1024 for dw of depth 1001 (32) 12 against 10.
+//   128 x 64 from 80 on: 300 x 2048 (96) 13 against 17 with 128 x 32, 77 x 8192 (128) 14 against 18; below, 200 x 2048 (64) 12
+//     and 12, with silu, gate and residual at k = 1024 13 against 11, 77 x 2048 at k = 8192 (32) 29 against 27.
+// Streaming kernels against 128 x 64 tiles: 1 x 2048 -> 24576 23 against 49, 3 rows 39 against 49, 4 rows 59 against 49 (and
+// 10 against 14 at 2048 -> 2048); dx of one row, 24576 -> 2048, 35 against 84, of four 59 against 68.
 template <bool kAmn, bool kBmn>
 static int gemm(const void* a, long long lda, const void* b, long long ldb, int m, int n, int k, const Epilogue& ep,
                 int* err, cudaStream_t stream) {
@@ -809,7 +821,7 @@ static int gemm(const void* a, long long lda, const void* b, long long ldb, int 
   auto tiles = [&](int tm, int tn) { return (static_cast<long long>(m) + tm - 1) / tm * ((n + tn - 1) / tn); };
   if (m > 128 && tiles(256, 256) >= 60) return launch_gemm<2, 256, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
   if (m > 128 && tiles(256, 128) >= 48) return launch_gemm<2, 128, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
-  if (kBmn || tiles(128, 64) >= 100) return launch_gemm<1, 64, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
+  if (kBmn || tiles(128, 64) >= 80) return launch_gemm<1, 64, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
   if constexpr (!kBmn) return launch_gemm<1, 32, kAmn, kBmn>(a, lda, b, ldb, g, ep, err, stream);
   return ORL_ERR_UNSUPPORTED;
 }
