@@ -37,6 +37,9 @@
 // one tile holds all keys of its queries (at most 64: then dS is a small difference of large terms; two keys: dq 0.0040
 // off in the 2-norm instead of 0.0024) a kDq block uses its own sum as well.
 //
+// Rounded to bf16 are P and dS, the A operands of the accumulating products (one rounding of each in dv, dq and dk), and the
+// gradients as they are stored; scores, exponentials, delta and the accumulators are fp32.
+//
 // What bounds it (figures: forward excluded, 5 products of useful work). 16 heads of 128, 22516 x 48212 rows in segments
 // of up to 14438 keys: 6.7 ms, 0.90 PFLOP/s useful and 1.26 computed, with the clock down at 1.7 GHz under the power cap:
 // the seven products run at 0.92 of the rate at which a library product is sustained under that cap. 16 heads of 64,

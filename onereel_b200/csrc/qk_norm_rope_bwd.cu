@@ -12,7 +12,7 @@
 // their weight sums in registers over all their rows, so the weight gradient costs a partial row per block; column_sum
 // adds the partial rows in a fixed order.
 // 22260 rows of 2048: 56 us, 0.80 of the measured copy rate (a block of 256 threads to a row, eight elements each and two
-// barriers of the block: 77 us).
+// barriers of the block: 77 us); with the column sums 64 us, over heads 78 us, rows of 5120 over three warps 199 us (0.54).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -1,6 +1,9 @@
 // Gradient of a pack: dst row i = sum of the packed rows that are copies of it (bf16 in and out, summed in fp32 in list
 // order: no atomics). HBM-bound: every packed row is read once, every source row written once; rows without copies get
-// zeros. One block per row and plane, 16 bytes per thread.
+// zeros. One block per row and plane, 16 bytes per thread. The copies' gradients come as the attention backward rounded them
+// to bf16 (as torch's gradient of a gather does): a source row's sum has one rounding for each of its copies besides its own;
+// fp32 copies would cost twice the memory of the packed dk and dv. 22260 rows of 2048 in two planes from 50880 copies: 160 us,
+// 0.57 of the measured copy rate (a row's copies lie far apart, and most rows have two).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -286,7 +286,8 @@ def attend_segments(plan: ScenePlan, q, eq, kp, vp, ov, ot, lse_v=None, lse_t=No
 
 class _PlanAttention(torch.autograd.Function):
     """attend_segments of a plan on one GPU, differentiable: the backward pass packs K / V again, takes the packed
-    gradients of all segments in one call and sums every source row's copies"""
+    gradients of all segments in one call and sums every source row's copies (in bf16, rounded once more where rotate turned
+    them back; the sums in fp32)"""
 
     @staticmethod
     def forward(ctx, plan, rotate, q, k, v, eq, ek, ev):
