@@ -40,10 +40,17 @@ inline int make_rows_map(CUtensorMap* map, const void* base, long long rows, lon
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld_elems) * 2};
   cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? ORL_OK : ORL_ERR_TENSOR_MAP;
+  auto encode = [&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encode()) return ORL_OK;
+  // A driver call: unlike the runtime's it does not bind the device's context to a thread that has made no call yet (a
+  // server's worker, autograd's thread in a process's first backward pass). cudaSetDevice does.
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return ORL_ERR_LAUNCH;
+  return encode() ? ORL_OK : ORL_ERR_TENSOR_MAP;
 }
 
 }  // namespace orl
