@@ -604,9 +604,11 @@ extern "C" int orl_attn_fwd(const void* q, const void* k, const void* v, void* o
                             long long nk, int heads, int head_dim, float scale, const AttnWork* work_dev,
                             int n_items, int* err_dev, void* stream_ptr) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || work_dev == nullptr || err_dev == nullptr)
-    return ORL_ERR_ARG;
   if (nq < 0 || nk < 0 || heads <= 0 || n_items < 0 || !(scale > 0.f)) return ORL_ERR_ARG;
+  // an empty tensor has no address
+  if ((nq > 0 && (q == nullptr || out == nullptr)) || (nk > 0 && (k == nullptr || v == nullptr)) || work_dev == nullptr ||
+      err_dev == nullptr)
+    return ORL_ERR_ARG;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
         reinterpret_cast<uintptr_t>(out)) & 15u) != 0)
     return ORL_ERR_ALIGN;
@@ -733,10 +735,10 @@ extern "C" int orl_attn_fwd_cu(const void* q, const void* k, const void* v, void
                                int* err_dev, void* stream_ptr) {
   using namespace orl;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || cu_q_dev == nullptr || cu_k_dev == nullptr ||
-      work_dev == nullptr || err_dev == nullptr)
-    return ORL_ERR_ARG;
   if (nq < 0 || nk < 0 || heads <= 0 || n_seg < 0 || !(scale > 0.f)) return ORL_ERR_ARG;
+  if ((nq > 0 && (q == nullptr || out == nullptr)) || (nk > 0 && (k == nullptr || v == nullptr)) || cu_q_dev == nullptr ||
+      cu_k_dev == nullptr || work_dev == nullptr || err_dev == nullptr)
+    return ORL_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return ORL_ERR_UNSUPPORTED;
   if (n_seg > kDevPlanMaxSeg) return ORL_ERR_CAPACITY;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |

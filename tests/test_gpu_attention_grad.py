@@ -427,3 +427,27 @@ def test_long_segment():
     out, lse = A.attend(q, k, v, *segs, lse=True)
     dq, dk, dv = A.attend_grad(q, k, v, out, lse, dout, *segs, dlse=dlse)
     check_all(dict(out=out, lse=lse, dq=dq, dk=dk, dv=dv), attention_grads(q, k, v, dout, *segs, dlse=dlse))
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('lq,lk', [([0, 0], [40, 7]), ([33, 150], [0, 0]), ([0], [0]), ([], [])])
+def test_no_queries_and_no_keys(lq, lk, D):
+    """tensors without rows on either side, through every entry point: zeros (log-sum-exp -inf) and zero gradients"""
+    from onereel_b200 import attention as A
+    H = 2
+    q, k, v, dout, _ = inputs(sum(lq), sum(lk), H, D, seed=1)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    cq, ck = A.cu_seqlens(lq), A.cu_seqlens(lk)
+    calls = [lambda *t: A.varlen_lse(*t, cq, ck, 200, 40), lambda *t: A.varlen_lse(*t, cq.tolist(), ck.tolist(), 200, 40)]
+    if len(lq) == 2:
+        calls.append(lambda *t: (A.overlapping_ranges(*t, [(0, lq[0]), (lq[0], sum(lq))], [(0, lk[0]), (lk[0], sum(lk))]), None))
+    for call in calls:
+        with torch.no_grad():
+            plain = call(q, k, v)
+        out, lse = call(*leaves)
+        assert out.shape == q.shape and not out.any() and torch.equal(out, plain[0])
+        assert lse is None or (lse == -float('inf')).all()
+        grads = torch.autograd.grad(out, leaves, dout)
+        assert all(g.shape == x.shape and not g.any() for g, x in zip(grads, leaves))
+    torch.cuda.synchronize()
+    A.check()

@@ -363,3 +363,59 @@ def test_phase_marks_with_and_without_gradients(monkeypatch):
         proc.scene(*(t.clone().requires_grad_(grad) for t in x))
         seen.append([name for name, _ in HY.PHASES])
     assert seen[0] == seen[1] and seen[0][0] == 'start' and 'near' in seen[0]
+
+
+@pytest.mark.parametrize('shared_pos', ['source', 'adjacent'])
+def test_captured_scene_step(shared_pos):
+    """a training step of Processor.scene captured after a first one, replayed on new values when the work-list caches have
+    been emptied of its layout since"""
+    from onereel_b200 import attention as A, hunyuan15 as HY, standin
+    from onereel_b200.layout import SceneLayout
+    lay = SceneLayout([3, 2, 4], halo=1, extra={0: [7], 2: [0]})
+    T, H, D, counts = 48, 2, 64, [7, 0, 5]
+    L = lay.n_frames * T
+    ctx = HY.Context(lay, T=T, counts={True: counts}, fwd=1, own=[(0, L)], shared_pos=shared_pos)
+    ctx._rot_full = tuple(t.cuda() for t in standin.rope_3d(lay.n_frames, 6, 8, D, axes=(8, 28, 28)))
+    proc = HY.Processor(ctx, 0)
+    x = [rand(n, H, D, seed=i) for i, n in enumerate((L, L, L, *[sum(counts)] * 3))]
+    gv, gt = rand(L, H, D, seed=10), rand(sum(counts), H, D, seed=11)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in x]
+        out = proc.scene(*leaves)
+        return (*(t.detach() for t in out), *torch.autograd.grad(out, leaves, (gv, gt)))
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for n in range(1, 700):
+        A.plan([0], [n], [0], [n], H, x[0].device)
+        A._plan_bwd([0], [n], [0], [n], H, n, n, x[0].device)
+    x[0].copy_(rand(L, H, D, seed=50))
+    x[4].copy_(rand(sum(counts), H, D, seed=51))
+    graph.replay()
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(res, want))
+    A.check()
+
+
+def test_scene_step_without_text_rows():
+    """sentences of no tokens: the text side is empty, the video side is the layer's without text"""
+    from onereel_b200 import attention as A, hunyuan15 as HY, wan
+    from onereel_b200.layout import SceneLayout
+    lay = SceneLayout([2, 3], halo=1, extra={0: [4]})
+    T, H, D = 16, 2, 64
+    L = lay.n_frames * T
+    x = [rand(n, H, D, seed=i).requires_grad_() for i, n in enumerate((L, L, L, 0, 0, 0))]
+    g = rand(L, H, D, seed=9)
+    proc = HY.Processor(HY.Context(lay, T=T, counts={True: [0, 0]}, fwd=1, own=[(0, L)]), 0)
+    with torch.no_grad():
+        want_v, want_t = proc.scene(*x)
+    ov, ot = proc.scene(*x)
+    assert torch.equal(ov, want_v) and ot.shape == want_t.shape == (0, H, D)
+    got = torch.autograd.grad((ov, ot), x, (g, torch.empty_like(ot)))
+    o = wan.Processor(wan.Context(lay, T=T, own=[(0, L)]), 'self', None, 0).ranges(*x[:3])
+    assert torch.equal(o, ov)
+    want = torch.autograd.grad(o, x[:3], g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(t.shape == (0, H, D) for t in got[3:])
+    A.check()
