@@ -159,7 +159,8 @@ extern "C" int orl_qk_norm_rope(const void* x, void* y, const void* weight, cons
                                 long long rows, int heads, int head_dim, int per_head, float eps, int sin_shift,
                                 long long rope_ld, const int32_t* row_map, void* stream_ptr) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (x == nullptr || y == nullptr || weight == nullptr || cos_t == nullptr || sin_t == nullptr) return ORL_ERR_ARG;
+  if (weight == nullptr) return ORL_ERR_ARG;
+  if (rows > 0 && (x == nullptr || y == nullptr || cos_t == nullptr || sin_t == nullptr)) return ORL_ERR_ARG;
   if (rows < 0 || heads <= 0 || head_dim <= 0 || (head_dim & 7) || sin_shift < 0 || sin_shift > 1 || rope_ld < head_dim)
     return ORL_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15u) return ORL_ERR_ALIGN;

@@ -57,7 +57,8 @@ def _table(t, rows: int, device):
     """a rotary table as the kernels read it: fp32 [rows, D], contiguous"""
     if t.dtype is torch.float32 and t.device == device and t.dim() == 2 and t.shape[0] == rows and t.is_contiguous():
         return t
-    return t.to(device=device, dtype=torch.float32).reshape(rows, -1).contiguous()
+    t = t.to(device=device, dtype=torch.float32)
+    return t.reshape(rows, -1 if rows else t.shape[-1]).contiguous()
 
 
 def _forward(x, w, c, s, heads, eps, per_head, sin_shift, out=None, row_map=None):

@@ -138,3 +138,18 @@ def test_gradients_without_and_with_a_large_epsilon(heads, dh, per_head, eps):
     wx, ww = reference(x, w, cos, sin, dy, heads, eps, per_head, 0)
     assert_close(dx, wx, 'dx')
     assert_close(dw, ww, 'dw')
+
+
+@pytest.mark.parametrize('per_head', [True, False])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float64])
+def test_no_rows(per_head, dtype):
+    from onereel_b200.rope import qk_norm_rope
+    heads, dh = 3, 64
+    x = torch.empty(0, heads * dh, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    w = torch.ones(dh if per_head else heads * dh, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    table = torch.empty(0, dh, device='cuda', dtype=dtype)
+    with torch.no_grad():
+        assert qk_norm_rope(x, w, table, table, heads, 1e-6, per_head, 0).shape == (0, heads, dh)
+    y = qk_norm_rope(x, w, table, table, heads, 1e-6, per_head, 0)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+    assert dx.shape == x.shape and dw.shape == w.shape and not dw.any()
