@@ -451,3 +451,28 @@ def test_no_queries_and_no_keys(lq, lk, D):
         assert all(g.shape == x.shape and not g.any() for g, x in zip(grads, leaves))
     torch.cuda.synchronize()
     A.check()
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('lq,lk', [([70, 300], [130, 200]), ([1, 129], [5, 64]), ([200, 57], [65, 400]), ([256, 128], [63, 1])])
+def test_a_segment_beside_a_bad_one(lq, lk, D):
+    """the next segment's q, k, v and dout all NaN: the first segment's gradients keep their bits, planned on either side"""
+    from onereel_b200 import attention as A
+    H = 2
+    data = inputs(sum(lq), sum(lk), H, D, seed=lq[0])[:4]
+    cq, ck = A.cu_seqlens(lq), A.cu_seqlens(lk)
+    for plan in (lambda c: c, lambda c: c.tolist()):
+        res = []
+        for bad in (False, True):
+            x = [t.clone() for t in data]
+            if bad:
+                for t, n in zip(x, (lq[0], lk[0], lk[0], lq[0])):
+                    t[n:] = float('nan')
+            leaves = [t.requires_grad_() for t in x[:3]]
+            out = A.varlen(*leaves, plan(cq), plan(ck), max(lq), max(lk))
+            dq, dk, dv = torch.autograd.grad(out, leaves, x[3])
+            res.append((out.detach()[:lq[0]], dq[:lq[0]], dk[:lk[0]], dv[:lk[0]]))
+        for a, b in zip(*res):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
+    torch.cuda.synchronize()
+    A.check()
