@@ -241,9 +241,9 @@ def _attend_split(q, k, v, q_start, q_len, k_start, k_len, out, lse, scale):
 
 
 def attend(q, k, v, q_start, q_len, k_start, k_len, out=None, lse=None, scale=None, stream=None, split_keys=False):
-    """the kernel call, without a backward pass: segment i = q rows q_start[i] + [0, q_len[i]) attending to k / v rows k_start[i] + [0, k_len[i]).
-    out [Nq, H, D] bf16 (allocated if None); lse None, True (allocate [H, Nq] fp32) or a tensor. split_keys: allow the
-    key split of coarse launches (see SPLIT_WAVES)."""
+    """the kernel call, without a backward pass: segment i = q rows q_start[i] + [0, q_len[i]) attending to k / v rows
+    k_start[i] + [0, k_len[i]). out [Nq, H, D] bf16 (allocated if None); lse None, True (allocate [H, Nq] fp32) or a tensor.
+    split_keys: allow the key split of coarse launches (see SPLIT_WAVES)."""
     _check_inputs(q, k, v)
     Nq, H, Dh = q.shape
     dev = q.device
@@ -270,8 +270,8 @@ def attend(q, k, v, q_start, q_len, k_start, k_len, out=None, lse=None, scale=No
 
 
 def attend_work(q, k, v, work, n_items: int, out, lse=None, scale=None, stream=None):
-    """the kernel call, without a backward pass, with a caller-held device work list (orl_attn_plan_ranges items, possibly edited on the
-    device since: the bounded memory sets each item's key count per head from its selection)"""
+    """the kernel call, without a backward pass, with a caller-held device work list (orl_attn_plan_ranges items, possibly
+    edited on the device since: the bounded memory sets each item's key count per head from its selection)"""
     _check_inputs(q, k, v)
     Nq, H, Dh = q.shape
     dev = q.device

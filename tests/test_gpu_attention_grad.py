@@ -440,7 +440,8 @@ def test_no_queries_and_no_keys(lq, lk, D):
     cq, ck = A.cu_seqlens(lq), A.cu_seqlens(lk)
     calls = [lambda *t: A.varlen_lse(*t, cq, ck, 200, 40), lambda *t: A.varlen_lse(*t, cq.tolist(), ck.tolist(), 200, 40)]
     if len(lq) == 2:
-        calls.append(lambda *t: (A.overlapping_ranges(*t, [(0, lq[0]), (lq[0], sum(lq))], [(0, lk[0]), (lk[0], sum(lk))]), None))
+        ranges = [(0, lq[0]), (lq[0], sum(lq))], [(0, lk[0]), (lk[0], sum(lk))]
+        calls.append(lambda *t: (A.overlapping_ranges(*t, *ranges), None))
     for call in calls:
         with torch.no_grad():
             plain = call(q, k, v)

@@ -1,4 +1,5 @@
-"""What the entry points refuse before they hand an address to a kernel (no GPU: tensors without storage stand for CUDA ones)."""
+"""What the entry points refuse before they hand an address to a kernel (no GPU: tensors without storage stand for CUDA
+ones)."""
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -82,6 +83,7 @@ def test_row_sum_refuses_parts_that_differ():
     with torch._subclasses.fake_tensor.unset_fake_temporarily():
         s = RowSum([0, 1, 1], [0, 1, 2], 2, 'cpu')
         part = lambda *shape, dtype=BF16: torch.zeros(*shape, dtype=dtype)
-        for parts in ([part(3, 1, 16), part(3, 1, 8)], [part(3, 1, 8), part(2, 1, 8)], [part(3, 1, 8), part(3, 1, 8, dtype=torch.half)]):
+        for parts in ([part(3, 1, 16), part(3, 1, 8)], [part(3, 1, 8), part(2, 1, 8)],
+                      [part(3, 1, 8), part(3, 1, 8, dtype=torch.half)]):
             with pytest.raises(ValueError, match='alike'):
                 s.run(parts)
