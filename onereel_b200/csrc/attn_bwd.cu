@@ -43,7 +43,7 @@
 // What bounds it (figures: forward excluded, 5 products of useful work). 16 heads of 128, 22516 x 48212 rows in segments
 // of up to 14438 keys: 6.7 ms, 0.90 PFLOP/s useful and 1.26 computed, with the clock down at 1.7 GHz under the power cap:
 // the seven products run at 0.92 of the rate at which a library product is sustained under that cap. 16 heads of 64,
-// 3 x 2048 rows: 273 us; a tile costs the compute warps as much as at D = 128 (exponentials, TMEM loads and barriers of
+// 3 x 2048 rows: 279 us; a tile costs the compute warps as much as at D = 128 (exponentials, TMEM loads and barriers of
 // some 1200 clocks per 64 keys), in which its MMAs take 450.
 //
 // Every mbarrier wait is bounded as in the forward: a stuck pipeline sets the error word and winds down. The compute warps'
